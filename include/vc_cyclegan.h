@@ -44,7 +44,8 @@ extern "C" {
 typedef struct vc_plan vc_plan;   /* opaque: geometry tables + workspace map for one (F, T) */
 
 /* ---- library ------------------------------------------------------------- */
-int         vc_version(void);          /* ABI revision: 116 (bumped whenever an entry point changes or is added) */
+int         vc_version(void);          /* ABI revision: 116 (bumped whenever an entry point above or below changes; the sequence operators came
+                                        * with no change to the others and carry a revision of their own: vc_seq_version) */
 int         vc_thread_is_product_run(void);   /* 1 when every test / tuning switch of vc_cyclegan_testing.h is at its production value in the
                                                * calling thread (model.CycleGAN.train and bench.py refuse to run otherwise: a forced tile
                                                * configuration left behind by a test must never be trained or benched with) */
@@ -208,6 +209,101 @@ int vc_l2_loss(const float* y, const float* y_hat, int64_t n, float* loss, float
  * after a summing all-reduce). */
 int vc_adam_tf_update(float* p, float* m, float* v, const float* g, int64_t n,
                       float alpha, float beta1, float beta2, float eps, float grad_scale, void* stream);
+
+/* ---- sequence operators: a frame's norm, the short causal convolution, the selective state space scan ----------------
+ * The networks above look ahead (SAME padding, module.py:32-40) and normalise over a whole utterance (module.py:135-146): they convert
+ * recordings.  These operators look back only, so a model built of them trains on packed utterances and runs on a live stream frame by frame.
+ *
+ * Layout: frame-major.  A tensor is rows x channels, channel stride 1, `*_ld` elements from row to row (a column slice of a wider product is
+ * passed in place; 0 repeats one row).  Row strides, pointers and channel counts need no alignment beyond the element's own.
+ * Types (`type`, the activations of one call): VC_F32, VC_BF16, VC_F16.  Parameters, recurrent states, statistics, and parameter gradients
+ * are fp32.  All sums are taken in fp32, in a fixed order: there are no atomics and two runs on the same inputs are bitwise equal.
+ * Utterances: `offsets` (device, int32, n_seqs + 1 entries, rising) packs n_seqs utterances of any length, zero included, one behind the
+ * other: utterance s is rows [offsets[s], offsets[s+1]).  NULL: n_seqs utterances of rows / n_seqs frames each.  Offsets are clamped into
+ * [0, rows] on the device (they are not read back), so wrong ones give wrong numbers and no access outside the tensors.
+ * Rows behind the last utterance are left as they were in every output, or cleared where `zero_tail` is set.
+ * Slots (`slots`, device, int32, one per row of a single-frame call): which entry of the state pool a row belongs to; NULL: row r has entry r.
+ * A row whose slot lies outside [0, n_slots), or that an earlier row of the call has already named, is padding: y gets zeros, no state moves. */
+#define VC_F32   0
+#define VC_BF16  1
+#define VC_F16   2
+int vc_seq_version(void);              /* revision of this section: 1 */
+
+/* RMS norm of every row with the residual's addition (beside vc_instnorm_glu_fwd mode 2, which adds the residual behind the norm):
+ *   t = x + residual, rounded to sum_type and stored in `sum`;   rstd = 1 / sqrt(mean(t^2) + eps);   y = t * rstd * gamma
+ * The norm reads t as it is stored, so the backward pass needs `sum` and rstd alone.  residual NULL: t = x (sum is not written and may be
+ * NULL, sum_type == type).  rstd [rows] may be NULL.  eps > 0: a row of zeros gives zeros.  sum_type: type or VC_F32.
+ * x, y, residual, sum: y may be x, sum may be residual. */
+int vc_rms_norm_fwd(const void* x, int64_t x_ld, const void* residual, int64_t res_ld, const float* gamma,
+                    void* y, int64_t y_ld, void* sum, int64_t sum_ld, float* rstd, float eps,
+                    int64_t rows, int cols, int type, int sum_type, void* stream);
+/* The same with y in 8 bits: q [rows][cols] OCP e4m3 (one byte each), y ~= q * scale.  group: columns that share a scale: 32, 64 or 128
+ * (dividing cols), or 0 for the whole row; scale [rows][cols/group or 1], contiguous.  scale = max|y| / 448 of the fp32 y (not below 2^-100 / 448),
+ * q = y / scale rounded to nearest even.  A group that holds a NaN or an infinity gets a NaN or infinite scale: it stands for no numbers. */
+int vc_rms_norm_e4m3(const void* x, int64_t x_ld, const void* residual, int64_t res_ld, const float* gamma,
+                     void* q, int64_t q_ld, float* scale, void* sum, int64_t sum_ld, float eps,
+                     int64_t rows, int cols, int group, int type, int sum_type, void* stream);
+/* Backward: t (`sum` of the forward, or x where it had no residual), rstd, dy and dsum (gradient of the stored sum, sum_type; may be NULL):
+ *   dt = dsum + rstd * (dy gamma - that * mean(dy gamma that)), that = t * rstd;   dgamma[c] = sum over rows of dy that (overwritten)
+ * dx (type) and dres (sum_type) both receive dt; either may be NULL.  work: vc_rms_norm_bwd_work(rows, cols) floats; dgamma NULL: none needed. */
+int64_t vc_rms_norm_bwd_work(int64_t rows, int cols);
+int vc_rms_norm_bwd(const void* dy, int64_t dy_ld, const void* dsum, int64_t dsum_ld, const void* sum, int64_t sum_ld,
+                    const float* rstd, const float* gamma, void* dx, int64_t dx_ld, void* dres, int64_t dres_ld, float* dgamma,
+                    float* work, int64_t work_floats, int64_t rows, int cols, int type, int sum_type, void* stream);
+
+/* Short causal convolution along the rows, one filter per channel (beside vc_conv2d_fwd, which pads both ends and mixes channels):
+ *   p[t][c] = bias[c] + sum_k w[k][c] x[t - (taps-1) + k][c];   y = p * sigmoid(p) (silu != 0) or p
+ * w [taps][cols], 2 <= taps <= 8; bias may be NULL.  Frames before an utterance come from initial [n_seqs][taps-1][cols] (type; oldest first;
+ * NULL: zeros).  final [n_seqs][taps-1][cols] (may be NULL) receives the last taps-1 frames, what the next call of a stream takes as initial;
+ * final may not be initial. */
+typedef struct {
+    const void* x; const float* w; const float* bias; const void* initial; const int32_t* offsets;
+    void* y; void* final_state;
+    int64_t x_ld, y_ld;
+    int64_t rows; int32_t cols, taps, n_seqs, type, silu, zero_tail;
+    /* backward only: dy (type), dfinal (type, may be NULL) in; dx, dinitial (type), dw [taps][cols], dbias [cols] (fp32, overwritten) out, each may be NULL */
+    const void* dy; const void* dfinal; void* dx; void* dinitial; float* dw; float* dbias;
+    int64_t dy_ld, dx_ld;
+    float* work; int64_t work_floats;              /* backward: vc_causal_conv1d_bwd_work floats */
+} vc_conv1d_args;
+int vc_causal_conv1d_fwd(const vc_conv1d_args* a, void* stream);
+int64_t vc_causal_conv1d_bwd_work(const vc_conv1d_args* a);
+int vc_causal_conv1d_bwd(const vc_conv1d_args* a, void* stream);
+/* One frame of `rows` streams: y from the row and its slot's taps-1 earlier frames; state [n_slots][taps-1][cols] (type) moves on by one frame. */
+int vc_causal_conv1d_step(const void* x, int64_t x_ld, void* state, const int32_t* slots, const float* w, const float* bias,
+                          void* y, int64_t y_ld, int rows, int n_slots, int cols, int taps, int type, int silu, void* stream);
+
+/* Selective state space scan along the rows:
+ *   delta = softplus(dt + dt_bias) (softplus != 0) or dt + dt_bias
+ *   h[t][c][n] = exp(delta[t][c] A[c][n]) h[t-1][c][n] + delta[t][c] x[t][c] B[t][g][n]
+ *   y[t][c] = (sum_n C[t][g][n] h[t][c][n] + D[c] x[t][c]) * z[t][c] sigmoid(z[t][c])
+ * with g = c / (cols / groups): the channels of a group share B and C.  A [cols][states] fp32, finite, 1 <= states <= 64.  D, z, dt_bias may be NULL
+ * (no skip, no gate, no bias).  B, C: row stride b_ld / c_ld, group g at + g * states.  initial [n_seqs][cols][states] fp32 (NULL: zeros);
+ * final_state likewise (NULL: not wanted); final_state may not be initial. */
+typedef struct {
+    const void *x, *dt, *z, *B, *C; const float *A, *D, *dt_bias; const float* initial; const int32_t* offsets;
+    void* y; float* final_state;
+    int64_t x_ld, dt_ld, z_ld, b_ld, c_ld, y_ld;
+    int64_t rows; int32_t cols, states, groups, n_seqs, type, softplus, zero_tail;
+    int32_t max_len;               /* longest utterance where the caller knows it, else 0: how the work is split, never what is computed */
+    /* Training: the states in front of every tile of rows, kept by the forward for the backward (NULL: not kept).  vc_selective_scan_saved floats. */
+    float* saved; int64_t saved_floats;
+    /* backward only: dy (type), dfinal (fp32, may be NULL) in; out: dx, ddt, dz, dB, dC (type; dB / dC with strides db_ld / dc_ld and groups like B / C), dA, dD,
+     * ddt_bias, dinitial (fp32).  dz, dD, ddt_bias, dinitial may be NULL. */
+    const void* dy; const float* dfinal; void *dx, *ddt, *dz, *dB, *dC; float *dA, *dD, *ddt_bias, *dinitial;
+    int64_t dy_ld, dx_ld, ddt_ld, dz_ld, db_ld, dc_ld;
+    float* work; int64_t work_floats;              /* vc_selective_scan_fwd_work / _bwd_work floats */
+} vc_scan_args;
+int64_t vc_selective_scan_saved(const vc_scan_args* a);
+int64_t vc_selective_scan_fwd_work(const vc_scan_args* a);
+int64_t vc_selective_scan_bwd_work(const vc_scan_args* a);
+int vc_selective_scan_fwd(const vc_scan_args* a, void* stream);
+int vc_selective_scan_bwd(const vc_scan_args* a, void* stream);
+/* One frame of `rows` streams; state [n_slots][cols][states] fp32 is moved on in place. */
+int vc_selective_scan_step(const void* x, int64_t x_ld, const void* dt, int64_t dt_ld, const void* z, int64_t z_ld,
+                           const void* B, int64_t b_ld, const void* C, int64_t c_ld, const float* A, const float* D, const float* dt_bias,
+                           float* state, const int32_t* slots, void* y, int64_t y_ld,
+                           int rows, int n_slots, int cols, int states, int groups, int type, int softplus, void* stream);
 
 /* ---- network level --------------------------------------------------------- */
 /* Geometry plan for num_features x n_frames inputs (n_frames % 4 == 0): geometry tables of every layer of both networks

@@ -1,0 +1,675 @@
+"""GPU: the sequence operators against the 64-bit oracle, through their public entry points.
+
+Tolerances.  A result of type t may be off by half a step of t (finfo(t).eps / 2 of its value) for its one rounding, and by K * 2^-24 of its magnitude --
+the same sum over absolute values, which the oracle gives -- for the fp32 arithmetic behind it, K being the number of roundings a term passes:
+  norm    each thread adds up to cols / 64 squares, then 6 + 4 steps across lanes and waves, and a few products: cols / 64 + 20
+  conv    taps products and sums, the bias, a sigmoid (exponential, reciprocal): taps + 20; its parameter gradients add over the rows as well
+  scan    a term is carried by exp(delta A) from frame to frame, 3 roundings each (the exponential's two and the product), for as many frames as it
+          lasts -- delta |A| >= 0.02 in these inputs, so 2^-24 of it is left after 17 / 0.02 = 850 frames; the argument's own error (10 units of
+          delta |A|, softplus and two products) adds 10 s e^-s < 4 in all; then the sums over the states.  Backwards the same twice, and the sums over rows
+          and channels.
+Nothing here is fitted to results."""
+import numpy as np
+import pytest
+import torch
+
+import vcgan_pkg  # noqa: F401
+from oracle import sequence_oracle as O
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+DEV = 'cuda:0'
+
+
+@pytest.fixture(scope='module')
+def S(built_lib):
+    assert torch.cuda.is_available()
+    from voice_converter_cyclegan_amd import sequence
+    return sequence
+
+
+def close(got, ref, mag, k, name=''):
+    got64, ref, mag = got.detach().cpu().double(), ref.double(), mag.double()
+    assert got64.shape == ref.shape, (name, got64.shape, ref.shape)
+    info = torch.finfo(got.dtype)
+    half = 0.0 if got.dtype == F32 else info.eps / 2
+    tol = half * ref.abs() + k * U * mag * (1 + half) + (info.smallest_normal * info.eps if got.dtype == F16 else 1e-37)
+    bad = ~((got64 - ref).abs() <= tol)
+    assert not bad.any(), '%s: %d of %d off, worst %.3g of its tolerance' % (name, int(bad.sum()), bad.numel(), float(((got64 - ref).abs() / tol).max()))
+
+
+def rnd(seed, *shape, dtype=F32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).to(DEV)
+
+
+# ------------------------------------------------------------------------------------------------------------------ norm
+
+NORM_SHAPES = [(1, 1), (1, 512), (3, 7), (5, 64), (2, 1001), (130, 1024), (7, 2048), (3, 2056), (4, 8192), (2, 8200), (2, 20001)]
+
+
+@pytest.mark.parametrize('rows,cols', NORM_SHAPES)
+@pytest.mark.parametrize('kind,stream', [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)])
+def test_norm_and_gradient(S, rows, cols, kind, stream):
+    x, res = rnd(1, rows, cols, dtype=kind), rnd(2, rows, cols, dtype=stream, scale=3.0)
+    gamma = 1 + rnd(3, cols, scale=0.1)
+    dy, ds = rnd(4, rows, cols, dtype=kind), rnd(5, rows, cols, dtype=stream)
+    for t in (x, res, gamma):
+        t.requires_grad_(True)
+    y, total = S.rms_norm(x, gamma, res, eps=1e-5)
+    want_total = (x.detach().float() + res.detach().float()).to(stream)
+    assert torch.equal(total.detach(), want_total)
+    k = cols / 64 + 20
+    ref, dt, dgamma = O.rms_norm(want_total, gamma, 1e-5, dy, ds)
+    _, dt_m, dgamma_m = O.rms_norm(want_total, gamma, 1e-5, dy, ds, absolute=True)
+    close(y, ref, ref.abs(), k, 'y')
+    dx, dres, dg = torch.autograd.grad((y, total), (x, res, gamma), (dy, ds))
+    close(dx, dt, dt_m, 3 * k, 'dx')
+    close(dres, dt, dt_m, 3 * k, 'dres')
+    close(dg, dgamma, dgamma_m, k + rows, 'dgamma')
+
+
+@pytest.mark.parametrize('kind', [F32, BF16])
+def test_norm_without_residual_and_partial_gradients(S, kind):
+    x, gamma, dy = rnd(1, 4, 9, 100, dtype=kind), 1 + rnd(2, 100, scale=0.1), rnd(3, 4, 9, 100, dtype=kind)
+    ref, dt, dgamma = O.rms_norm(x.view(36, 100), gamma, 1e-6, dy.view(36, 100))
+    _, dt_m, dg_m = O.rms_norm(x.view(36, 100), gamma, 1e-6, dy.view(36, 100), absolute=True)
+    with torch.no_grad():
+        close(S.rms_norm(x, gamma).view(36, 100), ref, ref.abs(), 22)
+    x.requires_grad_(True)
+    (dx,) = torch.autograd.grad(S.rms_norm(x, gamma), x, dy)
+    close(dx.view(36, 100), dt, dt_m, 66)
+    x.requires_grad_(False)
+    gamma.requires_grad_(True)
+    (dg,) = torch.autograd.grad(S.rms_norm(x, gamma), gamma, dy)
+    close(dg, dgamma, dg_m, 60)
+
+
+def test_norm_only_the_sum_has_a_gradient(S):
+    x, res, gamma = rnd(1, 5, 64).requires_grad_(True), rnd(2, 5, 64).requires_grad_(True), torch.ones(64, device=DEV)
+    _, total = S.rms_norm(x, gamma, res)
+    d = rnd(3, 5, 64)
+    dx, dr = torch.autograd.grad(total, (x, res), d)
+    assert torch.equal(dx, d) and torch.equal(dr, d)
+
+
+@pytest.mark.parametrize('kind,stream', [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F32)])
+@pytest.mark.parametrize('rows,cols,group', [(1, 64, 0), (3, 1000, 0), (5, 96, 32), (130, 1024, 128), (4, 2048, 64), (9, 4224, 128), (2, 9000, 0), (2, 20032, 64), (2, 20001, 0)])
+def test_norm_e4m3(S, kind, stream, rows, cols, group):
+    x, res, gamma = rnd(1, rows, cols, dtype=kind), rnd(2, rows, cols, dtype=stream, scale=3.0), 1 + rnd(3, cols, scale=0.1)
+    q, scale, total = S.rms_norm_e4m3(x, gamma, res, eps=1e-5, group=group)
+    want_total = (x.float() + res.float()).to(stream)
+    assert torch.equal(total, want_total) and q.dtype == torch.float8_e4m3fn and scale.shape == (rows, cols // group if group else 1)
+    y = O.rms_norm(want_total, gamma, 1e-5)
+    k = cols / 64 + 24
+    top = y.view(rows, -1, group or cols).abs().amax(-1)
+    close(scale, top / 448, top / 448, k, 'scale')
+    # a value is off by half a step of e4m3 (2^-4 of it, 2^-10 scales below the normal range), and the y it rounds by the arithmetic before it
+    wide = scale.double().cpu().repeat_interleave(group or cols, 1)
+    err = (q.float().double().cpu() * wide - y).abs()
+    assert (err <= y.abs() * (2.0 ** -4 + k * U) + wide * 2.0 ** -10).all(), float(err.max())
+    assert q.float().abs().max() <= 448
+
+
+def test_norm_e4m3_zeros_and_non_numbers(S):
+    x = rnd(1, 4, 256)
+    x[0] = 0
+    x[1, 130] = float('nan')
+    gamma = torch.ones(256, device=DEV)
+    q, scale = S.rms_norm_e4m3(x, gamma, group=128)
+    v = q.float().view(4, 2, 128) * scale[..., None]
+    assert (v[0] == 0).all() and torch.isfinite(scale[0]).all()
+    assert torch.isnan(v[1]).all()                                # the row's mean square is no number
+    assert torch.isfinite(v[2:]).all()
+    gamma2 = gamma.clone()
+    gamma2[200] = float('inf')
+    q, scale = S.rms_norm_e4m3(rnd(2, 1, 256), gamma2, group=128)
+    assert torch.isfinite(scale[0, 0]) and not torch.isfinite(scale[0, 1])
+
+
+def test_norm_zero_row_and_in_place_buffers(S):
+    x = torch.zeros(2, 32, device=DEV, requires_grad=True)
+    gamma = torch.ones(32, device=DEV, requires_grad=True)
+    y = S.rms_norm(x, gamma, eps=1e-6)
+    assert (y == 0).all()
+    dx, dg = torch.autograd.grad(y, (x, gamma), torch.ones_like(y))
+    assert torch.allclose(dx, torch.full_like(dx, 1e3)) and (dg == 0).all()
+
+
+# ----------------------------------------------------------------------------------------------------------- convolution
+
+LENGTHS = [[1], [5], [3, 3, 3], [0, 1, 2, 0, 7, 40], [17, 64, 65, 1], [150]]
+
+
+def offsets_of(lengths):
+    return torch.tensor(np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32), device=DEV)
+
+
+@pytest.mark.parametrize('lengths', LENGTHS)
+@pytest.mark.parametrize('cols,taps,kind,silu', [(1, 2, F32, True), (24, 4, F32, False), (300, 4, BF16, True), (257, 3, F16, True), (64, 8, F32, True), (1030, 4, BF16, True)])
+def test_conv_packed_with_states_and_a_tail(S, lengths, cols, taps, kind, silu):
+    n, live = len(lengths), sum(lengths)
+    rows = live + 3                                              # three rows behind the last utterance, which nothing may read
+    x, w, b = rnd(1, rows, cols, dtype=kind), rnd(2, taps, cols, scale=taps ** -0.5), rnd(3, cols, scale=0.1)
+    x[live:] = float('nan')
+    init = rnd(4, n, taps - 1, cols, dtype=kind)
+    dy, df = rnd(5, rows, cols, dtype=kind), rnd(6, n, taps - 1, cols, dtype=kind)
+    dy[live:] = float('nan')
+    leaves = [t.requires_grad_(True) for t in (x, w, b, init)]
+    y, final = S.causal_conv1d(x, w, b, initial_state=init, seq_offsets=offsets_of(lengths), silu=silu, return_final_state=True)
+    xc, dyc = x.detach().cpu(), dy.cpu().clone()
+    xc[live:], dyc[live:] = 0, 0
+    r = O.conv1d(xc, w, b, init, lengths, silu, dyc, df)
+    m = O.conv1d(xc, w, b, init, lengths, silu, dyc, df, absolute=True)
+    close(y, r['y'], m['p'], taps + 20, 'y')
+    assert (y[live:] == 0).all()
+    assert torch.equal(final.detach().double().cpu(), r['final'])
+    dx, dw, db, di = torch.autograd.grad((y, final), leaves, (dy, df))
+    close(dx, r['dx'], m['dx'], taps + 20, 'dx')
+    assert (dx[live:] == 0).all()
+    close(di, r['dinitial'], m['dinitial'], taps + 20, 'dinitial')
+    close(dw, r['dw'], m['dw'], taps + 20 + live, 'dw')
+    close(db, r['dbias'], m['dbias'], taps + 20 + live, 'dbias')
+
+
+@pytest.mark.parametrize('kind', [F32, BF16])
+def test_conv_batch_without_states(S, kind):
+    x, w = rnd(1, 5, 33, 130, dtype=kind), rnd(2, 4, 130, scale=0.5)
+    dy = rnd(3, 5, 33, 130, dtype=kind)
+    leaves = [t.requires_grad_(True) for t in (x, w)]
+    y = S.causal_conv1d(x, w)
+    flat = x.detach().view(-1, 130)
+    r = O.conv1d(flat, w, None, None, [33] * 5, True, dy.view(-1, 130))
+    m = O.conv1d(flat, w, None, None, [33] * 5, True, dy.view(-1, 130), absolute=True)
+    close(y.view(-1, 130), r['y'], m['p'], 24, 'y')
+    dx, dw = torch.autograd.grad(y, leaves, dy)
+    close(dx.view(-1, 130), r['dx'], m['dx'], 24, 'dx')
+    close(dw, r['dw'], m['dw'], 24 + 165, 'dw')
+
+
+@pytest.mark.parametrize('kind', [F32, BF16, F16])
+@pytest.mark.parametrize('cols', [5, 264])
+def test_conv_steps_equal_the_prompt(S, kind, cols):
+    n, t, taps = 3, 9, 4
+    x, w, b = rnd(1, n, t, cols, dtype=kind), rnd(2, taps, cols, scale=0.5), rnd(3, cols)
+    init = rnd(4, n, taps - 1, cols, dtype=kind)
+    y, final = S.causal_conv1d(x, w, b, initial_state=init, return_final_state=True)
+    pool = rnd(5, 7, taps - 1, cols, dtype=kind)
+    untouched = pool.clone()
+    slots = torch.tensor([6, 0, 3], dtype=torch.int32, device=DEV)
+    pool[slots.long()] = init
+    m = O.conv1d(x.view(-1, cols), w, b, init, [t] * n, True, absolute=True)['p'].view(n, t, cols)
+    for i in range(t):
+        yi = S.causal_conv1d_step(x[:, i], pool, w, b, slots=slots)
+        close(yi, y[:, i].cpu().double(), m[:, i] + (0 if kind == F32 else torch.finfo(kind).eps / U * y[:, i].cpu().double().abs()), 48, 'frame %d' % i)
+    assert torch.equal(pool[slots.long()], final)
+    for i in (1, 2, 4, 5):
+        assert torch.equal(pool[i], untouched[i])
+
+
+# ------------------------------------------------------------------------------------------------------------------ scan
+
+def scan_inputs(rows, cols, states, groups, kind, seqs, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    step = torch.exp(torch.rand(cols, generator=g) * 2.3 - 3.0)                  # 0.05 .. 0.5
+    A = -(0.4 + torch.rand(cols, states, generator=g) * 4)
+    v = dict(x=rnd(seed + 1, rows, cols, dtype=kind), dt=rnd(seed + 2, rows, cols, dtype=kind).clamp(-0.1, 0.5), A=A.to(DEV),
+             B=rnd(seed + 3, rows, groups, states, dtype=kind), C=rnd(seed + 4, rows, groups, states, dtype=kind), D=rnd(seed + 5, cols),
+             z=rnd(seed + 6, rows, cols, dtype=kind), dt_bias=(step + torch.log(-torch.expm1(-step))).to(DEV),
+             initial=rnd(seed + 7, seqs, cols, states))
+    return v
+
+
+def lasts(r, A, rows):
+    """frames a term of the recurrence lasts: until 2^-24 of it is left"""
+    weakest = float(r['delta'].abs().min() * A.detach().abs().min())
+    return min(rows, 17 / max(weakest, 1e-9))
+
+
+SCAN_SHAPES = [(4, 1, 1), (5, 3, 1), (16, 16, 1), (100, 16, 2), (130, 16, 1), (24, 21, 3), (12, 32, 1), (7, 64, 1), (10, 50, 2), (64, 8, 1), (33, 12, 1)]
+
+
+@pytest.mark.parametrize('lengths', LENGTHS)
+@pytest.mark.parametrize('cols,states,groups', SCAN_SHAPES)
+def test_scan_packed_with_states_and_a_tail(S, lengths, cols, states, groups):
+    kind = [F32, BF16, F16][(cols + len(lengths)) % 3]
+    n, live = len(lengths), sum(lengths)
+    rows = live + 5
+    v = scan_inputs(rows, cols, states, groups, kind, n)
+    for k in ('x', 'dt', 'z', 'B', 'C'):
+        v[k][live:] = float('nan')
+    dy, df = rnd(20, rows, cols, dtype=kind), rnd(21, n, cols, states)
+    dy[live:] = float('nan')
+    leaves = [t.requires_grad_(True) for t in v.values()]
+    y, final = S.selective_scan(v['x'], v['dt'], v['A'], v['B'], v['C'], D=v['D'], z=v['z'], dt_bias=v['dt_bias'], initial_state=v['initial'],
+                                seq_offsets=offsets_of(lengths), return_final_state=True)
+    clean = {k: t.detach().cpu().clone() for k, t in v.items()}
+    dyc = dy.cpu().clone()
+    for t in [clean[k] for k in ('x', 'dt', 'z', 'B', 'C')] + [dyc]:
+        t[live:] = 0
+    r = O.scan(**clean, lengths=lengths, dy=dyc, dfinal=df)
+    m = O.scan(**clean, lengths=lengths, dy=dyc, dfinal=df, absolute=True)
+    last = lasts(r, v['A'], max(lengths))
+    k = 3 * last + states + 40
+    close(y, r['y'], m['y'], k, 'y')
+    assert (y[live:] == 0).all()
+    close(final, r['final'], m['final'], k, 'final')
+    grads = torch.autograd.grad((y, final), leaves, (dy, df))
+    k = 6 * last + rows + cols + states + 60
+    for (name, _), got in zip(v.items(), grads):
+        close(got, r['d' + name], m['d' + name], k, 'd' + name)
+    for name, got in zip(v, grads):
+        if name in ('x', 'dt', 'z', 'B', 'C'):
+            assert (got[live:] == 0).all(), name
+
+
+@pytest.mark.parametrize('kind', [F32, BF16, F16])
+@pytest.mark.parametrize('softplus', [True, False])
+def test_scan_batch_without_extras(S, kind, softplus):
+    n, t, cols, states = 6, 37, 70, 16
+    v = scan_inputs(n * t, cols, states, 1, kind, n)
+    if not softplus:
+        v['dt'] = v['dt'].abs() * 0.3 + 0.05
+    dy = rnd(20, n, t, cols, dtype=kind)
+    use = {k: v[k].view(n, t, -1) if k in ('x', 'dt') else v[k].view(n, t, states) if k in 'BC' else v[k] for k in ('x', 'dt', 'A', 'B', 'C')}
+    leaves = [u.requires_grad_(True) for u in use.values()]
+    y = S.selective_scan(*use.values(), softplus=softplus)
+    plain = dict(x=v['x'], dt=v['dt'], A=v['A'], B=v['B'], C=v['C'], D=None, z=None, dt_bias=None, initial=None, lengths=[t] * n, softplus=softplus, dy=dy.view(-1, cols))
+    r, m = O.scan(**plain), O.scan(**plain, absolute=True)
+    last = lasts(r, v['A'], t)
+    close(y.view(-1, cols), r['y'], m['y'], 3 * last + 56, 'y')
+    for name, got in zip(use, torch.autograd.grad(y, leaves, dy)):
+        close(got.reshape(r['d' + name].shape), r['d' + name], m['d' + name], 6 * last + n * t + cols + 76, 'd' + name)
+
+
+@pytest.mark.parametrize('cols,states,kind', [(32, 16, F32), (20, 40, BF16)])
+@pytest.mark.parametrize('lengths,hint', [([1500], None), ([700, 3, 0, 800, 16], None), ([700, 3, 0, 800, 16], 800), ([31] * 40, 31), ([31] * 40, None)])
+def test_scan_long_and_many(S, cols, states, kind, lengths, hint):
+    """long axes that are split, and many short utterances; with the longest one told and not"""
+    n, rows = len(lengths), sum(lengths)
+    v = scan_inputs(rows, cols, states, 1, kind, n)
+    dy, df = rnd(20, rows, cols, dtype=kind), rnd(21, n, cols, states)
+    leaves = [t.requires_grad_(True) for t in v.values()]
+    y, final = S.selective_scan(v['x'], v['dt'], v['A'], v['B'], v['C'], D=v['D'], z=v['z'], dt_bias=v['dt_bias'], initial_state=v['initial'],
+                                seq_offsets=offsets_of(lengths), max_len=hint, return_final_state=True)
+    r = O.scan(**v, lengths=lengths, dy=dy, dfinal=df)
+    m = O.scan(**v, lengths=lengths, dy=dy, dfinal=df, absolute=True)
+    last = lasts(r, v['A'], max(lengths))
+    close(y, r['y'], m['y'], 3 * last + states + 40, 'y')
+    close(final, r['final'], m['final'], 3 * last + states + 40, 'final')
+    for (name, _), got in zip(v.items(), torch.autograd.grad((y, final), leaves, (dy, df))):
+        close(got, r['d' + name], m['d' + name], 6 * last + rows + cols + states + 60, 'd' + name)
+
+
+@pytest.mark.parametrize('kind', [F32, BF16])
+@pytest.mark.parametrize('cols,states,groups', [(6, 16, 1), (130, 16, 2), (9, 5, 3), (10, 64, 1)])
+def test_scan_steps_equal_the_prompt(S, kind, cols, states, groups):
+    n, t = 3, 11
+    v = scan_inputs(n * t, cols, states, groups, kind, n)
+    b = {k: v[k].view(n, t, *v[k].shape[1:]) for k in ('x', 'dt', 'z', 'B', 'C')}
+    y, final = S.selective_scan(b['x'], b['dt'], v['A'], b['B'], b['C'], D=v['D'], z=b['z'], dt_bias=v['dt_bias'], initial_state=v['initial'], return_final_state=True)
+    r = O.scan(**v, lengths=[t] * n)
+    m = O.scan(**v, lengths=[t] * n, absolute=True)
+    pool = rnd(30, 8, cols, states)
+    was = pool.clone()
+    slots = torch.tensor([5, 1, 7], dtype=torch.int32, device=DEV)
+    pool[slots.long()] = v['initial']
+    k = 3 * t + states + 40
+    for i in range(t):
+        yi = S.selective_scan_step(b['x'][:, i], b['dt'][:, i], v['A'], b['B'][:, i], b['C'][:, i], pool, D=v['D'], z=b['z'][:, i], dt_bias=v['dt_bias'], slots=slots)
+        close(yi, r['y'].view(n, t, cols)[:, i], m['y'].view(n, t, cols)[:, i], k, 'frame %d' % i)
+    close(pool[slots.long()], r['final'], m['final'], k, 'state')
+    close(final, r['final'], m['final'], k, 'final')
+    for i in (0, 2, 3, 4, 6):
+        assert torch.equal(pool[i], was[i])
+
+
+def test_steps_treat_strange_slots_as_padding(S):
+    cols, states = 40, 16
+    v = scan_inputs(6, cols, states, 1, F32, 1)
+    slots = torch.tensor([2, -1, 2, 9, 0, 2 ** 31 - 1], dtype=torch.int32, device=DEV)
+    pool = rnd(5, 4, cols, states)
+    alone = pool.clone()
+    args = [v[k] for k in ('x', 'dt', 'A')] + [v['B'][:, 0], v['C'][:, 0]]
+    y = S.selective_scan_step(*args, pool, D=v['D'], z=v['z'], dt_bias=v['dt_bias'], slots=slots)
+    keep = [0, 4]
+    rows = [a[keep] if a.shape[0] == 6 else a for a in (args[0], args[1])] + [args[2], args[3][keep], args[4][keep]]
+    y2 = S.selective_scan_step(*rows, alone, D=v['D'], z=v['z'][keep], dt_bias=v['dt_bias'], slots=slots[keep].contiguous())
+    assert torch.equal(y[keep], y2) and torch.equal(pool, alone)
+    assert (y[[1, 2, 3, 5]] == 0).all()
+    w, cpool = rnd(6, 4, cols), rnd(7, 4, 3, cols)
+    calone = cpool.clone()
+    y = S.causal_conv1d_step(v['x'], cpool, w, slots=slots)
+    y2 = S.causal_conv1d_step(v['x'][keep], calone, w, slots=slots[keep].contiguous())
+    assert torch.equal(y[keep], y2) and torch.equal(cpool, calone) and (y[[1, 2, 3, 5]] == 0).all()
+
+
+def test_a_non_number_stays_in_its_utterance(S):
+    lengths, cols = [20, 9, 33], 24
+    v = scan_inputs(62, cols, 16, 1, F32, 3)
+    w = rnd(9, 4, cols)
+    off = offsets_of(lengths)
+
+    def go():
+        leaves = [t.detach().clone().requires_grad_(True) for t in v.values()]
+        u = dict(zip(v, leaves))
+        c = S.causal_conv1d(u['x'], w, seq_offsets=off)
+        y = S.selective_scan(c, u['dt'], u['A'], u['B'], u['C'], D=u['D'], z=u['z'], dt_bias=u['dt_bias'], initial_state=u['initial'], seq_offsets=off)
+        g = torch.autograd.grad(y, [u[k] for k in ('x', 'dt', 'z', 'B', 'C', 'initial')], torch.ones_like(y))
+        return y, g
+    y0, g0 = go()
+    v['x'][22] = float('nan')
+    v['initial'][1, 3] = float('inf')
+    y1, g1 = go()
+    out = torch.cat([torch.arange(20), torch.arange(29, 62)]).to(DEV)
+    assert torch.isnan(y1[22:29]).any()
+    assert torch.equal(y0[out], y1[out])
+    for a, b in zip(g0[:5], g1[:5]):
+        assert torch.equal(a[out], b[out])
+    assert torch.equal(g0[5][[0, 2]], g1[5][[0, 2]])
+
+
+# ---------------------------------------------------------------------------------------------- how the calls may be made
+
+def layer(S, p, stream, off=None, states=None):
+    """a residual layer of the operators: norm -> product -> short convolution -> product -> scan (gated) -> product"""
+    cols, n = p['A'].shape
+    y, stream = S.rms_norm(p['x'] if stream is None else stream[0], p['gamma'], p['stream'] if stream is None else stream[1])
+    xz = y @ p['Win']
+    pack = dict(seq_offsets=off) if off is not None else {}
+    u = S.causal_conv1d(xz[..., :cols], p['w'], p['bias'], **pack)
+    s = u @ p['Wx']
+    v = S.selective_scan(u, s[..., 2 * n:] @ p['Wdt'], p['A'], s[..., :n], s[..., n:2 * n], D=p['D'], z=xz[..., cols:], dt_bias=p['dt_bias'], **pack)
+    return v @ p['Wout'], stream
+
+
+def layer_parameters(width=40, cols=72, n=16, rank=6):
+    v = scan_inputs(1, cols, n, 1, F32, 1)
+    return dict(gamma=1 + rnd(1, width, scale=0.1), Win=rnd(2, width, 2 * cols, scale=width ** -0.5), w=rnd(3, 4, cols, scale=0.5), bias=rnd(4, cols, scale=0.1),
+                Wx=rnd(5, cols, 2 * n + rank, scale=cols ** -0.5), Wdt=rnd(6, rank, cols, scale=0.3), A=v['A'], D=v['D'], dt_bias=v['dt_bias'],
+                Wout=rnd(7, cols, width, scale=cols ** -0.5))
+
+
+def plain_layer(p, x, stream, lengths):
+    """the same in 64 bits on the CPU, with torch's autograd"""
+    cols, n = p['A'].shape
+    t = x + stream
+    y = t / torch.sqrt(t.pow(2).mean(-1, keepdim=True) + 1e-6) * p['gamma']
+    xz = y @ p['Win']
+    outs, at = [], 0
+    for m in lengths:
+        axis = torch.cat([torch.zeros(3, cols, dtype=torch.float64), xz[at:at + m, :cols]])
+        c = sum(axis[j:j + m] * p['w'][j] for j in range(4)) + p['bias']
+        u = c * torch.sigmoid(c)
+        s = u @ p['Wx']
+        delta = torch.logaddexp(s[:, 2 * n:] @ p['Wdt'] + p['dt_bias'], torch.zeros((), dtype=torch.float64))
+        h, ys = torch.zeros(cols, n, dtype=torch.float64), []
+        for i in range(m):
+            h = torch.exp(delta[i][:, None] * p['A']) * h + (delta[i] * u[i])[:, None] * s[i, :n]
+            ys.append((h * s[i, n:2 * n]).sum(-1) + p['D'] * u[i])
+        z = xz[at:at + m, cols:]
+        outs.append(torch.stack(ys) * z * torch.sigmoid(z) if m else z)
+        at += m
+    return torch.cat(outs) @ p['Wout'], t
+
+
+def test_a_layer_of_them_trains_like_its_definition(S):
+    """norm, convolution and scan together, packed, with column slices of products as inputs: outputs and every gradient.  Tolerance: the three operators'
+    and four products' roundings follow one another; each passes on the relative error of what it is given with a factor that the magnitudes here keep
+    near one (norms of results and gradients are compared), so 200 roundings of 2^-24 a stage over 8 stages: 1e-4 of the largest element."""
+    lengths = [19, 0, 40, 1]
+    p = layer_parameters()
+    p.update(x=rnd(20, 60, 40), stream=rnd(21, 60, 40))
+    leaves = {k: t.requires_grad_(True) for k, t in p.items()}
+    out, stream = layer(S, p, None, offsets_of(lengths))
+    d1, d2 = rnd(22, 60, 40), rnd(23, 60, 40)
+    got = torch.autograd.grad((out, stream), list(leaves.values()), (d1, d2))
+    q = {k: t.detach().cpu().double().requires_grad_(True) for k, t in p.items()}
+    ref, rs = plain_layer(q, q['x'], q['stream'], lengths)
+    want = torch.autograd.grad((ref, rs), list(q.values()), (d1.cpu().double(), d2.cpu().double()))
+    assert (out.detach().cpu().double() - ref.detach()).abs().max() <= 1e-4 * ref.detach().abs().max()
+    for k, a, b in zip(leaves, got, want):
+        assert (a.cpu().double() - b).abs().max() <= 1e-4 * b.abs().max(), k
+
+
+def test_streaming_a_layer_frame_by_frame_equals_the_recording(S):
+    """the same layer on a live stream: single-frame calls with carried states against one call over all frames (same stages, same tolerance)"""
+    n, t, width = 2, 25, 40
+    p = layer_parameters()
+    cols, ns = p['A'].shape
+    p.update(x=rnd(20, n, t, width), stream=rnd(21, n, t, width))
+    out, _ = layer(S, p, None)
+    conv, state = torch.zeros(n, 3, cols, device=DEV), torch.zeros(n, cols, ns, device=DEV)
+    for i in range(t):
+        y, _ = S.rms_norm(p['x'][:, i], p['gamma'], p['stream'][:, i])
+        xz = y @ p['Win']
+        u = S.causal_conv1d_step(xz[:, :cols], conv, p['w'], p['bias'])
+        s = u @ p['Wx']
+        v = S.selective_scan_step(u, s[:, 2 * ns:] @ p['Wdt'], p['A'], s[:, :ns], s[:, ns:2 * ns], state, D=p['D'], z=xz[:, cols:], dt_bias=p['dt_bias'])
+        assert (v @ p['Wout'] - out[:, i]).abs().max() <= 1e-4 * out.abs().max(), i
+
+
+def test_strided_transposed_and_repeated_inputs(S):
+    """column slices, a time-contiguous tensor seen as frames, and one row for all: the same numbers as contiguous copies"""
+    rows, cols = 50, 36
+    wide = rnd(1, rows, 3 * cols + 5)
+    x, dt, z = wide[:, 1:cols + 1], wide[:, cols + 2:2 * cols + 2], wide[:, 2 * cols + 4:3 * cols + 4]
+    v = scan_inputs(rows, cols, 16, 1, F32, 1)
+    bc = rnd(2, rows, 40)
+    B, Cm = bc[:, 3:19], bc[:, 20:36]
+    off = offsets_of([20, 30])
+    a = S.selective_scan(x, dt, v['A'], B, Cm, D=v['D'], z=z, dt_bias=v['dt_bias'], seq_offsets=off)
+    b = S.selective_scan(x.contiguous(), dt.contiguous(), v['A'], B.contiguous(), Cm.contiguous(), D=v['D'], z=z.contiguous(), dt_bias=v['dt_bias'], seq_offsets=off)
+    assert torch.equal(a, b)
+    w = rnd(3, 4, cols)
+    assert torch.equal(S.causal_conv1d(x, w, seq_offsets=off), S.causal_conv1d(x.contiguous(), w, seq_offsets=off))
+    frames = rnd(4, 2, cols, 25).transpose(1, 2)                  # [batch, frames, channels] of a [batch, channels, frames] tensor
+    assert torch.equal(S.causal_conv1d(frames, w), S.causal_conv1d(frames.contiguous(), w))
+    gamma = torch.ones(cols, device=DEV)
+    assert torch.equal(S.rms_norm(frames, gamma), S.rms_norm(frames.contiguous(), gamma))
+    one = rnd(5, 1, cols).expand(rows, cols)
+    assert torch.equal(S.rms_norm(one, gamma, x)[0], S.rms_norm(one.contiguous(), gamma, x)[0])
+    leaf = rnd(6, 1, cols).requires_grad_(True)                   # gradient of a row that all rows share
+    (g,) = torch.autograd.grad(S.causal_conv1d(leaf.expand(rows, cols), w, seq_offsets=off).sum(), leaf)
+    many = leaf.detach().repeat(rows, 1).requires_grad_(True)
+    (h,) = torch.autograd.grad(S.causal_conv1d(many, w, seq_offsets=off).sum(), many)
+    assert torch.allclose(g, h.sum(0, keepdim=True), rtol=1e-5, atol=1e-5)
+
+
+def test_two_runs_are_bitwise_equal(S):
+    lengths = [300, 45, 200]
+    v = scan_inputs(545, 150, 16, 1, BF16, 3)
+    dy = rnd(20, 545, 150, dtype=BF16)
+
+    def go():
+        u = {k: t.detach().clone().requires_grad_(True) for k, t in v.items()}
+        w = rnd(9, 4, 150).requires_grad_(True)
+        gamma = torch.ones(150, device=DEV, requires_grad=True)
+        c = S.causal_conv1d(S.rms_norm(u['x'], gamma), w, seq_offsets=offsets_of(lengths))
+        y = S.selective_scan(c, u['dt'], u['A'], u['B'], u['C'], D=u['D'], z=u['z'], dt_bias=u['dt_bias'], initial_state=u['initial'], seq_offsets=offsets_of(lengths))
+        return torch.autograd.grad(y, list(u.values()) + [w, gamma], dy)
+    for a, b in zip(go(), go()):
+        assert torch.equal(a, b)
+
+
+def test_empty_calls(S):
+    w, A = rnd(1, 4, 8), -torch.ones(8, 4, device=DEV)
+    none = torch.empty(2, 0, 8, device=DEV)
+    bc = torch.empty(2, 0, 4, device=DEV)
+    init, h0 = rnd(2, 2, 3, 8), rnd(3, 2, 8, 4)
+    y, f = S.causal_conv1d(none, w, initial_state=init, return_final_state=True)
+    assert y.shape == none.shape and torch.equal(f, init)
+    y, f = S.selective_scan(none, none, A, bc, bc, initial_state=h0, return_final_state=True)
+    assert y.shape == none.shape and torch.equal(f, h0)
+    assert S.rms_norm(none, torch.ones(8, device=DEV)).shape == none.shape
+    assert S.rms_norm_e4m3(none, torch.ones(8, device=DEV))[1].shape == (2, 0, 1)
+    row = torch.empty(0, 8, device=DEV)
+    assert S.causal_conv1d_step(row, init, w).shape == (0, 8)
+    assert S.selective_scan_step(row, row, A, row[:, :4], row[:, :4], h0).shape == (0, 8)
+    leaves = [t.detach().clone().requires_grad_(True) for t in (none, w, A, init, h0)]
+    y, f = S.selective_scan(S.causal_conv1d(leaves[0], leaves[1], initial_state=leaves[3]), leaves[0], leaves[2], bc, bc, initial_state=leaves[4], return_final_state=True)
+    g = torch.autograd.grad((y, f), leaves, (y.detach(), torch.ones_like(f)))
+    assert g[0].shape == none.shape and (g[1] == 0).all() and (g[2] == 0).all() and (g[3] == 0).all() and (g[4] == 1).all()
+    x, gamma = none.clone().requires_grad_(True), torch.ones(8, device=DEV, requires_grad=True)
+    assert (torch.autograd.grad(S.rms_norm(x, gamma).sum(), gamma)[0] == 0).all()
+
+
+def test_refusals(S):
+    x, w = rnd(1, 2, 5, 8), rnd(2, 4, 8)
+    A, bc = -torch.ones(8, 4, device=DEV), rnd(3, 2, 5, 4)
+    ok = dict(A=A, B=bc, C=bc)
+
+    def no(f, *a, **k):
+        with pytest.raises((ValueError, RuntimeError)):
+            f(*a, **k)
+    no(S.rms_norm, x.double(), torch.ones(8, device=DEV))
+    no(S.rms_norm, x, torch.ones(7, device=DEV))
+    no(S.rms_norm, x, torch.ones(8, device=DEV, dtype=BF16))
+    no(S.rms_norm, x, torch.ones(8))
+    no(S.rms_norm, x, torch.ones(8, device=DEV), x[:1])
+    no(S.rms_norm, x, torch.ones(8, device=DEV), x.bfloat16())
+    no(S.rms_norm, x, torch.ones(8, device=DEV), eps=0.0)
+    no(S.rms_norm_e4m3, x, torch.ones(8, device=DEV), group=32)
+    no(S.rms_norm_e4m3, x, torch.ones(8, device=DEV, requires_grad=True))
+    no(S.causal_conv1d, x[0], w)                                  # rows without seq_offsets
+    no(S.causal_conv1d, x, w[:1])
+    no(S.causal_conv1d, x, rnd(4, 9, 8))
+    no(S.causal_conv1d, x, w.bfloat16())
+    no(S.causal_conv1d, x, w, initial_state=rnd(5, 2, 4, 8))
+    no(S.causal_conv1d, x, w, seq_offsets=torch.tensor([0, 5], dtype=torch.int32, device=DEV))
+    no(S.causal_conv1d, x[0], w, seq_offsets=torch.tensor([0, 5], device=DEV))
+    no(S.causal_conv1d, x[0], w, seq_offsets=torch.tensor([0, 5], dtype=torch.int32))
+    no(S.causal_conv1d, x[0], w, seq_offsets=torch.tensor([5], dtype=torch.int32, device=DEV))
+    no(S.causal_conv1d_step, x[:, 0], rnd(6, 1, 3, 8), w)         # two streams, one state
+    no(S.causal_conv1d_step, x[:, 0], rnd(6, 4, 3, 16)[..., ::2], w)
+    no(S.causal_conv1d_step, x[:, 0].clone().requires_grad_(True), rnd(6, 4, 3, 8), w)
+    no(S.causal_conv1d_step, x[:, 0], rnd(6, 4, 3, 8), w, slots=torch.tensor([0, 1], device=DEV))
+    no(S.selective_scan, x, x[:, :4], **ok)
+    no(S.selective_scan, x, x.bfloat16(), **ok)
+    no(S.selective_scan, x, x, A[:7], bc, bc)
+    no(S.selective_scan, x, x, A, bc[..., :3], bc)
+    no(S.selective_scan, x, x, A, rnd(7, 2, 5, 3, 4), rnd(8, 2, 5, 3, 4))                # three groups, eight channels
+    no(S.selective_scan, x, x, A, rnd(7, 2, 5, 2, 4), bc)
+    no(S.selective_scan, x, x, -torch.ones(8, 65, device=DEV), rnd(7, 2, 5, 65), rnd(8, 2, 5, 65))
+    no(S.selective_scan, x, x, z=x[..., :4], **ok)
+    no(S.selective_scan, x, x, D=torch.ones(8, device=DEV, dtype=F16), **ok)
+    no(S.selective_scan, x, x, initial_state=rnd(9, 2, 8, 5), **ok)
+    no(S.selective_scan, x, x, initial_state=rnd(9, 2, 8, 4, dtype=BF16), **ok)
+    no(S.selective_scan, x, x, max_len=-1, **ok)
+    no(S.selective_scan_step, x[:, 0], x[:, 0], A, bc[:, 0], bc[:, 0], rnd(9, 1, 8, 4))
+    no(S.selective_scan_step, x[:, 0], x[:, 0], A, bc[:, 0], bc[:, 0], rnd(9, 2, 8, 4).half())
+    no(S.selective_scan_step, x[:, 0], x[:, 0], A.clone().requires_grad_(True), bc[:, 0], bc[:, 0], rnd(9, 2, 8, 4))
+
+
+def test_another_stream(S):
+    v = scan_inputs(400, 64, 16, 1, F32, 1)
+    call = lambda: S.selective_scan(v['x'][None], v['dt'][None], v['A'], v['B'][None], v['C'][None], D=v['D'], z=v['z'][None], dt_bias=v['dt_bias'])  # noqa: E731
+    want = call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = call()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+def test_captured_calls_replay(S):
+    """two graphs of training passes and one of single frames, replayed in turn with eager work between, against eager results every time"""
+    lengths = [130, 1, 60]
+    off = offsets_of(lengths)
+    v = scan_inputs(191, 80, 16, 1, F32, 3)
+    w, gamma = rnd(9, 4, 80), 1 + rnd(10, 80, scale=0.1)
+    dy = rnd(20, 191, 80)
+
+    def train(u, w, gamma):
+        y, s = S.rms_norm(u['x'], gamma, u['z'])
+        c = S.causal_conv1d(y, w, seq_offsets=off)
+        o, f = S.selective_scan(c, u['dt'], u['A'], u['B'], u['C'], D=u['D'], z=u['z'], dt_bias=u['dt_bias'], initial_state=u['initial'], seq_offsets=off, return_final_state=True)
+        return [o, f] + list(torch.autograd.grad((o, f, s), list(u.values()) + [w, gamma], (dy, torch.ones_like(f), dy)))
+
+    def leaves():
+        return {k: t.detach().clone().requires_grad_(True) for k, t in v.items()}, w.clone().requires_grad_(True), gamma.clone().requires_grad_(True)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        train(*leaves())
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    sets, graphs, outs = [], [], []
+    for _ in range(2):
+        held = leaves()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = train(*held)
+        sets.append(held); graphs.append(g); outs.append(out)
+    pool, x1 = rnd(30, 5, 80, 16), rnd(31, 5, 80)
+    start = pool.clone()
+    gs = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gs):
+        ys = S.selective_scan_step(x1, v['dt'][:5], v['A'], v['B'][:5], v['C'][:5], pool, D=v['D'], z=v['z'][:5], dt_bias=v['dt_bias'])
+    eager_pool = start.clone()
+    pool.copy_(start)
+    for turn in range(4):
+        for i in (0, 1):
+            u = sets[i][0]
+            with torch.no_grad():
+                u['x'].copy_(rnd(100 + 10 * turn + i, 191, 80))
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            fresh = {k: t.detach().clone().requires_grad_(True) for k, t in u.items()}
+            want = train(fresh, sets[i][1].detach().clone().requires_grad_(True), sets[i][2].detach().clone().requires_grad_(True))
+            for a, b in zip(outs[i], want):
+                assert torch.equal(a, b), (turn, i)
+        gs.replay()
+        torch.cuda.synchronize()
+        ye = S.selective_scan_step(x1, v['dt'][:5], v['A'], v['B'][:5], v['C'][:5], eager_pool, D=v['D'], z=v['z'][:5], dt_bias=v['dt_bias'])
+        assert torch.equal(ys, ye) and torch.equal(pool, eager_pool), turn
+
+
+def test_wrong_offsets_stay_inside_the_tensors(S):
+    """offsets that fall, or reach outside: clamped on the device; what they give is not specified, that the guards around the outputs stay is"""
+    v = scan_inputs(64, 40, 16, 1, F32, 3)
+    from voice_converter_cyclegan_amd import _lib
+    import ctypes as C
+    for bad in ([0, 40, 20, 64], [-7, 10, 20, 1000], [50, 40, 30, 20], [0, 0, 0, 0], [2 ** 31 - 1, -2 ** 31, 5, 2 ** 31 - 1]):
+        off = torch.tensor(bad, dtype=torch.int32, device=DEV)
+        guard = torch.full((64 + 32, 40), 7.0, device=DEV)
+        y = guard[16:80]
+        final = torch.zeros(3, 40, 16, device=DEV)
+        a = _lib.ScanArgs(x=v['x'].data_ptr(), dt=v['dt'].data_ptr(), B=v['B'].data_ptr(), C=v['C'].data_ptr(), A=v['A'].data_ptr(), offsets=off.data_ptr(), y=y.data_ptr(),
+                          final_state=final.data_ptr(), x_ld=40, dt_ld=40, b_ld=16, c_ld=16, y_ld=40, rows=64, cols=40, states=16, groups=1, n_seqs=3, type=0, softplus=1)
+        a.work_floats = _lib.lib.vc_selective_scan_fwd_work(C.byref(a))
+        work = torch.empty(max(1, a.work_floats), device=DEV)
+        a.work = work.data_ptr()
+        _lib.check(_lib.lib.vc_selective_scan_fwd(C.byref(a), torch.cuda.current_stream().cuda_stream))
+        w = rnd(3, 4, 40)
+        cy = torch.full((64 + 32, 40), 7.0, device=DEV)
+        cf = torch.zeros(3, 3, 40, device=DEV)
+        ca = _lib.Conv1dArgs(x=v['x'].data_ptr(), w=w.data_ptr(), offsets=off.data_ptr(), y=cy[16:80].data_ptr(), final_state=cf.data_ptr(), x_ld=40, y_ld=40, rows=64, cols=40,
+                             taps=4, n_seqs=3, type=0, silu=1)
+        _lib.check(_lib.lib.vc_causal_conv1d_fwd(C.byref(ca), torch.cuda.current_stream().cuda_stream))
+        torch.cuda.synchronize()
+        for g in (guard, cy):
+            assert (g[:16] == 7).all() and (g[80:] == 7).all()
+
+
+def test_rows_behind_the_last_utterance_are_left_without_zero_tail(S):
+    from voice_converter_cyclegan_amd import _lib
+    import ctypes as C
+    v = scan_inputs(40, 24, 16, 1, F32, 2)
+    off = offsets_of([10, 21])
+    y = torch.full((40, 24), 7.0, device=DEV)
+    a = _lib.ScanArgs(x=v['x'].data_ptr(), dt=v['dt'].data_ptr(), B=v['B'].data_ptr(), C=v['C'].data_ptr(), A=v['A'].data_ptr(), offsets=off.data_ptr(), y=y.data_ptr(),
+                      x_ld=24, dt_ld=24, b_ld=16, c_ld=16, y_ld=24, rows=40, cols=24, states=16, groups=1, n_seqs=2, type=0, softplus=1)
+    a.work_floats = _lib.lib.vc_selective_scan_fwd_work(C.byref(a))
+    work = torch.empty(max(1, a.work_floats), device=DEV)
+    a.work = work.data_ptr()
+    _lib.check(_lib.lib.vc_selective_scan_fwd(C.byref(a), torch.cuda.current_stream().cuda_stream))
+    assert (y[31:] == 7).all() and (y[:31] != 7).all()
+    w = rnd(3, 4, 24)
+    y.fill_(7)
+    ca = _lib.Conv1dArgs(x=v['x'].data_ptr(), w=w.data_ptr(), offsets=off.data_ptr(), y=y.data_ptr(), x_ld=24, y_ld=24, rows=40, cols=24, taps=4, n_seqs=2, type=0, silu=1)
+    _lib.check(_lib.lib.vc_causal_conv1d_fwd(C.byref(ca), torch.cuda.current_stream().cuda_stream))
+    assert (y[31:] == 7).all() and (y[:31] != 7).all()

@@ -50,6 +50,23 @@ class ParamRec(C.Structure):
                 ('shape', C.c_int32 * 4), ('ld', C.c_int32)]
 
 
+def _fields(*groups):
+    return [(n, t) for t, names in groups for n in names.split()]
+
+
+class Conv1dArgs(C.Structure):
+    """vc_conv1d_args"""
+    _fields_ = _fields((vp, 'x w bias initial offsets y final_state'), (i64, 'x_ld y_ld rows'), (C.c_int32, 'cols taps n_seqs type silu zero_tail'),
+                       (vp, 'dy dfinal dx dinitial dw dbias'), (i64, 'dy_ld dx_ld'), (vp, 'work'), (i64, 'work_floats'))
+
+
+class ScanArgs(C.Structure):
+    """vc_scan_args"""
+    _fields_ = _fields((vp, 'x dt z B C A D dt_bias initial offsets y final_state'), (i64, 'x_ld dt_ld z_ld b_ld c_ld y_ld rows'),
+                       (C.c_int32, 'cols states groups n_seqs type softplus zero_tail max_len'), (vp, 'saved'), (i64, 'saved_floats'),
+                       (vp, 'dy dfinal dx ddt dz dB dC dA dD ddt_bias dinitial'), (i64, 'dy_ld dx_ld ddt_ld dz_ld db_ld dc_ld'), (vp, 'work'), (i64, 'work_floats'))
+
+
 # (name, restype, argtypes) -- every symbol declared in include/vc_cyclegan.h
 SIGNATURES = [
     ('vc_version', i32, []),
@@ -106,6 +123,21 @@ SIGNATURES = [
     ('vc_l1_loss', i32, [vp, vp, i64, vp, vp, vp]),
     ('vc_l2_loss', i32, [vp, vp, i64, vp, vp, vp]),
     ('vc_adam_tf_update', i32, [vp, vp, vp, vp, i64, f32, f32, f32, f32, f32, vp]),
+    ('vc_seq_version', i32, []),
+    ('vc_rms_norm_fwd', i32, [vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, f32, i64, i32, i32, i32, vp]),
+    ('vc_rms_norm_e4m3', i32, [vp, i64, vp, i64, vp, vp, i64, vp, vp, i64, f32, i64, i32, i32, i32, i32, vp]),
+    ('vc_rms_norm_bwd_work', i64, [i64, i32]),
+    ('vc_rms_norm_bwd', i32, [vp, i64, vp, i64, vp, i64, vp, vp, vp, i64, vp, i64, vp, vp, i64, i64, i32, i32, i32, vp]),
+    ('vc_causal_conv1d_fwd', i32, [C.POINTER(Conv1dArgs), vp]),
+    ('vc_causal_conv1d_bwd_work', i64, [C.POINTER(Conv1dArgs)]),
+    ('vc_causal_conv1d_bwd', i32, [C.POINTER(Conv1dArgs), vp]),
+    ('vc_causal_conv1d_step', i32, [vp, i64, vp, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, i32, vp]),
+    ('vc_selective_scan_saved', i64, [C.POINTER(ScanArgs)]),
+    ('vc_selective_scan_fwd_work', i64, [C.POINTER(ScanArgs)]),
+    ('vc_selective_scan_bwd_work', i64, [C.POINTER(ScanArgs)]),
+    ('vc_selective_scan_fwd', i32, [C.POINTER(ScanArgs), vp]),
+    ('vc_selective_scan_bwd', i32, [C.POINTER(ScanArgs), vp]),
+    ('vc_selective_scan_step', i32, [vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, i64] + [i32] * 7 + [vp]),
     ('vc_plan_create', i32, [i32, i32, C.POINTER(vp)]),
     ('vc_plan_create_inference', i32, [i32, i32, C.POINTER(vp)]),
     ('vc_plan_destroy', None, [vp]),

@@ -1,0 +1,47 @@
+// vc_seq.h -- what the translation units of the sequence operators share (vc_seq_norm.hip, vc_seq_conv.hip, vc_seq_scan.hip, vc_seq_scan_bwd.hip):
+// element types, utterance offsets, lane exchanges.
+#pragma once
+#include "vc_host.h"
+#include "vc_device_util.h"
+#include <type_traits>
+
+// VC_ARG inside a function that returns the status itself
+#define SEQ_TYPES(type, F, ...) ((type) == VC_F32 ? F<float>(__VA_ARGS__) : (type) == VC_BF16 ? F<__bf16>(__VA_ARGS__) : F<_Float16>(__VA_ARGS__))
+static inline int seq_esize(int type) { return type == VC_F32 ? 4 : 2; }
+static inline bool seq_type_ok(int type) { return type == VC_F32 || type == VC_BF16 || type == VC_F16; }
+
+// V elements in one access at any address the element type itself allows: gfx950 takes 16-byte global accesses at any alignment, so odd
+// channel counts and row strides need no second path
+template <class T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[V]; };
+template <class T, int V> __device__ __forceinline__ void load_vec(const T* p, float (&f)[V]) {
+    const Pack<T, V> q = *(const Pack<T, V>*)p;
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = (float)q.v[i];
+}
+template <class T, int V> __device__ __forceinline__ void store_vec(T* p, const float (&f)[V]) {
+    Pack<T, V> q;
+#pragma unroll
+    for (int i = 0; i < V; ++i) q.v[i] = (T)f[i];
+    *(Pack<T, V>*)p = q;
+}
+// the first n of V elements (the rest reads as zero)
+template <class T, int V> __device__ __forceinline__ void load_some(const T* p, float (&f)[V], int n) {
+    if (n >= V) { load_vec<T, V>(p, f); return; }
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = i < n ? (float)p[i] : 0.f;
+}
+template <class T, int V> __device__ __forceinline__ void store_some(T* p, const float (&f)[V], int n) {
+    if (n >= V) { store_vec<T, V>(p, f); return; }
+#pragma unroll
+    for (int i = 0; i < V; ++i) if (i < n) p[i] = (T)f[i];
+}
+
+// The utterances of one call.  begin / end clamp into [0, rows], whatever the device array holds.
+struct SeqMap { const int* off; int rows, n_seqs, len; };
+__device__ __forceinline__ int seq_begin(const SeqMap& m, int s) { return m.off ? min(max(m.off[s], 0), m.rows) : s * m.len; }
+__device__ __forceinline__ int seq_end(const SeqMap& m, int s, int begin) { return m.off ? max(seq_begin(m, s + 1), begin) : begin + m.len; }
+// rows behind the last utterance start here
+__device__ __forceinline__ int seq_tail(const SeqMap& m) { return m.off ? seq_begin(m, m.n_seqs) : m.rows; }
+
+// x * sigmoid(x) and its derivative's factor, sigmoid through one exponential: 1 / (1 + e^-x) (e^-x overflows to infinity, the reciprocal to 0)
+__device__ __forceinline__ float sigmoid_acc(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
