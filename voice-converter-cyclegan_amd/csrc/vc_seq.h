@@ -3,6 +3,7 @@
 #pragma once
 #include "vc_host.h"
 #include "vc_device_util.h"
+#include <algorithm>
 #include <type_traits>
 
 // VC_ARG inside a function that returns the status itself
@@ -45,3 +46,15 @@ __device__ __forceinline__ int seq_tail(const SeqMap& m) { return m.off ? seq_be
 
 // x * sigmoid(x) and its derivative's factor, sigmoid through one exponential: 1 / (1 + e^-x) (e^-x overflows to infinity, the reciprocal to 0)
 __device__ __forceinline__ float sigmoid_acc(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+
+// The slot row r works on, -1 where it is padding: outside the pool, or named by an earlier row of this call.  Every thread of the block calls it.
+__device__ __forceinline__ int claim_slot(const int* slots, int r, int n_slots) {
+    const int mine = slots ? slots[r] : r;
+    int taken = mine < 0 || mine >= n_slots;
+    if (slots)
+        for (int i = threadIdx.x; i < r; i += blockDim.x) taken |= slots[i] == mine;
+    return __syncthreads_or(taken) ? -1 : mine;
+}
+
+// dst[i] = sum over `parts` rows of part[parts][n], in order; columns [0, n0) go to dst0, the others to dst1 (either may be null).  vc_seq_norm.hip
+int seq_sum_parts(const float* part, int parts, int64_t n, float* dst0, int64_t n0, float* dst1, hipStream_t s);

@@ -1,10 +1,13 @@
 // vc_seq_conv.hip -- short causal convolution along the rows, one filter per channel: prompts, gradient, single frames.
 //   p[t] = bias + sum_k w[k] x[t - (K-1) + k];  y = p sigmoid(p) or p
+//   g = dy * (p sigmoid(p))';  dx[u] = sum_k w[k] g[u + (K-1) - k];  dw[k] = sum_t g[t] x[t - (K-1) + k];  dbias = sum_t g[t]
+// Bound by HBM.  A thread walks a run of rows for one 16-byte vector of channels with the last K frames in registers, so a row is fetched once,
+// apart from the K - 1 frames ahead of a run.
 #include "vc_seq.h"
 
-struct ConvArgs { vc_conv1d_args a; SeqMap m; };
+struct ConvArgs { vc_conv1d_args a; SeqMap m; int cv, cvb, runs; float* part; };
 
-// the utterance row r lies in: the last s with begin(s) <= r whose rows are not none; n_seqs where r lies behind the last utterance
+// the utterance row r lies in: the last s with begin(s) <= r; n_seqs where r lies behind the last utterance
 __device__ __forceinline__ int seq_of(const SeqMap& m, int r) {
     if (!m.off) return r / m.len;
     if (r >= seq_tail(m)) return m.n_seqs;
@@ -12,96 +15,252 @@ __device__ __forceinline__ int seq_of(const SeqMap& m, int r) {
     while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (seq_begin(m, mid) <= r) lo = mid; else hi = mid - 1; }
     return lo;
 }
-// frame t (counted from the utterance's first row b) of channel c: the utterance's own, or an earlier one from the initial state
-template <class T> __device__ __forceinline__ float frame(const vc_conv1d_args& a, int s, int b, int t, int c) {
-    if (t >= 0) return (float)((const T*)a.x)[(int64_t)(b + t) * a.x_ld + c];
-    return a.initial ? (float)((const T*)a.initial)[((int64_t)s * (a.taps - 1) + (a.taps - 1 + t)) * a.cols + c] : 0.f;
+// n channels of frame t (counted from the utterance's first row b): the utterance's own, or an earlier one from the initial state
+template <class T, int V> __device__ __forceinline__ void frame(const vc_conv1d_args& a, int s, int b, int t, int c, int n, float (&f)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = 0.f;
+    if (t >= 0) load_some<T, V>((const T*)a.x + (int64_t)(b + t) * a.x_ld + c, f, n);
+    else if (a.initial) load_some<T, V>((const T*)a.initial + ((int64_t)s * (a.taps - 1) + (a.taps - 1 + t)) * a.cols + c, f, n);
 }
-template <class T> __device__ __forceinline__ float pre(const vc_conv1d_args& a, int s, int b, int t, int c) {
-    float p = a.bias ? a.bias[c] : 0.f;
-    for (int k = 0; k < a.taps; ++k) p += a.w[k * a.cols + c] * frame<T>(a, s, b, t - (a.taps - 1) + k, c);
+template <class T, int K, int V> struct Filter {
+    float w[K][V], b[V];
+    __device__ __forceinline__ Filter(const vc_conv1d_args& a, int c, int n) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) b[e] = 0.f;
+        if (a.bias) load_some<float, V>(a.bias + c, b, n);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) w[k][e] = 0.f;
+            load_some<float, V>(a.w + (int64_t)k * a.cols + c, w[k], n);
+        }
+    }
+};
+// A block's threads: cvb vectors of channels (a power of two) next to each other, 256 / cvb runs of rows
+constexpr int FWD_RUN = 16, BWD_RUN = 16, AHEAD = 4;             // rows of a run; rows whose loads are issued together
+struct Place { int c, n, run; bool ok; };
+__device__ __forceinline__ Place place(const ConvArgs& k, int V) {
+    const int blocks = (k.cv + k.cvb - 1) / k.cvb;
+    Place p;
+    const int v = (int)(blockIdx.x % blocks) * k.cvb + threadIdx.x % k.cvb;
+    p.run = (int)(blockIdx.x / blocks) * (256 / k.cvb) + threadIdx.x / k.cvb;
+    p.c = v * V; p.n = k.a.cols - p.c; p.ok = v < k.cv;
     return p;
 }
-// gradient of the pre-activation of frame t
-template <class T> __device__ __forceinline__ float dpre(const vc_conv1d_args& a, int s, int b, int t, int c) {
-    const float g = (float)((const T*)a.dy)[(int64_t)(b + t) * a.dy_ld + c];
-    if (!a.silu) return g;
-    const float p = pre<T>(a, s, b, t, c), sg = sigmoid_acc(p);
-    return g * sg * (1.f + p * (1.f - sg));
-}
-template <class T> __global__ __launch_bounds__(256) void conv1d_fwd_kernel(const ConvArgs k) {
+
+template <class T, int K> __global__ __launch_bounds__(256) void conv1d_fwd_kernel(const ConvArgs k) {
+    constexpr int V = 16 / (int)sizeof(T);
     const vc_conv1d_args& a = k.a;
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= a.cols) return;
-    for (int r = blockIdx.y; r < a.rows; r += gridDim.y) {
-        const int s = seq_of(k.m, r);
-        if (s == k.m.n_seqs) { if (a.zero_tail) ((T*)a.y)[(int64_t)r * a.y_ld + c] = (T)0.f; continue; }
-        const int b = seq_begin(k.m, s);
-        const float p = pre<T>(a, s, b, r - b, c);
-        ((T*)a.y)[(int64_t)r * a.y_ld + c] = (T)(a.silu ? p * sigmoid_acc(p) : p);
-    }
-    if (a.final_state)
-        for (int s = blockIdx.y; s < k.m.n_seqs; s += gridDim.y) {
-            const int b = seq_begin(k.m, s), e = seq_end(k.m, s, b);
-            for (int i = 0; i < a.taps - 1; ++i)
-                ((T*)a.final_state)[((int64_t)s * (a.taps - 1) + i) * a.cols + c] = (T)frame<T>(a, s, b, e - b - (a.taps - 1) + i, c);
-        }
-}
-// gradient of frame t of the utterance (t < 0: of the initial state's)
-template <class T> __device__ __forceinline__ float dframe(const vc_conv1d_args& a, int s, int b, int n, int t, int c) {
-    float d = 0.f;
-    for (int k = 0; k < a.taps; ++k) { const int o = t + (a.taps - 1) - k; if (o >= 0 && o < n) d += a.w[k * a.cols + c] * dpre<T>(a, s, b, o, c); }
-    if (a.dfinal && t >= n - (a.taps - 1)) d += (float)((const T*)a.dfinal)[((int64_t)s * (a.taps - 1) + t - (n - (a.taps - 1))) * a.cols + c];
-    return d;
-}
-template <class T> __global__ __launch_bounds__(256) void conv1d_bwd_kernel(const ConvArgs k) {
-    const vc_conv1d_args& a = k.a;
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= a.cols) return;
-    if (a.dx)
-        for (int r = blockIdx.y; r < a.rows; r += gridDim.y) {
-            const int s = seq_of(k.m, r);
-            if (s == k.m.n_seqs) { if (a.zero_tail) ((T*)a.dx)[(int64_t)r * a.dx_ld + c] = (T)0.f; continue; }
-            const int b = seq_begin(k.m, s), e = seq_end(k.m, s, b);
-            ((T*)a.dx)[(int64_t)r * a.dx_ld + c] = (T)dframe<T>(a, s, b, e - b, r - b, c);
-        }
-    if (a.dinitial)
-        for (int s = blockIdx.y; s < k.m.n_seqs; s += gridDim.y) {
-            const int b = seq_begin(k.m, s), e = seq_end(k.m, s, b);
-            for (int i = 0; i < a.taps - 1; ++i)
-                ((T*)a.dinitial)[((int64_t)s * (a.taps - 1) + i) * a.cols + c] = (T)dframe<T>(a, s, b, e - b, i - (a.taps - 1), c);
-        }
-}
-template <class T> __global__ __launch_bounds__(64) void conv1d_dw_kernel(const ConvArgs k) {
-    const vc_conv1d_args& a = k.a;
-    const int c = blockIdx.x * 64 + threadIdx.x;
-    if (c >= a.cols) return;
-    float dw[8] = {}, db = 0.f;
-    for (int s = 0; s < k.m.n_seqs; ++s) {
-        const int b = seq_begin(k.m, s), n = seq_end(k.m, s, b) - b;
-        for (int t = 0; t < n; ++t) {
-            const float g = dpre<T>(a, s, b, t, c);
-            db += g;
+    const Place p = place(k, V);
+    if (!p.ok) return;
+    if (p.run >= k.runs) {                                       // behind the runs: one utterance's last K - 1 frames
+        const int s = p.run - k.runs;
+        if (!a.final_state || s >= k.m.n_seqs) return;
+        const int b = seq_begin(k.m, s), e = seq_end(k.m, s, b);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) if (j < a.taps) dw[j] += g * frame<T>(a, s, b, t - (a.taps - 1) + j, c);
+        for (int i = 0; i < K - 1; ++i) {
+            float f[V];
+            frame<T, V>(a, s, b, e - b - (K - 1) + i, p.c, p.n, f);
+            store_some<T, V>((T*)a.final_state + ((int64_t)s * (K - 1) + i) * a.cols + p.c, f, p.n);
+        }
+        return;
+    }
+    const Filter<T, K, V> w(a, p.c, p.n);
+    int r = p.run * FWD_RUN;
+    const int r1 = min(r + FWD_RUN, k.m.rows);
+    const T* x = (const T*)a.x + p.c;
+    T* y = (T*)a.y + p.c;
+    for (int s = seq_of(k.m, r); r < r1; ++s) {
+        if (s >= k.m.n_seqs) {                                   // rows behind the last utterance
+            float f[V] = {};
+            if (a.zero_tail) for (; r < r1; ++r) store_some<T, V>(y + (int64_t)r * a.y_ld, f, p.n);
+            return;
+        }
+        const int b = seq_begin(k.m, s), hi = min(seq_end(k.m, s, b), r1);
+        if (r >= hi) continue;                                   // an empty utterance
+        float win[K][V];
+#pragma unroll
+        for (int i = 0; i < K - 1; ++i) frame<T, V>(a, s, b, r - b - (K - 1) + i, p.c, p.n, win[i]);
+        auto step = [&](const float (&f)[V]) {
+            float o[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                win[K - 1][e] = f[e];
+                float q = w.b[e];
+#pragma unroll
+                for (int i = 0; i < K; ++i) q = fmaf(w.w[i][e], win[i][e], q);
+                o[e] = a.silu ? q * sigmoid_acc(q) : q;
+#pragma unroll
+                for (int i = 0; i < K - 1; ++i) win[i][e] = win[i + 1][e];
+            }
+            store_some<T, V>(y + (int64_t)r * a.y_ld, o, p.n);
+            ++r;
+        };
+        while (r + AHEAD <= hi) {
+            float f[AHEAD][V] = {};
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) load_some<T, V>(x + (int64_t)(r + i) * a.x_ld, f[i], p.n);
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) step(f[i]);
+        }
+        while (r < hi) {
+            float f[V] = {};
+            load_some<T, V>(x + (int64_t)r * a.x_ld, f, p.n);
+            step(f);
         }
     }
-    if (a.dbias) a.dbias[c] = db;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) if (j < a.taps && a.dw) a.dw[j * a.cols + c] = dw[j];
 }
+
+// g of one frame, from the K frames it looks at
+template <int K, int V> __device__ __forceinline__ void pre_gradient(const float (&win)[K][V], const float (&w)[K][V], const float (&b)[V], bool silu, float (&g)[V]) {
+    if (!silu) return;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        float q = b[e];
+#pragma unroll
+        for (int i = 0; i < K; ++i) q = fmaf(w[i][e], win[i][e], q);
+        const float sg = sigmoid_acc(q);
+        g[e] *= sg * fmaf(q, 1.f - sg, 1.f);
+    }
+}
+// A run's dx needs the K - 1 frames' g behind it as well: they are worked out again there.  dx of a frame gathers in a register ring while the
+// frames that look at it go by.
+template <class T, int K> __global__ __launch_bounds__(256) void conv1d_bwd_kernel(const ConvArgs k) {
+    constexpr int V = 16 / (int)sizeof(T);
+    __shared__ float red[256 * V];
+    const vc_conv1d_args& a = k.a;
+    const Place p = place(k, V);
+    float dw[K][V] = {}, db[V] = {};
+    if (p.ok && p.run < k.runs) {
+        const Filter<T, K, V> w(a, p.c, p.n);
+        int r = p.run * BWD_RUN;
+        const int r1 = min(r + BWD_RUN, k.m.rows);
+        const T *x = (const T*)a.x + p.c, *dy = (const T*)a.dy + p.c;
+        T* dx = a.dx ? (T*)a.dx + p.c : nullptr;
+        for (int s = seq_of(k.m, r); r < r1; ++s) {
+            if (s >= k.m.n_seqs) {
+                float f[V] = {};
+                if (a.zero_tail && dx) for (; r < r1; ++r) store_some<T, V>(dx + (int64_t)r * a.dx_ld, f, p.n);
+                break;
+            }
+            const int b = seq_begin(k.m, s), end = seq_end(k.m, s, b), lo = r, hi = min(end, r1);
+            if (lo >= hi) continue;
+            float win[K][V], ring[K][V] = {};                    // ring[i]: dx of frame r - (K-1) + i so far
+#pragma unroll
+            for (int i = 0; i < K - 1; ++i) frame<T, V>(a, s, b, lo - b - (K - 1) + i, p.c, p.n, win[i]);
+            auto emit = [&](int at, const float (&d)[V]) {       // row `at` has all but its share of the final state's gradient
+                if (!dx || at < lo || at >= hi) return;
+                float o[V] = {};
+                if (a.dfinal && at >= end - (K - 1))
+                    load_some<T, V>((const T*)a.dfinal + ((int64_t)s * (K - 1) + at - (end - (K - 1))) * a.cols + p.c, o, p.n);
+#pragma unroll
+                for (int e = 0; e < V; ++e) o[e] += d[e];
+                store_some<T, V>(dx + (int64_t)at * a.dx_ld, o, p.n);
+            };
+            auto step = [&](const float (&f)[V], float (&g)[V]) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) win[K - 1][e] = f[e];
+                pre_gradient<K, V>(win, w.w, w.b, a.silu, g);
+                if (r < hi) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        db[e] += g[e];
+#pragma unroll
+                        for (int i = 0; i < K; ++i) dw[i][e] = fmaf(g[e], win[i][e], dw[i][e]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+#pragma unroll
+                    for (int i = 0; i < K; ++i) ring[i][e] = fmaf(w.w[i][e], g[e], ring[i][e]);
+                emit(r - (K - 1), ring[0]);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+#pragma unroll
+                    for (int i = 0; i < K - 1; ++i) { win[i][e] = win[i + 1][e]; ring[i][e] = ring[i + 1][e]; }
+                    ring[K - 1][e] = 0.f;
+                }
+                ++r;
+            };
+            const int stop = min(end, hi + (dx ? K - 1 : 0));
+            while (r + AHEAD <= stop) {
+                float f[AHEAD][V] = {}, g[AHEAD][V] = {};
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    load_some<T, V>(x + (int64_t)(r + i) * a.x_ld, f[i], p.n);
+                    load_some<T, V>(dy + (int64_t)(r + i) * a.dy_ld, g[i], p.n);
+                }
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) step(f[i], g[i]);
+            }
+            while (r < stop) {
+                float f[V] = {}, g[V] = {};
+                load_some<T, V>(x + (int64_t)r * a.x_ld, f, p.n);
+                load_some<T, V>(dy + (int64_t)r * a.dy_ld, g, p.n);
+                step(f, g);
+            }
+#pragma unroll
+            for (int i = 0; i < K - 1; ++i) emit(stop - (K - 1) + i, ring[i]);      // the utterance's last frames, nothing behind them
+            r = hi;
+        }
+    } else if (p.ok && a.dinitial && p.run - k.runs < k.m.n_seqs) {
+        const int s = p.run - k.runs;                            // gradient of the K - 1 frames ahead of one utterance
+        const Filter<T, K, V> w(a, p.c, p.n);
+        const int b = seq_begin(k.m, s), len = seq_end(k.m, s, b) - b;
+        float win[K][V], ring[K - 1][V] = {};
+#pragma unroll
+        for (int i = 0; i < K - 1; ++i) frame<T, V>(a, s, b, i - (K - 1), p.c, p.n, win[i]);
+#pragma unroll
+        for (int t = 0; t < K - 1; ++t) {
+            if (t >= len) continue;
+            float g[V] = {};
+            frame<T, V>(a, s, b, t, p.c, p.n, win[K - 1]);
+            load_some<T, V>((const T*)a.dy + (int64_t)(b + t) * a.dy_ld + p.c, g, p.n);
+            pre_gradient<K, V>(win, w.w, w.b, a.silu, g);
+#pragma unroll
+            for (int i = 0; i < K - 1; ++i)                      // frame t's tap j looks at frame t - (K-1) + j = i - (K-1)
+                if (i - t >= 0)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) ring[i][e] = fmaf(w.w[i - t >= 0 ? i - t : 0][e], g[e], ring[i][e]);
+#pragma unroll
+            for (int i = 0; i < K - 1; ++i)
+#pragma unroll
+                for (int e = 0; e < V; ++e) win[i][e] = win[i + 1][e];
+        }
+#pragma unroll
+        for (int i = 0; i < K - 1; ++i) {
+            float o[V] = {};
+            if (a.dfinal && i >= len) load_some<T, V>((const T*)a.dfinal + ((int64_t)s * (K - 1) + i - len) * a.cols + p.c, o, p.n);
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] += ring[i][e];
+            store_some<T, V>((T*)a.dinitial + ((int64_t)s * (K - 1) + i) * a.cols + p.c, o, p.n);
+        }
+    }
+    if (!k.part) return;
+    const int blocks = (k.cv + k.cvb - 1) / k.cvb, row = blockIdx.x / blocks;
+    if (row * (256 / k.cvb) >= k.runs) return;                   // no run in this block
+    float* part = k.part + (int64_t)row * (K + 1) * a.cols;
+    auto combine = [&](const float (&v)[V], float* dst) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < V; ++e) red[e * 256 + threadIdx.x] = v[e];
+        __syncthreads();
+        if (threadIdx.x >= (unsigned)k.cvb || !p.ok) return;
+        float s[V] = {};
+        for (int i = threadIdx.x; i < 256; i += k.cvb)
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[e] += red[e * 256 + i];
+        store_some<float, V>(dst + p.c, s, p.n);
+    };
+#pragma unroll
+    for (int i = 0; i < K; ++i) combine(dw[i], part + (int64_t)i * a.cols);
+    combine(db, part + (int64_t)K * a.cols);
+}
+
 struct ConvStepArgs {
     const void* x; void* state; const int* slots; const float *w, *bias; void* y;
     int64_t x_ld, y_ld; int rows, n_slots, cols, taps, silu;
 };
-// The slot row r works on, -1 where it is padding: outside the pool, or named by an earlier row of this call.  Every thread of the block calls it.
-__device__ __forceinline__ int claim_slot(const int* slots, int r, int n_slots) {
-    const int mine = slots ? slots[r] : r;
-    int taken = mine < 0 || mine >= n_slots;
-    if (slots)
-        for (int i = threadIdx.x; i < r; i += blockDim.x) taken |= slots[i] == mine;
-    return __syncthreads_or(taken) ? -1 : mine;
-}
 template <class T> __global__ __launch_bounds__(256) void conv1d_step_kernel(const ConvStepArgs a) {
     const int r = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
     const int slot = claim_slot(a.slots, r, a.n_slots);
@@ -111,12 +270,14 @@ template <class T> __global__ __launch_bounds__(256) void conv1d_step_kernel(con
     T* st = (T*)a.state + (int64_t)slot * (a.taps - 1) * a.cols + c;
     const T x = ((const T*)a.x)[(int64_t)r * a.x_ld + c];
     float p = (a.bias ? a.bias[c] : 0.f);
-    for (int k = 0; k < a.taps - 1; ++k) {
+#pragma unroll
+    for (int k = 0; k < 7; ++k) {
+        if (k >= a.taps - 1) break;
         const T v = st[(int64_t)k * a.cols];
-        p += a.w[k * a.cols + c] * (float)v;
+        p = fmaf(a.w[(int64_t)k * a.cols + c], (float)v, p);
         if (k) st[(int64_t)(k - 1) * a.cols] = v;
     }
-    p += a.w[(a.taps - 1) * a.cols + c] * (float)x;
+    p = fmaf(a.w[(int64_t)(a.taps - 1) * a.cols + c], (float)x, p);
     st[(int64_t)(a.taps - 2) * a.cols] = x;
     *y = (T)(a.silu ? p * sigmoid_acc(p) : p);
 }
@@ -129,21 +290,34 @@ static int check_conv1d(const char* who, const vc_conv1d_args* a, ConvArgs* k) {
     VC_ARG(a->offsets || a->rows % a->n_seqs == 0, "%s: without offsets the rows divide into n_seqs equal utterances", who);
     k->a = *a;
     k->m = SeqMap{a->offsets, (int)a->rows, a->n_seqs, (int)(a->rows / a->n_seqs)};
+    const int v = 16 / seq_esize(a->type);
+    k->cv = (a->cols + v - 1) / v;
+    for (k->cvb = 1; k->cvb < k->cv && k->cvb < 32;) k->cvb *= 2;
+    k->part = nullptr;
     return 0;
 }
-template <class T> static int conv1d_fwd(const ConvArgs& k, hipStream_t s) {
-    const int n = (int)std::max<int64_t>(k.a.rows, k.a.n_seqs);
-    hipLaunchKernelGGL((conv1d_fwd_kernel<T>), dim3((k.a.cols + 255) / 256, std::min(n, 32768)), dim3(256), 0, s, k);
+static int conv_grid(const char* who, const ConvArgs& k, bool seqs, unsigned* grid) {
+    const int per = 256 / k.cvb;
+    const int64_t g = (int64_t)((k.cv + k.cvb - 1) / k.cvb) * (((int64_t)k.runs + (seqs ? k.m.n_seqs : 0) + per - 1) / per);
+    VC_ARG(g < (1LL << 31), "%s: too many rows and channels for one launch", who);
+    *grid = (unsigned)g;
+    return 0;
+}
+template <class T, int K> static int fwd_k(const ConvArgs& k, unsigned grid, hipStream_t s) {
+    hipLaunchKernelGGL((conv1d_fwd_kernel<T, K>), dim3(grid), dim3(256), 0, s, k);
     VC_HIP(hipGetLastError());
     return 0;
 }
-template <class T> static int conv1d_bwd(const ConvArgs& k, hipStream_t s) {
-    const int n = (int)std::max<int64_t>(k.a.rows, k.a.n_seqs);
-    hipLaunchKernelGGL((conv1d_bwd_kernel<T>), dim3((k.a.cols + 255) / 256, std::min(n, 32768)), dim3(256), 0, s, k);
-    if (k.a.dw || k.a.dbias) hipLaunchKernelGGL((conv1d_dw_kernel<T>), dim3((k.a.cols + 63) / 64), dim3(64), 0, s, k);
+template <class T, int K> static int bwd_k(const ConvArgs& k, unsigned grid, hipStream_t s) {
+    hipLaunchKernelGGL((conv1d_bwd_kernel<T, K>), dim3(grid), dim3(256), 0, s, k);
     VC_HIP(hipGetLastError());
     return 0;
 }
+#define CONV_TAPS(T, taps, F, ...) \
+    ((taps) == 2 ? F<T, 2>(__VA_ARGS__) : (taps) == 3 ? F<T, 3>(__VA_ARGS__) : (taps) == 4 ? F<T, 4>(__VA_ARGS__) : (taps) == 5 ? F<T, 5>(__VA_ARGS__) : \
+     (taps) == 6 ? F<T, 6>(__VA_ARGS__) : (taps) == 7 ? F<T, 7>(__VA_ARGS__) : F<T, 8>(__VA_ARGS__))
+template <class T> static int conv1d_fwd(const ConvArgs& k, unsigned grid, hipStream_t s) { return CONV_TAPS(T, k.a.taps, fwd_k, k, grid, s); }
+template <class T> static int conv1d_bwd(const ConvArgs& k, unsigned grid, hipStream_t s) { return CONV_TAPS(T, k.a.taps, bwd_k, k, grid, s); }
 template <class T> static int conv1d_step(const ConvStepArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((conv1d_step_kernel<T>), dim3((a.cols + 255) / 256, a.rows), dim3(256), 0, s, a);
     VC_HIP(hipGetLastError());
@@ -154,13 +328,29 @@ extern "C" int vc_causal_conv1d_fwd(const vc_conv1d_args* a, void* stream) {
     VC_ARG(a->w && (a->rows == 0 || (a->x && a->y)), "vc_causal_conv1d_fwd: null pointer");
     VC_ARG(!a->final_state || a->final_state != a->initial, "vc_causal_conv1d_fwd: final_state may not be initial");
     if (a->rows == 0 && !a->final_state) return 0;
-    return SEQ_TYPES(a->type, conv1d_fwd, k, (hipStream_t)stream);
+    k.runs = (k.m.rows + FWD_RUN - 1) / FWD_RUN;
+    unsigned grid; VC_CHECK(conv_grid("vc_causal_conv1d_fwd", k, a->final_state != nullptr, &grid));
+    return SEQ_TYPES(a->type, conv1d_fwd, k, grid, (hipStream_t)stream);
 }
-extern "C" int64_t vc_causal_conv1d_bwd_work(const vc_conv1d_args* a) { return 0; }
+// rows of `part`: one for each block's runs
+static int conv_parts(const ConvArgs& k) { const int per = 256 / k.cvb; return (k.runs + per - 1) / per; }
+extern "C" int64_t vc_causal_conv1d_bwd_work(const vc_conv1d_args* a) {
+    ConvArgs k; if (check_conv1d("vc_causal_conv1d_bwd_work", a, &k)) return VC_E_ARG;
+    k.runs = (k.m.rows + BWD_RUN - 1) / BWD_RUN;
+    return (int64_t)conv_parts(k) * (a->taps + 1) * a->cols;
+}
 extern "C" int vc_causal_conv1d_bwd(const vc_conv1d_args* a, void* stream) {
     ConvArgs k; VC_CHECK(check_conv1d("vc_causal_conv1d_bwd", a, &k));
     VC_ARG(a->w && (a->rows == 0 || (a->x && a->dy)), "vc_causal_conv1d_bwd: null pointer");
-    return SEQ_TYPES(a->type, conv1d_bwd, k, (hipStream_t)stream);
+    k.runs = (k.m.rows + BWD_RUN - 1) / BWD_RUN;
+    const bool params = a->dw || a->dbias;
+    const int64_t need = (int64_t)conv_parts(k) * (a->taps + 1) * a->cols;
+    if (params && need && (!a->work || a->work_floats < need)) { vc_set_error("vc_causal_conv1d_bwd: work is too small (%lld floats needed)", (long long)need); return VC_E_NOMEM; }
+    if (params) k.part = a->work;
+    unsigned grid; VC_CHECK(conv_grid("vc_causal_conv1d_bwd", k, a->dinitial != nullptr, &grid));
+    if (grid) VC_CHECK(SEQ_TYPES(a->type, conv1d_bwd, k, grid, (hipStream_t)stream));
+    // no rows: no parts, and the sums are zeros
+    return params ? seq_sum_parts(k.part, conv_parts(k), (int64_t)(a->taps + 1) * a->cols, a->dw, (int64_t)a->taps * a->cols, a->dbias, (hipStream_t)stream) : 0;
 }
 extern "C" int vc_causal_conv1d_step(const void* x, int64_t x_ld, void* state, const int32_t* slots, const float* w, const float* bias,
                                      void* y, int64_t y_ld, int rows, int n_slots, int cols, int taps, int type, int silu, void* stream) {

@@ -1,110 +1,384 @@
 // vc_seq_norm.hip -- RMS norm of a frame's channels with the residual's addition, its 8-bit form, its gradient.
 //   t = x + residual (as stored);  y = t * rstd * gamma,  rstd = 1 / sqrt(mean(t^2) + eps)
+//   dt = dsum + rstd * (g - that * mean(g * that)),  g = dy * gamma, that = t * rstd;   dgamma = sum over rows of dy * that
+// All of it is bound by HBM: a row is read once into registers (TPR threads hold it, ITEMS 16-byte vectors each), its sum taken there, and written.
 #include "vc_seq.h"
 
 struct NormRowArgs {
     const void* x; const void* res; const float* gamma; void* y; void* sum; float* rstd; float* scale;
-    const void* dy; const void* dsum; void* dx; void* dres;
+    const void* dy; const void* dsum; void* dx; void* dres; float* part;
     int64_t x_ld, res_ld, y_ld, sum_ld, dy_ld, dsum_ld, dx_ld, dres_ld;
     float eps; int64_t rows; int cols, group;
 };
 
-template <class T, class S> __global__ __launch_bounds__(256) void rms_fwd_kernel(const NormRowArgs a) {
-    __shared__ float red[4];
-    const int64_t r = blockIdx.x;
-    const T* x = (const T*)a.x + r * a.x_ld;
-    const S* res = a.res ? (const S*)a.res + r * a.res_ld : nullptr;
-    S* sum = a.sum ? (S*)a.sum + r * a.sum_ld : nullptr;
-    float ss = 0.f;
-    for (int c = threadIdx.x; c < a.cols; c += 256) {
-        const float t = res ? (float)(S)((float)x[c] + (float)res[c]) : (float)x[c];
-        ss += t * t;
+// sum / largest over the TPR threads of a row; every one gets it.  TPR = 64: a wave, no barrier; else the block
+template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red) {
+    v = wave_sum_dpp(v);
+    if constexpr (TPR > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int i = 0; i < TPR / 64; ++i) v += red[i];
     }
-    ss = block_sum_256(ss, red);
-    const float rstd = 1.f / sqrtf(ss / (float)a.cols + a.eps);
-    if (a.rstd && threadIdx.x == 0) a.rstd[r] = rstd;
-    for (int c = threadIdx.x; c < a.cols; c += 256) {
-        const float t = res ? (float)(S)((float)x[c] + (float)res[c]) : (float)x[c];
-        if (sum && res) sum[c] = (S)t;
-        ((T*)a.y)[r * a.y_ld + c] = (T)(t * rstd * a.gamma[c]);
+    return v;
+}
+template <int LANES> __device__ __forceinline__ unsigned lanes_max(unsigned v) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
+    return v;
+}
+template <int TPR> __device__ __forceinline__ unsigned row_max(unsigned v, float* red) {
+    v = lanes_max<64>(v);
+    if constexpr (TPR > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = __uint_as_float(v);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TPR / 64; ++i) v = max(v, __float_as_uint(red[i]));
+    }
+    return v;
+}
+// four (V = 4) or eight values as e4m3: rounded to nearest even by the conversion instruction; |f| <= 448 (1 + 2^-23), which rounds to 448
+template <int V> __device__ __forceinline__ void store_e4m3(unsigned char* p, const float (&f)[V], int n) {
+    unsigned w[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+        int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i], f[4 * i + 1], 0, false);
+        w[i] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2], f[4 * i + 3], lo, true);
+    }
+    if (n >= V) {
+        struct __attribute__((packed, aligned(1))) W { unsigned v[V / 4]; } q;
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) q.v[i] = w[i];
+        *(W*)p = q;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) if (i < n) p[i] = (unsigned char)(w[i / 4] >> (8 * (i % 4)));
     }
 }
-template <class T, class S> __global__ __launch_bounds__(256) void rms_e4m3_kernel(const NormRowArgs a) {
-    __shared__ float red[4];
-    __shared__ unsigned top;
-    const int64_t r = blockIdx.x;
-    const T* x = (const T*)a.x + r * a.x_ld;
-    const S* res = a.res ? (const S*)a.res + r * a.res_ld : nullptr;
-    float ss = 0.f;
-    for (int c = threadIdx.x; c < a.cols; c += 256) {
-        const float t = res ? (float)(S)((float)x[c] + (float)res[c]) : (float)x[c];
-        ss += t * t;
-    }
-    ss = block_sum_256(ss, red);
-    const float rstd = 1.f / sqrtf(ss / (float)a.cols + a.eps);
-    const int w = a.group ? a.group : a.cols, ng = a.cols / w;
-    for (int g = 0; g < ng; ++g) {
-        __syncthreads();
-        if (threadIdx.x == 0) top = __float_as_uint(0x1p-100f);
-        __syncthreads();
-        for (int c = g * w + threadIdx.x; c < (g + 1) * w; c += 256) {
-            const float t = res ? (float)(S)((float)x[c] + (float)res[c]) : (float)x[c];
-            atomicMax(&top, __float_as_uint(fabsf(t * rstd * a.gamma[c])));      // as integers: NaN is above infinity, and stays
-        }
-        __syncthreads();
-        const float m = __uint_as_float(top);
-        const float inv = 448.f / m;
-        if (threadIdx.x == 0) a.scale[r * ng + g] = m / 448.f;
-        for (int c = g * w + threadIdx.x; c < (g + 1) * w; c += 256) {
-            const float t = res ? (float)(S)((float)x[c] + (float)res[c]) : (float)x[c];
-            if (a.sum && res) ((S*)a.sum)[r * a.sum_ld + c] = (S)t;
-            const float v = t * rstd * a.gamma[c] * inv;
-            ((unsigned char*)a.y)[r * a.y_ld + c] = (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false);
-        }
-    }
-}
-template <class T, class S> __global__ __launch_bounds__(256) void rms_bwd_kernel(const NormRowArgs a) {
-    __shared__ float red[4];
-    const int64_t r = blockIdx.x;
-    const S* t = (const S*)a.sum + r * a.sum_ld;
-    const T* dy = (const T*)a.dy + r * a.dy_ld;
-    const S* ds = a.dsum ? (const S*)a.dsum + r * a.dsum_ld : nullptr;
-    const float rstd = a.rstd[r];
-    float m = 0.f;
-    for (int c = threadIdx.x; c < a.cols; c += 256) m += (float)dy[c] * a.gamma[c] * ((float)t[c] * rstd);
-    m = block_sum_256(m, red) / (float)a.cols;
-    for (int c = threadIdx.x; c < a.cols; c += 256) {
-        const float g = (float)dy[c] * a.gamma[c];
-        const float d = (ds ? (float)ds[c] : 0.f) + rstd * (g - (float)t[c] * rstd * m);
-        if (a.dx) ((T*)a.dx)[r * a.dx_ld + c] = (T)d;
-        if (a.dres) ((S*)a.dres)[r * a.dres_ld + c] = (S)d;
-    }
-}
-template <class T, class S> __global__ __launch_bounds__(64) void rms_dgamma_kernel(const NormRowArgs a, float* dgamma) {
-    const int c = blockIdx.x * 64 + threadIdx.x;
-    if (c >= a.cols) return;
-    float s = 0.f;
-    for (int64_t r = 0; r < a.rows; ++r) s += (float)((const T*)a.dy)[r * a.dy_ld + c] * ((float)((const S*)a.sum)[r * a.sum_ld + c] * a.rstd[r]);
-    dgamma[c] = s;
+// The largest |y| of a group as an integer: ordered like the numbers, a NaN above infinity (fmaxf would drop it)
+constexpr float E4M3_TOP = 448.f, LEAST_TOP = 0x1p-100f;
+template <int V> __device__ __forceinline__ unsigned top_of(const float (&f)[V], unsigned m) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(fabsf(f[i])));
+    return m;
 }
 
-template <class T, class S> static int norm_fwd_t(const NormRowArgs& a, bool e4m3, hipStream_t s) {
-    if (e4m3) hipLaunchKernelGGL((rms_e4m3_kernel<T, S>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((rms_fwd_kernel<T, S>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+// A row of up to TPR * ITEMS vectors in registers.  Threads walk the rows with a stride of the grid, so gamma is read once for all of them.
+template <class T, class S, bool E4M3, int TPR, int ITEMS> __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(const NormRowArgs a) {
+    constexpr int V = 16 / (int)sizeof(T), RPB = TPR < 256 ? 256 / TPR : 1;
+    __shared__ float red[TPR / 64 > 0 ? TPR / 64 : 1];
+    const int t = threadIdx.x % TPR;
+    float gm[ITEMS][V];
+    int left[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int c = (i * TPR + t) * V;
+        left[i] = a.cols - c;
+#pragma unroll
+        for (int e = 0; e < V; ++e) gm[i][e] = 0.f;
+        if (left[i] > 0) load_some<float, V>(a.gamma + c, gm[i], left[i]);
+    }
+    const float inv_cols = 1.f / (float)a.cols;
+    for (int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; r < a.rows; r += (int64_t)gridDim.x * RPB) {
+        float f[ITEMS][V];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int c = (i * TPR + t) * V;
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[i][e] = 0.f;
+            if (left[i] > 0) load_some<T, V>((const T*)a.x + r * a.x_ld + c, f[i], left[i]);
+        }
+        if (a.res) {
+            float g[ITEMS][V];
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int c = (i * TPR + t) * V;
+#pragma unroll
+                for (int e = 0; e < V; ++e) g[i][e] = 0.f;
+                if (left[i] > 0) load_some<S, V>((const S*)a.res + r * a.res_ld + c, g[i], left[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int c = (i * TPR + t) * V;
+#pragma unroll
+                for (int e = 0; e < V; ++e) f[i][e] = (float)(S)(f[i][e] + g[i][e]);
+                if (left[i] > 0) store_some<S, V>((S*)a.sum + r * a.sum_ld + c, f[i], left[i]);
+            }
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) ss = fmaf(f[i][e], f[i][e], ss);
+        const float rstd = 1.f / sqrtf(row_sum<TPR>(ss, red) * inv_cols + a.eps);
+        if (a.rstd && t == 0) a.rstd[r] = rstd;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[i][e] = f[i][e] * rstd * gm[i][e];
+        if constexpr (!E4M3) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (left[i] > 0) store_some<T, V>((T*)a.y + r * a.y_ld + (i * TPR + t) * V, f[i], left[i]);
+        } else {
+            unsigned top[ITEMS];
+            if (a.group == 0) {
+                unsigned m = __float_as_uint(LEAST_TOP);
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i) m = top_of<V>(f[i], m);
+                m = row_max<TPR>(m, red);
+                if (t == 0) a.scale[r] = __uint_as_float(m) / E4M3_TOP;
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i) top[i] = m;
+            } else {
+                const int gl = a.group / V;                      // lanes that share a scale: 4 to 32, next to each other
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i) {
+                    unsigned m = top_of<V>(f[i], __float_as_uint(LEAST_TOP));
+                    m = max(m, (unsigned)__shfl_xor((int)m, 1, 64));
+                    m = max(m, (unsigned)__shfl_xor((int)m, 2, 64));
+                    if (gl > 4) m = max(m, (unsigned)__shfl_xor((int)m, 4, 64));
+                    if (gl > 8) m = max(m, (unsigned)__shfl_xor((int)m, 8, 64));
+                    if (gl > 16) m = max(m, (unsigned)__shfl_xor((int)m, 16, 64));
+                    top[i] = m;
+                    if (left[i] > 0 && t % gl == 0) a.scale[r * (a.cols / a.group) + (i * TPR + t) / gl] = __uint_as_float(m) / E4M3_TOP;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const float inv = E4M3_TOP / __uint_as_float(top[i]);
+                float q[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) q[e] = f[i][e] * inv;
+                if (left[i] > 0) store_e4m3<V>((unsigned char*)a.y + r * a.y_ld + (i * TPR + t) * V, q, left[i]);
+            }
+        }
+    }
+}
+// Rows longer than the registers of a block hold: one block a row, which it reads again for each pass (out of L2)
+template <class T, class S, bool E4M3> __global__ __launch_bounds__(1024) void rms_fwd_long_kernel(const NormRowArgs a) {
+    __shared__ float red[16];
+    const int64_t r = blockIdx.x;
+    const T* x = (const T*)a.x + r * a.x_ld;
+    const S* res = a.res ? (const S*)a.res + r * a.res_ld : nullptr;
+    S* sum = a.res ? (S*)a.sum + r * a.sum_ld : nullptr;
+    float ss = 0.f;
+    for (int c = threadIdx.x; c < a.cols; c += 1024) {
+        float f = (float)x[c];
+        if (res) { const S q = (S)(f + (float)res[c]); sum[c] = q; f = (float)q; }
+        ss = fmaf(f, f, ss);
+    }
+    const float rstd = 1.f / sqrtf(row_sum<1024>(ss, red) / (float)a.cols + a.eps);
+    if (a.rstd && threadIdx.x == 0) a.rstd[r] = rstd;
+    auto y = [&](int c) { return (sum ? (float)sum[c] : (float)x[c]) * rstd * a.gamma[c]; };      // a thread reads back what it wrote itself
+    if constexpr (!E4M3) {
+        for (int c = threadIdx.x; c < a.cols; c += 1024) ((T*)a.y)[r * a.y_ld + c] = (T)y(c);
+    } else {
+        // scales: a wave for each group of 64 threads' columns would leave most idle, so each pass of the block covers 1024 columns: 8 to 32 groups
+        unsigned whole = __float_as_uint(LEAST_TOP);
+        if (a.group == 0) {
+            for (int c = threadIdx.x; c < a.cols; c += 1024) whole = max(whole, __float_as_uint(fabsf(y(c))));
+            whole = row_max<1024>(whole, red);
+            if (threadIdx.x == 0) a.scale[r] = __uint_as_float(whole) / E4M3_TOP;
+        }
+        __shared__ unsigned top[1024 / 32];
+        for (int c0 = 0; c0 < a.cols; c0 += 1024) {
+            const int c = c0 + threadIdx.x;
+            const float v = c < a.cols ? y(c) : 0.f;
+            unsigned m = whole;
+            if (a.group) {
+                m = lanes_max<32>(max(whole, __float_as_uint(fabsf(v))));
+                __syncthreads();
+                if (threadIdx.x % 32 == 0) top[threadIdx.x / 32] = m;
+                __syncthreads();
+                const int per = a.group / 32, first = threadIdx.x / a.group * per;
+                for (int i = 0; i < per; ++i) m = max(m, top[first + i]);
+                if (c < a.cols && threadIdx.x % a.group == 0) a.scale[r * (a.cols / a.group) + c / a.group] = __uint_as_float(m) / E4M3_TOP;
+            }
+            const float q = v * (E4M3_TOP / __uint_as_float(m));
+            if (c < a.cols) ((unsigned char*)a.y)[r * a.y_ld + c] = (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(q, q, 0, false);
+        }
+    }
+}
+
+// Gradient.  Every thread keeps its columns' share of dgamma over all rows it walks; a block leaves one row of `part`.
+template <class T, class S, int TPR, int ITEMS> __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(const NormRowArgs a) {
+    constexpr int V = 16 / (int)sizeof(T), RPB = TPR < 256 ? 256 / TPR : 1;
+    __shared__ float red[TPR / 64 > 0 ? TPR / 64 : 1];
+    const int t = threadIdx.x % TPR;
+    float gm[ITEMS][V], dg[ITEMS][V];
+    int left[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int c = (i * TPR + t) * V;
+        left[i] = a.cols - c;
+#pragma unroll
+        for (int e = 0; e < V; ++e) { gm[i][e] = 0.f; dg[i][e] = 0.f; }
+        if (left[i] > 0) load_some<float, V>(a.gamma + c, gm[i], left[i]);
+    }
+    const float inv_cols = 1.f / (float)a.cols;
+    for (int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; r < a.rows; r += (int64_t)gridDim.x * RPB) {
+        float th[ITEMS][V], g[ITEMS][V], ds[ITEMS][V];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int c = (i * TPR + t) * V;
+#pragma unroll
+            for (int e = 0; e < V; ++e) { th[i][e] = 0.f; g[i][e] = 0.f; ds[i][e] = 0.f; }
+            if (left[i] > 0) {
+                load_some<S, V>((const S*)a.sum + r * a.sum_ld + c, th[i], left[i]);
+                load_some<T, V>((const T*)a.dy + r * a.dy_ld + c, g[i], left[i]);
+                if (a.dsum) load_some<S, V>((const S*)a.dsum + r * a.dsum_ld + c, ds[i], left[i]);
+            }
+        }
+        const float rstd = a.rstd[r];
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                th[i][e] *= rstd;
+                dg[i][e] = fmaf(g[i][e], th[i][e], dg[i][e]);
+                g[i][e] *= gm[i][e];
+                m = fmaf(g[i][e], th[i][e], m);
+            }
+        if (!a.dx && !a.dres) continue;                          // the same for all threads
+        m = row_sum<TPR>(m, red) * inv_cols;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int c = (i * TPR + t) * V;
+#pragma unroll
+            for (int e = 0; e < V; ++e) g[i][e] = fmaf(rstd, fmaf(-th[i][e], m, g[i][e]), ds[i][e]);
+            if (left[i] <= 0) continue;
+            if (a.dx) store_some<T, V>((T*)a.dx + r * a.dx_ld + c, g[i], left[i]);
+            if (a.dres) store_some<S, V>((S*)a.dres + r * a.dres_ld + c, g[i], left[i]);
+        }
+    }
+    if (!a.part) return;
+    if constexpr (RPB > 1) {                                     // the block's rows of threads, one behind the other
+        __shared__ float acc[TPR * ITEMS * V];
+        for (int w = 0; w < RPB; ++w) {
+            if ((int)threadIdx.x / TPR == w)
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        float& p = acc[(i * V + e) * TPR + t];
+                        dg[i][e] += w ? p : 0.f;
+                        p = dg[i][e];
+                    }
+            __syncthreads();
+        }
+        if ((int)threadIdx.x / TPR != RPB - 1) return;           // the last one holds the sums
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+        if (left[i] > 0) store_some<float, V>(a.part + (int64_t)blockIdx.x * a.cols + (i * TPR + t) * V, dg[i], left[i]);
+}
+template <class T, class S> __global__ __launch_bounds__(1024) void rms_bwd_long_kernel(const NormRowArgs a) {
+    __shared__ float red[16];
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const S* t = (const S*)a.sum + r * a.sum_ld;
+        const T* dy = (const T*)a.dy + r * a.dy_ld;
+        const S* ds = a.dsum ? (const S*)a.dsum + r * a.dsum_ld : nullptr;
+        const float rstd = a.rstd[r];
+        float* part = a.part ? a.part + (int64_t)blockIdx.x * a.cols : nullptr;
+        float m = 0.f;
+        for (int c = threadIdx.x; c < a.cols; c += 1024) {
+            const float th = (float)t[c] * rstd, d = (float)dy[c];
+            m = fmaf(d * a.gamma[c], th, m);
+            if (part) part[c] = (r == blockIdx.x ? 0.f : part[c]) + d * th;
+        }
+        m = row_sum<1024>(m, red) / (float)a.cols;
+        for (int c = threadIdx.x; c < a.cols; c += 1024) {
+            const float d = fmaf(rstd, (float)dy[c] * a.gamma[c] - (float)t[c] * rstd * m, ds ? (float)ds[c] : 0.f);
+            if (a.dx) ((T*)a.dx)[r * a.dx_ld + c] = (T)d;
+            if (a.dres) ((S*)a.dres)[r * a.dres_ld + c] = (S)d;
+        }
+    }
+}
+
+// 64 columns a block, 16 threads a column
+__global__ __launch_bounds__(1024) void sum_parts_kernel(const float* part, int parts, int64_t n, float* dst0, int64_t n0, float* dst1) {
+    __shared__ float red[16][64];
+    const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+    const int w = threadIdx.x >> 6;
+    float s = 0.f;
+    if (c < n) {
+        int p = w;
+        for (; p + 48 < parts; p += 64) {
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = part[(int64_t)(p + 16 * i) * n + c];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s += v[i];
+        }
+        for (; p < parts; p += 16) s += part[(int64_t)p * n + c];
+    }
+    red[w][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (w || c >= n) return;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += red[i][threadIdx.x];
+    float* dst = c < n0 ? dst0 : dst1;
+    if (dst) dst[c < n0 ? c : c - n0] = s;
+}
+int seq_sum_parts(const float* part, int parts, int64_t n, float* dst0, int64_t n0, float* dst1, hipStream_t s) {
+    hipLaunchKernelGGL(sum_parts_kernel, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, s, part, parts, n, dst0, n0, dst1);
+    VC_HIP(hipGetLastError());
+    return 0;
+}
+
+// How a row of nv vectors is held: a wave up to 4 vectors a thread, then a block of 256, then of 1024
+#define NORM_LAYOUT(nv, F) \
+    ((nv) <= 64 ? F(64, 1) : (nv) <= 128 ? F(64, 2) : (nv) <= 256 ? F(64, 4) : (nv) <= 512 ? F(256, 2) : (nv) <= 1024 ? F(256, 4) : F(1024, 4))
+static int norm_tpr(int64_t nv) { return nv <= 256 ? 64 : nv <= 1024 ? 256 : 1024; }
+constexpr int64_t NORM_MOST = 4096;                              // vectors of the longest row that registers hold
+static int64_t norm_vectors(int cols, int type) { const int v = 16 / seq_esize(type); return (cols + v - 1) / v; }
+
+template <class T, class S, bool E, int TPR, int ITEMS> static void launch_fwd(const NormRowArgs& a, hipStream_t s) {
+    const int64_t rpb = TPR < 256 ? 256 / TPR : 1, want = (a.rows + rpb - 1) / rpb;
+    const int64_t most = TPR == 1024 ? 1024 : 4096;
+    hipLaunchKernelGGL((rms_fwd_kernel<T, S, E, TPR, ITEMS>), dim3((unsigned)std::min(want, most)), dim3(TPR < 256 ? 256 : TPR), 0, s, a);
+}
+template <class T, class S, bool E> static int norm_fwd_e(const NormRowArgs& a, hipStream_t s) {
+    const int64_t nv = (a.cols + 16 / (int)sizeof(T) - 1) / (16 / (int)sizeof(T));
+    if (nv > NORM_MOST) hipLaunchKernelGGL((rms_fwd_long_kernel<T, S, E>), dim3((unsigned)a.rows), dim3(1024), 0, s, a);
+    else {
+#define F(TPR, ITEMS) launch_fwd<T, S, E, TPR, ITEMS>(a, s)
+        NORM_LAYOUT(nv, F);
+#undef F
+    }
     VC_HIP(hipGetLastError());
     return 0;
 }
 template <class T> static int norm_fwd(const NormRowArgs& a, bool wide, bool e4m3, hipStream_t s) {
-    return wide ? norm_fwd_t<T, float>(a, e4m3, s) : norm_fwd_t<T, T>(a, e4m3, s);
+    if (wide) return e4m3 ? norm_fwd_e<T, float, true>(a, s) : norm_fwd_e<T, float, false>(a, s);
+    return e4m3 ? norm_fwd_e<T, T, true>(a, s) : norm_fwd_e<T, T, false>(a, s);
 }
-template <class T, class S> static int norm_bwd_t(const NormRowArgs& a, float* dgamma, hipStream_t s) {
-    if (a.dx || a.dres) hipLaunchKernelGGL((rms_bwd_kernel<T, S>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
-    if (dgamma) hipLaunchKernelGGL((rms_dgamma_kernel<T, S>), dim3((a.cols + 63) / 64), dim3(64), 0, s, a, dgamma);
+// Blocks of the gradient: enough to fill the card, few enough that their rows of `part` cost little beside the activations
+static int norm_bwd_blocks(int64_t rows, int cols, int type) {
+    const int64_t nv = norm_vectors(cols, type);
+    const int64_t rpb = nv <= 256 ? 4 : 1, most = norm_tpr(nv) == 1024 ? 256 : 512;
+    return (int)std::min<int64_t>((rows + rpb - 1) / rpb, most);
+}
+template <class T, class S> static int norm_bwd_t(const NormRowArgs& a, int type, float* dgamma, hipStream_t s) {
+    const int64_t nv = norm_vectors(a.cols, type);
+    const int blocks = norm_bwd_blocks(a.rows, a.cols, type);
+    if (nv > NORM_MOST / 2) hipLaunchKernelGGL((rms_bwd_long_kernel<T, S>), dim3(blocks), dim3(1024), 0, s, a);
+    else {
+#define F(TPR, ITEMS) hipLaunchKernelGGL((rms_bwd_kernel<T, S, TPR, ITEMS>), dim3(blocks), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
+        if (nv <= 64) F(64, 1); else if (nv <= 128) F(64, 2); else if (nv <= 256) F(64, 4); else if (nv <= 512) F(256, 2); else if (nv <= 1024) F(256, 4); else F(1024, 2);
+#undef F
+    }
     VC_HIP(hipGetLastError());
-    return 0;
+    return dgamma ? seq_sum_parts(a.part, blocks, a.cols, dgamma, a.cols, nullptr, s) : 0;
 }
-template <class T> static int norm_bwd(const NormRowArgs& a, bool wide, float* dgamma, hipStream_t s) {
-    return wide ? norm_bwd_t<T, float>(a, dgamma, s) : norm_bwd_t<T, T>(a, dgamma, s);
+template <class T> static int norm_bwd(const NormRowArgs& a, bool wide, int type, float* dgamma, hipStream_t s) {
+    return wide ? norm_bwd_t<T, float>(a, type, dgamma, s) : norm_bwd_t<T, T>(a, type, dgamma, s);
 }
 
 static int check_norm(const char* who, int64_t rows, int cols, int type, int sum_type) {
@@ -140,7 +414,10 @@ extern "C" int vc_rms_norm_e4m3(const void* x, int64_t x_ld, const void* residua
     a.eps = eps; a.rows = rows; a.cols = cols; a.group = group;
     return norm_entry("vc_rms_norm_e4m3", a, type, sum_type, true, stream);
 }
-extern "C" int64_t vc_rms_norm_bwd_work(int64_t rows, int cols) { return 0; }
+extern "C" int64_t vc_rms_norm_bwd_work(int64_t rows, int cols) {
+    VC_CHECK(check_norm("vc_rms_norm_bwd_work", rows, cols, VC_F32, VC_F32));
+    return (int64_t)std::max(norm_bwd_blocks(rows, cols, VC_F32), norm_bwd_blocks(rows, cols, VC_BF16)) * cols;
+}
 extern "C" int vc_rms_norm_bwd(const void* dy, int64_t dy_ld, const void* dsum, int64_t dsum_ld, const void* sum, int64_t sum_ld,
                                const float* rstd, const float* gamma, void* dx, int64_t dx_ld, void* dres, int64_t dres_ld, float* dgamma,
                                float* work, int64_t work_floats, int64_t rows, int cols, int type, int sum_type, void* stream) {
@@ -150,10 +427,11 @@ extern "C" int vc_rms_norm_bwd(const void* dy, int64_t dy_ld, const void* dsum, 
         return 0;
     }
     VC_ARG(dy && sum && rstd && gamma && (dx || dres || dgamma), "vc_rms_norm_bwd: null pointer");
+    if (dgamma && (!work || work_floats < vc_rms_norm_bwd_work(rows, cols))) { vc_set_error("vc_rms_norm_bwd: work is too small"); return VC_E_NOMEM; }
     NormRowArgs a{};
     a.dy = dy; a.dy_ld = dy_ld; a.dsum = dsum; a.dsum_ld = dsum_ld; a.sum = (void*)sum; a.sum_ld = sum_ld; a.rstd = (float*)rstd; a.gamma = gamma;
-    a.dx = dx; a.dx_ld = dx_ld; a.dres = dres; a.dres_ld = dres_ld; a.rows = rows; a.cols = cols;
-    return SEQ_TYPES(type, norm_bwd, a, sum_type == VC_F32 && type != VC_F32, dgamma, (hipStream_t)stream);
+    a.dx = dx; a.dx_ld = dx_ld; a.dres = dres; a.dres_ld = dres_ld; a.rows = rows; a.cols = cols; a.part = dgamma ? work : nullptr;
+    return SEQ_TYPES(type, norm_bwd, a, sum_type == VC_F32 && type != VC_F32, type, dgamma, (hipStream_t)stream);
 }
 
 extern "C" int vc_seq_version(void) { return 1; }

@@ -72,14 +72,6 @@ struct ScanStepArgs {
     const void *x, *dt, *z, *B, *C; const float *A, *D, *dt_bias; float* state; const int* slots; void* y;
     int64_t x_ld, dt_ld, z_ld, b_ld, c_ld, y_ld; int rows, n_slots, cols, states, groups, softplus;
 };
-// The slot row r works on, -1 where it is padding: outside the pool, or named by an earlier row of this call.  Every thread of the block calls it.
-__device__ __forceinline__ int claim_slot(const int* slots, int r, int n_slots) {
-    const int mine = slots ? slots[r] : r;
-    int taken = mine < 0 || mine >= n_slots;
-    if (slots)
-        for (int i = threadIdx.x; i < r; i += blockDim.x) taken |= slots[i] == mine;
-    return __syncthreads_or(taken) ? -1 : mine;
-}
 template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_step_kernel(const ScanStepArgs a) {
     const int r = blockIdx.y, j = threadIdx.x % L, c = blockIdx.x * (256 / L) + threadIdx.x / L;
     const int slot = claim_slot(a.slots, r, a.n_slots);

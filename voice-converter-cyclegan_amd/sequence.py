@@ -23,6 +23,7 @@ from . import _lib
 from ._lib import lib, check
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _require(ok, text, *args):
@@ -34,24 +35,16 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
-
-
-class _on:
-    """The tensors' device as the current one, where it is another."""
-
-    def __init__(self, t):
-        self.want = t.device.index
-
-    def __enter__(self):
-        self.had = torch.cuda.current_device()
-        if self.had != self.want:
-            torch.cuda.set_device(self.want)
-
-    def __exit__(self, *_):
-        if self.had != self.want:
-            torch.cuda.set_device(self.had)
+def _launch(f, name, ref, *args):
+    """f(*args, stream) on ref's device and that device's current stream."""
+    index = ref.device.index
+    if torch.cuda.current_device() == index:
+        rc = f(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = f(*args, _raw_stream(index))
+    if rc:
+        check(rc, name)
 
 
 def _activation(t, name):
@@ -63,10 +56,10 @@ def _activation(t, name):
 def _like(t, ref, name, shape=None, dtype=None):
     """t on ref's device, with this shape and type."""
     dtype = dtype or ref.dtype
-    _require(isinstance(t, torch.Tensor) and t.device == ref.device and t.dtype == dtype, '%s must be a %s tensor on %s', name, dtype, ref.device)
-    if shape is not None:
-        _require(tuple(t.shape) == tuple(shape), '%s must have shape %s, got %s', name, tuple(shape), tuple(t.shape))
-    return t
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == ref.device and (shape is None or t.shape == shape):
+        return t
+    _require(isinstance(t, torch.Tensor) and t.device == ref.device and t.dtype is dtype, '%s must be a %s tensor on %s', name, dtype, ref.device)
+    raise ValueError('%s must have shape %s, got %s' % (name, tuple(shape), tuple(t.shape)))
 
 
 def _parameter(t, ref, name, shape):
@@ -75,6 +68,10 @@ def _parameter(t, ref, name, shape):
 
 def _rows(t, tail=1):
     """[..., channels] (or [..., groups, states] with tail = 2) as rows with one stride between them: (tensor, stride).  Copies only what cannot be seen so."""
+    if t.is_contiguous():
+        return t, t.shape[-1] if tail == 1 else t.shape[-1] * t.shape[-2]
+    if tail == 1 and t.dim() == 2 and t.stride(1) == 1:
+        return t, t.stride(0)
     inner = t.shape[t.dim() - tail:]
     width = 1
     for n in inner:
@@ -85,8 +82,29 @@ def _rows(t, tail=1):
     return flat, flat.stride(0) if flat.shape[0] > 1 else width
 
 
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _no_grad(what, *tensors):
+    _require(not _wants_grad(*tensors), '%s has no gradient: call it under torch.no_grad() or on detached tensors', what)
+
+
 def _fresh(shape, ref, dtype=None):
-    return torch.empty(shape, dtype=dtype or ref.dtype, device=ref.device)
+    return ref.new_empty(shape, dtype=dtype)
+
+
+def _fresh_like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _once(grad):
+    """The backward of a Function that cannot be differentiated again: refuses that where a graph of the backward is built, costs nothing where none is."""
+    guarded = once_differentiable(grad)
+
+    def backward(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else grad)(ctx, *grads)
+    return backward
 
 
 # ------------------------------------------------------------------------------------------------------------------ norm
@@ -103,30 +121,35 @@ def _norm_inputs(x, gamma, residual, eps):
     return gamma
 
 
+def _norm_forward(x, gamma, residual, eps, keep):
+    cols = x.shape[-1]
+    rows = x.numel() // cols
+    x2, x_ld = _rows(x)
+    y = _fresh_like(x)
+    kind = stream_kind = _TYPES[x.dtype]
+    total, r2, r_ld = None, None, 0
+    if residual is not None:
+        total = _fresh_like(residual)
+        r2, r_ld = _rows(residual)
+        stream_kind = _TYPES[residual.dtype]
+    rstd = _fresh((rows,), gamma) if keep else None
+    _launch(lib.vc_rms_norm_fwd, 'vc_rms_norm_fwd', x, _p(x2), x_ld, _p(r2), r_ld, _p(gamma), _p(y), cols, _p(total), cols, _p(rstd), eps, rows, cols,
+            kind, stream_kind)
+    return y, total, rstd, (kind, stream_kind)
+
+
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gamma, residual, eps, keep):
-        shape, cols = x.shape, x.shape[-1]
-        x2, x_ld = _rows(x)
-        rows = x2.shape[0]
-        y = _fresh(shape, x)
-        total = _fresh(shape, x, residual.dtype) if residual is not None else None
-        rstd = _fresh((rows,), x, torch.float32) if keep else None
-        r2, r_ld = _rows(residual) if residual is not None else (None, 0)
-        kind = _TYPES[x.dtype]
-        stream_kind = _TYPES[residual.dtype] if residual is not None else kind
-        with _on(x):
-            check(lib.vc_rms_norm_fwd(_p(x2), x_ld, _p(r2), r_ld, _p(gamma), _p(y), cols, _p(total), cols, _p(rstd), eps, rows, cols,
-                                      kind, stream_kind, _stream(x)), 'vc_rms_norm_fwd')
-        if keep:
-            ctx.kinds, ctx.x_dtype = (kind, stream_kind), x.dtype
-            ctx.save_for_backward(x if total is None else total, gamma, rstd)
-            ctx.has_residual = residual is not None
-            ctx.set_materialize_grads(False)
-        return y if residual is None else (y, total)
+    def forward(ctx, x, gamma, residual, eps):
+        y, total, rstd, ctx.kinds = _norm_forward(x, gamma, residual, eps, True)
+        ctx.x_dtype = x.dtype
+        ctx.has_residual = residual is not None
+        ctx.save_for_backward(x if total is None else total, gamma, rstd)
+        ctx.set_materialize_grads(False)
+        return y if total is None else (y, total)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dtotal=None):
         total, gamma, rstd = ctx.saved_tensors
         cols = total.shape[-1]
@@ -135,7 +158,7 @@ class _RmsNorm(torch.autograd.Function):
         t2, t_ld = _rows(total)
         dy2, dy_ld = _rows(dy)
         ds2, ds_ld = _rows(dtotal) if dtotal is not None else (None, 0)
-        rows = t2.shape[0]
+        rows = total.numel() // cols
         need_x, need_g, need_r = ctx.needs_input_grad[:3]
         need_r = need_r and ctx.has_residual
         one = ctx.kinds[0] == ctx.kinds[1]                       # one gradient serves both summands where they have one type
@@ -145,10 +168,9 @@ class _RmsNorm(torch.autograd.Function):
         floats = lib.vc_rms_norm_bwd_work(rows, cols) if need_g else 0
         work = _fresh((floats,), gamma) if floats else None
         if rows:
-            with _on(total):
-                check(lib.vc_rms_norm_bwd(_p(dy2), dy_ld, _p(ds2), ds_ld, _p(t2), t_ld, _p(rstd), _p(gamma), _p(dx), cols, _p(dres), cols,
-                                          _p(dgamma), _p(work), floats, rows, cols, *ctx.kinds, _stream(total)), 'vc_rms_norm_bwd')
-        return dx if need_x else None, dgamma, (dx if one else dres) if need_r else None, None, None
+            _launch(lib.vc_rms_norm_bwd, 'vc_rms_norm_bwd', total, _p(dy2), dy_ld, _p(ds2), ds_ld, _p(t2), t_ld, _p(rstd), _p(gamma), _p(dx), cols,
+                    _p(dres), cols, _p(dgamma), _p(work), floats, rows, cols, *ctx.kinds)
+        return dx if need_x else None, dgamma, (dx if one else dres) if need_r else None, None
 
 
 def rms_norm(x, gamma, residual=None, eps=1e-6):
@@ -156,8 +178,10 @@ def rms_norm(x, gamma, residual=None, eps=1e-6):
 
     The sum has the residual's type and is what the norm sees: y = gamma * sum / sqrt(mean(sum^2) + eps)."""
     gamma = _norm_inputs(x, gamma, residual, eps)
-    keep = torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or (residual is not None and residual.requires_grad))
-    return _RmsNorm.apply(x, gamma, residual, eps, keep)
+    if _wants_grad(x, gamma, residual):
+        return _RmsNorm.apply(x, gamma, residual, eps)
+    y, total, _, _ = _norm_forward(x, gamma, residual, eps, False)
+    return y if total is None else (y, total)
 
 
 def rms_norm_e4m3(x, gamma, residual=None, eps=1e-6, group=0):
@@ -167,18 +191,16 @@ def rms_norm_e4m3(x, gamma, residual=None, eps=1e-6, group=0):
     gamma = _norm_inputs(x, gamma, residual, eps)
     cols = x.shape[-1]
     _require(group in (0, 32, 64, 128) and (group == 0 or cols % group == 0), 'group must be 0, 32, 64 or 128 and divide the channels')
-    _require(not (torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or (residual is not None and residual.requires_grad))),
-             'rms_norm_e4m3 has no gradient: call it under torch.no_grad() or on detached tensors')
+    _no_grad('rms_norm_e4m3', x, gamma, residual)
+    rows = x.numel() // cols
     x2, x_ld = _rows(x)
-    rows = x2.shape[0]
     q = _fresh(x.shape, x, torch.float8_e4m3fn)
     scale = _fresh((*x.shape[:-1], cols // group if group else 1), x, torch.float32)
-    total = _fresh(x.shape, x, residual.dtype) if residual is not None else None
+    total = _fresh_like(residual) if residual is not None else None
     r2, r_ld = _rows(residual) if residual is not None else (None, 0)
     kind = _TYPES[x.dtype]
-    with _on(x):
-        check(lib.vc_rms_norm_e4m3(_p(x2), x_ld, _p(r2), r_ld, _p(gamma), _p(q), cols, _p(scale), _p(total), cols, eps, rows, cols, group, kind,
-                                   _TYPES[residual.dtype] if residual is not None else kind, _stream(x)), 'vc_rms_norm_e4m3')
+    _launch(lib.vc_rms_norm_e4m3, 'vc_rms_norm_e4m3', x, _p(x2), x_ld, _p(r2), r_ld, _p(gamma), _p(q), cols, _p(scale), _p(total), cols,
+            eps, rows, cols, group, kind, _TYPES[residual.dtype] if residual is not None else kind)
     return (q, scale) if residual is None else (q, scale, total)
 
 
@@ -213,22 +235,26 @@ def _conv_args(x, w, bias, initial, offsets, seqs, rows, silu):
     return a, x2
 
 
+def _conv_forward(x, w, bias, initial, offsets, plan, want_final):
+    seqs, rows, silu = plan
+    a, x2 = _conv_args(x, w, bias, initial, offsets, seqs, rows, silu)
+    y = _fresh_like(x)
+    final = _fresh((seqs, a.taps - 1, a.cols), x) if want_final else None
+    a.y, a.y_ld, a.final_state = _p(y), a.cols, _p(final)
+    _launch(lib.vc_causal_conv1d_fwd, 'vc_causal_conv1d_fwd', x, C.byref(a))
+    return (y, final) if want_final else y
+
+
 class _CausalConv1d(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, bias, initial, offsets, seqs, rows, silu, want_final):
-        a, x2 = _conv_args(x, w, bias, initial, offsets, seqs, rows, silu)
-        y = _fresh(x.shape, x)
-        final = _fresh((seqs, a.taps - 1, a.cols), x) if want_final else None
-        a.y, a.y_ld, a.final_state = _p(y), a.cols, _p(final)
-        with _on(x):
-            check(lib.vc_causal_conv1d_fwd(C.byref(a), _stream(x)), 'vc_causal_conv1d_fwd')
+    def forward(ctx, x, w, bias, initial, offsets, plan, want_final):
         ctx.save_for_backward(x, w, bias, initial, offsets)
-        ctx.plan = seqs, rows, silu
+        ctx.plan = plan
         ctx.set_materialize_grads(False)
-        return (y, final) if want_final else y
+        return _conv_forward(x, w, bias, initial, offsets, plan, want_final)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dfinal=None):
         x, w, bias, initial, offsets = ctx.saved_tensors
         seqs, rows, silu = ctx.plan
@@ -239,17 +265,16 @@ class _CausalConv1d(torch.autograd.Function):
         if dfinal is not None:
             dfinal = dfinal.contiguous()
         need = ctx.needs_input_grad
-        dx = _fresh(x.shape, x) if need[0] else None
-        dw = _fresh(w.shape, w) if need[1] else None
+        dx = _fresh_like(x) if need[0] else None
+        dw = _fresh_like(w) if need[1] else None
         dbias = _fresh(bias.shape, bias) if bias is not None and need[2] else None
         dinitial = _fresh(initial.shape, initial) if initial is not None and need[3] else None
         a.dy, a.dfinal, a.dx, a.dx_ld, a.dw, a.dbias, a.dinitial = _p(dy2), _p(dfinal), _p(dx), a.cols, _p(dw), _p(dbias), _p(dinitial)
         a.work_floats = lib.vc_causal_conv1d_bwd_work(C.byref(a))
         work = _fresh((a.work_floats,), w) if a.work_floats else None
         a.work = _p(work)
-        with _on(x):
-            check(lib.vc_causal_conv1d_bwd(C.byref(a), _stream(x)), 'vc_causal_conv1d_bwd')
-        return dx, dw, dbias, dinitial, None, None, None, None, None
+        _launch(lib.vc_causal_conv1d_bwd, 'vc_causal_conv1d_bwd', x, C.byref(a))
+        return dx, dw, dbias, dinitial, None, None, None
 
 
 def _conv_weights(x, w, bias, cols):
@@ -269,12 +294,8 @@ def causal_conv1d(x, w, bias=None, initial_state=None, seq_offsets=None, silu=Tr
         initial_state = _like(initial_state, x, 'initial_state', (seqs, w.shape[0] - 1, x.shape[-1])).contiguous()
     if seq_offsets is not None:
         seq_offsets = seq_offsets.contiguous()
-    return _CausalConv1d.apply(x, w, bias, initial_state, seq_offsets, seqs, rows, bool(silu), bool(return_final_state))
-
-
-def _no_grad(what, *tensors):
-    _require(not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors),
-             '%s has no gradient: call it under torch.no_grad() or on detached tensors', what)
+    args = x, w, bias, initial_state, seq_offsets, (seqs, rows, bool(silu)), bool(return_final_state)
+    return (_CausalConv1d.apply if _wants_grad(x, w, bias, initial_state) else _conv_forward)(*args)
 
 
 def causal_conv1d_step(x, state, w, bias=None, slots=None, silu=True):
@@ -292,10 +313,9 @@ def causal_conv1d_step(x, state, w, bias=None, slots=None, silu=True):
     _no_grad('causal_conv1d_step', x, state, w, bias)
     slots = _slots(slots, rows, state.shape[0], x)
     x2, x_ld = _rows(x)
-    y = _fresh(x.shape, x)
-    with _on(x):
-        check(lib.vc_causal_conv1d_step(_p(x2), x_ld, _p(state), _p(slots), _p(w), _p(bias), _p(y), cols, rows, state.shape[0], cols, w.shape[0],
-                                        _TYPES[x.dtype], int(silu), _stream(x)), 'vc_causal_conv1d_step')
+    y = _fresh_like(x)
+    _launch(lib.vc_causal_conv1d_step, 'vc_causal_conv1d_step', x, _p(x2), x_ld, _p(state), _p(slots), _p(w), _p(bias), _p(y), cols, rows,
+            state.shape[0], cols, w.shape[0], _TYPES[x.dtype], int(silu))
     return y
 
 
@@ -334,31 +354,35 @@ def _scan_args(x, dt, A, B, C_, D, z, dt_bias, initial, offsets, plan):
     return a, held
 
 
+def _scan_forward(x, dt, A, B, C_, D, z, dt_bias, initial, offsets, plan, want_final, keep=False):
+    a, held = _scan_args(x, dt, A, B, C_, D, z, dt_bias, initial, offsets, plan)
+    y = _fresh_like(x)
+    final = _fresh((plan[0], a.cols, a.states), A) if want_final else None
+    a.y, a.y_ld, a.final_state = _p(y), a.cols, _p(final)
+    saved = None
+    if keep:
+        a.saved_floats = lib.vc_selective_scan_saved(C.byref(a))
+        saved = _fresh((a.saved_floats,), A)
+        a.saved = _p(saved)
+    a.work_floats = lib.vc_selective_scan_fwd_work(C.byref(a))
+    work = _fresh((a.work_floats,), A) if a.work_floats > 0 else None
+    a.work = _p(work)
+    _launch(lib.vc_selective_scan_fwd, 'vc_selective_scan_fwd', x, C.byref(a))
+    out = (y, final) if want_final else y
+    return (out, saved) if keep else out
+
+
 class _SelectiveScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, dt, A, B, C_, D, z, dt_bias, initial, offsets, plan, want_final, keep):
-        a, held = _scan_args(x, dt, A, B, C_, D, z, dt_bias, initial, offsets, plan)
-        y = _fresh(x.shape, x)
-        final = _fresh((plan[0], a.cols, a.states), x, torch.float32) if want_final else None
-        a.y, a.y_ld, a.final_state = _p(y), a.cols, _p(final)
-        saved = None
-        if keep:
-            a.saved_floats = lib.vc_selective_scan_saved(C.byref(a))
-            saved = _fresh((a.saved_floats,), A)
-            a.saved = _p(saved)
-        a.work_floats = lib.vc_selective_scan_fwd_work(C.byref(a))
-        work = _fresh((a.work_floats,), A) if a.work_floats > 0 else None
-        a.work = _p(work)
-        with _on(x):
-            check(lib.vc_selective_scan_fwd(C.byref(a), _stream(x)), 'vc_selective_scan_fwd')
-        if keep:
-            ctx.save_for_backward(x, dt, A, B, C_, D, z, dt_bias, initial, offsets, saved)
-            ctx.plan = plan
-            ctx.set_materialize_grads(False)
-        return (y, final) if want_final else y
+    def forward(ctx, x, dt, A, B, C_, D, z, dt_bias, initial, offsets, plan, want_final):
+        out, saved = _scan_forward(x, dt, A, B, C_, D, z, dt_bias, initial, offsets, plan, want_final, True)
+        ctx.save_for_backward(x, dt, A, B, C_, D, z, dt_bias, initial, offsets, saved)
+        ctx.plan = plan
+        ctx.set_materialize_grads(False)
+        return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dfinal=None):
         x, dt, A, B, C_, D, z, dt_bias, initial, offsets, saved = ctx.saved_tensors
         a, held = _scan_args(x, dt, A, B, C_, D, z, dt_bias, initial, offsets, ctx.plan)
@@ -368,8 +392,8 @@ class _SelectiveScan(torch.autograd.Function):
         if dfinal is not None:
             dfinal = dfinal.contiguous()
         need = ctx.needs_input_grad
-        dx, ddt, dB, dC, dA = _fresh(x.shape, x), _fresh(x.shape, x), _fresh(B.shape, x), _fresh(C_.shape, x), _fresh(A.shape, A)
-        dz = _fresh(x.shape, x) if z is not None else None
+        dx, ddt, dB, dC, dA = _fresh_like(x), _fresh_like(x), _fresh_like(B), _fresh_like(C_), _fresh_like(A)
+        dz = _fresh_like(x) if z is not None else None
         dD = _fresh(D.shape, A) if D is not None else None
         dbias = _fresh(dt_bias.shape, A) if dt_bias is not None else None
         dinitial = _fresh(initial.shape, A) if initial is not None and need[8] else None
@@ -382,10 +406,9 @@ class _SelectiveScan(torch.autograd.Function):
         a.work_floats = lib.vc_selective_scan_bwd_work(C.byref(a))
         work = _fresh((a.work_floats,), A)
         a.work = _p(work)
-        with _on(x):
-            check(lib.vc_selective_scan_bwd(C.byref(a), _stream(x)), 'vc_selective_scan_bwd')
+        _launch(lib.vc_selective_scan_bwd, 'vc_selective_scan_bwd', x, C.byref(a))
         grads = (dx, ddt, dA, dB, dC, dD, dz, dbias, dinitial)
-        return tuple(g if n else None for g, n in zip(grads, need)) + (None,) * 4
+        return tuple(g if n else None for g, n in zip(grads, need)) + (None,) * 3
 
 
 def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, initial_state=None, seq_offsets=None, max_len=None, softplus=True, return_final_state=False):
@@ -405,11 +428,10 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, initial_state=N
         initial_state = _like(initial_state, x, 'initial_state', (seqs, *A.shape), torch.float32).contiguous()
     _require(max_len is None or max_len >= 0, 'max_len must not be negative')
     tensors = (x, dt, A, B, C, D, z, dt_bias, initial_state)
-    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
     if seq_offsets is not None:
         seq_offsets = seq_offsets.contiguous()
     plan = seqs, rows, int(max_len or 0), bool(softplus)
-    return _SelectiveScan.apply(*tensors, seq_offsets, plan, bool(return_final_state), keep)
+    return (_SelectiveScan.apply if _wants_grad(*tensors) else _scan_forward)(*tensors, seq_offsets, plan, bool(return_final_state))
 
 
 def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, slots=None, softplus=True):
@@ -426,9 +448,7 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, slo
     slots = _slots(slots, rows, state.shape[0], x)
     (x2, x_ld), (t2, t_ld), (b2, b_ld), (c2, c_ld) = _rows(x), _rows(dt), _rows(B, 2), _rows(C, 2)
     z2, z_ld = _rows(z) if z is not None else (None, 0)
-    y = _fresh(x.shape, x)
-    with _on(x):
-        check(lib.vc_selective_scan_step(_p(x2), x_ld, _p(t2), t_ld, _p(z2), z_ld, _p(b2), b_ld, _p(c2), c_ld, _p(A), _p(D), _p(dt_bias), _p(state), _p(slots),
-                                         _p(y), cols, rows, state.shape[0], cols, A.shape[1], B.shape[-2], _TYPES[x.dtype], int(softplus), _stream(x)),
-              'vc_selective_scan_step')
+    y = _fresh_like(x)
+    _launch(lib.vc_selective_scan_step, 'vc_selective_scan_step', x, _p(x2), x_ld, _p(t2), t_ld, _p(z2), z_ld, _p(b2), b_ld, _p(c2), c_ld,
+            _p(A), _p(D), _p(dt_bias), _p(state), _p(slots), _p(y), cols, rows, state.shape[0], cols, A.shape[1], B.shape[-2], _TYPES[x.dtype], int(softplus))
     return y
