@@ -14,31 +14,63 @@
 #include "vc_seq.h"
 
 constexpr int TILE = 16;
-constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f, LOG2E_REST = 1.92596299112661746887e-8f;     // log2 e = LOG2E + LOG2E_REST
 
 struct ScanK {
     vc_scan_args a; SeqMap m;
     int cg, nblk;                  // channels of a group; blocks that cover them
     int slots;                     // slots in all
+    // How the time axis is shared out: items are whole utterances (chunk = 0), or runs of `chunk` slots whatever utterances these belong to.
+    // In the second form a first pass works out what each run does to a state that enters it, h -> exp(A sum_delta) h + edge, and the main pass begins
+    // with the sum of what the runs before it hand on.  `cut` marks the runs that hand on nothing of what enters (an utterance begins or ends there).
+    int items, chunk;
+    float *edge, *sum_delta; int* cut;             // [items][cols][states], [items][cols], [items]
     float *part, *dapart, *chpart; // backward: partial sums of dB / dC, dA, and of dD and ddt_bias
 };
 
 __device__ __forceinline__ int slot_base(const SeqMap& m, int s) { return seq_begin(m, s) / TILE + s; }
 
+// the same in all lanes, and the compiler is to know it: addresses of rows then take a scalar base
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// The utterance that the slots being walked belong to
+struct Cursor {
+    const SeqMap& m;
+    int s, base, next, begin, end, tiles;
+    __device__ __forceinline__ explicit Cursor(const SeqMap& map) : m(map) {}
+    __device__ __forceinline__ void load(int i) {
+        s = uniform(i); begin = uniform(seq_begin(m, s)); end = uniform(seq_end(m, s, begin)); base = begin / TILE + s; tiles = (end - begin + TILE - 1) / TILE;
+        next = s + 1 < m.n_seqs ? uniform(slot_base(m, s + 1)) : 0x7fffffff;
+    }
+    __device__ __forceinline__ void find(int q) {
+        int lo = 0, hi = m.n_seqs - 1;
+        while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (slot_base(m, mid) <= q) lo = mid; else hi = mid - 1; }
+        load(lo);
+    }
+};
+// the slots of an item
+__device__ __forceinline__ void item_slots(const ScanK& k, int item, int& q0, int& q1) {
+    if (k.chunk) { q0 = item * k.chunk; q1 = min(q0 + k.chunk, k.slots); }
+    else { q0 = slot_base(k.m, item); q1 = item + 1 < k.m.n_seqs ? slot_base(k.m, item + 1) : k.slots; }
+}
+
 template <int I, int N, class F> __device__ __forceinline__ void static_for(F&& f) {
     if constexpr (I < N) { f(std::integral_constant<int, I>()); static_for<I + 1, N>(f); }
 }
+// dpp_read where every lane has a source: nothing to keep of the destination's old value, which lets the move become part of the instruction that uses it
+template <int CTRL> __device__ __forceinline__ float dpp_all(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
 // lane i's value of the L lanes that share a channel
 template <int L, int I> __device__ __forceinline__ float from_lane(float v) {
-    if constexpr (L == 4) return dpp_read<I * 0x55>(v);          // quad_perm [i,i,i,i]
-    else return dpp_read<0x150 + I>(v);                          // row_newbcast:i
+    if constexpr (L == 4) return dpp_all<I * 0x55>(v);          // quad_perm [i,i,i,i]
+    else return dpp_all<0x150 + I>(v);                          // row_newbcast:i
 }
 // one step of sums_by_row: rows kept by bit BIT of the lane, the others handed to the lane that keeps them
 template <int CTRL, int N> __device__ __forceinline__ void halve(float (&v)[N], bool up) {
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
         const float keep = up ? v[i + N / 2] : v[i], send = up ? v[i] : v[i + N / 2];
-        v[i] = keep + dpp_read<CTRL>(send);
+        v[i] = keep + dpp_all<CTRL>(send);
     }
 }
 // v[i] = this lane's share of row i; lane j gets the sum of row j over the L lanes (L - 1 additions in place of L log2 L)
@@ -66,14 +98,18 @@ template <int L> __device__ __forceinline__ float sums_by_row(float (&v)[L], int
 // sum over the L lanes of a channel, in all of them
 template <int L> __device__ __forceinline__ float channel_sum(float v) {
     if constexpr (L == 16) return row16_sum(v);
-    v += dpp_read<0xB1>(v);
-    return v + dpp_read<0x4E>(v);
+    v += dpp_all<0xB1>(v);
+    return v + dpp_all<0x4E>(v);
 }
 
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|) in (0, 1], and its slope.  log(1 + e) = 2 atanh(e / (2 + e)) by its series: the argument is at
 // most 1/3, seven terms leave 1.4e-8, and a small e keeps all its bits (a logarithm of the rounded 1 + e would lose them: steps of 0.001 are ordinary here)
 __device__ __forceinline__ float softplus(float v, float& slope) {
-    const float e = expf(-fabsf(v));
+    // e^-|v| with what the product with log2 e rounds off put back: the exponential alone would be off by |v| 2^-24 of itself
+    const float av = fabsf(v), t = -av * LOG2E, lo = fmaf(-av, LOG2E, -t) - av * LOG2E_REST;
+    float e = exp2_fast(t);
+    e = fmaf(e, lo * LN2, e);
     const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
     float p = 1.f / 13.f;
     p = fmaf(p, q, 1.f / 11.f); p = fmaf(p, q, 1.f / 9.f); p = fmaf(p, q, 1.f / 7.f); p = fmaf(p, q, 1.f / 5.f); p = fmaf(p, q, 1.f / 3.f); p = fmaf(p, q, 1.f);
@@ -81,19 +117,60 @@ __device__ __forceinline__ float softplus(float v, float& slope) {
     slope = v >= 0.f ? r : e * r;
     return fmaxf(v, 0.f) + 2.f * s * p + (v - v);                // v - v: a NaN stays one (fmaxf drops it)
 }
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Rows [row0, row0 + nr) of B or C (group g) as fp32 into dst[TILE][NP]: four lanes a row, NP / 4 states each; zeros where there is no row or state
-template <class T, int NP> __device__ __forceinline__ void stage_states(const T* src, int64_t ld, int row0, int nr, int states, float* dst, int lane) {
-    constexpr int W = NP / 4;
-    const int r = lane >> 2, n = (lane & 3) * W;
-    float f[W];
+// A tensor of rows as a lane uses it: through a buffer descriptor of the tile's rows, whose bounds check gives zeros for the rows that a short tile
+// lacks (where rows do not overlap) and drops stores to them, and those of lanes without a channel.  Host code keeps row strides within MAX_LD: the
+// offsets in a tile fit 31 bits.
+constexpr int64_t MAX_LD = 1 << 25;
+template <class T, int L> struct Rows {
+    const T* p; int ld, width; unsigned at, step;
+    __device__ __forceinline__ Rows(const void* base, int64_t stride, int cols, int c, int j, bool ok = true)
+        : p((const T*)base), ld((int)stride), width(cols * (int)sizeof(T)),
+          at(ok ? (unsigned)(j * (int)stride + c) * (unsigned)sizeof(T) : 0x80000000u), step((unsigned)(L * (int)stride) * (unsigned)sizeof(T)) {}
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile(int row0, int nr) const {
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(p + (int64_t)row0 * ld), 0, (nr - 1) * ld * (int)sizeof(T) + width, 0x00020000);
+    }
+    // rows b * L + j of a tile
+    template <int NB> __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t t, T (&v)[NB]) const {
 #pragma unroll
-    for (int i = 0; i < W; ++i) f[i] = 0.f;
-    if (r < nr) load_some<T, W>(src + (int64_t)(row0 + r) * ld + n, f, states - n);
+        for (int b = 0; b < NB; ++b) {
+            if constexpr (sizeof(T) == 4) v[b] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(t, at + b * step, 0, 0));
+            else v[b] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(t, at + b * step, 0, 0));
+        }
+    }
+    template <int NB> __device__ __forceinline__ void load(int row0, int nr, T (&v)[NB]) const { load(tile(row0, nr), v); }
+    __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t t, int b, float f) const {
+        if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, f), t, at + b * step, 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (T)f), t, at + b * step, 0, 0);
+    }
+    // rows from `first` on, one after the other by the lanes of a channel
+    __device__ __forceinline__ void clear(int first, int rows, int c, int j) const {
+        if (at != 0x80000000u) for (int r = first + j; r < rows; r += L) ((T*)p)[(int64_t)r * ld + c] = (T)0.f;
+    }
+};
+// A tile of B or C (a group's states contiguous): four lanes a row, NP / 4 states each, in registers until the tile before it is done with
+template <class T, int NP> struct States {
+    static constexpr int W = NP / 4;
+    const T* p; int ld, states, r, n;
+    __device__ __forceinline__ States(const void* base, int64_t stride, int g, int count, int lane) : p((const T*)base + g * count), ld((int)stride), states(count), r(lane >> 2), n((lane & 3) * W) {}
+    __device__ __forceinline__ void load(int row0, int nr, T (&v)[W]) const {
+        const char* base = (const char*)(p + (int64_t)row0 * ld);
+        const unsigned row = (unsigned)(min(r, nr - 1) * ld) * (unsigned)sizeof(T);      // a short tile's missing rows read its last one
+        if (states == NP) {
+            const Pack<T, W> q = *(const Pack<T, W>*)(base + (row + n * (unsigned)sizeof(T)));
 #pragma unroll
-    for (int i = 0; i < W; ++i) dst[r * NP + n + i] = f[i];
-}
+            for (int i = 0; i < W; ++i) v[i] = q.v[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = *(const T*)(base + (row + min(n + i, states - 1) * (unsigned)sizeof(T)));
+        }
+    }
+    // as fp32 into dst[TILE][NP], zeros where there is no row or state
+    __device__ __forceinline__ void stage(const T (&v)[W], int nr, float* dst) const {
+#pragma unroll
+        for (int i = 0; i < W; ++i) dst[r * NP + n + i] = r < nr && n + i < states ? (float)v[i] : 0.f;
+    }
+};
 // LDS of one wave: what its lanes wrote is there for all of them (the hardware keeps a wave's LDS accesses in order; this keeps the compiler's)
 __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -104,7 +181,7 @@ __device__ __forceinline__ void wave_lds_fence() {
 template <int L, int NS> struct Lane {
     int lane, wave, j, c, n0, nn; bool ok; int g;
     __device__ __forceinline__ Lane(const ScanK& k, int waves, int blk) {
-        lane = threadIdx.x & 63; wave = threadIdx.x >> 6;
+        lane = threadIdx.x & 63; wave = uniform(threadIdx.x >> 6);
         j = lane % L;
         g = blk / k.nblk;
         const int cw = 64 / L, cb = (blk - g * k.nblk) * waves * cw + wave * cw + lane / L;
@@ -121,4 +198,8 @@ template <int NS> __device__ __forceinline__ void load_state(const float* p, flo
     ((states) <= 8 ? F<T, 4, 2>(__VA_ARGS__) : (states) <= 16 ? F<T, 4, 4>(__VA_ARGS__) : (states) <= 32 ? F<T, 16, 2>(__VA_ARGS__) : F<T, 16, 4>(__VA_ARGS__))
 static inline int scan_lanes(int states) { return states <= 16 ? 4 : 16; }
 static inline int scan_padded(int states) { return states <= 8 ? 8 : states <= 16 ? 16 : states <= 32 ? 32 : 64; }
-int scan_setup(const char* who, const vc_scan_args* a, bool bwd, ScanK* k);
+int scan_setup(const char* who, const vc_scan_args* a, int waves, ScanK* k);
+int64_t scan_edge_floats(const ScanK& k);                        // of edge, sum_delta and cut
+void scan_edge_place(ScanK* k, float* work);
+// edge[r]: what run r hands on -> what enters it from the runs before it (behind it where !FORWARD)
+int scan_carry(const ScanK& k, bool forward, hipStream_t s);

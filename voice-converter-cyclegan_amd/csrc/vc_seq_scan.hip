@@ -1,71 +1,205 @@
 // vc_seq_scan.hip -- selective state space scan: prompts and single frames (vc_seq_scan.h says how the work is laid out).
 #include "vc_seq_scan.h"
+#include <cstdlib>
 
 constexpr int FWD_WAVES = 4;
 
-// One block walks one utterance for FWD_WAVES * 64 / L channels, tile by tile.
+// First pass of a split axis: what each run hands on.  Only rows from the last utterance's beginning on matter.
+template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_edge_kernel(const ScanK k) {
+    constexpr int NP = L * NS, NB = TILE / L;
+    __shared__ float lds[FWD_WAVES][TILE * NP];
+    const vc_scan_args& a = k.a;
+    const int nblk = a.groups * k.nblk, item = blockIdx.x / nblk, blk = blockIdx.x - item * nblk;
+    const Lane<L, NS> w(k, FWD_WAVES, blk);
+    const int c = w.c, j = w.j, n0 = w.n0, nn = w.nn;
+    const Rows<T, L> X(a.x, a.x_ld, a.cols, c, j), DT(a.dt, a.dt_ld, a.cols, c, j);
+    const States<T, NP> B(a.B, a.b_ld, w.g, a.states, w.lane);
+    float A2[NS], h[NS];
+    load_state<NS>(a.A + (int64_t)c * a.states + n0, A2, nn);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) { A2[i] *= LOG2E; h[i] = 0.f; }
+    const float bias = a.dt_bias ? a.dt_bias[c] : 0.f;
+    int q0, q1;
+    item_slots(k, item, q0, q1);
+    Cursor cur(k.m);
+    cur.find(q1 - 1);
+    const bool cut = cur.base >= q0;                             // an utterance begins in this run
+    if (cut && a.initial) load_state<NS>(a.initial + ((int64_t)cur.s * a.cols + c) * a.states + n0, h, nn);
+    float* Bs = lds[w.wave];
+    float sd = 0.f;
+    const int k0 = max(q0 - cur.base, 0), k1 = min(cur.tiles, q1 - cur.base);
+    T xr[NB], tr[NB], br[NP / 4];
+    auto fetch = [&](int kt) {
+        const int row0 = cur.begin + kt * TILE, nr = min(TILE, cur.end - row0);
+        X.load(row0, nr, xr); DT.load(row0, nr, tr); B.load(row0, nr, br);
+    };
+    if (k0 < k1) fetch(k0);
+    for (int kt = k0; kt < k1; ++kt) {
+        const int nr = min(TILE, cur.end - cur.begin - kt * TILE);
+        B.stage(br, nr, Bs);
+        float delta[NB], dtx[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            float slope;
+            const float v = (float)tr[b] + bias, d = a.softplus ? softplus(v, slope) : v;
+            delta[b] = b * L + j < nr ? d : 0.f;
+            dtx[b] = b * L + j < nr ? d * (float)xr[b] : 0.f;
+            sd += delta[b];
+        }
+        if (kt + 1 < k1) fetch(kt + 1);
+        wave_lds_fence();
+        static_for<0, NB>([&](auto b) {
+            static_for<0, L>([&](auto i) {
+                const float dl = from_lane<L, i>(delta[b]), dx = from_lane<L, i>(dtx[b]);
+                const float* Br = Bs + (b * L + i) * NP + n0;
+#pragma unroll
+                for (int e = 0; e < NS; ++e) h[e] = fmaf(exp2_fast(dl * A2[e]), h[e], dx * Br[e]);
+            });
+        });
+        wave_lds_fence();
+    }
+    sd = channel_sum<L>(sd);
+    if (w.ok) {
+        store_some<float, NS>(k.edge + ((int64_t)item * a.cols + c) * a.states + n0, h, nn);
+        if (j == 0) k.sum_delta[(int64_t)item * a.cols + c] = sd;
+    }
+    if (blk == 0 && threadIdx.x == 0) k.cut[item] = cut;
+}
+
+// Second pass of a split axis: from what every run hands on to what enters it, run by run for one state a thread.  Reads ahead: the chain is one
+// multiply-add a run.
+__global__ __launch_bounds__(64) void scan_carry_kernel(const ScanK k, bool forward) {
+    constexpr int AHEAD = 16;
+    const vc_scan_args& a = k.a;
+    const int64_t n = (int64_t)a.cols * a.states, i = (int64_t)blockIdx.x * 64 + threadIdx.x;
+    if (i >= n) return;
+    const int c = (int)(i / a.states);
+    const float A2 = a.A[i] * LOG2E;
+    float h = 0.f;
+    for (int r0 = 0; r0 < k.items; r0 += AHEAD) {
+        float e[AHEAD], sd[AHEAD]; int cut[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int at = min(r0 + u, k.items - 1), r = forward ? at : k.items - 1 - at;
+            e[u] = k.edge[r * n + i]; sd[u] = k.sum_delta[(int64_t)r * a.cols + c]; cut[u] = k.cut[r];
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (r0 + u >= k.items) break;
+            k.edge[(forward ? r0 + u : k.items - 1 - r0 - u) * n + i] = h;
+            h = cut[u] ? e[u] : fmaf(exp2_fast(A2 * sd[u]), h, e[u]);
+        }
+    }
+}
+int scan_carry(const ScanK& k, bool forward, hipStream_t s) {
+    hipLaunchKernelGGL(scan_carry_kernel, dim3((unsigned)(((int64_t)k.a.cols * k.a.states + 63) / 64)), dim3(64), 0, s, k, forward);
+    VC_HIP(hipGetLastError());
+    return 0;
+}
+
+template <int NS> struct RowPair {                                // B and C of two rows, a lane's states
+    float b[2][NS], c[2][NS];
+    __device__ __forceinline__ void read(const float* pb, const float* pc, int stride) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < NS; ++e) { b[u][e] = pb[u * stride + e]; c[u][e] = pc[u * stride + e]; }
+    }
+};
+
+// One block walks the slots of one item for FWD_WAVES * 64 / L channels.  The next tile's rows are on their way while a tile is worked on.
 template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_fwd_kernel(const ScanK k) {
     constexpr int NP = L * NS, NB = TILE / L;
     __shared__ float lds[FWD_WAVES][2][TILE * NP];
     const vc_scan_args& a = k.a;
-    const int nblk = a.groups * k.nblk, s = blockIdx.x / nblk, blk = blockIdx.x - s * nblk;
+    const int nblk = a.groups * k.nblk, item = blockIdx.x / nblk, blk = blockIdx.x - item * nblk;
     const Lane<L, NS> w(k, FWD_WAVES, blk);
     const int c = w.c, j = w.j, n0 = w.n0, nn = w.nn;
-    const T *x = (const T*)a.x + c, *dt = (const T*)a.dt + c, *z = a.z ? (const T*)a.z + c : nullptr;
-    const T *B = (const T*)a.B + w.g * a.states, *C = (const T*)a.C + w.g * a.states;
-    T* y = (T*)a.y + c;
-    if (s == k.m.n_seqs) {                                       // rows behind the last utterance
-        if (w.ok) for (int r = seq_tail(k.m) + j; r < k.m.rows; r += L) y[(int64_t)r * a.y_ld] = (T)0.f;
+    const Rows<T, L> Y(a.y, a.y_ld, a.cols, c, j, w.ok);
+    if (item == k.items) {                                       // rows behind the last utterance
+        Y.clear(seq_tail(k.m), k.m.rows, c, j);
         return;
     }
+    const bool has_z = a.z != nullptr;
+    const Rows<T, L> X(a.x, a.x_ld, a.cols, c, j), DT(a.dt, a.dt_ld, a.cols, c, j), Z(has_z ? a.z : a.x, has_z ? a.z_ld : a.x_ld, a.cols, c, j);
+    const States<T, NP> B(a.B, a.b_ld, w.g, a.states, w.lane), C(a.C, a.c_ld, w.g, a.states, w.lane);
     float A2[NS], h[NS];
     load_state<NS>(a.A + (int64_t)c * a.states + n0, A2, nn);
 #pragma unroll
     for (int i = 0; i < NS; ++i) { A2[i] *= LOG2E; h[i] = 0.f; }
     const float Dc = a.D ? a.D[c] : 0.f, bias = a.dt_bias ? a.dt_bias[c] : 0.f;
-    const int begin = seq_begin(k.m, s), end = seq_end(k.m, s, begin), base = slot_base(k.m, s);
-    const int64_t hs = ((int64_t)s * a.cols + c) * a.states + n0;
-    if (a.initial) load_state<NS>(a.initial + hs, h, nn);
+    int q0, q1;
+    item_slots(k, item, q0, q1);
+    Cursor cur(k.m);
+    if (k.chunk) cur.find(q0); else cur.load(item);
+    if (k.chunk && q0 > cur.base) load_state<NS>(k.edge + ((int64_t)item * a.cols + c) * a.states + n0, h, nn);
     float *Bs = lds[w.wave][0], *Cs = lds[w.wave][1];
-    for (int row0 = begin, q = base; row0 < end; row0 += TILE, ++q) {
-        const int nr = min(TILE, end - row0);
-        if (a.saved && w.ok) store_some<float, NS>(a.saved + ((int64_t)q * a.cols + c) * a.states + n0, h, nn);
-        stage_states<T, NP>(B, a.b_ld, row0, nr, a.states, Bs, w.lane);
-        stage_states<T, NP>(C, a.c_ld, row0, nr, a.states, Cs, w.lane);
-        float delta[NB], dtx[NB], gate[NB], skip[NB];
+    for (int q = q0; q < q1;) {                                  // the utterances of the item
+        const int64_t hs = ((int64_t)cur.s * a.cols + c) * a.states + n0;
+        const int k0 = max(q - cur.base, 0), k1 = min(cur.tiles, q1 - cur.base);
+        if (q == cur.base) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const bool ok = b * L + j < nr;
-            const int64_t r = row0 + b * L + j;
-            const float xv = ok ? (float)x[r * a.x_ld] : 0.f, zv = ok && z ? (float)z[r * a.z_ld] : 0.f;
-            const float v = (ok ? (float)dt[r * a.dt_ld] : 0.f) + bias;
-            float slope;
-            const float d = a.softplus ? softplus(v, slope) : v;
-            delta[b] = ok ? d : 0.f;
-            dtx[b] = delta[b] * xv;
-            gate[b] = z ? zv * sigmoid_acc(zv) : 1.f;
-            skip[b] = Dc * xv;
+            for (int i = 0; i < NS; ++i) h[i] = 0.f;
+            if (a.initial) load_state<NS>(a.initial + hs, h, nn);
         }
-        wave_lds_fence();
-        static_for<0, NB>([&](auto b) {
-            float acc[L];
-            static_for<0, L>([&](auto i) {
-                const float dl = from_lane<L, i>(delta[b]), dx = from_lane<L, i>(dtx[b]);
-                const float *Br = Bs + (b * L + i) * NP + n0, *Cr = Cs + (b * L + i) * NP + n0;
-                float sum = 0.f;
+        T xr[NB], tr[NB], zr[NB], br[NP / 4], cr[NP / 4];
+        auto fetch = [&](int kt) {
+            const int row0 = cur.begin + kt * TILE, nr = min(TILE, cur.end - row0);
+            X.load(row0, nr, xr); DT.load(row0, nr, tr);
+            if (has_z) Z.load(row0, nr, zr);
+            B.load(row0, nr, br); C.load(row0, nr, cr);
+        };
+        if (k0 < k1) fetch(k0);
+        for (int kt = k0; kt < k1; ++kt) {
+            const int row0 = cur.begin + kt * TILE, nr = min(TILE, cur.end - row0);
+            if (a.saved && w.ok) store_some<float, NS>(a.saved + ((int64_t)(cur.base + kt) * a.cols + c) * a.states + n0, h, nn);
+            B.stage(br, nr, Bs); C.stage(cr, nr, Cs);
+            float delta[NB], dtx[NB], gate[NB], skip[NB];
 #pragma unroll
-                for (int e = 0; e < NS; ++e) {
-                    h[e] = fmaf(exp2_fast(dl * A2[e]), h[e], dx * Br[e]);
-                    sum = fmaf(Cr[e], h[e], sum);
-                }
-                acc[i] = sum;
+            for (int b = 0; b < NB; ++b) {
+                float slope;
+                const float v = (float)tr[b] + bias, d = a.softplus ? softplus(v, slope) : v, xv = (float)xr[b];
+                delta[b] = b * L + j < nr ? d : 0.f;
+                dtx[b] = b * L + j < nr ? d * xv : 0.f;
+                gate[b] = has_z ? (float)zr[b] * sigmoid_acc((float)zr[b]) : 1.f;
+                skip[b] = Dc * xv;
+            }
+            if (kt + 1 < k1) fetch(kt + 1);
+            const auto yt = Y.tile(row0, nr);
+            wave_lds_fence();
+            RowPair<NS> bc[2];
+            bc[0].read(Bs + n0, Cs + n0, NP);
+            static_for<0, NB>([&](auto b) {
+                float acc[L];
+                static_for<0, L / 2>([&](auto ii) {
+                    constexpr int i = 2 * ii, t = b * L + i;
+                    // the next two rows' B and C are fetched before these two are worked on; left alone, the scheduler asks for them when they are needed
+                    if constexpr (t + 2 < TILE) bc[(t / 2 + 1) & 1].read(Bs + (t + 2) * NP + n0, Cs + (t + 2) * NP + n0, NP);
+                    __builtin_amdgcn_sched_barrier(0);
+                    const RowPair<NS>& r = bc[(t / 2) & 1];
+                    const float dl[2] = {from_lane<L, i>(delta[b]), from_lane<L, i + 1>(delta[b])}, dx[2] = {from_lane<L, i>(dtx[b]), from_lane<L, i + 1>(dtx[b])};
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        float sum = 0.f;
+#pragma unroll
+                        for (int e = 0; e < NS; ++e) {
+                            h[e] = fmaf(exp2_fast(dl[u] * A2[e]), h[e], dx[u] * r.b[u][e]);
+                            sum = fmaf(r.c[u][e], h[e], sum);
+                        }
+                        acc[i + u] = sum;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+                const float out = (sums_by_row<L>(acc, j) + skip[b]) * gate[b];
+                Y.store(yt, b, out);
             });
-            const float out = (sums_by_row<L>(acc, j) + skip[b]) * gate[b];
-            if (w.ok && b * L + j < nr) y[(int64_t)(row0 + b * L + j) * a.y_ld] = (T)out;
-        });
-        wave_lds_fence();
+            wave_lds_fence();
+        }
+        if (a.final_state && w.ok && (cur.tiles ? k0 < cur.tiles && k1 == cur.tiles : q == cur.base)) store_some<float, NS>(a.final_state + hs, h, nn);
+        if (cur.next >= q1) break;
+        q = max(cur.next, q + 1);
+        cur.load(cur.s + 1);
     }
-    if (a.final_state && w.ok) store_some<float, NS>(a.final_state + hs, h, nn);
 }
 
 struct ScanStepArgs {
@@ -100,41 +234,82 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_st
     if (j == 0) *y = (T)(a.z ? sum * (z * sigmoid_acc(z)) : sum);
 }
 
-int scan_setup(const char* who, const vc_scan_args* a, bool bwd, ScanK* k) {
+// Whole utterances where these fill the card, else runs of slots.  A run costs its first pass on top, about as much again as 0.75 of the main pass, so
+// runs are for axes that are long beside the number of channels and utterances.
+int scan_setup(const char* who, const vc_scan_args* a, int waves, ScanK* k) {
     VC_ARG(a, "%s: null pointer", who);
     VC_ARG(seq_type_ok(a->type), "%s: type must be VC_F32, VC_BF16 or VC_F16", who);
     VC_ARG(a->states >= 1 && a->states <= 64, "%s: 1 to 64 states, got %d", who, a->states);
     VC_ARG(a->cols > 0 && a->groups > 0 && a->cols % a->groups == 0, "%s: groups (%d) must divide cols (%d)", who, a->groups, a->cols);
     VC_ARG(a->rows >= 0 && a->n_seqs > 0 && a->rows + (int64_t)TILE * a->n_seqs < (1LL << 31), "%s: bad sizes (rows %lld, n_seqs %d)", who, (long long)a->rows, a->n_seqs);
     VC_ARG(a->offsets || a->rows % a->n_seqs == 0, "%s: without offsets the rows divide into n_seqs equal utterances", who);
+    for (int64_t ld : {a->x_ld, a->dt_ld, a->z ? a->z_ld : 0, a->b_ld, a->c_ld, a->y ? a->y_ld : 0, a->dy ? a->dy_ld : 0})
+        VC_ARG(ld >= 0 && ld <= MAX_LD && a->cols <= MAX_LD, "%s: row strides lie between 0 and 2^25 elements", who);
+    if (a->rows > 1) {
+        VC_ARG(!a->y || a->y_ld >= a->cols, "%s: rows of y overlap", who);
+        VC_ARG(!a->dx || (a->dx_ld >= a->cols && a->dx_ld <= MAX_LD && a->ddt_ld >= a->cols && a->ddt_ld <= MAX_LD), "%s: row strides of dx and ddt lie between cols and 2^25", who);
+        VC_ARG(!a->dz || (a->dz_ld >= a->cols && a->dz_ld <= MAX_LD), "%s: row strides of dz lie between cols and 2^25", who);
+        VC_ARG(!a->dB || std::min(a->db_ld, a->dc_ld) >= (int64_t)a->groups * a->states, "%s: rows of dB or dC overlap", who);
+    }
+    *k = ScanK{};
     k->a = *a;
     k->m = SeqMap{a->offsets, (int)a->rows, a->n_seqs, (int)(a->rows / a->n_seqs)};
     k->cg = a->cols / a->groups;
     k->slots = (int)(a->rows / TILE) + a->n_seqs;
+    const int per = waves * 64 / scan_lanes(a->states);          // channels of a block
+    k->nblk = (k->cg + per - 1) / per;
+    const int64_t row_waves = (int64_t)a->groups * ((k->cg + 64 / scan_lanes(a->states) - 1) / (64 / scan_lanes(a->states)));      // waves that a frame's channels fill
+    static const int T1 = getenv("SC_T1") ? atoi(getenv("SC_T1")) : 512, T2 = getenv("SC_T2") ? atoi(getenv("SC_T2")) : 2048;
+    const int64_t longest = !a->offsets ? k->m.len : a->max_len > 0 ? a->max_len : a->rows;
+    // utterances that run side by side for as long as the longest lasts
+    const int64_t side = longest > 0 ? std::max<int64_t>(1, a->rows / longest) : a->n_seqs;
+    k->items = a->n_seqs; k->chunk = 0;
+    if (side * row_waves < T1 && longest >= 8 * TILE) {
+        const int64_t want = std::max<int64_t>(1, T2 / row_waves);
+        k->chunk = (int)std::max<int64_t>(4, (k->slots + want - 1) / want);
+        k->items = (k->slots + k->chunk - 1) / k->chunk;
+        if (k->items == 1) { k->items = a->n_seqs; k->chunk = 0; }
+    }
     return 0;
 }
+int64_t scan_edge_floats(const ScanK& k) { return k.chunk ? (int64_t)k.items * ((int64_t)k.a.cols * (k.a.states + 1) + 1) : 0; }
+void scan_edge_place(ScanK* k, float* work) {
+    k->edge = work;
+    k->sum_delta = work + (int64_t)k->items * k->a.cols * k->a.states;
+    k->cut = (int*)(k->sum_delta + (int64_t)k->items * k->a.cols);
+}
 extern "C" int64_t vc_selective_scan_saved(const vc_scan_args* a) {
-    ScanK k; if (scan_setup("vc_selective_scan_saved", a, false, &k)) return VC_E_ARG;
+    ScanK k; if (scan_setup("vc_selective_scan_saved", a, FWD_WAVES, &k)) return VC_E_ARG;
     return (int64_t)k.slots * a->cols * a->states;
 }
-extern "C" int64_t vc_selective_scan_fwd_work(const vc_scan_args* a) { ScanK k; return scan_setup("vc_selective_scan_fwd_work", a, false, &k) ? VC_E_ARG : 0; }
+extern "C" int64_t vc_selective_scan_fwd_work(const vc_scan_args* a) {
+    ScanK k; if (scan_setup("vc_selective_scan_fwd_work", a, FWD_WAVES, &k)) return VC_E_ARG;
+    return scan_edge_floats(k);
+}
 
 template <class T, int L, int NS> static int scan_fwd_l(const ScanK& k, hipStream_t s) {
-    const int64_t blocks = (int64_t)k.a.groups * k.nblk * (k.m.n_seqs + (k.a.zero_tail && k.m.off ? 1 : 0));
+    const int64_t per = (int64_t)k.a.groups * k.nblk, blocks = per * (k.items + (k.a.zero_tail && k.m.off ? 1 : 0));
     VC_ARG(blocks < (1LL << 31), "vc_selective_scan_fwd: too many utterances and channels for one launch");
+    if (k.chunk) {
+        hipLaunchKernelGGL((scan_edge_kernel<T, L, NS>), dim3((unsigned)(per * k.items)), dim3(64 * FWD_WAVES), 0, s, k);
+        VC_CHECK(scan_carry(k, true, s));
+    }
     hipLaunchKernelGGL((scan_fwd_kernel<T, L, NS>), dim3((unsigned)blocks), dim3(64 * FWD_WAVES), 0, s, k);
     VC_HIP(hipGetLastError());
     return 0;
 }
 template <class T> static int scan_fwd_t(const ScanK& k, hipStream_t s) { return SCAN_LAYOUT(T, k.a.states, scan_fwd_l, k, s); }
 extern "C" int vc_selective_scan_fwd(const vc_scan_args* a, void* stream) {
-    ScanK k{}; VC_CHECK(scan_setup("vc_selective_scan_fwd", a, false, &k));
+    ScanK k; VC_CHECK(scan_setup("vc_selective_scan_fwd", a, FWD_WAVES, &k));
     VC_ARG(a->A && (a->rows == 0 || (a->x && a->dt && a->B && a->C && a->y)), "vc_selective_scan_fwd: null pointer");
     VC_ARG(!a->final_state || a->final_state != a->initial, "vc_selective_scan_fwd: final_state may not be initial");
-    if (a->saved && a->saved_floats < vc_selective_scan_saved(a)) { vc_set_error("vc_selective_scan_fwd: saved is too small"); return VC_E_NOMEM; }
+    if (a->saved && a->saved_floats < (int64_t)k.slots * a->cols * a->states) { vc_set_error("vc_selective_scan_fwd: saved is too small"); return VC_E_NOMEM; }
+    if (scan_edge_floats(k) > 0 && (!a->work || a->work_floats < scan_edge_floats(k))) {
+        vc_set_error("vc_selective_scan_fwd: work is too small (%lld floats needed)", (long long)scan_edge_floats(k));
+        return VC_E_NOMEM;
+    }
+    if (k.chunk) scan_edge_place(&k, a->work);
     if (a->rows == 0 && !a->final_state) return 0;
-    const int per = FWD_WAVES * 64 / scan_lanes(a->states);
-    k.nblk = (k.cg + per - 1) / per;
     return SEQ_TYPES(a->type, scan_fwd_t, k, (hipStream_t)stream);
 }
 

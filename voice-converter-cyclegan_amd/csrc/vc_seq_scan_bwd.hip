@@ -6,6 +6,13 @@
 
 template <int L> constexpr int BWD_WAVES = L == 4 ? 8 : 4;      // LDS: B and C of each wave, and its share of dB and dC
 
+template <int NS> struct Row {                                    // B and C of a row, a lane's states
+    float b[NS], c[NS];
+    __device__ __forceinline__ void read(const float* pb, const float* pc) {
+#pragma unroll
+        for (int e = 0; e < NS; ++e) { b[e] = pb[e]; c[e] = pc[e]; }
+    }
+};
 // sum over the channels of a wave of its 2 NS values: the first steps hand one half of the values to the other half of the lanes.
 template <int N> __device__ __forceinline__ void across_32(float (&v)[N]) {
 #pragma unroll
@@ -61,90 +68,190 @@ template <int L, int NS> __device__ __forceinline__ float gather_item(const floa
     }
 }
 
+// First pass of a split axis: what each run hands on to the one before it.  Only rows up to the end of the run's first utterance matter.
+constexpr int EDGE_WAVES = 4;
+template <class T, int L, int NS> __global__ __launch_bounds__(64 * EDGE_WAVES) void scan_bwd_edge_kernel(const ScanK k, int nblk1) {
+    constexpr int NP = L * NS, NB = TILE / L;
+    __shared__ float lds[EDGE_WAVES][TILE * NP];
+    const vc_scan_args& a = k.a;
+    const int nblk = a.groups * nblk1, item = blockIdx.x / nblk, blk = blockIdx.x - item * nblk;
+    ScanK kk = k; kk.nblk = nblk1;
+    const Lane<L, NS> w(kk, EDGE_WAVES, blk);
+    const int c = w.c, j = w.j, n0 = w.n0, nn = w.nn;
+    const bool has_z = a.z != nullptr;
+    const Rows<T, L> DT(a.dt, a.dt_ld, a.cols, c, j), DY(a.dy, a.dy_ld, a.cols, c, j), Z(has_z ? a.z : a.dy, has_z ? a.z_ld : a.dy_ld, a.cols, c, j);
+    const States<T, NP> C(a.C, a.c_ld, w.g, a.states, w.lane);
+    float A2[NS], dhc[NS];
+    load_state<NS>(a.A + (int64_t)c * a.states + n0, A2, nn);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) { A2[i] *= LOG2E; dhc[i] = 0.f; }
+    const float bias = a.dt_bias ? a.dt_bias[c] : 0.f;
+    int q0, q1;
+    item_slots(k, item, q0, q1);
+    Cursor cur(k.m);
+    cur.find(q0);
+    const bool begins = q0 <= cur.base, ends = cur.base + cur.tiles <= q1;
+    if (ends && a.dfinal && w.ok) load_state<NS>(a.dfinal + ((int64_t)cur.s * a.cols + c) * a.states + n0, dhc, nn);
+    float* Cs = lds[w.wave];
+    float sd = 0.f;
+    const int k0 = max(q0 - cur.base, 0), k1 = begins ? k0 : min(cur.tiles, q1 - cur.base);
+    T tr[NB], gr[NB], zr[NB], cr[NP / 4];
+    auto fetch = [&](int kt) {
+        const int row0 = cur.begin + kt * TILE, nr = min(TILE, cur.end - row0);
+        DT.load(row0, nr, tr); DY.load(row0, nr, gr);
+        if (has_z) Z.load(row0, nr, zr);
+        C.load(row0, nr, cr);
+    };
+    if (k0 < k1) fetch(k1 - 1);
+    for (int kt = k1 - 1; kt >= k0; --kt) {
+        const int nr = min(TILE, cur.end - cur.begin - kt * TILE);
+        C.stage(cr, nr, Cs);
+        float delta[NB], dp[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const bool ok = w.ok && b * L + j < nr;
+            float slope;
+            const float v = (float)tr[b] + bias, d = a.softplus ? softplus(v, slope) : v;
+            delta[b] = ok ? d : 0.f;
+            sd += delta[b];
+            dp[b] = ok ? has_z ? (float)gr[b] * ((float)zr[b] * sigmoid_acc((float)zr[b])) : (float)gr[b] : 0.f;
+        }
+        if (kt > k0) fetch(kt - 1);
+        wave_lds_fence();
+        static_for<0, NB>([&](auto bb) {
+            constexpr int b = NB - 1 - bb;
+            static_for<0, L>([&](auto ii) {
+                constexpr int i = L - 1 - ii;
+                const float dl = from_lane<L, i>(delta[b]), dpl = from_lane<L, i>(dp[b]);
+                const float* Cr = Cs + (b * L + i) * NP + n0;
+#pragma unroll
+                for (int e = 0; e < NS; ++e) dhc[e] = exp2_fast(dl * A2[e]) * fmaf(dpl, Cr[e], dhc[e]);
+            });
+        });
+        wave_lds_fence();
+    }
+    sd = channel_sum<L>(sd);
+    if (w.ok) {
+        store_some<float, NS>(k.edge + ((int64_t)item * a.cols + c) * a.states + n0, dhc, nn);
+        if (j == 0) k.sum_delta[(int64_t)item * a.cols + c] = sd;
+    }
+    if (blk == 0 && threadIdx.x == 0) k.cut[item] = begins || ends;
+}
+
+// Rows whose decays are worked out a second time on the way back: 4 NS registers for 4 NS exponentials of a tile, without which some would spill
+template <class T> constexpr int AGAIN = sizeof(T) == 4 ? 5 : 4;
 template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES<L>, 1) void scan_bwd_kernel(const ScanK k) {
     constexpr int NP = L * NS, NB = TILE / L, WV = BWD_WAVES<L>, R = RED<L, NS>;
     __shared__ float lds[WV][2][TILE * NP];
-    __shared__ float red[WV][TILE * R];
+    __shared__ float red[2][WV][TILE * R];                       // two of them: one barrier a tile
     const vc_scan_args& a = k.a;
-    const int nblk = a.groups * k.nblk, s = blockIdx.x / nblk, blk = blockIdx.x - s * nblk;
+    const int nblk = a.groups * k.nblk, item = blockIdx.x / nblk, blk = blockIdx.x - item * nblk;
     const Lane<L, NS> w(k, WV, blk);
     const int c = w.c, j = w.j, n0 = w.n0, nn = w.nn;
-    T *dxo = (T*)a.dx + c, *ddt = (T*)a.ddt + c, *dzo = a.dz ? (T*)a.dz + c : nullptr;
-    if (s == k.m.n_seqs) {
-        if (w.ok)
-            for (int r = seq_tail(k.m) + j; r < k.m.rows; r += L) {
-                dxo[(int64_t)r * a.dx_ld] = (T)0.f; ddt[(int64_t)r * a.ddt_ld] = (T)0.f;
-                if (dzo) dzo[(int64_t)r * a.dz_ld] = (T)0.f;
-            }
+    const bool has_z = a.z != nullptr;
+    const Rows<T, L> DX(a.dx, a.dx_ld, a.cols, c, j, w.ok), DDT(a.ddt, a.ddt_ld, a.cols, c, j, w.ok), DZ(a.dz, a.dz_ld, a.cols, c, j, w.ok);
+    if (item == k.items) {                                       // rows behind the last utterance
+        const int tail = seq_tail(k.m);
+        DX.clear(tail, k.m.rows, c, j); DDT.clear(tail, k.m.rows, c, j);
+        if (has_z) DZ.clear(tail, k.m.rows, c, j);
         return;
     }
-    const T *x = (const T*)a.x + c, *dt = (const T*)a.dt + c, *z = a.z ? (const T*)a.z + c : nullptr, *dy = (const T*)a.dy + c;
-    const T *B = (const T*)a.B + w.g * a.states, *C = (const T*)a.C + w.g * a.states;
+    const Rows<T, L> X(a.x, a.x_ld, a.cols, c, j), DT(a.dt, a.dt_ld, a.cols, c, j), DY(a.dy, a.dy_ld, a.cols, c, j), Z(has_z ? a.z : a.dy, has_z ? a.z_ld : a.dy_ld, a.cols, c, j);
+    const States<T, NP> B(a.B, a.b_ld, w.g, a.states, w.lane), C(a.C, a.c_ld, w.g, a.states, w.lane);
     float A2[NS], dA[NS], dhc[NS];
     load_state<NS>(a.A + (int64_t)c * a.states + n0, A2, nn);
 #pragma unroll
     for (int i = 0; i < NS; ++i) { A2[i] *= LOG2E; dA[i] = 0.f; dhc[i] = 0.f; }
     const float Dc = a.D ? a.D[c] : 0.f, bias = a.dt_bias ? a.dt_bias[c] : 0.f;
-    const int begin = seq_begin(k.m, s), end = seq_end(k.m, s, begin), base = slot_base(k.m, s);
-    const int64_t hs = ((int64_t)s * a.cols + c) * a.states + n0;
-    if (a.dfinal && w.ok) load_state<NS>(a.dfinal + hs, dhc, nn);
+    int q0, q1;
+    item_slots(k, item, q0, q1);
+    Cursor cur(k.m);
+    if (k.chunk) cur.find(q1 - 1); else cur.load(item);
+    if (k.chunk && cur.base + cur.tiles > q1) load_state<NS>(k.edge + ((int64_t)item * a.cols + c) * a.states + n0, dhc, nn);
     float dDacc = 0.f, dbacc = 0.f;
-    float *Bs = lds[w.wave][0], *Cs = lds[w.wave][1], *mine = red[w.wave];
-    for (int kt = (end - begin + TILE - 1) / TILE - 1; kt >= 0; --kt) {
-        const int row0 = begin + kt * TILE, nr = min(TILE, end - row0);
-        stage_states<T, NP>(B, a.b_ld, row0, nr, a.states, Bs, w.lane);
-        stage_states<T, NP>(C, a.c_ld, row0, nr, a.states, Cs, w.lane);
-        float h0[NS];
-        load_state<NS>(a.saved + ((int64_t)(base + kt) * a.cols + c) * a.states + n0, h0, nn);
+    float *Bs = lds[w.wave][0], *Cs = lds[w.wave][1];
+    int turn = 0;
+    for (int q = q1 - 1; q >= q0;) {                             // the utterances of the item, the last one first
+      const int64_t hs = ((int64_t)cur.s * a.cols + c) * a.states + n0;
+      const int k0 = max(q0 - cur.base, 0), k1 = min(cur.tiles, q + 1 - cur.base);
+      if (cur.base + cur.tiles <= q1) {                          // its end lies in this item
+#pragma unroll
+        for (int i = 0; i < NS; ++i) dhc[i] = 0.f;
+        if (a.dfinal && w.ok) load_state<NS>(a.dfinal + hs, dhc, nn);
+      }
+      T xr[NB], tr[NB], gr[NB], zr[NB], br[NP / 4], cr[NP / 4];
+      float h0[NS];
+      auto fetch = [&](int kt) {
+        const int row0 = cur.begin + kt * TILE, nr = min(TILE, cur.end - row0);
+        X.load(row0, nr, xr); DT.load(row0, nr, tr); DY.load(row0, nr, gr);
+        if (has_z) Z.load(row0, nr, zr);
+        B.load(row0, nr, br); C.load(row0, nr, cr);
+      };
+      if (k0 < k1) fetch(k1 - 1);
+      for (int kt = k1 - 1; kt >= k0; --kt) {
+        const int row0 = cur.begin + kt * TILE, nr = min(TILE, cur.end - row0);
+        float* mine = red[turn][w.wave];
+        load_state<NS>(a.saved + ((int64_t)(cur.base + kt) * a.cols + c) * a.states + n0, h0, nn);
+        B.stage(br, nr, Bs); C.stage(cr, nr, Cs);
         float xv[NB], delta[NB], slope[NB], dtx[NB], dp[NB], dzf[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             const bool ok = w.ok && b * L + j < nr;
-            const int64_t r = row0 + b * L + j;
-            xv[b] = ok ? (float)x[r * a.x_ld] : 0.f;
-            const float g = ok ? (float)dy[r * a.dy_ld] : 0.f, v = (ok ? (float)dt[r * a.dt_ld] : 0.f) + bias;
+            const float g = ok ? (float)gr[b] : 0.f, v = (float)tr[b] + bias;
+            xv[b] = ok ? (float)xr[b] : 0.f;
             slope[b] = 1.f;
             const float d = a.softplus ? softplus(v, slope[b]) : v;
             delta[b] = ok ? d : 0.f;
             dtx[b] = delta[b] * xv[b];
             dp[b] = g; dzf[b] = 0.f;
-            if (z) {
-                const float zv = ok ? (float)z[r * a.z_ld] : 0.f, sg = sigmoid_acc(zv);
+            if (has_z) {
+                const float zv = ok ? (float)zr[b] : 0.f, sg = sigmoid_acc(zv);
                 dp[b] = g * (zv * sg);
                 dzf[b] = g * (sg * (1.f + zv * (1.f - sg)));
             }
         }
         wave_lds_fence();
-        float av[TILE][NS], h[TILE][NS];
+        const auto xt = DX.tile(row0, nr), tt = DDT.tile(row0, nr), zt = DZ.tile(row0, nr);
+        float av[TILE][NS], h[TILE][NS];                         // (av of the first AGAIN rows is not kept)
+        Row<NS> bc[2];
+        bc[0].read(Bs + n0, Cs + n0);
         static_for<0, NB>([&](auto b) {
             float acc[L];
             static_for<0, L>([&](auto i) {
                 constexpr int t = b * L + i;
+                if constexpr (t + 1 < TILE) bc[(t + 1) & 1].read(Bs + (t + 1) * NP + n0, Cs + (t + 1) * NP + n0);
+                __builtin_amdgcn_sched_barrier(0);
                 const float dl = from_lane<L, i>(delta[b]), dx = from_lane<L, i>(dtx[b]);
-                const float *Br = Bs + t * NP + n0, *Cr = Cs + t * NP + n0;
+                const float (&Br)[NS] = bc[t & 1].b, (&Cr)[NS] = bc[t & 1].c;
                 float sum = 0.f;
 #pragma unroll
                 for (int e = 0; e < NS; ++e) {
                     const float hp = t ? h[t ? t - 1 : 0][e] : h0[e];
-                    av[t][e] = exp2_fast(dl * A2[e]);
-                    h[t][e] = fmaf(av[t][e], hp, dx * Br[e]);
+                    const float ae = exp2_fast(dl * A2[e]);
+                    if constexpr (t >= AGAIN<T>) av[t][e] = ae;
+                    h[t][e] = fmaf(ae, hp, dx * Br[e]);
                     sum = fmaf(Cr[e], h[t][e], sum);
                 }
                 acc[i] = sum;
-                __builtin_amdgcn_sched_barrier(0);      // B and C of later rows wait in LDS, not in registers: 128 of them hold a and h
+                __builtin_amdgcn_sched_barrier(0);      // one row ahead and no more: 128 registers hold a and h
             });
-            if (dzo) {
+            if (has_z) {
                 const float yp = sums_by_row<L>(acc, j) + Dc * xv[b];
-                if (w.ok && b * L + j < nr) dzo[(int64_t)(row0 + b * L + j) * a.dz_ld] = (T)(dzf[b] * yp);
+                DZ.store(zt, b, dzf[b] * yp);
             }
         });
         static_for<0, NB>([&](auto bb) {
             constexpr int b = NB - 1 - bb;
-            float gacc[L], qacc[L];
+            float gacc[L], qacc[L], xb = xv[b];
+            asm("" : "+v"(xb));                                  // delta x is worked out again: kept, it would cost a register for each row of a lane
+            const float dtxb = delta[b] * xb;
+            if (b == (NB > 1 ? NB / 2 - 1 : 0) && kt > k0) fetch(kt - 1);      // half of a and h is done with: their registers take the next tile's rows
             static_for<0, L>([&](auto ii) {
                 constexpr int i = L - 1 - ii, t = b * L + i;
-                const float dl = from_lane<L, i>(delta[b]), dx = from_lane<L, i>(dtx[b]), dpl = from_lane<L, i>(dp[b]);
-                const float *Br = Bs + t * NP + n0, *Cr = Cs + t * NP + n0;
+                if constexpr (t > 0) bc[(t - 1) & 1].read(Bs + (t - 1) * NP + n0, Cs + (t - 1) * NP + n0);
+                __builtin_amdgcn_sched_barrier(0);
+                const float dl = from_lane<L, i>(delta[b]), dx = from_lane<L, i>(dtxb), dpl = from_lane<L, i>(dp[b]);
+                const float (&Br)[NS] = bc[t & 1].b, (&Cr)[NS] = bc[t & 1].c;
                 float v[2 * NS], g = 0.f, qs = 0.f;
 #pragma unroll
                 for (int e = 0; e < NS; ++e) {
@@ -153,7 +260,8 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES<L>
                     v[NS + e] = dpl * h[t][e];
                     v[e] = dh * dx;
                     g = fmaf(dh, Br[e], g);
-                    dhc[e] = av[t][e] * dh;
+                    if constexpr (t >= AGAIN<T>) dhc[e] = av[t][e] * dh;
+                    else dhc[e] = exp2_fast(dl * A2[e]) * dh;
                     const float q = dhc[e] * hp;
                     qs = fmaf(q, A2[e], qs);
                     dA[e] = fmaf(q, dl, dA[e]);
@@ -165,31 +273,30 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES<L>
             const float g = sums_by_row<L>(gacc, j), q = sums_by_row<L>(qacc, j) * LN2;
             const float dv = (q + xv[b] * g) * slope[b];
             dDacc = fmaf(dp[b], xv[b], dDacc);
-            if (w.ok && b * L + j < nr) {
-                dbacc += dv;
-                const int64_t r = row0 + b * L + j;
-                dxo[r * a.dx_ld] = (T)fmaf(delta[b], g, dp[b] * Dc);
-                ddt[r * a.ddt_ld] = (T)dv;
-            }
+            dbacc += w.ok && b * L + j < nr ? dv : 0.f;
+            DX.store(xt, b, fmaf(delta[b], g, dp[b] * Dc));
+            DDT.store(tt, b, dv);
         });
         __syncthreads();
         for (int o = threadIdx.x; o < nr * 2 * NP; o += 64 * WV) {
             const int t = o / (2 * NP), e = o % (2 * NP), n = e % NP, it = (e / NP) * NS + n % NS;
             float sum = 0.f;
 #pragma unroll
-            for (int v = 0; v < WV; ++v) sum += gather_item<L, NS>(red[v] + t * R, it, n / NS);
+            for (int v = 0; v < WV; ++v) sum += gather_item<L, NS>(red[turn][v] + t * R, it, n / NS);
             k.part[((int64_t)blk * k.m.rows + row0 + t) * (2 * NP) + e] = sum;
         }
-        __syncthreads();
+        turn ^= 1;
+      }
+      if (cur.base >= q0 && a.dinitial && w.ok) store_some<float, NS>(a.dinitial + hs, dhc, nn);       // its beginning lies in this item
+      if (cur.base <= q0 || cur.s == 0) break;
+      q = min(cur.base, q) - 1;
+      cur.load(cur.s - 1);
     }
-    if (w.ok) {
-        if (a.dinitial) store_some<float, NS>(a.dinitial + hs, dhc, nn);
-        store_some<float, NS>(k.dapart + hs, dA, nn);
-    }
+    if (w.ok) store_some<float, NS>(k.dapart + ((int64_t)item * a.cols + c) * a.states + n0, dA, nn);
     const float d = channel_sum<L>(dDacc), b = channel_sum<L>(dbacc);
     if (w.ok && j == 0) {
-        k.chpart[((int64_t)s * 2) * a.cols + c] = d;
-        k.chpart[((int64_t)s * 2 + 1) * a.cols + c] = b;
+        k.chpart[((int64_t)item * 2) * a.cols + c] = d;
+        k.chpart[((int64_t)item * 2 + 1) * a.cols + c] = b;
     }
 }
 
@@ -209,54 +316,43 @@ template <class T> __global__ __launch_bounds__(256) void scan_dbc_kernel(const 
     for (int b = 0; b < k.nblk; ++b) s += k.part[((int64_t)(g * k.nblk + b) * k.m.rows + r) * (2 * np) + m];
     *dst = (T)s;
 }
-// dA, dD, ddt_bias: sum over the utterances
-__global__ __launch_bounds__(256) void scan_param_kernel(const ScanK k, int items) {
-    const vc_scan_args& a = k.a;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, na = (int64_t)a.cols * a.states;
-    if (i < na) {
-        float s = 0.f;
-        for (int q = 0; q < items; ++q) s += k.dapart[q * na + i];
-        a.dA[i] = s;
-    } else if (i < na + 2 * a.cols) {
-        const int64_t e = i - na;
-        float* dst = e < a.cols ? a.dD : a.ddt_bias;
-        if (!dst) return;
-        float s = 0.f;
-        for (int q = 0; q < items; ++q) s += k.chpart[(int64_t)q * 2 * a.cols + e];
-        dst[e % a.cols] = s;
-    }
-}
-
 static int bwd_setup(const char* who, const vc_scan_args* a, ScanK* k, int64_t* floats) {
-    VC_CHECK(scan_setup(who, a, true, k));
-    const int per = (scan_lanes(a->states) == 4 ? BWD_WAVES<4> : BWD_WAVES<16>) * 64 / scan_lanes(a->states);
-    k->nblk = (k->cg + per - 1) / per;
+    VC_ARG(a, "%s: null pointer", who);
+    VC_CHECK(scan_setup(who, a, a->states <= 16 ? BWD_WAVES<4> : BWD_WAVES<16>, k));
     const int64_t part = (int64_t)a->groups * k->nblk * a->rows * 2 * scan_padded(a->states);
-    const int64_t da = (int64_t)a->n_seqs * a->cols * a->states, ch = (int64_t)a->n_seqs * 2 * a->cols;
-    *floats = part + da + ch;
-    k->part = a->work; k->dapart = a->work + part; k->chpart = a->work + part + da;
+    const int64_t da = (int64_t)k->items * a->cols * a->states, ch = (int64_t)k->items * 2 * a->cols;
+    *floats = part + da + ch + scan_edge_floats(*k);
+    k->part = a->work; k->dapart = a->work + part; k->chpart = k->dapart + da;
+    scan_edge_place(k, k->chpart + ch);
     return 0;
 }
 extern "C" int64_t vc_selective_scan_bwd_work(const vc_scan_args* a) {
-    ScanK k{}; int64_t n;
+    ScanK k; int64_t n;
     return bwd_setup("vc_selective_scan_bwd_work", a, &k, &n) ? VC_E_ARG : n;
 }
 template <class T, int L, int NS> static int scan_bwd_l(const ScanK& k, hipStream_t s) {
-    const int64_t blocks = (int64_t)k.a.groups * k.nblk * (k.m.n_seqs + (k.a.zero_tail && k.m.off ? 1 : 0));
-    const int64_t bc = ((int64_t)k.m.rows * 2 * L * NS * k.a.groups + 255) / 256, pr = ((int64_t)k.a.cols * (k.a.states + 2) + 255) / 256;
-    VC_ARG(blocks < (1LL << 31) && bc < (1LL << 31), "vc_selective_scan_bwd: too many utterances and channels for one launch");
+    const int64_t blocks = (int64_t)k.a.groups * k.nblk * (k.items + (k.a.zero_tail && k.m.off ? 1 : 0));
+    const int64_t bc = ((int64_t)k.m.rows * 2 * L * NS * k.a.groups + 255) / 256;
+    const int per = EDGE_WAVES * 64 / L, nblk1 = (k.cg + per - 1) / per;
+    const int64_t eb = (int64_t)k.a.groups * nblk1 * k.items;
+    VC_ARG(blocks < (1LL << 31) && bc < (1LL << 31) && eb < (1LL << 31), "vc_selective_scan_bwd: too many utterances and channels for one launch");
+    if (k.chunk) {
+        hipLaunchKernelGGL((scan_bwd_edge_kernel<T, L, NS>), dim3((unsigned)eb), dim3(64 * EDGE_WAVES), 0, s, k, nblk1);
+        VC_CHECK(scan_carry(k, false, s));
+    }
     hipLaunchKernelGGL((scan_bwd_kernel<T, L, NS>), dim3((unsigned)blocks), dim3(64 * BWD_WAVES<L>), 0, s, k);
     if (bc) hipLaunchKernelGGL((scan_dbc_kernel<T>), dim3((unsigned)bc), dim3(256), 0, s, k, L * NS);
-    hipLaunchKernelGGL(scan_param_kernel, dim3((unsigned)pr), dim3(256), 0, s, k, k.m.n_seqs);
     VC_HIP(hipGetLastError());
-    return 0;
+    const int64_t na = (int64_t)k.a.cols * k.a.states;
+    VC_CHECK(seq_sum_parts(k.dapart, k.items, na, k.a.dA, na, nullptr, s));
+    return k.a.dD || k.a.ddt_bias ? seq_sum_parts(k.chpart, k.items, 2 * (int64_t)k.a.cols, k.a.dD, k.a.cols, k.a.ddt_bias, s) : 0;
 }
 template <class T> static int scan_bwd_t(const ScanK& k, hipStream_t s) { return SCAN_LAYOUT(T, k.a.states, scan_bwd_l, k, s); }
 extern "C" int vc_selective_scan_bwd(const vc_scan_args* a, void* stream) {
-    ScanK k{}; int64_t need;
+    ScanK k; int64_t need;
     VC_CHECK(bwd_setup("vc_selective_scan_bwd", a, &k, &need));
     VC_ARG(a->A && a->dA && (a->rows == 0 || (a->x && a->dt && a->B && a->C && a->dy && a->dx && a->ddt && a->dB && a->dC && a->saved)), "vc_selective_scan_bwd: null pointer");
-    VC_ARG(!a->z || a->dz, "vc_selective_scan_bwd: z has a gradient, dz is null");
+    VC_ARG(!a->z || a->dz || a->rows == 0, "vc_selective_scan_bwd: z has a gradient, dz is null");
     if (!a->z) k.a.dz = nullptr;
     if (a->saved_floats < vc_selective_scan_saved(a) && a->rows) { vc_set_error("vc_selective_scan_bwd: saved is too small"); return VC_E_NOMEM; }
     if (a->work_floats < need || !a->work) { vc_set_error("vc_selective_scan_bwd: work is too small (%lld floats needed)", (long long)need); return VC_E_NOMEM; }
