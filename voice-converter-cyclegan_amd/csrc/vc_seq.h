@@ -44,9 +44,8 @@ __device__ __forceinline__ int seq_end(const SeqMap& m, int s, int begin) { retu
 // rows behind the last utterance start here
 __device__ __forceinline__ int seq_tail(const SeqMap& m) { return m.off ? seq_begin(m, m.n_seqs) : m.rows; }
 
-// x * sigmoid(x) and its derivative's factor, sigmoid through one exponential: 1 / (1 + e^-x) (e^-x overflows to infinity, the reciprocal to 0)
-__device__ __forceinline__ float sigmoid_acc(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
-
+// 1 / (1 + e^-x) through the reciprocal instruction (one unit in the last place; e^-x overflows to infinity, whose reciprocal is 0)
+__device__ __forceinline__ float sigmoid_acc(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
 // The slot row r works on, -1 where it is padding: outside the pool, or named by an earlier row of this call.  Every thread of the block calls it.
 __device__ __forceinline__ int claim_slot(const int* slots, int r, int n_slots) {
     const int mine = slots ? slots[r] : r;

@@ -5,7 +5,7 @@
 // apart from the K - 1 frames ahead of a run.
 #include "vc_seq.h"
 
-struct ConvArgs { vc_conv1d_args a; SeqMap m; int cv, cvb, runs; float* part; };
+struct ConvArgs { vc_conv1d_args a; SeqMap m; int v, cv, cvb, runs; float* part; };     // v channels a thread, cv such vectors, cvb of them next to each other
 
 // the utterance row r lies in: the last s with begin(s) <= r; n_seqs where r lies behind the last utterance
 __device__ __forceinline__ int seq_of(const SeqMap& m, int r) {
@@ -15,41 +15,67 @@ __device__ __forceinline__ int seq_of(const SeqMap& m, int r) {
     while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (seq_begin(m, mid) <= r) lo = mid; else hi = mid - 1; }
     return lo;
 }
-// n channels of frame t (counted from the utterance's first row b): the utterance's own, or an earlier one from the initial state
-template <class T, int V> __device__ __forceinline__ void frame(const vc_conv1d_args& a, int s, int b, int t, int c, int n, float (&f)[V]) {
+// V channels of frame t (counted from the utterance's first row b): the utterance's own, or an earlier one from the initial state
+template <class T, int V> __device__ __forceinline__ void frame(const vc_conv1d_args& a, int s, int b, int t, int c, float (&f)[V]) {
 #pragma unroll
     for (int e = 0; e < V; ++e) f[e] = 0.f;
-    if (t >= 0) load_some<T, V>((const T*)a.x + (int64_t)(b + t) * a.x_ld + c, f, n);
-    else if (a.initial) load_some<T, V>((const T*)a.initial + ((int64_t)s * (a.taps - 1) + (a.taps - 1 + t)) * a.cols + c, f, n);
+    if (t >= 0) load_vec<T, V>((const T*)a.x + (int64_t)(b + t) * a.x_ld + c, f);
+    else if (a.initial) load_vec<T, V>((const T*)a.initial + ((int64_t)s * (a.taps - 1) + (a.taps - 1 + t)) * a.cols + c, f);
 }
 template <class T, int K, int V> struct Filter {
     float w[K][V], b[V];
-    __device__ __forceinline__ Filter(const vc_conv1d_args& a, int c, int n) {
+    __device__ __forceinline__ Filter(const vc_conv1d_args& a, int c) {
 #pragma unroll
         for (int e = 0; e < V; ++e) b[e] = 0.f;
-        if (a.bias) load_some<float, V>(a.bias + c, b, n);
+        if (a.bias) load_vec<float, V>(a.bias + c, b);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
 #pragma unroll
             for (int e = 0; e < V; ++e) w[k][e] = 0.f;
-            load_some<float, V>(a.w + (int64_t)k * a.cols + c, w[k], n);
+            load_vec<float, V>(a.w + (int64_t)k * a.cols + c, w[k]);
         }
     }
 };
 // A block's threads: cvb vectors of channels (a power of two) next to each other, 256 / cvb runs of rows
-constexpr int FWD_RUN = 16, BWD_RUN = 16, AHEAD = 4;             // rows of a run; rows whose loads are issued together
-struct Place { int c, n, run; bool ok; };
+// Rows of a run, and rows whose loads are issued together while as many are worked on.  8192 x 2048 bf16, 4 taps, forward and backward: 46.5 us
+// with (8, 16; 4, 2); 49.6 with (16, 16; 4, 4), 51.9 with (16, 16; 2, 2), 47.4 with (32, 32; 4, 4), which gives small calls too few threads.
+constexpr int FWD_RUN = 8, BWD_RUN = 16, FWD_AHEAD = 4, BWD_AHEAD = 2;
+constexpr int BWD_V = 4;                                         // channels of a thread of the gradient
+constexpr int FWD_WIDE = 32, BWD_WIDE = 64;                      // most vectors of channels next to each other in a block
+struct Place { int c, run; bool ok; };
 __device__ __forceinline__ Place place(const ConvArgs& k, int V) {
     const int blocks = (k.cv + k.cvb - 1) / k.cvb;
     Place p;
     const int v = (int)(blockIdx.x % blocks) * k.cvb + threadIdx.x % k.cvb;
     p.run = (int)(blockIdx.x / blocks) * (256 / k.cvb) + threadIdx.x / k.cvb;
-    p.c = v * V; p.n = k.a.cols - p.c; p.ok = v < k.cv;
+    // the last vector ends with the last channel: where V does not divide the channels it works out some of its neighbour's once more, to the same
+    // values, and no access has to ask how many channels are left (fewer than V of them: V = 1)
+    p.c = min(v * V, k.a.cols - V); p.ok = v < k.cv;
     return p;
 }
 
-template <class T, int K> __global__ __launch_bounds__(256) void conv1d_fwd_kernel(const ConvArgs k) {
-    constexpr int V = 16 / (int)sizeof(T);
+// V elements as they came: 16-bit ones two to a register
+template <class T, int V> struct Raw {
+    static constexpr int N = (V * (int)sizeof(T) + 3) / 4;
+    unsigned w[N];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (V * sizeof(T) % 4 != 0) w[0] = __builtin_bit_cast(unsigned short, *p);
+        else {
+            struct __attribute__((packed, aligned(sizeof(T)))) W { unsigned v[N]; };
+            const W q = *(const W*)p;
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[i] = q.v[i];
+        }
+    }
+    __device__ __forceinline__ void get(float (&f)[V]) const {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if constexpr (sizeof(T) == 4) f[i] = __builtin_bit_cast(float, w[i]);
+            else f[i] = (float)__builtin_bit_cast(T, (unsigned short)(w[i / 2] >> (16 * (i % 2))));
+        }
+    }
+};
+template <class T, int K, int V> __global__ __launch_bounds__(256) void conv1d_fwd_kernel(const ConvArgs k) {
     const vc_conv1d_args& a = k.a;
     const Place p = place(k, V);
     if (!p.ok) return;
@@ -60,12 +86,12 @@ template <class T, int K> __global__ __launch_bounds__(256) void conv1d_fwd_kern
 #pragma unroll
         for (int i = 0; i < K - 1; ++i) {
             float f[V];
-            frame<T, V>(a, s, b, e - b - (K - 1) + i, p.c, p.n, f);
-            store_some<T, V>((T*)a.final_state + ((int64_t)s * (K - 1) + i) * a.cols + p.c, f, p.n);
+            frame<T, V>(a, s, b, e - b - (K - 1) + i, p.c, f);
+            store_vec<T, V>((T*)a.final_state + ((int64_t)s * (K - 1) + i) * a.cols + p.c, f);
         }
         return;
     }
-    const Filter<T, K, V> w(a, p.c, p.n);
+    const Filter<T, K, V> w(a, p.c);
     int r = p.run * FWD_RUN;
     const int r1 = min(r + FWD_RUN, k.m.rows);
     const T* x = (const T*)a.x + p.c;
@@ -73,14 +99,14 @@ template <class T, int K> __global__ __launch_bounds__(256) void conv1d_fwd_kern
     for (int s = seq_of(k.m, r); r < r1; ++s) {
         if (s >= k.m.n_seqs) {                                   // rows behind the last utterance
             float f[V] = {};
-            if (a.zero_tail) for (; r < r1; ++r) store_some<T, V>(y + (int64_t)r * a.y_ld, f, p.n);
+            if (a.zero_tail) for (; r < r1; ++r) store_vec<T, V>(y + (int64_t)r * a.y_ld, f);
             return;
         }
         const int b = seq_begin(k.m, s), hi = min(seq_end(k.m, s, b), r1);
         if (r >= hi) continue;                                   // an empty utterance
         float win[K][V];
 #pragma unroll
-        for (int i = 0; i < K - 1; ++i) frame<T, V>(a, s, b, r - b - (K - 1) + i, p.c, p.n, win[i]);
+        for (int i = 0; i < K - 1; ++i) frame<T, V>(a, s, b, r - b - (K - 1) + i, p.c, win[i]);
         auto step = [&](const float (&f)[V]) {
             float o[V];
 #pragma unroll
@@ -93,20 +119,28 @@ template <class T, int K> __global__ __launch_bounds__(256) void conv1d_fwd_kern
 #pragma unroll
                 for (int i = 0; i < K - 1; ++i) win[i][e] = win[i + 1][e];
             }
-            store_some<T, V>(y + (int64_t)r * a.y_ld, o, p.n);
+            store_vec<T, V>(y + (int64_t)r * a.y_ld, o);
             ++r;
         };
-        while (r + AHEAD <= hi) {
-            float f[AHEAD][V] = {};
+        // FWD_AHEAD rows are worked on while the next are on their way; rows past the end read the last one and are not used
+        Raw<T, V> next[FWD_AHEAD];
+        auto fetch = [&](int at) {
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) load_some<T, V>(x + (int64_t)(r + i) * a.x_ld, f[i], p.n);
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) step(f[i]);
-        }
+            for (int i = 0; i < FWD_AHEAD; ++i) next[i].load(x + (int64_t)min(at + i, hi - 1) * a.x_ld);
+        };
+        fetch(r);
         while (r < hi) {
-            float f[V] = {};
-            load_some<T, V>(x + (int64_t)r * a.x_ld, f, p.n);
-            step(f);
+            Raw<T, V> now[FWD_AHEAD];
+#pragma unroll
+            for (int i = 0; i < FWD_AHEAD; ++i) now[i] = next[i];
+            if (r + FWD_AHEAD < hi) fetch(r + FWD_AHEAD);
+#pragma unroll
+            for (int i = 0; i < FWD_AHEAD; ++i) {
+                if (r >= hi) break;
+                float f[V];
+                now[i].get(f);
+                step(f);
+            }
         }
     }
 }
@@ -125,14 +159,14 @@ template <int K, int V> __device__ __forceinline__ void pre_gradient(const float
 }
 // A run's dx needs the K - 1 frames' g behind it as well: they are worked out again there.  dx of a frame gathers in a register ring while the
 // frames that look at it go by.
-template <class T, int K> __global__ __launch_bounds__(256) void conv1d_bwd_kernel(const ConvArgs k) {
-    constexpr int V = 16 / (int)sizeof(T);
+// Four channels a thread: eight would fill the registers (filter, window, ring and its share of dw are K vectors each) and leave too few waves to wait with.
+template <class T, int K, int V> __global__ __launch_bounds__(256) void conv1d_bwd_kernel(const ConvArgs k) {
     __shared__ float red[256 * V];
     const vc_conv1d_args& a = k.a;
     const Place p = place(k, V);
     float dw[K][V] = {}, db[V] = {};
     if (p.ok && p.run < k.runs) {
-        const Filter<T, K, V> w(a, p.c, p.n);
+        const Filter<T, K, V> w(a, p.c);
         int r = p.run * BWD_RUN;
         const int r1 = min(r + BWD_RUN, k.m.rows);
         const T *x = (const T*)a.x + p.c, *dy = (const T*)a.dy + p.c;
@@ -140,22 +174,22 @@ template <class T, int K> __global__ __launch_bounds__(256) void conv1d_bwd_kern
         for (int s = seq_of(k.m, r); r < r1; ++s) {
             if (s >= k.m.n_seqs) {
                 float f[V] = {};
-                if (a.zero_tail && dx) for (; r < r1; ++r) store_some<T, V>(dx + (int64_t)r * a.dx_ld, f, p.n);
+                if (a.zero_tail && dx) for (; r < r1; ++r) store_vec<T, V>(dx + (int64_t)r * a.dx_ld, f);
                 break;
             }
             const int b = seq_begin(k.m, s), end = seq_end(k.m, s, b), lo = r, hi = min(end, r1);
             if (lo >= hi) continue;
             float win[K][V], ring[K][V] = {};                    // ring[i]: dx of frame r - (K-1) + i so far
 #pragma unroll
-            for (int i = 0; i < K - 1; ++i) frame<T, V>(a, s, b, lo - b - (K - 1) + i, p.c, p.n, win[i]);
+            for (int i = 0; i < K - 1; ++i) frame<T, V>(a, s, b, lo - b - (K - 1) + i, p.c, win[i]);
             auto emit = [&](int at, const float (&d)[V]) {       // row `at` has all but its share of the final state's gradient
                 if (!dx || at < lo || at >= hi) return;
                 float o[V] = {};
                 if (a.dfinal && at >= end - (K - 1))
-                    load_some<T, V>((const T*)a.dfinal + ((int64_t)s * (K - 1) + at - (end - (K - 1))) * a.cols + p.c, o, p.n);
+                    load_vec<T, V>((const T*)a.dfinal + ((int64_t)s * (K - 1) + at - (end - (K - 1))) * a.cols + p.c, o);
 #pragma unroll
                 for (int e = 0; e < V; ++e) o[e] += d[e];
-                store_some<T, V>(dx + (int64_t)at * a.dx_ld, o, p.n);
+                store_vec<T, V>(dx + (int64_t)at * a.dx_ld, o);
             };
             auto step = [&](const float (&f)[V], float (&g)[V]) {
 #pragma unroll
@@ -183,21 +217,28 @@ template <class T, int K> __global__ __launch_bounds__(256) void conv1d_bwd_kern
                 ++r;
             };
             const int stop = min(end, hi + (dx ? K - 1 : 0));
-            while (r + AHEAD <= stop) {
-                float f[AHEAD][V] = {}, g[AHEAD][V] = {};
+            // BWD_AHEAD rows are worked on while the next are on their way; rows past the end read the last one and are not used
+            Raw<T, V> xn[BWD_AHEAD], gn[BWD_AHEAD];
+            auto fetch = [&](int at) {
 #pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    load_some<T, V>(x + (int64_t)(r + i) * a.x_ld, f[i], p.n);
-                    load_some<T, V>(dy + (int64_t)(r + i) * a.dy_ld, g[i], p.n);
+                for (int i = 0; i < BWD_AHEAD; ++i) {
+                    const int64_t row = min(at + i, stop - 1);
+                    xn[i].load(x + row * a.x_ld); gn[i].load(dy + row * a.dy_ld);
                 }
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) step(f[i], g[i]);
-            }
+            };
+            fetch(r);
             while (r < stop) {
-                float f[V] = {}, g[V] = {};
-                load_some<T, V>(x + (int64_t)r * a.x_ld, f, p.n);
-                load_some<T, V>(dy + (int64_t)r * a.dy_ld, g, p.n);
-                step(f, g);
+                Raw<T, V> xc[BWD_AHEAD], gc[BWD_AHEAD];
+#pragma unroll
+                for (int i = 0; i < BWD_AHEAD; ++i) { xc[i] = xn[i]; gc[i] = gn[i]; }
+                if (r + BWD_AHEAD < stop) fetch(r + BWD_AHEAD);
+#pragma unroll
+                for (int i = 0; i < BWD_AHEAD; ++i) {
+                    if (r >= stop) break;
+                    float f[V], g[V];
+                    xc[i].get(f); gc[i].get(g);
+                    step(f, g);
+                }
             }
 #pragma unroll
             for (int i = 0; i < K - 1; ++i) emit(stop - (K - 1) + i, ring[i]);      // the utterance's last frames, nothing behind them
@@ -205,17 +246,17 @@ template <class T, int K> __global__ __launch_bounds__(256) void conv1d_bwd_kern
         }
     } else if (p.ok && a.dinitial && p.run - k.runs < k.m.n_seqs) {
         const int s = p.run - k.runs;                            // gradient of the K - 1 frames ahead of one utterance
-        const Filter<T, K, V> w(a, p.c, p.n);
+        const Filter<T, K, V> w(a, p.c);
         const int b = seq_begin(k.m, s), len = seq_end(k.m, s, b) - b;
         float win[K][V], ring[K - 1][V] = {};
 #pragma unroll
-        for (int i = 0; i < K - 1; ++i) frame<T, V>(a, s, b, i - (K - 1), p.c, p.n, win[i]);
+        for (int i = 0; i < K - 1; ++i) frame<T, V>(a, s, b, i - (K - 1), p.c, win[i]);
 #pragma unroll
         for (int t = 0; t < K - 1; ++t) {
             if (t >= len) continue;
             float g[V] = {};
-            frame<T, V>(a, s, b, t, p.c, p.n, win[K - 1]);
-            load_some<T, V>((const T*)a.dy + (int64_t)(b + t) * a.dy_ld + p.c, g, p.n);
+            frame<T, V>(a, s, b, t, p.c, win[K - 1]);
+            load_vec<T, V>((const T*)a.dy + (int64_t)(b + t) * a.dy_ld + p.c, g);
             pre_gradient<K, V>(win, w.w, w.b, a.silu, g);
 #pragma unroll
             for (int i = 0; i < K - 1; ++i)                      // frame t's tap j looks at frame t - (K-1) + j = i - (K-1)
@@ -230,10 +271,10 @@ template <class T, int K> __global__ __launch_bounds__(256) void conv1d_bwd_kern
 #pragma unroll
         for (int i = 0; i < K - 1; ++i) {
             float o[V] = {};
-            if (a.dfinal && i >= len) load_some<T, V>((const T*)a.dfinal + ((int64_t)s * (K - 1) + i - len) * a.cols + p.c, o, p.n);
+            if (a.dfinal && i >= len) load_vec<T, V>((const T*)a.dfinal + ((int64_t)s * (K - 1) + i - len) * a.cols + p.c, o);
 #pragma unroll
             for (int e = 0; e < V; ++e) o[e] += ring[i][e];
-            store_some<T, V>((T*)a.dinitial + ((int64_t)s * (K - 1) + i) * a.cols + p.c, o, p.n);
+            store_vec<T, V>((T*)a.dinitial + ((int64_t)s * (K - 1) + i) * a.cols + p.c, o);
         }
     }
     if (!k.part) return;
@@ -250,7 +291,7 @@ template <class T, int K> __global__ __launch_bounds__(256) void conv1d_bwd_kern
         for (int i = threadIdx.x; i < 256; i += k.cvb)
 #pragma unroll
             for (int e = 0; e < V; ++e) s[e] += red[e * 256 + i];
-        store_some<float, V>(dst + p.c, s, p.n);
+        store_vec<float, V>(dst + p.c, s);
     };
 #pragma unroll
     for (int i = 0; i < K; ++i) combine(dw[i], part + (int64_t)i * a.cols);
@@ -282,7 +323,7 @@ template <class T> __global__ __launch_bounds__(256) void conv1d_step_kernel(con
     *y = (T)(a.silu ? p * sigmoid_acc(p) : p);
 }
 
-static int check_conv1d(const char* who, const vc_conv1d_args* a, ConvArgs* k) {
+static int check_conv1d(const char* who, const vc_conv1d_args* a, int v, int most, ConvArgs* k) {
     VC_ARG(a, "%s: null pointer", who);
     VC_ARG(seq_type_ok(a->type), "%s: type must be VC_F32, VC_BF16 or VC_F16", who);
     VC_ARG(a->taps >= 2 && a->taps <= 8, "%s: 2 to 8 taps, got %d", who, a->taps);
@@ -290,9 +331,9 @@ static int check_conv1d(const char* who, const vc_conv1d_args* a, ConvArgs* k) {
     VC_ARG(a->offsets || a->rows % a->n_seqs == 0, "%s: without offsets the rows divide into n_seqs equal utterances", who);
     k->a = *a;
     k->m = SeqMap{a->offsets, (int)a->rows, a->n_seqs, (int)(a->rows / a->n_seqs)};
-    const int v = 16 / seq_esize(a->type);
-    k->cv = (a->cols + v - 1) / v;
-    for (k->cvb = 1; k->cvb < k->cv && k->cvb < 32;) k->cvb *= 2;
+    k->v = a->cols < v ? 1 : v;
+    k->cv = (a->cols + k->v - 1) / k->v;
+    for (k->cvb = 1; k->cvb < k->cv && k->cvb < most;) k->cvb *= 2;
     k->part = nullptr;
     return 0;
 }
@@ -304,12 +345,14 @@ static int conv_grid(const char* who, const ConvArgs& k, bool seqs, unsigned* gr
     return 0;
 }
 template <class T, int K> static int fwd_k(const ConvArgs& k, unsigned grid, hipStream_t s) {
-    hipLaunchKernelGGL((conv1d_fwd_kernel<T, K>), dim3(grid), dim3(256), 0, s, k);
+    if (k.v == 1) hipLaunchKernelGGL((conv1d_fwd_kernel<T, K, 1>), dim3(grid), dim3(256), 0, s, k);
+    else hipLaunchKernelGGL((conv1d_fwd_kernel<T, K, 16 / (int)sizeof(T)>), dim3(grid), dim3(256), 0, s, k);
     VC_HIP(hipGetLastError());
     return 0;
 }
 template <class T, int K> static int bwd_k(const ConvArgs& k, unsigned grid, hipStream_t s) {
-    hipLaunchKernelGGL((conv1d_bwd_kernel<T, K>), dim3(grid), dim3(256), 0, s, k);
+    if (k.v == 1) hipLaunchKernelGGL((conv1d_bwd_kernel<T, K, 1>), dim3(grid), dim3(256), 0, s, k);
+    else hipLaunchKernelGGL((conv1d_bwd_kernel<T, K, BWD_V>), dim3(grid), dim3(256), 0, s, k);
     VC_HIP(hipGetLastError());
     return 0;
 }
@@ -324,7 +367,8 @@ template <class T> static int conv1d_step(const ConvStepArgs& a, hipStream_t s) 
     return 0;
 }
 extern "C" int vc_causal_conv1d_fwd(const vc_conv1d_args* a, void* stream) {
-    ConvArgs k; VC_CHECK(check_conv1d("vc_causal_conv1d_fwd", a, &k));
+    VC_ARG(a, "vc_causal_conv1d_fwd: null pointer");
+    ConvArgs k; VC_CHECK(check_conv1d("vc_causal_conv1d_fwd", a, a->type == VC_F32 ? 4 : 8, FWD_WIDE, &k));
     VC_ARG(a->w && (a->rows == 0 || (a->x && a->y)), "vc_causal_conv1d_fwd: null pointer");
     VC_ARG(!a->final_state || a->final_state != a->initial, "vc_causal_conv1d_fwd: final_state may not be initial");
     if (a->rows == 0 && !a->final_state) return 0;
@@ -335,12 +379,12 @@ extern "C" int vc_causal_conv1d_fwd(const vc_conv1d_args* a, void* stream) {
 // rows of `part`: one for each block's runs
 static int conv_parts(const ConvArgs& k) { const int per = 256 / k.cvb; return (k.runs + per - 1) / per; }
 extern "C" int64_t vc_causal_conv1d_bwd_work(const vc_conv1d_args* a) {
-    ConvArgs k; if (check_conv1d("vc_causal_conv1d_bwd_work", a, &k)) return VC_E_ARG;
+    ConvArgs k; if (check_conv1d("vc_causal_conv1d_bwd_work", a, BWD_V, BWD_WIDE, &k)) return VC_E_ARG;
     k.runs = (k.m.rows + BWD_RUN - 1) / BWD_RUN;
     return (int64_t)conv_parts(k) * (a->taps + 1) * a->cols;
 }
 extern "C" int vc_causal_conv1d_bwd(const vc_conv1d_args* a, void* stream) {
-    ConvArgs k; VC_CHECK(check_conv1d("vc_causal_conv1d_bwd", a, &k));
+    ConvArgs k; VC_CHECK(check_conv1d("vc_causal_conv1d_bwd", a, BWD_V, BWD_WIDE, &k));
     VC_ARG(a->w && (a->rows == 0 || (a->x && a->dy)), "vc_causal_conv1d_bwd: null pointer");
     k.runs = (k.m.rows + BWD_RUN - 1) / BWD_RUN;
     const bool params = a->dw || a->dbias;

@@ -65,7 +65,7 @@ template <int L, int I> __device__ __forceinline__ float from_lane(float v) {
     if constexpr (L == 4) return dpp_all<I * 0x55>(v);          // quad_perm [i,i,i,i]
     else return dpp_all<0x150 + I>(v);                          // row_newbcast:i
 }
-// one step of sums_by_row: rows kept by bit BIT of the lane, the others handed to the lane that keeps them
+// one step of sums_by_row: rows kept by one bit of the lane, the others handed to the lane that keeps them
 template <int CTRL, int N> __device__ __forceinline__ void halve(float (&v)[N], bool up) {
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {

@@ -1,6 +1,5 @@
 // vc_seq_scan.hip -- selective state space scan: prompts and single frames (vc_seq_scan.h says how the work is laid out).
 #include "vc_seq_scan.h"
-#include <cstdlib>
 
 constexpr int FWD_WAVES = 4;
 
@@ -234,8 +233,10 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_st
     if (j == 0) *y = (T)(a.z ? sum * (z * sigmoid_acc(z)) : sum);
 }
 
-// Whole utterances where these fill the card, else runs of slots.  A run costs its first pass on top, about as much again as 0.75 of the main pass, so
-// runs are for axes that are long beside the number of channels and utterances.
+// Whole utterances where these fill the card side by side (WALK_WAVES: two waves a SIMD), else runs of slots, as many as make RUN_WAVES waves.  Runs cost
+// their first pass on top, about 0.7 of the main pass.  1 x 8192 x 1024 bf16, 16 states: 2880 us as one walk, 162 / 112 / 103 / 103 us with runs for
+// 1024 / 2048 / 4096 / 8192 waves; 64 x 128 x 1024 (4096 waves side by side): 54 us walked, 94 with runs.
+constexpr int64_t WALK_WAVES = 2048, RUN_WAVES = 4096;
 int scan_setup(const char* who, const vc_scan_args* a, int waves, ScanK* k) {
     VC_ARG(a, "%s: null pointer", who);
     VC_ARG(seq_type_ok(a->type), "%s: type must be VC_F32, VC_BF16 or VC_F16", who);
@@ -259,13 +260,12 @@ int scan_setup(const char* who, const vc_scan_args* a, int waves, ScanK* k) {
     const int per = waves * 64 / scan_lanes(a->states);          // channels of a block
     k->nblk = (k->cg + per - 1) / per;
     const int64_t row_waves = (int64_t)a->groups * ((k->cg + 64 / scan_lanes(a->states) - 1) / (64 / scan_lanes(a->states)));      // waves that a frame's channels fill
-    static const int T1 = getenv("SC_T1") ? atoi(getenv("SC_T1")) : 512, T2 = getenv("SC_T2") ? atoi(getenv("SC_T2")) : 2048;
     const int64_t longest = !a->offsets ? k->m.len : a->max_len > 0 ? a->max_len : a->rows;
     // utterances that run side by side for as long as the longest lasts
     const int64_t side = longest > 0 ? std::max<int64_t>(1, a->rows / longest) : a->n_seqs;
     k->items = a->n_seqs; k->chunk = 0;
-    if (side * row_waves < T1 && longest >= 8 * TILE) {
-        const int64_t want = std::max<int64_t>(1, T2 / row_waves);
+    if (side * row_waves < WALK_WAVES && longest >= 8 * TILE) {
+        const int64_t want = std::max<int64_t>(1, RUN_WAVES / row_waves);
         k->chunk = (int)std::max<int64_t>(4, (k->slots + want - 1) / want);
         k->items = (k->slots + k->chunk - 1) / k->chunk;
         if (k->items == 1) { k->items = a->n_seqs; k->chunk = 0; }

@@ -39,7 +39,7 @@ template <int L, int NS> __device__ __forceinline__ void reduce_to_lds(float (&v
         across_16<4>(w);
         u[0] = w[0]; u[1] = w[1];
         if constexpr (L == 4) {
-            halve<0x128, 2>(u, lane & 8);
+            halve<0x128, 2>(u, lane & 8);                        // row_ror:8
             dst[lane] = u[0];
         } else {
             dst[lane] = u[0]; dst[64 + lane] = u[1];
@@ -53,19 +53,12 @@ template <int L, int NS> __device__ __forceinline__ void reduce_to_lds(float (&v
     }
 }
 template <int L, int NS> constexpr int RED = (L == 16 && NS == 4) ? 128 : 64;      // floats a wave leaves for one row
-// sum of item `it` (0..NS-1 dB, NS.. dC) of lane j of the channels, from what one wave left
-template <int L, int NS> __device__ __forceinline__ float gather_item(const float* src, int it, int j) {
-    if constexpr (L == 4 && NS == 4) {
-        const int l = ((it & 1) << 3) + ((it & 2) << 3) + ((it & 4) << 3) + j;
-        return src[l] + src[l + 4];
-    } else if constexpr (L == 4) {
-        const int l = ((it & 1) << 4) + ((it & 2) << 4) + j;
-        return (src[l] + src[l + 4]) + (src[l + 8] + src[l + 12]);
-    } else if constexpr (NS == 4) {
-        return src[(it & 1) * 64 + ((it & 2) << 3) + ((it & 4) << 3) + j];
-    } else {
-        return src[((it & 1) << 4) + ((it & 2) << 4) + j];
-    }
+// what one wave left of item `it` (0..NS-1 dB, NS.. dC) of lane j of the channels: SPLIT numbers to be added
+template <int L, int NS> constexpr int SPLIT = L == 16 ? 1 : NS == 4 ? 2 : 4;
+template <int L, int NS> __device__ __forceinline__ int item_at(int it, int j) {
+    if constexpr (L == 4 && NS == 4) return ((it & 1) << 3) + ((it & 2) << 3) + ((it & 4) << 3) + j;
+    else if constexpr (NS == 4) return (it & 1) * 64 + ((it & 2) << 3) + ((it & 4) << 3) + j;
+    else return ((it & 1) << 4) + ((it & 2) << 4) + j;
 }
 
 // First pass of a split axis: what each run hands on to the one before it.  Only rows up to the end of the run's first utterance matter.
@@ -280,9 +273,15 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES<L>
         __syncthreads();
         for (int o = threadIdx.x; o < nr * 2 * NP; o += 64 * WV) {
             const int t = o / (2 * NP), e = o % (2 * NP), n = e % NP, it = (e / NP) * NS + n % NS;
+            const float* at = red[turn][0] + t * R + item_at<L, NS>(it, n / NS);
+            float f[WV * SPLIT<L, NS>];
+#pragma unroll
+            for (int v = 0; v < WV; ++v)
+#pragma unroll
+                for (int u = 0; u < SPLIT<L, NS>; ++u) f[v * SPLIT<L, NS> + u] = at[v * TILE * R + 4 * u];
             float sum = 0.f;
 #pragma unroll
-            for (int v = 0; v < WV; ++v) sum += gather_item<L, NS>(red[turn][v] + t * R, it, n / NS);
+            for (int v = 0; v < WV * SPLIT<L, NS>; ++v) sum += f[v];
             k.part[((int64_t)blk * k.m.rows + row0 + t) * (2 * NP) + e] = sum;
         }
         turn ^= 1;
@@ -300,22 +299,53 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES<L>
     }
 }
 
-// dB, dC: sum over the blocks of a group, rounded once
-template <class T> __global__ __launch_bounds__(256) void scan_dbc_kernel(const ScanK k, int np) {
+// What the main pass left in parts: dB and dC are summed over the blocks of a group and rounded once (blocks [0, bc)), dA, dD and ddt_bias over the items
+// (one column of sums for 64 lanes and 4 waves).
+template <class T> __global__ __launch_bounds__(256) void scan_finish_kernel(const ScanK k, int np, int bc) {
+    __shared__ float red[4][64];
     const vc_scan_args& a = k.a;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int w = 2 * np * a.groups, tail = seq_tail(k.m);
-    if (i >= (int64_t)k.m.rows * w) return;
-    const int64_t r = i / w;
-    const int e = (int)(i - r * w), g = e / (2 * np), m = e % (2 * np), n = m % np;
-    if (n >= a.states) return;
-    T* dst = m < np ? (T*)a.dB + r * a.db_ld : (T*)a.dC + r * a.dc_ld;
-    dst += g * a.states + n;
-    if (r >= tail) { if (a.zero_tail) *dst = (T)0.f; return; }
+    if ((int)blockIdx.x < bc) {
+        const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+        const int w = 2 * np * a.groups, tail = seq_tail(k.m);
+        if (i >= (int64_t)k.m.rows * w) return;
+        const int64_t r = i / w;
+        const int e = (int)(i - r * w), g = e / (2 * np), m = e % (2 * np), n = m % np;
+        if (n >= a.states) return;
+        T* dst = m < np ? (T*)a.dB + r * a.db_ld : (T*)a.dC + r * a.dc_ld;
+        dst += g * a.states + n;
+        if (r >= tail) { if (a.zero_tail) *dst = (T)0.f; return; }
+        float s = 0.f;
+        for (int b = 0; b < k.nblk; ++b) s += k.part[((int64_t)(g * k.nblk + b) * k.m.rows + r) * (2 * np) + m];
+        *dst = (T)s;
+        return;
+    }
+    // dapart [items][cols * states], chpart [items][2 * cols]
+    const int64_t na = (int64_t)a.cols * a.states, i = (int64_t)(blockIdx.x - bc) * 64 + (threadIdx.x & 63);
+    const bool second = i >= na;
+    const int64_t e = second ? i - na : i, width = second ? 2 * (int64_t)a.cols : na;
+    const float* src = second ? k.chpart : k.dapart;
+    const int w = threadIdx.x >> 6;
     float s = 0.f;
-    for (int b = 0; b < k.nblk; ++b) s += k.part[((int64_t)(g * k.nblk + b) * k.m.rows + r) * (2 * np) + m];
-    *dst = (T)s;
+    if (e < width) {
+        int q = w;
+        for (; q + 28 < k.items; q += 32) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = src[(q + 4 * u) * width + e];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
+        for (; q < k.items; q += 4) s += src[q * width + e];
+    }
+    red[w][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (w || e >= width) return;
+    s = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+    if (!second) a.dA[e] = s;
+    else if (e < a.cols) { if (a.dD) a.dD[e] = s; }
+    else if (a.ddt_bias) a.ddt_bias[e - a.cols] = s;
 }
+
 static int bwd_setup(const char* who, const vc_scan_args* a, ScanK* k, int64_t* floats) {
     VC_ARG(a, "%s: null pointer", who);
     VC_CHECK(scan_setup(who, a, a->states <= 16 ? BWD_WAVES<4> : BWD_WAVES<16>, k));
@@ -341,11 +371,11 @@ template <class T, int L, int NS> static int scan_bwd_l(const ScanK& k, hipStrea
         VC_CHECK(scan_carry(k, false, s));
     }
     hipLaunchKernelGGL((scan_bwd_kernel<T, L, NS>), dim3((unsigned)blocks), dim3(64 * BWD_WAVES<L>), 0, s, k);
-    if (bc) hipLaunchKernelGGL((scan_dbc_kernel<T>), dim3((unsigned)bc), dim3(256), 0, s, k, L * NS);
+    const int64_t pc = ((int64_t)k.a.cols * (k.a.states + 2) + 63) / 64;
+    VC_ARG(bc + pc < (1LL << 31), "vc_selective_scan_bwd: too many rows and channels for one launch");
+    hipLaunchKernelGGL((scan_finish_kernel<T>), dim3((unsigned)(bc + pc)), dim3(256), 0, s, k, L * NS, (int)bc);
     VC_HIP(hipGetLastError());
-    const int64_t na = (int64_t)k.a.cols * k.a.states;
-    VC_CHECK(seq_sum_parts(k.dapart, k.items, na, k.a.dA, na, nullptr, s));
-    return k.a.dD || k.a.ddt_bias ? seq_sum_parts(k.chpart, k.items, 2 * (int64_t)k.a.cols, k.a.dD, k.a.cols, k.a.ddt_bias, s) : 0;
+    return 0;
 }
 template <class T> static int scan_bwd_t(const ScanK& k, hipStream_t s) { return SCAN_LAYOUT(T, k.a.states, scan_bwd_l, k, s); }
 extern "C" int vc_selective_scan_bwd(const vc_scan_args* a, void* stream) {

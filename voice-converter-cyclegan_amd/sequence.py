@@ -26,9 +26,8 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _require(ok, text, *args):
-    if not ok:
-        raise ValueError(text % args)
+def _refuse(text, *args):
+    raise ValueError(text % args)
 
 
 def _p(t):
@@ -37,7 +36,7 @@ def _p(t):
 
 def _launch(f, name, ref, *args):
     """f(*args, stream) on ref's device and that device's current stream."""
-    index = ref.device.index
+    index = ref.get_device()
     if torch.cuda.current_device() == index:
         rc = f(*args, _raw_stream(index))
     else:
@@ -48,17 +47,20 @@ def _launch(f, name, ref, *args):
 
 
 def _activation(t, name):
-    _require(isinstance(t, torch.Tensor) and t.is_cuda, '%s must be a tensor on a GPU (there is no CPU path)', name)
-    _require(t.dtype in _TYPES, '%s must be float32, bfloat16 or float16, got %s', name, t.dtype)
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        _refuse('%s must be a tensor on a GPU (there is no CPU path)', name)
+    if t.dtype not in _TYPES:
+        _refuse('%s must be float32, bfloat16 or float16, got %s', name, t.dtype)
     return t
 
 
 def _like(t, ref, name, shape=None, dtype=None):
     """t on ref's device, with this shape and type."""
     dtype = dtype or ref.dtype
-    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == ref.device and (shape is None or t.shape == shape):
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == ref.get_device() and (shape is None or t.shape == shape):
         return t
-    _require(isinstance(t, torch.Tensor) and t.device == ref.device and t.dtype is dtype, '%s must be a %s tensor on %s', name, dtype, ref.device)
+    if not (isinstance(t, torch.Tensor) and t.device == ref.device and t.dtype is dtype):
+        _refuse('%s must be a %s tensor on %s', name, dtype, ref.device)
     raise ValueError('%s must have shape %s, got %s' % (name, tuple(shape), tuple(t.shape)))
 
 
@@ -83,11 +85,16 @@ def _rows(t, tail=1):
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _no_grad(what, *tensors):
-    _require(not _wants_grad(*tensors), '%s has no gradient: call it under torch.no_grad() or on detached tensors', what)
+    if _wants_grad(*tensors):
+        _refuse('%s has no gradient: call it under torch.no_grad() or on detached tensors', what)
 
 
 def _fresh(shape, ref, dtype=None):
@@ -111,12 +118,16 @@ def _once(grad):
 
 def _norm_inputs(x, gamma, residual, eps):
     _activation(x, 'x')
-    _require(x.dim() >= 1 and x.shape[-1] > 0, 'x must be [..., channels]')
-    _require(eps > 0, 'eps must be positive')
+    if not (x.dim() >= 1 and x.shape[-1] > 0):
+        _refuse('x must be [..., channels]')
+    if not eps > 0:
+        _refuse('eps must be positive')
     gamma = _parameter(gamma, x, 'gamma', (x.shape[-1],))
-    _require(gamma is not None, 'gamma is missing')
+    if gamma is None:
+        _refuse('gamma is missing')
     if residual is not None:
-        _require(isinstance(residual, torch.Tensor) and residual.dtype in (x.dtype, torch.float32), 'residual must be a tensor of %s or float32', x.dtype)
+        if not (isinstance(residual, torch.Tensor) and residual.dtype in (x.dtype, torch.float32)):
+            _refuse('residual must be a tensor of %s or float32', x.dtype)
         _like(residual, x, 'residual', x.shape, residual.dtype)
     return gamma
 
@@ -190,7 +201,8 @@ def rms_norm_e4m3(x, gamma, residual=None, eps=1e-6, group=0):
     q * scale stands for the norm.  group: columns that share a scale, 32, 64 or 128; 0: the whole row.  It has no gradient."""
     gamma = _norm_inputs(x, gamma, residual, eps)
     cols = x.shape[-1]
-    _require(group in (0, 32, 64, 128) and (group == 0 or cols % group == 0), 'group must be 0, 32, 64 or 128 and divide the channels')
+    if not (group in (0, 32, 64, 128) and (group == 0 or cols % group == 0)):
+        _refuse('group must be 0, 32, 64 or 128 and divide the channels')
     _no_grad('rms_norm_e4m3', x, gamma, residual)
     rows = x.numel() // cols
     x2, x_ld = _rows(x)
@@ -206,21 +218,26 @@ def rms_norm_e4m3(x, gamma, residual=None, eps=1e-6, group=0):
 
 # ------------------------------------------------------------------------------------------------------------ utterances
 
-def _utterances(x, seq_offsets, tail=1):
+def _utterances(x, seq_offsets):
     """(utterances, rows) of [batch, frames, ...] or of packed [rows, ...]."""
     if seq_offsets is None:
-        _require(x.dim() == 3, 'x must be [batch, frames, channels], or [rows, channels] with seq_offsets; got %s', tuple(x.shape))
-        _require(x.shape[0] > 0, 'x holds no utterance')
+        if x.dim() != 3:
+            _refuse('x must be [batch, frames, channels], or [rows, channels] with seq_offsets; got %s', tuple(x.shape))
+        if x.shape[0] == 0:
+            _refuse('x holds no utterance')
         return x.shape[0], x.shape[0] * x.shape[1]
-    _require(x.dim() == 2, 'with seq_offsets x must be [rows, channels], got %s', tuple(x.shape))
-    _require(isinstance(seq_offsets, torch.Tensor) and seq_offsets.dtype == torch.int32 and seq_offsets.device == x.device and seq_offsets.dim() == 1 and
-             seq_offsets.numel() >= 2, 'seq_offsets must be an int32 tensor [utterances + 1] on %s', x.device)
+    if x.dim() != 2:
+        _refuse('with seq_offsets x must be [rows, channels], got %s', tuple(x.shape))
+    if not (isinstance(seq_offsets, torch.Tensor) and seq_offsets.dtype == torch.int32 and seq_offsets.device == x.device and seq_offsets.dim() == 1 and
+            seq_offsets.numel() >= 2):
+        _refuse('seq_offsets must be an int32 tensor [utterances + 1] on %s', x.device)
     return seq_offsets.numel() - 1, x.shape[0]
 
 
 def _slots(slots, rows, pool, ref):
     if slots is None:
-        _require(rows <= pool, '%d frames without slots, and a state of %d', rows, pool)
+        if rows > pool:
+            _refuse('%d frames without slots, and a state of %d', rows, pool)
         return None
     _like(slots, ref, 'slots', (rows,), torch.int32)
     return slots.contiguous()
@@ -278,7 +295,8 @@ class _CausalConv1d(torch.autograd.Function):
 
 
 def _conv_weights(x, w, bias, cols):
-    _require(isinstance(w, torch.Tensor) and w.dim() == 2 and 2 <= w.shape[0] <= 8 and w.shape[1] == cols, 'w must be [taps, %d] with 2 to 8 taps', cols)
+    if not (isinstance(w, torch.Tensor) and w.dim() == 2 and 2 <= w.shape[0] <= 8 and w.shape[1] == cols):
+        _refuse('w must be [taps, %d] with 2 to 8 taps', cols)
     return _parameter(w, x, 'w', w.shape), _parameter(bias, x, 'bias', (cols,))
 
 
@@ -304,12 +322,15 @@ def causal_conv1d_step(x, state, w, bias=None, slots=None, silu=True):
     slots (int32 [streams]): the stream's entry in the pool; without them stream i has entry i.  A stream whose slot lies outside the pool, or is
     named by an earlier stream of the call, is padding: its y is zero and no state moves."""
     _activation(x, 'x')
-    _require(x.dim() == 2 and x.shape[1] > 0, 'x must be [streams, channels], got %s', tuple(x.shape))
+    if not (x.dim() == 2 and x.shape[1] > 0):
+        _refuse('x must be [streams, channels], got %s', tuple(x.shape))
     rows, cols = x.shape
     w, bias = _conv_weights(x, w, bias, cols)
-    _require(isinstance(state, torch.Tensor) and state.dim() == 3, 'state must be [pool, taps - 1, channels]')
+    if not (isinstance(state, torch.Tensor) and state.dim() == 3):
+        _refuse('state must be [pool, taps - 1, channels]')
     _like(state, x, 'state', (state.shape[0], w.shape[0] - 1, cols))
-    _require(state.is_contiguous(), 'state must be contiguous: it is moved on in place')
+    if not state.is_contiguous():
+        _refuse('state must be contiguous: it is moved on in place')
     _no_grad('causal_conv1d_step', x, state, w, bias)
     slots = _slots(slots, rows, state.shape[0], x)
     x2, x_ld = _rows(x)
@@ -323,11 +344,12 @@ def causal_conv1d_step(x, state, w, bias=None, slots=None, silu=True):
 
 def _grouped(t, lead, states, ref, name):
     """B or C as [..., groups, states]."""
-    _require(isinstance(t, torch.Tensor) and t.device == ref.device and t.dtype == ref.dtype, '%s must be a %s tensor on %s', name, ref.dtype, ref.device)
+    if not (isinstance(t, torch.Tensor) and t.dtype is ref.dtype and t.get_device() == ref.get_device()):
+        _refuse('%s must be a %s tensor on %s', name, ref.dtype, ref.device)
     if t.dim() == len(lead) + 1:
         t = t.unsqueeze(-2)
-    _require(t.dim() == len(lead) + 2 and tuple(t.shape[:-2]) == tuple(lead) and t.shape[-1] == states and t.shape[-2] > 0,
-             '%s must be %s + [groups, %d] or + [%d], got %s', name, tuple(lead), states, states, tuple(t.shape))
+    if not (t.dim() == len(lead) + 2 and t.shape[:-2] == lead and t.shape[-1] == states and t.shape[-2] > 0):
+        _refuse('%s must be %s + [groups, %d] or + [%d], got %s', name, tuple(lead), states, states, tuple(t.shape))
     return t
 
 
@@ -336,11 +358,13 @@ def _scan_inputs(x, dt, A, B, C_, D, z, dt_bias):
     _like(dt, x, 'dt', x.shape)
     if z is not None:
         _like(z, x, 'z', x.shape)
-    _require(isinstance(A, torch.Tensor) and A.dim() == 2 and A.shape[0] == cols and 1 <= A.shape[1] <= 64, 'A must be [%d, states] with 1 to 64 states', cols)
+    if not (isinstance(A, torch.Tensor) and A.dim() == 2 and A.shape[0] == cols and 1 <= A.shape[1] <= 64):
+        _refuse('A must be [%d, states] with 1 to 64 states', cols)
     A = _parameter(A, x, 'A', A.shape)
     B = _grouped(B, x.shape[:-1], A.shape[1], x, 'B')
     C_ = _grouped(C_, x.shape[:-1], A.shape[1], x, 'C')
-    _require(B.shape[-2] == C_.shape[-2] and cols % B.shape[-2] == 0, 'B and C must have the same groups, and these divide the channels')
+    if not (B.shape[-2] == C_.shape[-2] and cols % B.shape[-2] == 0):
+        _refuse('B and C must have the same groups, and these divide the channels')
     return A, B, C_, _parameter(D, x, 'D', (cols,)), _parameter(dt_bias, x, 'dt_bias', (cols,))
 
 
@@ -422,11 +446,13 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, initial_state=N
     max_len: the longest utterance where the program knows it: how a packed call is split, never what it gives."""
     _activation(x, 'x')
     seqs, rows = _utterances(x, seq_offsets)
-    _require(x.shape[-1] > 0, 'x has no channels')
+    if x.shape[-1] == 0:
+        _refuse('x has no channels')
     A, B, C, D, dt_bias = _scan_inputs(x, dt, A, B, C, D, z, dt_bias)
     if initial_state is not None:
         initial_state = _like(initial_state, x, 'initial_state', (seqs, *A.shape), torch.float32).contiguous()
-    _require(max_len is None or max_len >= 0, 'max_len must not be negative')
+    if not (max_len is None or max_len >= 0):
+        _refuse('max_len must not be negative')
     tensors = (x, dt, A, B, C, D, z, dt_bias, initial_state)
     if seq_offsets is not None:
         seq_offsets = seq_offsets.contiguous()
@@ -438,12 +464,15 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, slo
     """One frame of each of x's [streams, channels] (dt, z alike; B, C [streams, states] or [streams, groups, states]): y, and `state`
     [pool, channels, states] (float32) moved on in place.  slots as in causal_conv1d_step."""
     _activation(x, 'x')
-    _require(x.dim() == 2 and x.shape[1] > 0, 'x must be [streams, channels], got %s', tuple(x.shape))
+    if not (x.dim() == 2 and x.shape[1] > 0):
+        _refuse('x must be [streams, channels], got %s', tuple(x.shape))
     rows, cols = x.shape
     A, B, C, D, dt_bias = _scan_inputs(x, dt, A, B, C, D, z, dt_bias)
-    _require(isinstance(state, torch.Tensor) and state.dim() == 3, 'state must be [pool, channels, states]')
+    if not (isinstance(state, torch.Tensor) and state.dim() == 3):
+        _refuse('state must be [pool, channels, states]')
     _like(state, x, 'state', (state.shape[0], *A.shape), torch.float32)
-    _require(state.is_contiguous(), 'state must be contiguous: it is moved on in place')
+    if not state.is_contiguous():
+        _refuse('state must be contiguous: it is moved on in place')
     _no_grad('selective_scan_step', x, dt, A, B, C, state, D, z, dt_bias)
     slots = _slots(slots, rows, state.shape[0], x)
     (x2, x_ld), (t2, t_ld), (b2, b_ld), (c2, c_ld) = _rows(x), _rows(dt), _rows(B, 2), _rows(C, 2)
