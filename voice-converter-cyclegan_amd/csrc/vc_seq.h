@@ -46,13 +46,16 @@ __device__ __forceinline__ int seq_tail(const SeqMap& m) { return m.off ? seq_be
 
 // 1 / (1 + e^-x) through the reciprocal instruction (one unit in the last place; e^-x overflows to infinity, whose reciprocal is 0)
 __device__ __forceinline__ float sigmoid_acc(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
-// The slot row r works on, -1 where it is padding: outside the pool, or named by an earlier row of this call.  Every thread of the block calls it.
-__device__ __forceinline__ int claim_slot(const int* slots, int r, int n_slots) {
-    const int mine = slots ? slots[r] : r;
-    int taken = mine < 0 || mine >= n_slots;
-    if (slots)
-        for (int i = threadIdx.x; i < r; i += blockDim.x) taken |= slots[i] == mine;
-    return __syncthreads_or(taken) ? -1 : mine;
+// Single-frame calls.  The slot row r names; whether it is padding: a slot outside the pool, or one that an earlier row of the call names.  A wave looks
+// through the earlier rows itself (no barrier); MAX_SLOT_ROWS bounds how many there are.
+constexpr int MAX_SLOT_ROWS = 4096;
+__device__ __forceinline__ bool slot_is_padding(const int* slots, int r, int mine, int n_slots) {
+    bool taken = mine < 0 || mine >= n_slots;
+    if (slots) {
+#pragma unroll 4
+        for (int i = threadIdx.x & 63; i < r; i += 64) taken |= slots[i] == mine;
+    }
+    return __any(taken);
 }
 
 // dst[i] = sum over `parts` rows of part[parts][n], in order; columns [0, n0) go to dst0, the others to dst1 (either may be null).  vc_seq_norm.hip

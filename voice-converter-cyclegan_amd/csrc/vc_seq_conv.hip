@@ -304,23 +304,29 @@ struct ConvStepArgs {
 };
 template <class T> __global__ __launch_bounds__(256) void conv1d_step_kernel(const ConvStepArgs a) {
     const int r = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
-    const int slot = claim_slot(a.slots, r, a.n_slots);
-    if (c >= a.cols) return;
-    T* y = (T*)a.y + (int64_t)r * a.y_ld + c;
-    if (slot < 0) { *y = (T)0.f; return; }
-    T* st = (T*)a.state + (int64_t)slot * (a.taps - 1) * a.cols + c;
-    const T x = ((const T*)a.x)[(int64_t)r * a.x_ld + c];
-    float p = (a.bias ? a.bias[c] : 0.f);
+    const int mine = a.slots ? a.slots[r] : r, at = mine >= 0 && mine < a.n_slots ? mine : 0, cc = min(c, a.cols - 1);
+    const T* from = (const T*)a.state + (int64_t)at * (a.taps - 1) * a.cols + cc;
+    const T x = ((const T*)a.x)[(int64_t)r * a.x_ld + cc];
+    T f[7];
+    float p = a.bias ? a.bias[cc] : 0.f;
 #pragma unroll
     for (int k = 0; k < 7; ++k) {
         if (k >= a.taps - 1) break;
-        const T v = st[(int64_t)k * a.cols];
-        p = fmaf(a.w[(int64_t)k * a.cols + c], (float)v, p);
-        if (k) st[(int64_t)(k - 1) * a.cols] = v;
+        f[k] = from[(int64_t)k * a.cols];
+        p = fmaf(a.w[(int64_t)k * a.cols + cc], (float)f[k], p);
     }
-    p = fmaf(a.w[(int64_t)(a.taps - 1) * a.cols + c], (float)x, p);
-    st[(int64_t)(a.taps - 2) * a.cols] = x;
+    p = fmaf(a.w[(int64_t)(a.taps - 1) * a.cols + cc], (float)x, p);
+    const bool padding = slot_is_padding(a.slots, r, mine, a.n_slots);
+    if (c >= a.cols) return;
+    T* y = (T*)a.y + (int64_t)r * a.y_ld + c;
+    if (padding) { *y = (T)0.f; return; }
     *y = (T)(a.silu ? p * sigmoid_acc(p) : p);
+    T* to = (T*)a.state + (int64_t)mine * (a.taps - 1) * a.cols + c;
+#pragma unroll
+    for (int k = 0; k < 7; ++k) {
+        if (k >= a.taps - 1) break;
+        to[(int64_t)k * a.cols] = k < 6 && k + 1 < a.taps - 1 ? f[k + 1 < 7 ? k + 1 : 6] : x;
+    }
 }
 
 static int check_conv1d(const char* who, const vc_conv1d_args* a, int v, int most, ConvArgs* k) {
@@ -402,6 +408,7 @@ extern "C" int vc_causal_conv1d_step(const void* x, int64_t x_ld, void* state, c
     VC_ARG(taps >= 2 && taps <= 8, "vc_causal_conv1d_step: 2 to 8 taps, got %d", taps);
     VC_ARG(rows >= 0 && rows <= 65535 && n_slots > 0 && cols > 0, "vc_causal_conv1d_step: bad sizes (rows %d, n_slots %d, cols %d)", rows, n_slots, cols);
     VC_ARG(slots || rows <= n_slots, "vc_causal_conv1d_step: %d rows without slots, and %d slots", rows, n_slots);
+    VC_ARG(!slots || rows <= MAX_SLOT_ROWS, "vc_causal_conv1d_step: at most %d rows with slots, got %d", MAX_SLOT_ROWS, rows);
     if (rows == 0) return 0;
     VC_ARG(x && state && w && y, "vc_causal_conv1d_step: null pointer");
     const ConvStepArgs a{x, state, slots, w, bias, y, x_ld, y_ld, rows, n_slots, cols, taps, silu};

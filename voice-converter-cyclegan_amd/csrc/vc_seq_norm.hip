@@ -58,17 +58,27 @@ template <int V> __device__ __forceinline__ void store_e4m3(unsigned char* p, co
         for (int i = 0; i < V; ++i) if (i < n) p[i] = (unsigned char)(w[i / 4] >> (8 * (i % 4)));
     }
 }
-// The largest |y| of a group as an integer: ordered like the numbers, a NaN above infinity (fmaxf would drop it)
+// The largest |t gamma| of a group as an integer: ordered like the numbers, a NaN above infinity (fmaxf would drop it)
 constexpr float E4M3_TOP = 448.f, LEAST_TOP = 0x1p-100f;
 template <int V> __device__ __forceinline__ unsigned top_of(const float (&f)[V], unsigned m) {
 #pragma unroll
     for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(fabsf(f[i])));
     return m;
 }
+// y / scale of a group whose largest |t gamma| is `top`: rstd falls out of it, so a value passes three roundings on its way to the eight bits (t gamma, the
+// factor, the product).  A group under the least scale (rows of zeros, above all) takes that: the factor has rstd in it then.
+struct Quant { float first, factor, scale; };
+__device__ __forceinline__ Quant quant_of(unsigned bits, float rstd) {
+    const float top = __uint_as_float(bits), y = top * rstd;
+    Quant q;
+    if (y >= LEAST_TOP) { q.first = 1.f; q.factor = E4M3_TOP / top; q.scale = y / E4M3_TOP; }
+    else { q.first = rstd; q.factor = E4M3_TOP / LEAST_TOP; q.scale = y != y ? y : LEAST_TOP / E4M3_TOP; }
+    return q;
+}
 
 // A row of up to TPR * ITEMS vectors in registers.  Threads walk the rows with a stride of the grid, so gamma is read once for all of them.
-template <class T, class S, bool E4M3, int TPR, int ITEMS> __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(const NormRowArgs a) {
-    constexpr int V = 16 / (int)sizeof(T), RPB = TPR < 256 ? 256 / TPR : 1;
+template <class T, class S, bool E4M3, int TPR, int ITEMS> __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_fwd_kernel(const NormRowArgs a) {
+    constexpr int V = 16 / (int)sizeof(T), RPB = TPR == 64 ? 4 : 1;
     __shared__ float red[TPR / 64 > 0 ? TPR / 64 : 1];
     const int t = threadIdx.x % TPR;
     float gm[ITEMS][V];
@@ -118,7 +128,7 @@ template <class T, class S, bool E4M3, int TPR, int ITEMS> __global__ __launch_b
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-            for (int e = 0; e < V; ++e) f[i][e] = f[i][e] * rstd * gm[i][e];
+            for (int e = 0; e < V; ++e) f[i][e] = E4M3 ? f[i][e] * gm[i][e] : f[i][e] * rstd * gm[i][e];
         if constexpr (!E4M3) {
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i)
@@ -126,33 +136,33 @@ template <class T, class S, bool E4M3, int TPR, int ITEMS> __global__ __launch_b
         } else {
             unsigned top[ITEMS];
             if (a.group == 0) {
-                unsigned m = __float_as_uint(LEAST_TOP);
+                unsigned m = 0;
 #pragma unroll
                 for (int i = 0; i < ITEMS; ++i) m = top_of<V>(f[i], m);
                 m = row_max<TPR>(m, red);
-                if (t == 0) a.scale[r] = __uint_as_float(m) / E4M3_TOP;
+                if (t == 0) a.scale[r] = quant_of(m, rstd).scale;
 #pragma unroll
                 for (int i = 0; i < ITEMS; ++i) top[i] = m;
             } else {
                 const int gl = a.group / V;                      // lanes that share a scale: 4 to 32, next to each other
 #pragma unroll
                 for (int i = 0; i < ITEMS; ++i) {
-                    unsigned m = top_of<V>(f[i], __float_as_uint(LEAST_TOP));
+                    unsigned m = top_of<V>(f[i], 0);
                     m = max(m, (unsigned)__shfl_xor((int)m, 1, 64));
                     m = max(m, (unsigned)__shfl_xor((int)m, 2, 64));
                     if (gl > 4) m = max(m, (unsigned)__shfl_xor((int)m, 4, 64));
                     if (gl > 8) m = max(m, (unsigned)__shfl_xor((int)m, 8, 64));
                     if (gl > 16) m = max(m, (unsigned)__shfl_xor((int)m, 16, 64));
                     top[i] = m;
-                    if (left[i] > 0 && t % gl == 0) a.scale[r * (a.cols / a.group) + (i * TPR + t) / gl] = __uint_as_float(m) / E4M3_TOP;
+                    if (left[i] > 0 && t % gl == 0) a.scale[r * (a.cols / a.group) + (i * TPR + t) / gl] = quant_of(m, rstd).scale;
                 }
             }
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
-                const float inv = E4M3_TOP / __uint_as_float(top[i]);
+                const Quant k = quant_of(top[i], rstd);
                 float q[V];
 #pragma unroll
-                for (int e = 0; e < V; ++e) q[e] = f[i][e] * inv;
+                for (int e = 0; e < V; ++e) q[e] = f[i][e] * k.first * k.factor;
                 if (left[i] > 0) store_e4m3<V>((unsigned char*)a.y + r * a.y_ld + (i * TPR + t) * V, q, left[i]);
             }
         }
@@ -173,21 +183,21 @@ template <class T, class S, bool E4M3> __global__ __launch_bounds__(1024) void r
     }
     const float rstd = 1.f / sqrtf(row_sum<1024>(ss, red) / (float)a.cols + a.eps);
     if (a.rstd && threadIdx.x == 0) a.rstd[r] = rstd;
-    auto y = [&](int c) { return (sum ? (float)sum[c] : (float)x[c]) * rstd * a.gamma[c]; };      // a thread reads back what it wrote itself
+    auto t = [&](int c) { return sum ? (float)sum[c] : (float)x[c]; };                            // a thread reads back what it wrote itself
     if constexpr (!E4M3) {
-        for (int c = threadIdx.x; c < a.cols; c += 1024) ((T*)a.y)[r * a.y_ld + c] = (T)y(c);
+        for (int c = threadIdx.x; c < a.cols; c += 1024) ((T*)a.y)[r * a.y_ld + c] = (T)(t(c) * rstd * a.gamma[c]);
     } else {
         // scales: a wave for each group of 64 threads' columns would leave most idle, so each pass of the block covers 1024 columns: 8 to 32 groups
-        unsigned whole = __float_as_uint(LEAST_TOP);
+        unsigned whole = 0;
         if (a.group == 0) {
-            for (int c = threadIdx.x; c < a.cols; c += 1024) whole = max(whole, __float_as_uint(fabsf(y(c))));
+            for (int c = threadIdx.x; c < a.cols; c += 1024) whole = max(whole, __float_as_uint(fabsf(t(c) * a.gamma[c])));
             whole = row_max<1024>(whole, red);
-            if (threadIdx.x == 0) a.scale[r] = __uint_as_float(whole) / E4M3_TOP;
+            if (threadIdx.x == 0) a.scale[r] = quant_of(whole, rstd).scale;
         }
         __shared__ unsigned top[1024 / 32];
         for (int c0 = 0; c0 < a.cols; c0 += 1024) {
             const int c = c0 + threadIdx.x;
-            const float v = c < a.cols ? y(c) : 0.f;
+            const float v = c < a.cols ? t(c) * a.gamma[c] : 0.f;
             unsigned m = whole;
             if (a.group) {
                 m = lanes_max<32>(max(whole, __float_as_uint(fabsf(v))));
@@ -196,17 +206,18 @@ template <class T, class S, bool E4M3> __global__ __launch_bounds__(1024) void r
                 __syncthreads();
                 const int per = a.group / 32, first = threadIdx.x / a.group * per;
                 for (int i = 0; i < per; ++i) m = max(m, top[first + i]);
-                if (c < a.cols && threadIdx.x % a.group == 0) a.scale[r * (a.cols / a.group) + c / a.group] = __uint_as_float(m) / E4M3_TOP;
+                if (c < a.cols && threadIdx.x % a.group == 0) a.scale[r * (a.cols / a.group) + c / a.group] = quant_of(m, rstd).scale;
             }
-            const float q = v * (E4M3_TOP / __uint_as_float(m));
+            const Quant k = quant_of(m, rstd);
+            const float q = v * k.first * k.factor;
             if (c < a.cols) ((unsigned char*)a.y)[r * a.y_ld + c] = (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(q, q, 0, false);
         }
     }
 }
 
 // Gradient.  Every thread keeps its columns' share of dgamma over all rows it walks; a block leaves one row of `part`.
-template <class T, class S, int TPR, int ITEMS> __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(const NormRowArgs a) {
-    constexpr int V = 16 / (int)sizeof(T), RPB = TPR < 256 ? 256 / TPR : 1;
+template <class T, class S, int TPR, int ITEMS> __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_bwd_kernel(const NormRowArgs a) {
+    constexpr int V = 16 / (int)sizeof(T), RPB = TPR == 64 ? 4 : 1;
     __shared__ float red[TPR / 64 > 0 ? TPR / 64 : 1];
     const int t = threadIdx.x % TPR;
     float gm[ITEMS][V], dg[ITEMS][V];
@@ -332,17 +343,19 @@ int seq_sum_parts(const float* part, int parts, int64_t n, float* dst0, int64_t 
     return 0;
 }
 
-// How a row of nv vectors is held: a wave up to 4 vectors a thread, then a block of 256, then of 1024
+// How a row of nv vectors is held: by a wave with up to two vectors a thread, which needs no barrier; longer ones by a block of 256, then of 1024.
+// Rows of 2048 bf16 with 8-bit output (8832 of them): 58 us by a wave with four vectors a thread, whose registers leave four waves a SIMD, 53 by 128
+// threads, 45 by 256; rows of 1024: 32 us by a wave, 40 by 128 or 256 threads.
 #define NORM_LAYOUT(nv, F) \
-    ((nv) <= 64 ? F(64, 1) : (nv) <= 128 ? F(64, 2) : (nv) <= 256 ? F(64, 4) : (nv) <= 512 ? F(256, 2) : (nv) <= 1024 ? F(256, 4) : F(1024, 4))
-static int norm_tpr(int64_t nv) { return nv <= 256 ? 64 : nv <= 1024 ? 256 : 1024; }
+    ((nv) <= 64 ? F(64, 1) : (nv) <= 128 ? F(64, 2) : (nv) <= 256 ? F(256, 1) : (nv) <= 512 ? F(256, 2) : (nv) <= 1024 ? F(256, 4) : F(1024, 4))
+static int norm_tpr(int64_t nv) { return nv <= 128 ? 64 : nv <= 1024 ? 256 : 1024; }
 constexpr int64_t NORM_MOST = 4096;                              // vectors of the longest row that registers hold
 static int64_t norm_vectors(int cols, int type) { const int v = 16 / seq_esize(type); return (cols + v - 1) / v; }
 
 template <class T, class S, bool E, int TPR, int ITEMS> static void launch_fwd(const NormRowArgs& a, hipStream_t s) {
-    const int64_t rpb = TPR < 256 ? 256 / TPR : 1, want = (a.rows + rpb - 1) / rpb;
+    const int64_t rpb = TPR == 64 ? 4 : 1, want = (a.rows + rpb - 1) / rpb;
     const int64_t most = TPR == 1024 ? 1024 : 4096;
-    hipLaunchKernelGGL((rms_fwd_kernel<T, S, E, TPR, ITEMS>), dim3((unsigned)std::min(want, most)), dim3(TPR < 256 ? 256 : TPR), 0, s, a);
+    hipLaunchKernelGGL((rms_fwd_kernel<T, S, E, TPR, ITEMS>), dim3((unsigned)std::min(want, most)), dim3(TPR == 64 ? 256 : TPR), 0, s, a);
 }
 template <class T, class S, bool E> static int norm_fwd_e(const NormRowArgs& a, hipStream_t s) {
     const int64_t nv = (a.cols + 16 / (int)sizeof(T) - 1) / (16 / (int)sizeof(T));
@@ -362,7 +375,7 @@ template <class T> static int norm_fwd(const NormRowArgs& a, bool wide, bool e4m
 // Blocks of the gradient: enough to fill the card, few enough that their rows of `part` cost little beside the activations
 static int norm_bwd_blocks(int64_t rows, int cols, int type) {
     const int64_t nv = norm_vectors(cols, type);
-    const int64_t rpb = nv <= 256 ? 4 : 1, most = norm_tpr(nv) == 1024 ? 256 : 512;
+    const int64_t rpb = nv <= 128 ? 4 : 1, most = norm_tpr(nv) == 1024 ? 256 : 1024;
     return (int)std::min<int64_t>((rows + rpb - 1) / rpb, most);
 }
 template <class T, class S> static int norm_bwd_t(const NormRowArgs& a, int type, float* dgamma, hipStream_t s) {
@@ -370,8 +383,8 @@ template <class T, class S> static int norm_bwd_t(const NormRowArgs& a, int type
     const int blocks = norm_bwd_blocks(a.rows, a.cols, type);
     if (nv > NORM_MOST / 2) hipLaunchKernelGGL((rms_bwd_long_kernel<T, S>), dim3(blocks), dim3(1024), 0, s, a);
     else {
-#define F(TPR, ITEMS) hipLaunchKernelGGL((rms_bwd_kernel<T, S, TPR, ITEMS>), dim3(blocks), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
-        if (nv <= 64) F(64, 1); else if (nv <= 128) F(64, 2); else if (nv <= 256) F(64, 4); else if (nv <= 512) F(256, 2); else if (nv <= 1024) F(256, 4); else F(1024, 2);
+#define F(TPR, ITEMS) hipLaunchKernelGGL((rms_bwd_kernel<T, S, TPR, ITEMS>), dim3(blocks), dim3(TPR == 64 ? 256 : TPR), 0, s, a)
+        if (nv <= 64) F(64, 1); else if (nv <= 128) F(64, 2); else if (nv <= 256) F(256, 1); else if (nv <= 512) F(256, 2); else if (nv <= 1024) F(256, 4); else F(1024, 2);
 #undef F
     }
     VC_HIP(hipGetLastError());

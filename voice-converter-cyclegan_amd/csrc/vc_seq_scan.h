@@ -201,5 +201,32 @@ static inline int scan_padded(int states) { return states <= 8 ? 8 : states <= 1
 int scan_setup(const char* who, const vc_scan_args* a, int waves, ScanK* k);
 int64_t scan_edge_floats(const ScanK& k);                        // of edge, sum_delta and cut
 void scan_edge_place(ScanK* k, float* work);
-// edge[r]: what run r hands on -> what enters it from the runs before it (behind it where !FORWARD)
+// What enters run `item` from the runs before it (behind it where !FORWARD).  Up to CARRY_ITEMS runs every wave goes through them itself, which saves a
+// launch; more are gone through once for all by scan_carry, which puts what enters a run in the place of what it hands on.
+constexpr int CARRY_ITEMS = 64;
 int scan_carry(const ScanK& k, bool forward, hipStream_t s);
+template <int NS, bool FORWARD> __device__ __forceinline__ void carry_in(const ScanK& k, int item, int c, int n0, int nn, const float (&A2)[NS], float (&h)[NS]) {
+    constexpr int AT_ONCE = 8;                                   // runs whose loads are on their way together: the chain itself is one multiply-add a run
+    const vc_scan_args& a = k.a;
+    if (k.items > CARRY_ITEMS) {
+        load_state<NS>(k.edge + ((int64_t)item * a.cols + c) * a.states + n0, h, nn);
+        return;
+    }
+    const int n = FORWARD ? item : k.items - 1 - item;           // runs to go through, the farthest first
+    for (int i0 = 0; i0 < n; i0 += AT_ONCE) {
+        float e[AT_ONCE][NS], sd[AT_ONCE]; int cut[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const int at = min(i0 + i, n - 1), r = FORWARD ? at : k.items - 1 - at;
+            load_state<NS>(k.edge + ((int64_t)r * a.cols + c) * a.states + n0, e[i], nn);
+            sd[i] = k.sum_delta[(int64_t)r * a.cols + c];
+            cut[i] = k.cut[r];
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            if (i0 + i >= n) break;
+#pragma unroll
+            for (int j = 0; j < NS; ++j) h[j] = cut[i] ? e[i][j] : fmaf(exp2_fast(A2[j] * sd[i]), h[j], e[i][j]);
+        }
+    }
+}

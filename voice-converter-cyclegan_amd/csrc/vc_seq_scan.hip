@@ -91,6 +91,7 @@ __global__ __launch_bounds__(64) void scan_carry_kernel(const ScanK k, bool forw
     }
 }
 int scan_carry(const ScanK& k, bool forward, hipStream_t s) {
+    if (k.items <= CARRY_ITEMS) return 0;
     hipLaunchKernelGGL(scan_carry_kernel, dim3((unsigned)(((int64_t)k.a.cols * k.a.states + 63) / 64)), dim3(64), 0, s, k, forward);
     VC_HIP(hipGetLastError());
     return 0;
@@ -131,7 +132,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_fw
     item_slots(k, item, q0, q1);
     Cursor cur(k.m);
     if (k.chunk) cur.find(q0); else cur.load(item);
-    if (k.chunk && q0 > cur.base) load_state<NS>(k.edge + ((int64_t)item * a.cols + c) * a.states + n0, h, nn);
+    if (k.chunk && q0 > cur.base) carry_in<NS, true>(k, item, c, n0, nn, A2, h);
     float *Bs = lds[w.wave][0], *Cs = lds[w.wave][1];
     for (int q = q0; q < q1;) {                                  // the utterances of the item
         const int64_t hs = ((int64_t)cur.s * a.cols + c) * a.states + n0;
@@ -205,32 +206,48 @@ struct ScanStepArgs {
     const void *x, *dt, *z, *B, *C; const float *A, *D, *dt_bias; float* state; const int* slots; void* y;
     int64_t x_ld, dt_ld, z_ld, b_ld, c_ld, y_ld; int rows, n_slots, cols, states, groups, softplus;
 };
+// Bound by the state's traffic: L lanes a channel as in the scan, STEP_U channels a lane group.  Everything is asked for before the earlier rows' slots are
+// looked through; a slot outside the pool reads entry 0 and drops it.
+constexpr int STEP_U = 2;
 template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_step_kernel(const ScanStepArgs a) {
-    const int r = blockIdx.y, j = threadIdx.x % L, c = blockIdx.x * (256 / L) + threadIdx.x / L;
-    const int slot = claim_slot(a.slots, r, a.n_slots);
-    if (c >= a.cols) return;
-    T* y = (T*)a.y + (int64_t)r * a.y_ld + c;
-    if (slot < 0) { if (j == 0) *y = (T)0.f; return; }
-    const int n0 = j * NS, nn = max(0, min(NS, a.states - n0)), g = c / (a.cols / a.groups);
-    float* st = a.state + ((int64_t)slot * a.cols + c) * a.states + n0;
-    float h[NS], A[NS], B[NS], C[NS];
-    load_state<NS>(st, h, nn);
-    load_state<NS>(a.A + (int64_t)c * a.states + n0, A, nn);
-    load_some<T, NS>((const T*)a.B + r * a.b_ld + g * a.states + n0, B, nn);
-    load_some<T, NS>((const T*)a.C + r * a.c_ld + g * a.states + n0, C, nn);
-    const float x = (float)((const T*)a.x)[r * a.x_ld + c], z = a.z ? (float)((const T*)a.z)[r * a.z_ld + c] : 0.f;
-    const float v = (float)((const T*)a.dt)[r * a.dt_ld + c] + (a.dt_bias ? a.dt_bias[c] : 0.f);
-    float slope;
-    const float d = a.softplus ? softplus(v, slope) : v;
-    float sum = 0.f;
+    constexpr int G = 256 / L;                                   // lane groups of a block
+    const int r = blockIdx.y, j = threadIdx.x % L, c0 = blockIdx.x * (G * STEP_U) + threadIdx.x / L;
+    const int mine = a.slots ? a.slots[r] : r, at = mine >= 0 && mine < a.n_slots ? mine : 0;
+    const int n0 = j * NS, nn = max(0, min(NS, a.states - n0)), wide = a.cols / a.groups;
+    const bool full = a.states == L * NS;                        // no lane lacks states: whole vectors without a question
+    float h[STEP_U][NS], A[STEP_U][NS], B[STEP_U][NS], C[STEP_U][NS], x[STEP_U], z[STEP_U], v[STEP_U], D[STEP_U];
 #pragma unroll
-    for (int e = 0; e < NS; ++e) {
-        h[e] = fmaf(exp2_fast(d * (A[e] * LOG2E)), h[e], d * x * B[e]);
-        sum = fmaf(C[e], h[e], sum);
+    for (int u = 0; u < STEP_U; ++u) {
+        const int c = min(c0 + u * G, a.cols - 1), g = c / wide;
+        const float *hp = a.state + ((int64_t)at * a.cols + c) * a.states + n0, *ap = a.A + (int64_t)c * a.states + n0;
+        const T *bp = (const T*)a.B + r * a.b_ld + g * a.states + n0, *cp = (const T*)a.C + r * a.c_ld + g * a.states + n0;
+        if (full) { load_vec<float, NS>(hp, h[u]); load_vec<float, NS>(ap, A[u]); load_vec<T, NS>(bp, B[u]); load_vec<T, NS>(cp, C[u]); }
+        else { load_some<float, NS>(hp, h[u], nn); load_some<float, NS>(ap, A[u], nn); load_some<T, NS>(bp, B[u], nn); load_some<T, NS>(cp, C[u], nn); }
+        x[u] = (float)((const T*)a.x)[r * a.x_ld + c];
+        v[u] = (float)((const T*)a.dt)[r * a.dt_ld + c] + (a.dt_bias ? a.dt_bias[c] : 0.f);
+        z[u] = a.z ? (float)((const T*)a.z)[r * a.z_ld + c] : 0.f;
+        D[u] = a.D ? a.D[c] : 0.f;
     }
-    store_some<float, NS>(st, h, nn);
-    sum = channel_sum<L>(sum) + (a.D ? a.D[c] * x : 0.f);
-    if (j == 0) *y = (T)(a.z ? sum * (z * sigmoid_acc(z)) : sum);
+    const bool padding = slot_is_padding(a.slots, r, mine, a.n_slots);
+#pragma unroll
+    for (int u = 0; u < STEP_U; ++u) {
+        const int c = c0 + u * G;
+        if (c >= a.cols) break;
+        T* y = (T*)a.y + (int64_t)r * a.y_ld + c;
+        if (padding) { if (j == 0) *y = (T)0.f; continue; }
+        float slope;
+        const float d = a.softplus ? softplus(v[u], slope) : v[u];
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < NS; ++e) {
+            h[u][e] = fmaf(exp2_fast(d * (A[u][e] * LOG2E)), h[u][e], d * x[u] * B[u][e]);
+            sum = fmaf(C[u][e], h[u][e], sum);
+        }
+        float* hp = a.state + ((int64_t)mine * a.cols + c) * a.states + n0;
+        if (full) store_vec<float, NS>(hp, h[u]); else store_some<float, NS>(hp, h[u], nn);
+        sum = channel_sum<L>(sum) + D[u] * x[u];
+        if (j == 0) *y = (T)(a.z ? sum * (z[u] * sigmoid_acc(z[u])) : sum);
+    }
 }
 
 // Whole utterances where these fill the card side by side (WALK_WAVES: two waves a SIMD), else runs of slots, as many as make RUN_WAVES waves.  Runs cost
@@ -314,7 +331,7 @@ extern "C" int vc_selective_scan_fwd(const vc_scan_args* a, void* stream) {
 }
 
 template <class T, int L, int NS> static int scan_step_l(const ScanStepArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL((scan_step_kernel<T, L, NS>), dim3((a.cols + 256 / L - 1) / (256 / L), a.rows), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((scan_step_kernel<T, L, NS>), dim3((a.cols + STEP_U * 256 / L - 1) / (STEP_U * 256 / L), a.rows), dim3(256), 0, s, a);
     VC_HIP(hipGetLastError());
     return 0;
 }
@@ -328,6 +345,7 @@ extern "C" int vc_selective_scan_step(const void* x, int64_t x_ld, const void* d
     VC_ARG(rows >= 0 && rows <= 65535 && n_slots > 0 && cols > 0 && groups > 0 && cols % groups == 0,
            "vc_selective_scan_step: bad sizes (rows %d, n_slots %d, cols %d, groups %d)", rows, n_slots, cols, groups);
     VC_ARG(slots || rows <= n_slots, "vc_selective_scan_step: %d rows without slots, and %d slots", rows, n_slots);
+    VC_ARG(!slots || rows <= MAX_SLOT_ROWS, "vc_selective_scan_step: at most %d rows with slots, got %d", MAX_SLOT_ROWS, rows);
     if (rows == 0) return 0;
     VC_ARG(x && dt && B && C && A && state && y, "vc_selective_scan_step: null pointer");
     const ScanStepArgs a{x, dt, z, B, C, A, D, dt_bias, state, slots, y, x_ld, dt_ld, z_ld, b_ld, c_ld, y_ld, rows, n_slots, cols, states, groups, softplus};

@@ -160,7 +160,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES<L>
     item_slots(k, item, q0, q1);
     Cursor cur(k.m);
     if (k.chunk) cur.find(q1 - 1); else cur.load(item);
-    if (k.chunk && cur.base + cur.tiles > q1) load_state<NS>(k.edge + ((int64_t)item * a.cols + c) * a.states + n0, dhc, nn);
+    if (k.chunk && cur.base + cur.tiles > q1) carry_in<NS, false>(k, item, c, n0, nn, A2, dhc);
     float dDacc = 0.f, dbacc = 0.f;
     float *Bs = lds[w.wave][0], *Cs = lds[w.wave][1];
     int turn = 0;
