@@ -40,6 +40,18 @@ template <int TPR> __device__ __forceinline__ unsigned row_max(unsigned v, float
     }
     return v;
 }
+template <int TPR> __device__ __forceinline__ float row_maxf(float v, float* red) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    if constexpr (TPR > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TPR / 64; ++i) v = fmaxf(v, red[i]);
+    }
+    return v;
+}
 // four (V = 4) or eight values as e4m3: rounded to nearest even by the conversion instruction; |f| <= 448 (1 + 2^-23), which rounds to 448
 template <int V> __device__ __forceinline__ void store_e4m3(unsigned char* p, const float (&f)[V], int n) {
     unsigned w[V / 4];
@@ -65,16 +77,30 @@ template <int V> __device__ __forceinline__ unsigned top_of(const float (&f)[V],
     for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(fabsf(f[i])));
     return m;
 }
-// y / scale of a group whose largest |t gamma| is `top`: rstd falls out of it, so a value passes three roundings on its way to the eight bits (t gamma, the
-// factor, the product).  A group under the least scale (rows of zeros, above all) takes that: the factor has rstd in it then.
-struct Quant { float first, factor, scale; };
-__device__ __forceinline__ Quant quant_of(unsigned bits, float rstd) {
+// y / scale of a group.  rstd falls out of it: q = t gamma * 448 / max|t gamma|.  A quotient next to a border between two of the 8-bit values goes to the
+// wrong one where its fp32 error reaches across (a few in a million elements), so what the products and the division round off is carried along: e is
+// the rounding error of t gamma (rest: that of the largest), one multiply-add each.  A group under the least scale (rows of zeros, above all) takes that.
+struct Quant { float first, factor, correction, scale; };
+__device__ __forceinline__ Quant quant_of(unsigned bits, float rest, float rstd) {
     const float top = __uint_as_float(bits), y = top * rstd;
     Quant q;
-    if (y >= LEAST_TOP) { q.first = 1.f; q.factor = E4M3_TOP / top; q.scale = y / E4M3_TOP; }
-    else { q.first = rstd; q.factor = E4M3_TOP / LEAST_TOP; q.scale = y != y ? y : LEAST_TOP / E4M3_TOP; }
+    if (y >= LEAST_TOP) {
+        q.first = 1.f; q.factor = E4M3_TOP / top; q.scale = y / E4M3_TOP;
+        q.correction = (fmaf(-q.factor, top, E4M3_TOP) - q.factor * rest) / E4M3_TOP;
+    } else { q.first = rstd; q.factor = E4M3_TOP / LEAST_TOP; q.correction = 0.f; q.scale = y != y ? y : LEAST_TOP / E4M3_TOP; }
     return q;
 }
+__device__ __forceinline__ float quantised(const Quant& k, float p, float e) {
+    const float v = p * k.first, q = v * k.factor;
+    return q + (fmaf(v, k.factor, -q) + fmaf(e * k.first, k.factor, q * k.correction));
+}
+// the rounding error of the largest |t gamma|: of several, the one that makes it largest
+template <int V> __device__ __forceinline__ float rest_of(const float (&p)[V], const float (&e)[V], unsigned top, float m) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) m = __float_as_uint(fabsf(p[i])) == top ? fmaxf(m, copysignf(1.f, p[i]) * e[i]) : m;
+    return m;
+}
+constexpr float NO_REST = -3.0e38f;
 
 // A row of up to TPR * ITEMS vectors in registers.  Threads walk the rows with a stride of the grid, so gamma is read once for all of them.
 template <class T, class S, bool E4M3, int TPR, int ITEMS> __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_fwd_kernel(const NormRowArgs a) {
@@ -125,44 +151,49 @@ template <class T, class S, bool E4M3, int TPR, int ITEMS> __global__ __launch_b
             for (int e = 0; e < V; ++e) ss = fmaf(f[i][e], f[i][e], ss);
         const float rstd = 1.f / sqrtf(row_sum<TPR>(ss, red) * inv_cols + a.eps);
         if (a.rstd && t == 0) a.rstd[r] = rstd;
+        float err[E4M3 ? ITEMS : 1][V];
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-            for (int e = 0; e < V; ++e) f[i][e] = E4M3 ? f[i][e] * gm[i][e] : f[i][e] * rstd * gm[i][e];
+            for (int e = 0; e < V; ++e) {
+                if constexpr (E4M3) { const float p = f[i][e] * gm[i][e]; err[i][e] = fmaf(f[i][e], gm[i][e], -p); f[i][e] = p; }
+                else f[i][e] = f[i][e] * rstd * gm[i][e];
+            }
         if constexpr (!E4M3) {
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i)
                 if (left[i] > 0) store_some<T, V>((T*)a.y + r * a.y_ld + (i * TPR + t) * V, f[i], left[i]);
         } else {
-            unsigned top[ITEMS];
+            Quant k[ITEMS];
             if (a.group == 0) {
                 unsigned m = 0;
 #pragma unroll
                 for (int i = 0; i < ITEMS; ++i) m = top_of<V>(f[i], m);
                 m = row_max<TPR>(m, red);
-                if (t == 0) a.scale[r] = quant_of(m, rstd).scale;
+                float rest = NO_REST;
 #pragma unroll
-                for (int i = 0; i < ITEMS; ++i) top[i] = m;
+                for (int i = 0; i < ITEMS; ++i) rest = rest_of<V>(f[i], err[i], m, rest);
+                k[0] = quant_of(m, row_maxf<TPR>(rest, red), rstd);
+                if (t == 0) a.scale[r] = k[0].scale;
+#pragma unroll
+                for (int i = 1; i < ITEMS; ++i) k[i] = k[0];
             } else {
                 const int gl = a.group / V;                      // lanes that share a scale: 4 to 32, next to each other
 #pragma unroll
                 for (int i = 0; i < ITEMS; ++i) {
                     unsigned m = top_of<V>(f[i], 0);
-                    m = max(m, (unsigned)__shfl_xor((int)m, 1, 64));
-                    m = max(m, (unsigned)__shfl_xor((int)m, 2, 64));
-                    if (gl > 4) m = max(m, (unsigned)__shfl_xor((int)m, 4, 64));
-                    if (gl > 8) m = max(m, (unsigned)__shfl_xor((int)m, 8, 64));
-                    if (gl > 16) m = max(m, (unsigned)__shfl_xor((int)m, 16, 64));
-                    top[i] = m;
-                    if (left[i] > 0 && t % gl == 0) a.scale[r * (a.cols / a.group) + (i * TPR + t) / gl] = quant_of(m, rstd).scale;
+                    for (int o = 1; o < gl; o <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
+                    float rest = rest_of<V>(f[i], err[i], m, NO_REST);
+                    for (int o = 1; o < gl; o <<= 1) rest = fmaxf(rest, __shfl_xor(rest, o, 64));
+                    k[i] = quant_of(m, rest, rstd);
+                    if (left[i] > 0 && t % gl == 0) a.scale[r * (a.cols / a.group) + (i * TPR + t) / gl] = k[i].scale;
                 }
             }
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
-                const Quant k = quant_of(top[i], rstd);
                 float q[V];
 #pragma unroll
-                for (int e = 0; e < V; ++e) q[e] = f[i][e] * k.first * k.factor;
+                for (int e = 0; e < V; ++e) q[e] = quantised(k[i], f[i][e], err[i][e]);
                 if (left[i] > 0) store_e4m3<V>((unsigned char*)a.y + r * a.y_ld + (i * TPR + t) * V, q, left[i]);
             }
         }
@@ -188,28 +219,41 @@ template <class T, class S, bool E4M3> __global__ __launch_bounds__(1024) void r
         for (int c = threadIdx.x; c < a.cols; c += 1024) ((T*)a.y)[r * a.y_ld + c] = (T)(t(c) * rstd * a.gamma[c]);
     } else {
         // scales: a wave for each group of 64 threads' columns would leave most idle, so each pass of the block covers 1024 columns: 8 to 32 groups
-        unsigned whole = 0;
+        auto product = [&](int c, float& e) { const float f = t(c), g = a.gamma[c], p = f * g; e = fmaf(f, g, -p); return p; };
+        Quant k{};
         if (a.group == 0) {
-            for (int c = threadIdx.x; c < a.cols; c += 1024) whole = max(whole, __float_as_uint(fabsf(t(c) * a.gamma[c])));
-            whole = row_max<1024>(whole, red);
-            if (threadIdx.x == 0) a.scale[r] = quant_of(whole, rstd).scale;
+            unsigned m = 0;
+            float e, rest = NO_REST;
+            for (int c = threadIdx.x; c < a.cols; c += 1024) m = max(m, __float_as_uint(fabsf(product(c, e))));
+            m = row_max<1024>(m, red);
+            for (int c = threadIdx.x; c < a.cols; c += 1024) { const float p[1] = {product(c, e)}, q[1] = {e}; rest = rest_of<1>(p, q, m, rest); }
+            k = quant_of(m, row_maxf<1024>(rest, red), rstd);
+            if (threadIdx.x == 0) a.scale[r] = k.scale;
         }
         __shared__ unsigned top[1024 / 32];
-        for (int c0 = 0; c0 < a.cols; c0 += 1024) {
+        __shared__ float most[1024 / 32];
+        for (int c0 = 0; c0 < a.cols; c0 += 1024) {              // 1024 columns at a time: 8 to 32 groups
             const int c = c0 + threadIdx.x;
-            const float v = c < a.cols ? t(c) * a.gamma[c] : 0.f;
-            unsigned m = whole;
+            float e = 0.f;
+            const float p = c < a.cols ? product(c, e) : 0.f;
             if (a.group) {
-                m = lanes_max<32>(max(whole, __float_as_uint(fabsf(v))));
+                const int per = a.group / 32, first = threadIdx.x / a.group * per;
+                unsigned m = lanes_max<32>(__float_as_uint(fabsf(p)));
                 __syncthreads();
                 if (threadIdx.x % 32 == 0) top[threadIdx.x / 32] = m;
                 __syncthreads();
-                const int per = a.group / 32, first = threadIdx.x / a.group * per;
                 for (int i = 0; i < per; ++i) m = max(m, top[first + i]);
-                if (c < a.cols && threadIdx.x % a.group == 0) a.scale[r * (a.cols / a.group) + c / a.group] = quant_of(m, rstd).scale;
+                const float p1[1] = {p}, e1[1] = {e};
+                float rest = rest_of<1>(p1, e1, m, NO_REST);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) rest = fmaxf(rest, __shfl_xor(rest, o, 64));
+                if (threadIdx.x % 32 == 0) most[threadIdx.x / 32] = rest;
+                __syncthreads();
+                for (int i = 0; i < per; ++i) rest = fmaxf(rest, most[first + i]);
+                k = quant_of(m, rest, rstd);
+                if (c < a.cols && threadIdx.x % a.group == 0) a.scale[r * (a.cols / a.group) + c / a.group] = k.scale;
             }
-            const Quant k = quant_of(m, rstd);
-            const float q = v * k.first * k.factor;
+            const float q = quantised(k, p, e);
             if (c < a.cols) ((unsigned char*)a.y)[r * a.y_ld + c] = (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(q, q, 0, false);
         }
     }
@@ -347,9 +391,9 @@ int seq_sum_parts(const float* part, int parts, int64_t n, float* dst0, int64_t 
 // Rows of 2048 bf16 with 8-bit output (8832 of them): 58 us by a wave with four vectors a thread, whose registers leave four waves a SIMD, 53 by 128
 // threads, 45 by 256; rows of 1024: 32 us by a wave, 40 by 128 or 256 threads.
 #define NORM_LAYOUT(nv, F) \
-    ((nv) <= 64 ? F(64, 1) : (nv) <= 128 ? F(64, 2) : (nv) <= 256 ? F(256, 1) : (nv) <= 512 ? F(256, 2) : (nv) <= 1024 ? F(256, 4) : F(1024, 4))
+    ((nv) <= 64 ? F(64, 1) : (nv) <= 128 ? F(64, 2) : (nv) <= 256 ? F(256, 1) : (nv) <= 512 ? F(256, 2) : (nv) <= 1024 ? F(256, 4) : F(1024, 2))
 static int norm_tpr(int64_t nv) { return nv <= 128 ? 64 : nv <= 1024 ? 256 : 1024; }
-constexpr int64_t NORM_MOST = 4096;                              // vectors of the longest row that registers hold
+constexpr int64_t NORM_MOST = 2048;                              // vectors of the longest row that registers hold
 static int64_t norm_vectors(int cols, int type) { const int v = 16 / seq_esize(type); return (cols + v - 1) / v; }
 
 template <class T, class S, bool E, int TPR, int ITEMS> static void launch_fwd(const NormRowArgs& a, hipStream_t s) {
@@ -381,7 +425,7 @@ static int norm_bwd_blocks(int64_t rows, int cols, int type) {
 template <class T, class S> static int norm_bwd_t(const NormRowArgs& a, int type, float* dgamma, hipStream_t s) {
     const int64_t nv = norm_vectors(a.cols, type);
     const int blocks = norm_bwd_blocks(a.rows, a.cols, type);
-    if (nv > NORM_MOST / 2) hipLaunchKernelGGL((rms_bwd_long_kernel<T, S>), dim3(blocks), dim3(1024), 0, s, a);
+    if (nv > NORM_MOST) hipLaunchKernelGGL((rms_bwd_long_kernel<T, S>), dim3(blocks), dim3(1024), 0, s, a);
     else {
 #define F(TPR, ITEMS) hipLaunchKernelGGL((rms_bwd_kernel<T, S, TPR, ITEMS>), dim3(blocks), dim3(TPR == 64 ? 256 : TPR), 0, s, a)
         if (nv <= 64) F(64, 1); else if (nv <= 128) F(64, 2); else if (nv <= 256) F(256, 1); else if (nv <= 512) F(256, 2); else if (nv <= 1024) F(256, 4); else F(1024, 2);
