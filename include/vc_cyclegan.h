@@ -223,7 +223,8 @@ int vc_adam_tf_update(float* p, float* m, float* v, const float* g, int64_t n,
  * [0, rows] on the device (they are not read back), so wrong ones give wrong numbers and no access outside the tensors.
  * Rows behind the last utterance are left as they were in every output, or cleared where `zero_tail` is set.
  * Slots (`slots`, device, int32, one per row of a single-frame call): which entry of the state pool a row belongs to; NULL: row r has entry r.
- * A row whose slot lies outside [0, n_slots), or that an earlier row of the call has already named, is padding: y gets zeros, no state moves. */
+ * A row whose slot lies outside [0, n_slots), or that an earlier row of the call has already named, is padding: y gets zeros, no state moves.  At most
+ * 4096 rows a call with slots, 65535 without. */
 #define VC_F32   0
 #define VC_BF16  1
 #define VC_F16   2
@@ -279,7 +280,7 @@ int vc_causal_conv1d_step(const void* x, int64_t x_ld, void* state, const int32_
  *   y[t][c] = (sum_n C[t][g][n] h[t][c][n] + D[c] x[t][c]) * z[t][c] sigmoid(z[t][c])
  * with g = c / (cols / groups): the channels of a group share B and C.  A [cols][states] fp32, finite, 1 <= states <= 64.  D, z, dt_bias may be NULL
  * (no skip, no gate, no bias).  B, C: row stride b_ld / c_ld, group g at + g * states.  initial [n_seqs][cols][states] fp32 (NULL: zeros);
- * final_state likewise (NULL: not wanted); final_state may not be initial. */
+ * final_state likewise (NULL: not wanted); final_state may not be initial.  Row strides: at most 2^24 elements, those of outputs at least their row. */
 typedef struct {
     const void *x, *dt, *z, *B, *C; const float *A, *D, *dt_bias; const float* initial; const int32_t* offsets;
     void* y; float* final_state;

@@ -157,6 +157,7 @@ def test_conv_refusals(L):
         a.work, a.work_floats = 4096, need - 1
         assert b(C.byref(a), NULL_STREAM) == -2
     s = L.lib.vc_causal_conv1d_step
+    assert s(ONE, 8, ONE, ONE, ONE, None, ONE, 8, 4097, 5000, 8, 4, 0, 1, NULL_STREAM) == -1      # more rows with slots than a wave looks through
     args = [ONE, 8, ONE, None, ONE, None, ONE, 8, 2, 4, 8, 4, 0, 1, NULL_STREAM]
     for i, v in ((0, None), (2, None), (4, None), (6, None), (8, -1), (8, 65536), (9, 1), (9, 0), (10, 0), (11, 1), (11, 9), (12, 3)):
         bad = list(args)
@@ -174,7 +175,8 @@ def _scan(L, **kw):
 def test_scan_refusals(L):
     f = L.lib.vc_selective_scan_fwd
     for bad in (dict(x=None), dict(dt=None), dict(A=None), dict(B=None), dict(C=None), dict(y=None), dict(states=0), dict(states=65), dict(groups=3), dict(groups=0), dict(cols=0),
-                dict(n_seqs=0), dict(rows=-1), dict(rows=1 << 31), dict(rows=13), dict(type=3), dict(initial=4096, final_state=4096)):
+                dict(n_seqs=0), dict(rows=-1), dict(rows=1 << 31), dict(rows=13), dict(type=3), dict(initial=4096, final_state=4096),
+                dict(x_ld=-1), dict(dt_ld=(1 << 24) + 1), dict(b_ld=1 << 25), dict(c_ld=-8), dict(y_ld=7), dict(y_ld=1 << 25), dict(z=4096, z_ld=1 << 25)):
         assert f(C.byref(_scan(L, **bad)), NULL_STREAM) == -1, bad
     assert f(None, NULL_STREAM) == -1
     a = _scan(L)
@@ -188,13 +190,15 @@ def test_scan_refusals(L):
     work = L.lib.vc_selective_scan_bwd_work(C.byref(a))
     assert work > 0
     full.update(work=4096, work_floats=work)
-    for bad in (dict(dy=None), dict(dx=None), dict(ddt=None), dict(dB=None), dict(dC=None), dict(dA=None), dict(saved=None), dict(z=4096), dict(states=65)):
+    for bad in (dict(dy=None), dict(dx=None), dict(ddt=None), dict(dB=None), dict(dC=None), dict(dA=None), dict(saved=None), dict(z=4096), dict(states=65),
+                dict(dx_ld=7), dict(ddt_ld=1 << 25), dict(z=4096, dz=4096, dz_ld=7), dict(db_ld=15), dict(dc_ld=3), dict(dy_ld=-1)):
         assert b(C.byref(_scan(L, **{**full, **bad})), NULL_STREAM) == -1, bad
     for bad in (dict(saved_floats=need - 1), dict(work_floats=work - 1), dict(work=None)):
         assert b(C.byref(_scan(L, **{**full, **bad})), NULL_STREAM) == -2, bad
     assert L.lib.vc_selective_scan_saved(C.byref(_scan(L, states=70))) == -1
     s = L.lib.vc_selective_scan_step
     args = [ONE, 8, ONE, 8, None, 0, ONE, 16, ONE, 16, ONE, None, None, ONE, None, ONE, 8, 2, 4, 8, 16, 1, 0, 1, NULL_STREAM]
+    assert s(*args[:14], ONE, ONE, 8, 4097, 5000, *args[19:]) == -1
     for i, v in ((0, None), (2, None), (6, None), (8, None), (10, None), (13, None), (15, None), (17, -1), (17, 65536), (18, 1), (18, 0), (19, 0), (20, 0), (20, 65), (21, 3), (22, 4)):
         bad = list(args)
         bad[i] = v

@@ -302,6 +302,41 @@ def test_scan_long_and_many(S, cols, states, kind, lengths, hint):
         close(got, r['d' + name], m['d' + name], 6 * last + rows + cols + states + 60, 'd' + name)
 
 
+def test_scan_of_many_short_utterances(S):
+    """more utterances than any split has parts: runs that hold many of them, some of no frames, one long at the end"""
+    g = torch.Generator().manual_seed(4)
+    lengths = torch.randint(0, 4, (5000,), generator=g).tolist() + [90]
+    n, rows, cols = len(lengths), sum(lengths), 5
+    v = scan_inputs(rows, cols, 4, 1, F32, n)
+    dy, df = rnd(20, rows, cols), rnd(21, n, cols, 4)
+    leaves = [t.requires_grad_(True) for t in v.values()]
+    for hint in (None, 90):
+        y, final = S.selective_scan(v['x'], v['dt'], v['A'], v['B'], v['C'], D=v['D'], z=v['z'], dt_bias=v['dt_bias'], initial_state=v['initial'],
+                                    seq_offsets=offsets_of(lengths), max_len=hint, return_final_state=True)
+        r = O.scan(**v, lengths=lengths, dy=dy, dfinal=df)
+        m = O.scan(**v, lengths=lengths, dy=dy, dfinal=df, absolute=True)
+        close(y, r['y'], m['y'], 3 * 90 + 44, 'y')
+        close(final, r['final'], m['final'], 3 * 90 + 44, 'final')
+        for (name, _), got in zip(v.items(), torch.autograd.grad((y, final), leaves, (dy, df))):
+            close(got, r['d' + name], m['d' + name], 6 * 90 + rows + cols + 64, 'd' + name)
+
+
+def test_scan_that_grows(S):
+    """A > 0: states grow by e^0.05 a frame, over 3000 frames further than fp32 reaches; while nothing has come in they stay zero, and what is small enough
+    stays finite, also where a run's whole factor is not.  Errors relative to what has grown: 3 roundings a frame and 50 units of the exponent's sum."""
+    t, cols = 3000, 8
+    x = torch.zeros(1, t, cols, device=DEV)
+    x[0, 1400:] = rnd(1, t - 1400, cols) * 1e-20
+    dt = torch.full((1, t, cols), 0.05, device=DEV)
+    A, bc = torch.ones(cols, 4, device=DEV), torch.ones(1, t, 4, device=DEV)
+    y, final = S.selective_scan(x, dt, A, bc, bc, softplus=False, return_final_state=True)
+    r = O.scan(x[0], dt[0], A, bc[0, :, None], bc[0, :, None], None, None, None, None, [t], softplus=False)
+    m = O.scan(x[0], dt[0], A, bc[0, :, None], bc[0, :, None], None, None, None, None, [t], softplus=False, absolute=True)
+    assert (y[0, :1400] == 0).all() and torch.isfinite(r['y'].float()).all()
+    close(y[0], r['y'], m['y'], 3 * 1600 + 50 * 80, 'y')
+    close(final, r['final'], m['final'], 3 * 1600 + 50 * 80, 'final')
+
+
 @pytest.mark.parametrize('kind', [F32, BF16])
 @pytest.mark.parametrize('cols,states,groups', [(6, 16, 1), (130, 16, 2), (9, 5, 3), (10, 64, 1)])
 def test_scan_steps_equal_the_prompt(S, kind, cols, states, groups):

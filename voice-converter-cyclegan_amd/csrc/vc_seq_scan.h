@@ -121,7 +121,7 @@ __device__ __forceinline__ float softplus(float v, float& slope) {
 // A tensor of rows as a lane uses it: through a buffer descriptor of the tile's rows, whose bounds check gives zeros for the rows that a short tile
 // lacks (where rows do not overlap) and drops stores to them, and those of lanes without a channel.  Host code keeps row strides within MAX_LD: the
 // offsets in a tile fit 31 bits.
-constexpr int64_t MAX_LD = 1 << 25;
+constexpr int64_t MAX_LD = 1 << 24;
 template <class T, int L> struct Rows {
     const T* p; int ld, width; unsigned at, step;
     __device__ __forceinline__ Rows(const void* base, int64_t stride, int cols, int c, int j, bool ok = true)
@@ -204,6 +204,12 @@ void scan_edge_place(ScanK* k, float* work);
 // What enters run `item` from the runs before it (behind it where !FORWARD).  Up to CARRY_ITEMS runs every wave goes through them itself, which saves a
 // launch; more are gone through once for all by scan_carry, which puts what enters a run in the place of what it hands on.
 constexpr int CARRY_ITEMS = 64;
+// exp2(p) h + e, or e where nothing is handed on.  In two halves: the factor of a whole run may leave the range of fp32 where its product with h does not
+// (frame by frame it would not either), and a state of zero stays one under any factor.
+__device__ __forceinline__ float carried(float p, float h, float e, int cut) {
+    const float f = exp2_fast(0.5f * p);
+    return cut || h == 0.f ? e : fmaf(f * h, f, e);
+}
 int scan_carry(const ScanK& k, bool forward, hipStream_t s);
 template <int NS, bool FORWARD> __device__ __forceinline__ void carry_in(const ScanK& k, int item, int c, int n0, int nn, const float (&A2)[NS], float (&h)[NS]) {
     constexpr int AT_ONCE = 8;                                   // runs whose loads are on their way together: the chain itself is one multiply-add a run
@@ -226,7 +232,7 @@ template <int NS, bool FORWARD> __device__ __forceinline__ void carry_in(const S
         for (int i = 0; i < AT_ONCE; ++i) {
             if (i0 + i >= n) break;
 #pragma unroll
-            for (int j = 0; j < NS; ++j) h[j] = cut[i] ? e[i][j] : fmaf(exp2_fast(A2[j] * sd[i]), h[j], e[i][j]);
+            for (int j = 0; j < NS; ++j) h[j] = carried(A2[j] * sd[i], h[j], e[i][j], cut[i]);
         }
     }
 }

@@ -86,7 +86,7 @@ __global__ __launch_bounds__(64) void scan_carry_kernel(const ScanK k, bool forw
         for (int u = 0; u < AHEAD; ++u) {
             if (r0 + u >= k.items) break;
             k.edge[(forward ? r0 + u : k.items - 1 - r0 - u) * n + i] = h;
-            h = cut[u] ? e[u] : fmaf(exp2_fast(A2 * sd[u]), h, e[u]);
+            h = carried(A2 * sd[u], h, e[u], cut[u]);
         }
     }
 }
@@ -262,11 +262,11 @@ int scan_setup(const char* who, const vc_scan_args* a, int waves, ScanK* k) {
     VC_ARG(a->rows >= 0 && a->n_seqs > 0 && a->rows + (int64_t)TILE * a->n_seqs < (1LL << 31), "%s: bad sizes (rows %lld, n_seqs %d)", who, (long long)a->rows, a->n_seqs);
     VC_ARG(a->offsets || a->rows % a->n_seqs == 0, "%s: without offsets the rows divide into n_seqs equal utterances", who);
     for (int64_t ld : {a->x_ld, a->dt_ld, a->z ? a->z_ld : 0, a->b_ld, a->c_ld, a->y ? a->y_ld : 0, a->dy ? a->dy_ld : 0})
-        VC_ARG(ld >= 0 && ld <= MAX_LD && a->cols <= MAX_LD, "%s: row strides lie between 0 and 2^25 elements", who);
+        VC_ARG(ld >= 0 && ld <= MAX_LD && a->cols <= MAX_LD, "%s: row strides lie between 0 and 2^24 elements", who);
     if (a->rows > 1) {
         VC_ARG(!a->y || a->y_ld >= a->cols, "%s: rows of y overlap", who);
-        VC_ARG(!a->dx || (a->dx_ld >= a->cols && a->dx_ld <= MAX_LD && a->ddt_ld >= a->cols && a->ddt_ld <= MAX_LD), "%s: row strides of dx and ddt lie between cols and 2^25", who);
-        VC_ARG(!a->dz || (a->dz_ld >= a->cols && a->dz_ld <= MAX_LD), "%s: row strides of dz lie between cols and 2^25", who);
+        VC_ARG(!a->dx || (a->dx_ld >= a->cols && a->dx_ld <= MAX_LD && a->ddt_ld >= a->cols && a->ddt_ld <= MAX_LD), "%s: row strides of dx and ddt lie between cols and 2^24", who);
+        VC_ARG(!a->dz || (a->dz_ld >= a->cols && a->dz_ld <= MAX_LD), "%s: row strides of dz lie between cols and 2^24", who);
         VC_ARG(!a->dB || std::min(a->db_ld, a->dc_ld) >= (int64_t)a->groups * a->states, "%s: rows of dB or dC overlap", who);
     }
     *k = ScanK{};
@@ -281,8 +281,9 @@ int scan_setup(const char* who, const vc_scan_args* a, int waves, ScanK* k) {
     // utterances that run side by side for as long as the longest lasts
     const int64_t side = longest > 0 ? std::max<int64_t>(1, a->rows / longest) : a->n_seqs;
     k->items = a->n_seqs; k->chunk = 0;
-    if (side * row_waves < WALK_WAVES && longest >= 8 * TILE) {
-        const int64_t want = std::max<int64_t>(1, RUN_WAVES / row_waves);
+    const int64_t want = std::max<int64_t>(1, RUN_WAVES / row_waves);
+    // ... and runs where utterances are many and short: their first pass then has little to do, and the sums over items stay few
+    if ((side * row_waves < WALK_WAVES && longest >= 8 * TILE) || a->n_seqs > 4 * want) {
         k->chunk = (int)std::max<int64_t>(4, (k->slots + want - 1) / want);
         k->items = (k->slots + k->chunk - 1) / k->chunk;
         if (k->items == 1) { k->items = a->n_seqs; k->chunk = 0; }

@@ -320,7 +320,7 @@ def causal_conv1d_step(x, state, w, bias=None, slots=None, silu=True):
     """One frame of each of x's [streams, channels]: y, and `state` [pool, taps - 1, channels] moved on by a frame in place.
 
     slots (int32 [streams]): the stream's entry in the pool; without them stream i has entry i.  A stream whose slot lies outside the pool, or is
-    named by an earlier stream of the call, is padding: its y is zero and no state moves."""
+    named by an earlier stream of the call, is padding: its y is zero and no state moves.  At most 4096 streams a call with slots."""
     _activation(x, 'x')
     if not (x.dim() == 2 and x.shape[1] > 0):
         _refuse('x must be [streams, channels], got %s', tuple(x.shape))
