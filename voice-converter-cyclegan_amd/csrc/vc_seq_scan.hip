@@ -1,5 +1,6 @@
 // vc_seq_scan.hip -- selective state space scan: prompts and single frames (vc_seq_scan.h says how the work is laid out).
 #include "vc_seq_scan.h"
+#include <cmath>
 
 constexpr int FWD_WAVES = 4;
 
@@ -250,11 +251,13 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_st
     }
 }
 
-// Whole utterances where these fill the card side by side (WALK_WAVES: two waves a SIMD), else runs of slots, as many as make RUN_WAVES waves.  Runs cost
-// their first pass on top, about 0.7 of the main pass.  1 x 8192 x 1024 bf16, 16 states: 2880 us as one walk, 162 / 112 / 103 / 103 us with runs for
-// 1024 / 2048 / 4096 / 8192 waves; 64 x 128 x 1024 (4096 waves side by side): 54 us walked, 94 with runs.
-constexpr int64_t WALK_WAVES = 2048, RUN_WAVES = 4096;
-int scan_setup(const char* who, const vc_scan_args* a, int waves, ScanK* k) {
+// Whole utterances where these fill the card side by side (WALK_WAVES: two waves a SIMD), else runs of slots: as many as make run_waves waves, though
+// of no fewer than sqrt(slots / 32) slots, for a wave goes through all runs before its own.  Runs cost their first pass on top, 0.7 of the main pass.
+// Measured, bf16, 16 states: 1 x 8192 frames x 1024 channels 2880 us as one walk, 162 / 112 / 103 / 103 us in runs for 1024 / 2048 / 4096 / 8192 waves;
+// 1 x 128 x 1024 20 us walked, 10 in runs; 64 x 128 x 1024 (4096 waves side by side) 54 us walked, 94 in runs; 16 x 512 x 1024 (1024) 92 and 103, its
+// training step 380 and 332.
+constexpr int64_t WALK_WAVES = 2048, FWD_RUN_WAVES = 4096;
+int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_waves, ScanK* k) {
     VC_ARG(a, "%s: null pointer", who);
     VC_ARG(seq_type_ok(a->type), "%s: type must be VC_F32, VC_BF16 or VC_F16", who);
     VC_ARG(a->states >= 1 && a->states <= 64, "%s: 1 to 64 states, got %d", who, a->states);
@@ -281,10 +284,10 @@ int scan_setup(const char* who, const vc_scan_args* a, int waves, ScanK* k) {
     // utterances that run side by side for as long as the longest lasts
     const int64_t side = longest > 0 ? std::max<int64_t>(1, a->rows / longest) : a->n_seqs;
     k->items = a->n_seqs; k->chunk = 0;
-    const int64_t want = std::max<int64_t>(1, RUN_WAVES / row_waves);
+    const int64_t want = std::max<int64_t>(1, run_waves / row_waves);
     // ... and runs where utterances are many and short: their first pass then has little to do, and the sums over items stay few
-    if ((side * row_waves < WALK_WAVES && longest >= 8 * TILE) || a->n_seqs > 4 * want) {
-        k->chunk = (int)std::max<int64_t>(4, (k->slots + want - 1) / want);
+    if ((side * row_waves < WALK_WAVES && longest > 4 * TILE) || a->n_seqs > 4 * want) {
+        k->chunk = (int)std::max<int64_t>((int64_t)ceil(sqrt(k->slots / 32.0)), (k->slots + want - 1) / want);
         k->items = (k->slots + k->chunk - 1) / k->chunk;
         if (k->items == 1) { k->items = a->n_seqs; k->chunk = 0; }
     }
@@ -297,11 +300,11 @@ void scan_edge_place(ScanK* k, float* work) {
     k->cut = (int*)(k->sum_delta + (int64_t)k->items * k->a.cols);
 }
 extern "C" int64_t vc_selective_scan_saved(const vc_scan_args* a) {
-    ScanK k; if (scan_setup("vc_selective_scan_saved", a, FWD_WAVES, &k)) return VC_E_ARG;
+    ScanK k; if (scan_setup("vc_selective_scan_saved", a, FWD_WAVES, FWD_RUN_WAVES, &k)) return VC_E_ARG;
     return (int64_t)k.slots * a->cols * a->states;
 }
 extern "C" int64_t vc_selective_scan_fwd_work(const vc_scan_args* a) {
-    ScanK k; if (scan_setup("vc_selective_scan_fwd_work", a, FWD_WAVES, &k)) return VC_E_ARG;
+    ScanK k; if (scan_setup("vc_selective_scan_fwd_work", a, FWD_WAVES, FWD_RUN_WAVES, &k)) return VC_E_ARG;
     return scan_edge_floats(k);
 }
 
@@ -318,7 +321,7 @@ template <class T, int L, int NS> static int scan_fwd_l(const ScanK& k, hipStrea
 }
 template <class T> static int scan_fwd_t(const ScanK& k, hipStream_t s) { return SCAN_LAYOUT(T, k.a.states, scan_fwd_l, k, s); }
 extern "C" int vc_selective_scan_fwd(const vc_scan_args* a, void* stream) {
-    ScanK k; VC_CHECK(scan_setup("vc_selective_scan_fwd", a, FWD_WAVES, &k));
+    ScanK k; VC_CHECK(scan_setup("vc_selective_scan_fwd", a, FWD_WAVES, FWD_RUN_WAVES, &k));
     VC_ARG(a->A && (a->rows == 0 || (a->x && a->dt && a->B && a->C && a->y)), "vc_selective_scan_fwd: null pointer");
     VC_ARG(!a->final_state || a->final_state != a->initial, "vc_selective_scan_fwd: final_state may not be initial");
     if (a->saved && a->saved_floats < (int64_t)k.slots * a->cols * a->states) { vc_set_error("vc_selective_scan_fwd: saved is too small"); return VC_E_NOMEM; }
