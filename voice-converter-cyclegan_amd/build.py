@@ -71,7 +71,46 @@ def needs_build():
     return open(ID_FILE).read().strip() != build_id(os.environ.get('VC_EXTRA_FLAGS', '').split())
 
 
+# ---- the torch binding of the sequence operators (host code; everything it calls of the library it gets by address at import)
+BINDING_SOURCE = os.path.join(CSRC, 'vc_seq_torch.cpp')
+BINDING = os.path.join(HERE, '_seq.so')
+BINDING_FLAGS = ['-O2', '-std=c++17', '-fPIC', '-shared', '-Wall']
+
+
+def binding_id():
+    """Content hash of the binding's source, the header it is written against, its flags and the torch and Python it is built for."""
+    import hashlib
+    import sys
+    import torch
+    h = hashlib.sha256()
+    for f in (BINDING_SOURCE, os.path.join(HERE, '..', 'include', 'vc_cyclegan.h')):
+        with open(f, 'rb') as fh:
+            h.update(fh.read())
+        h.update(b'\0')
+    h.update(' '.join(BINDING_FLAGS + [torch.__version__, sys.version]).encode())
+    return h.hexdigest()[:16]
+
+
+def build_binding(force=False, verbose=True):
+    import sysconfig
+    import torch
+    bid, stamp = binding_id(), BINDING + '.buildid'
+    if not force and os.path.exists(BINDING) and os.path.exists(stamp) and open(stamp).read().strip() == bid:
+        return BINDING
+    root = os.path.dirname(torch.__file__)
+    cmd = [os.environ.get('CXX', 'g++')] + BINDING_FLAGS + ['-I' + os.path.join(root, 'include'), '-I' + os.path.join(root, 'include', 'torch', 'csrc', 'api', 'include'),
+           '-I' + sysconfig.get_paths()['include'], '-DVC_BINDING_ID="%s"' % bid, BINDING_SOURCE, '-o', BINDING, '-L' + os.path.join(root, 'lib'),
+           '-lc10', '-ltorch_cpu', '-ltorch', '-ltorch_python']
+    if verbose:
+        print('[vcgan] ' + ' '.join(cmd), flush=True)
+    _run(cmd, CSRC)
+    with open(stamp, 'w') as fh:
+        fh.write(bid + '\n')
+    return BINDING
+
+
 def build(force=False, verbose=True):
+    build_binding(force, verbose)
     if not force and not needs_build():
         return LIB
     hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
