@@ -179,7 +179,7 @@ __device__ __forceinline__ void wave_lds_fence() {
 
 // Where a lane works
 template <int L, int NS> struct Lane {
-    int lane, wave, j, c, n0, nn; bool ok; int g;
+    int lane, wave, j, c, n0, nn; bool ok, full; int g;
     __device__ __forceinline__ Lane(const ScanK& k, int waves, int blk) {
         lane = threadIdx.x & 63; wave = uniform(threadIdx.x >> 6);
         j = lane % L;
@@ -189,9 +189,16 @@ template <int L, int NS> struct Lane {
         c = g * k.cg + min(cb, k.cg - 1);
         n0 = j * NS;
         nn = max(0, min(NS, k.a.states - n0));
+        full = k.a.states == L * NS;
     }
 };
-template <int NS> __device__ __forceinline__ void load_state(const float* p, float (&h)[NS], int nn) { load_some<float, NS>(p, h, nn); }
+// a lane's states of a channel at p; `full` (the same in all lanes): none lacks any, so nothing waits for the answer of a branch
+template <int NS> __device__ __forceinline__ void load_state(const float* p, float (&h)[NS], int nn, bool full) {
+    if (full) load_vec<float, NS>(p, h); else load_some<float, NS>(p, h, nn);
+}
+template <int NS> __device__ __forceinline__ void store_state(float* p, const float (&h)[NS], int nn, bool full) {
+    if (full) store_vec<float, NS>(p, h); else store_some<float, NS>(p, h, nn);
+}
 
 // which register layout serves a number of states, and how many channels a block of `waves` waves covers
 #define SCAN_LAYOUT(T, states, F, ...) \
@@ -211,11 +218,11 @@ __device__ __forceinline__ float carried(float p, float h, float e, int cut) {
     return cut || h == 0.f ? e : fmaf(f * h, f, e);
 }
 int scan_carry(const ScanK& k, bool forward, hipStream_t s);
-template <int NS, bool FORWARD> __device__ __forceinline__ void carry_in(const ScanK& k, int item, int c, int n0, int nn, const float (&A2)[NS], float (&h)[NS]) {
+template <int NS, bool FORWARD> __device__ __forceinline__ void carry_in(const ScanK& k, int item, int c, int n0, int nn, bool full, const float (&A2)[NS], float (&h)[NS]) {
     constexpr int AT_ONCE = 8;                                   // runs whose loads are on their way together: the chain itself is one multiply-add a run
     const vc_scan_args& a = k.a;
     if (k.items > CARRY_ITEMS) {
-        load_state<NS>(k.edge + ((int64_t)item * a.cols + c) * a.states + n0, h, nn);
+        load_state<NS>(k.edge + ((int64_t)item * a.cols + c) * a.states + n0, h, nn, full);
         return;
     }
     const int n = FORWARD ? item : k.items - 1 - item;           // runs to go through, the farthest first
@@ -224,7 +231,7 @@ template <int NS, bool FORWARD> __device__ __forceinline__ void carry_in(const S
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
             const int at = min(i0 + i, n - 1), r = FORWARD ? at : k.items - 1 - at;
-            load_state<NS>(k.edge + ((int64_t)r * a.cols + c) * a.states + n0, e[i], nn);
+            load_state<NS>(k.edge + ((int64_t)r * a.cols + c) * a.states + n0, e[i], nn, full);
             sd[i] = k.sum_delta[(int64_t)r * a.cols + c];
             cut[i] = k.cut[r];
         }

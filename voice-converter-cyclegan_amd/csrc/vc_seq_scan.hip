@@ -15,7 +15,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_ed
     const Rows<T, L> X(a.x, a.x_ld, a.cols, c, j), DT(a.dt, a.dt_ld, a.cols, c, j);
     const States<T, NP> B(a.B, a.b_ld, w.g, a.states, w.lane);
     float A2[NS], h[NS];
-    load_state<NS>(a.A + (int64_t)c * a.states + n0, A2, nn);
+    load_state<NS>(a.A + (int64_t)c * a.states + n0, A2, nn, w.full);
 #pragma unroll
     for (int i = 0; i < NS; ++i) { A2[i] *= LOG2E; h[i] = 0.f; }
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f;
@@ -24,7 +24,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_ed
     Cursor cur(k.m);
     cur.find(q1 - 1);
     const bool cut = cur.base >= q0;                             // an utterance begins in this run
-    if (cut && a.initial) load_state<NS>(a.initial + ((int64_t)cur.s * a.cols + c) * a.states + n0, h, nn);
+    if (cut && a.initial) load_state<NS>(a.initial + ((int64_t)cur.s * a.cols + c) * a.states + n0, h, nn, w.full);
     float* Bs = lds[w.wave];
     float sd = 0.f;
     const int k0 = max(q0 - cur.base, 0), k1 = min(cur.tiles, q1 - cur.base);
@@ -60,7 +60,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_ed
     }
     sd = channel_sum<L>(sd);
     if (w.ok) {
-        store_some<float, NS>(k.edge + ((int64_t)item * a.cols + c) * a.states + n0, h, nn);
+        store_state<NS>(k.edge + ((int64_t)item * a.cols + c) * a.states + n0, h, nn, w.full);
         if (j == 0) k.sum_delta[(int64_t)item * a.cols + c] = sd;
     }
     if (blk == 0 && threadIdx.x == 0) k.cut[item] = cut;
@@ -125,7 +125,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_fw
     const Rows<T, L> X(a.x, a.x_ld, a.cols, c, j), DT(a.dt, a.dt_ld, a.cols, c, j), Z(has_z ? a.z : a.x, has_z ? a.z_ld : a.x_ld, a.cols, c, j);
     const States<T, NP> B(a.B, a.b_ld, w.g, a.states, w.lane), C(a.C, a.c_ld, w.g, a.states, w.lane);
     float A2[NS], h[NS];
-    load_state<NS>(a.A + (int64_t)c * a.states + n0, A2, nn);
+    load_state<NS>(a.A + (int64_t)c * a.states + n0, A2, nn, w.full);
 #pragma unroll
     for (int i = 0; i < NS; ++i) { A2[i] *= LOG2E; h[i] = 0.f; }
     const float Dc = a.D ? a.D[c] : 0.f, bias = a.dt_bias ? a.dt_bias[c] : 0.f;
@@ -133,7 +133,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_fw
     item_slots(k, item, q0, q1);
     Cursor cur(k.m);
     if (k.chunk) cur.find(q0); else cur.load(item);
-    if (k.chunk && q0 > cur.base) carry_in<NS, true>(k, item, c, n0, nn, A2, h);
+    if (k.chunk && q0 > cur.base) carry_in<NS, true>(k, item, c, n0, nn, w.full, A2, h);
     float *Bs = lds[w.wave][0], *Cs = lds[w.wave][1];
     for (int q = q0; q < q1;) {                                  // the utterances of the item
         const int64_t hs = ((int64_t)cur.s * a.cols + c) * a.states + n0;
@@ -141,7 +141,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_fw
         if (q == cur.base) {
 #pragma unroll
             for (int i = 0; i < NS; ++i) h[i] = 0.f;
-            if (a.initial) load_state<NS>(a.initial + hs, h, nn);
+            if (a.initial) load_state<NS>(a.initial + hs, h, nn, w.full);
         }
         T xr[NB], tr[NB], zr[NB], br[NP / 4], cr[NP / 4];
         auto fetch = [&](int kt) {
@@ -153,7 +153,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_fw
         if (k0 < k1) fetch(k0);
         for (int kt = k0; kt < k1; ++kt) {
             const int row0 = cur.begin + kt * TILE, nr = min(TILE, cur.end - row0);
-            if (a.saved && w.ok) store_some<float, NS>(a.saved + ((int64_t)(cur.base + kt) * a.cols + c) * a.states + n0, h, nn);
+            if (a.saved && w.ok) store_state<NS>(a.saved + ((int64_t)(cur.base + kt) * a.cols + c) * a.states + n0, h, nn, w.full);
             B.stage(br, nr, Bs); C.stage(cr, nr, Cs);
             float delta[NB], dtx[NB], gate[NB], skip[NB];
 #pragma unroll
@@ -196,7 +196,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_fw
             });
             wave_lds_fence();
         }
-        if (a.final_state && w.ok && (cur.tiles ? k0 < cur.tiles && k1 == cur.tiles : q == cur.base)) store_some<float, NS>(a.final_state + hs, h, nn);
+        if (a.final_state && w.ok && (cur.tiles ? k0 < cur.tiles && k1 == cur.tiles : q == cur.base)) store_state<NS>(a.final_state + hs, h, nn, w.full);
         if (cur.next >= q1) break;
         q = max(cur.next, q + 1);
         cur.load(cur.s + 1);
@@ -222,8 +222,9 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_st
         const int c = min(c0 + u * G, a.cols - 1), g = c / wide;
         const float *hp = a.state + ((int64_t)at * a.cols + c) * a.states + n0, *ap = a.A + (int64_t)c * a.states + n0;
         const T *bp = (const T*)a.B + r * a.b_ld + g * a.states + n0, *cp = (const T*)a.C + r * a.c_ld + g * a.states + n0;
-        if (full) { load_vec<float, NS>(hp, h[u]); load_vec<float, NS>(ap, A[u]); load_vec<T, NS>(bp, B[u]); load_vec<T, NS>(cp, C[u]); }
-        else { load_some<float, NS>(hp, h[u], nn); load_some<float, NS>(ap, A[u], nn); load_some<T, NS>(bp, B[u], nn); load_some<T, NS>(cp, C[u], nn); }
+        load_state<NS>(hp, h[u], nn, full); load_state<NS>(ap, A[u], nn, full);
+        if (full) { load_vec<T, NS>(bp, B[u]); load_vec<T, NS>(cp, C[u]); }
+        else { load_some<T, NS>(bp, B[u], nn); load_some<T, NS>(cp, C[u], nn); }
         x[u] = (float)((const T*)a.x)[r * a.x_ld + c];
         v[u] = (float)((const T*)a.dt)[r * a.dt_ld + c] + (a.dt_bias ? a.dt_bias[c] : 0.f);
         z[u] = a.z ? (float)((const T*)a.z)[r * a.z_ld + c] : 0.f;
@@ -245,7 +246,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_st
             sum = fmaf(C[u][e], h[u][e], sum);
         }
         float* hp = a.state + ((int64_t)mine * a.cols + c) * a.states + n0;
-        if (full) store_vec<float, NS>(hp, h[u]); else store_some<float, NS>(hp, h[u], nn);
+        store_state<NS>(hp, h[u], nn, full);
         sum = channel_sum<L>(sum) + D[u] * x[u];
         if (j == 0) *y = (T)(a.z ? sum * (z[u] * sigmoid_acc(z[u])) : sum);
     }

@@ -4,7 +4,7 @@
 // A tile's states are worked out again from the one the forward kept in front of it: a and h of its 16 rows stay in registers for the way back.
 #include "vc_seq_scan.h"
 
-template <int L> constexpr int BWD_WAVES = L == 4 ? 8 : 4;      // LDS: B and C of each wave, and its share of dB and dC
+constexpr int BWD_WAVES = 4;                                     // of a block.  8 leave half as many partial sums of dB and dC and cost 2 %: more waves stand at a barrier together
 
 template <int NS> struct Row {                                    // B and C of a row, a lane's states
     float b[NS], c[NS];
@@ -75,7 +75,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * EDGE_WAVES) 
     const Rows<T, L> DT(a.dt, a.dt_ld, a.cols, c, j), DY(a.dy, a.dy_ld, a.cols, c, j), Z(has_z ? a.z : a.dy, has_z ? a.z_ld : a.dy_ld, a.cols, c, j);
     const States<T, NP> C(a.C, a.c_ld, w.g, a.states, w.lane);
     float A2[NS], dhc[NS];
-    load_state<NS>(a.A + (int64_t)c * a.states + n0, A2, nn);
+    load_state<NS>(a.A + (int64_t)c * a.states + n0, A2, nn, w.full);
 #pragma unroll
     for (int i = 0; i < NS; ++i) { A2[i] *= LOG2E; dhc[i] = 0.f; }
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f;
@@ -84,7 +84,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * EDGE_WAVES) 
     Cursor cur(k.m);
     cur.find(q0);
     const bool begins = q0 <= cur.base, ends = cur.base + cur.tiles <= q1;
-    if (ends && a.dfinal && w.ok) load_state<NS>(a.dfinal + ((int64_t)cur.s * a.cols + c) * a.states + n0, dhc, nn);
+    if (ends && a.dfinal && w.ok) load_state<NS>(a.dfinal + ((int64_t)cur.s * a.cols + c) * a.states + n0, dhc, nn, w.full);
     float* Cs = lds[w.wave];
     float sd = 0.f;
     const int k0 = max(q0 - cur.base, 0), k1 = begins ? k0 : min(cur.tiles, q1 - cur.base);
@@ -125,16 +125,16 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * EDGE_WAVES) 
     }
     sd = channel_sum<L>(sd);
     if (w.ok) {
-        store_some<float, NS>(k.edge + ((int64_t)item * a.cols + c) * a.states + n0, dhc, nn);
+        store_state<NS>(k.edge + ((int64_t)item * a.cols + c) * a.states + n0, dhc, nn, w.full);
         if (j == 0) k.sum_delta[(int64_t)item * a.cols + c] = sd;
     }
     if (blk == 0 && threadIdx.x == 0) k.cut[item] = begins || ends;
 }
 
 // Rows whose decays are worked out a second time on the way back: 4 NS registers for 4 NS exponentials of a tile, without which some would spill
-template <class T> constexpr int AGAIN = sizeof(T) == 4 ? 5 : 4;
-template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES<L>, 1) void scan_bwd_kernel(const ScanK k) {
-    constexpr int NP = L * NS, NB = TILE / L, WV = BWD_WAVES<L>, R = RED<L, NS>;
+template <class T> constexpr int AGAIN = sizeof(T) == 4 ? 6 : 4;
+template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES, L == 16 && NS == 4 ? 1 : 2) void scan_bwd_kernel(const ScanK k) {
+    constexpr int NP = L * NS, NB = TILE / L, WV = BWD_WAVES, R = RED<L, NS>;
     __shared__ float lds[WV][2][TILE * NP];
     __shared__ float red[2][WV][TILE * R];                       // two of them: one barrier a tile
     const vc_scan_args& a = k.a;
@@ -152,7 +152,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES<L>
     const Rows<T, L> X(a.x, a.x_ld, a.cols, c, j), DT(a.dt, a.dt_ld, a.cols, c, j), DY(a.dy, a.dy_ld, a.cols, c, j), Z(has_z ? a.z : a.dy, has_z ? a.z_ld : a.dy_ld, a.cols, c, j);
     const States<T, NP> B(a.B, a.b_ld, w.g, a.states, w.lane), C(a.C, a.c_ld, w.g, a.states, w.lane);
     float A2[NS], dA[NS], dhc[NS];
-    load_state<NS>(a.A + (int64_t)c * a.states + n0, A2, nn);
+    load_state<NS>(a.A + (int64_t)c * a.states + n0, A2, nn, w.full);
 #pragma unroll
     for (int i = 0; i < NS; ++i) { A2[i] *= LOG2E; dA[i] = 0.f; dhc[i] = 0.f; }
     const float Dc = a.D ? a.D[c] : 0.f, bias = a.dt_bias ? a.dt_bias[c] : 0.f;
@@ -160,7 +160,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES<L>
     item_slots(k, item, q0, q1);
     Cursor cur(k.m);
     if (k.chunk) cur.find(q1 - 1); else cur.load(item);
-    if (k.chunk && cur.base + cur.tiles > q1) carry_in<NS, false>(k, item, c, n0, nn, A2, dhc);
+    if (k.chunk && cur.base + cur.tiles > q1) carry_in<NS, false>(k, item, c, n0, nn, w.full, A2, dhc);
     float dDacc = 0.f, dbacc = 0.f;
     float *Bs = lds[w.wave][0], *Cs = lds[w.wave][1];
     int turn = 0;
@@ -170,21 +170,24 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES<L>
       if (cur.base + cur.tiles <= q1) {                          // its end lies in this item
 #pragma unroll
         for (int i = 0; i < NS; ++i) dhc[i] = 0.f;
-        if (a.dfinal && w.ok) load_state<NS>(a.dfinal + hs, dhc, nn);
+        if (a.dfinal && w.ok) load_state<NS>(a.dfinal + hs, dhc, nn, w.full);
       }
       T xr[NB], tr[NB], gr[NB], zr[NB], br[NP / 4], cr[NP / 4];
-      float h0[NS];
+      float hn[NS];                                              // the state in front of the tile
       auto fetch = [&](int kt) {
         const int row0 = cur.begin + kt * TILE, nr = min(TILE, cur.end - row0);
         X.load(row0, nr, xr); DT.load(row0, nr, tr); DY.load(row0, nr, gr);
         if (has_z) Z.load(row0, nr, zr);
         B.load(row0, nr, br); C.load(row0, nr, cr);
+        load_state<NS>(a.saved + ((int64_t)(cur.base + kt) * a.cols + c) * a.states + n0, hn, nn, w.full);
       };
       if (k0 < k1) fetch(k1 - 1);
       for (int kt = k1 - 1; kt >= k0; --kt) {
         const int row0 = cur.begin + kt * TILE, nr = min(TILE, cur.end - row0);
         float* mine = red[turn][w.wave];
-        load_state<NS>(a.saved + ((int64_t)(cur.base + kt) * a.cols + c) * a.states + n0, h0, nn);
+        float h0[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) h0[i] = hn[i];
         B.stage(br, nr, Bs); C.stage(cr, nr, Cs);
         float xv[NB], delta[NB], slope[NB], dtx[NB], dp[NB], dzf[NB];
 #pragma unroll
@@ -286,12 +289,12 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES<L>
         }
         turn ^= 1;
       }
-      if (cur.base >= q0 && a.dinitial && w.ok) store_some<float, NS>(a.dinitial + hs, dhc, nn);       // its beginning lies in this item
+      if (cur.base >= q0 && a.dinitial && w.ok) store_state<NS>(a.dinitial + hs, dhc, nn, w.full);       // its beginning lies in this item
       if (cur.base <= q0 || cur.s == 0) break;
       q = min(cur.base, q) - 1;
       cur.load(cur.s - 1);
     }
-    if (w.ok) store_some<float, NS>(k.dapart + ((int64_t)item * a.cols + c) * a.states + n0, dA, nn);
+    if (w.ok) store_state<NS>(k.dapart + ((int64_t)item * a.cols + c) * a.states + n0, dA, nn, w.full);
     const float d = channel_sum<L>(dDacc), b = channel_sum<L>(dbacc);
     if (w.ok && j == 0) {
         k.chpart[((int64_t)item * 2) * a.cols + c] = d;
@@ -349,7 +352,7 @@ template <class T> __global__ __launch_bounds__(256) void scan_finish_kernel(con
 constexpr int64_t BWD_RUN_WAVES = 2048;                          // two waves a SIMD is what its registers allow
 static int bwd_setup(const char* who, const vc_scan_args* a, ScanK* k, int64_t* floats) {
     VC_ARG(a, "%s: null pointer", who);
-    VC_CHECK(scan_setup(who, a, a->states <= 16 ? BWD_WAVES<4> : BWD_WAVES<16>, BWD_RUN_WAVES, k));
+    VC_CHECK(scan_setup(who, a, BWD_WAVES, BWD_RUN_WAVES, k));
     const int64_t part = (int64_t)a->groups * k->nblk * a->rows * 2 * scan_padded(a->states);
     const int64_t da = (int64_t)k->items * a->cols * a->states, ch = (int64_t)k->items * 2 * a->cols;
     *floats = part + da + ch + scan_edge_floats(*k);
@@ -371,7 +374,7 @@ template <class T, int L, int NS> static int scan_bwd_l(const ScanK& k, hipStrea
         hipLaunchKernelGGL((scan_bwd_edge_kernel<T, L, NS>), dim3((unsigned)eb), dim3(64 * EDGE_WAVES), 0, s, k, nblk1);
         VC_CHECK(scan_carry(k, false, s));
     }
-    hipLaunchKernelGGL((scan_bwd_kernel<T, L, NS>), dim3((unsigned)blocks), dim3(64 * BWD_WAVES<L>), 0, s, k);
+    hipLaunchKernelGGL((scan_bwd_kernel<T, L, NS>), dim3((unsigned)blocks), dim3(64 * BWD_WAVES), 0, s, k);
     const int64_t pc = ((int64_t)k.a.cols * (k.a.states + 2) + 63) / 64;
     VC_ARG(bc + pc < (1LL << 31), "vc_selective_scan_bwd: too many rows and channels for one launch");
     hipLaunchKernelGGL((scan_finish_kernel<T>), dim3((unsigned)(bc + pc)), dim3(256), 0, s, k, L * NS, (int)bc);
