@@ -5,7 +5,7 @@
 // apart from the K - 1 frames ahead of a run.
 #include "vc_seq.h"
 
-struct ConvArgs { vc_conv1d_args a; SeqMap m; int v, cv, cvb, runs; float* part; };     // v channels a thread, cv such vectors, cvb of them next to each other
+struct ConvArgs { vc_conv1d_args a; SeqMap m; int v, cv, cvb, run, runs; float* part; };   // v channels a thread, cv such vectors, cvb of them next to each other; runs of `run` rows
 
 // the utterance row r lies in: the last s with begin(s) <= r; n_seqs where r lies behind the last utterance
 __device__ __forceinline__ int seq_of(const SeqMap& m, int r) {
@@ -37,35 +37,59 @@ template <class T, int K, int V> struct Filter {
     }
 };
 // A block's threads: cvb vectors of channels (a power of two) next to each other, 256 / cvb runs of rows
-// Rows of a run, and rows whose loads are issued together while as many are worked on.  8192 x 2048 bf16, 4 taps, forward and backward: 46.5 us
-// with (8, 16; 4, 2); 49.6 with (16, 16; 4, 4), 51.9 with (16, 16; 2, 2), 47.4 with (32, 32; 4, 4), which gives small calls too few threads.
-constexpr int FWD_RUN = 8, BWD_RUN = 16, FWD_AHEAD = 4, BWD_AHEAD = 2;
+// Longest and shortest run of rows, and the waves below which a run is halved.  Long runs repeat fewer frames ahead of them (the gradient: and behind
+// them, with their sigmoids), short ones leave enough threads.  Gradient of 8192 x 2048 bf16, 4 taps, with its forward pass: 45.7 us by runs of 32, 51.7
+// by 16, 55.8 by 64; of 1024 x 512: 16 by 8, 18.6 by 16, 23.7 by 32.  Forward alone, 9001 x 1000 fp32: 17.2 by 8, 17.7 by 4 and by 16.
+constexpr int FWD_RUN = 8, FWD_SHORT = 4, BWD_RUN = 32, BWD_SHORT = 8, RUN_WAVES = 1024;
+// Rows worked on while as many are on their way: with two in the forward pass 18.0 us in place of 17.2, in the gradient 48.9 in place of 45.7.
+constexpr int AHEAD = 4;
 constexpr int BWD_V = 4;                                         // channels of a thread of the gradient
 constexpr int FWD_WIDE = 32, BWD_WIDE = 64;                      // most vectors of channels next to each other in a block
-struct Place { int c, run; bool ok; };
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+struct Place { int c, run, base; bool ok; };                     // base: first row of the block's first run
 __device__ __forceinline__ Place place(const ConvArgs& k, int V) {
     const int blocks = (k.cv + k.cvb - 1) / k.cvb;
     Place p;
     const int v = (int)(blockIdx.x % blocks) * k.cvb + threadIdx.x % k.cvb;
-    p.run = (int)(blockIdx.x / blocks) * (256 / k.cvb) + threadIdx.x / k.cvb;
+    const int first = (int)(blockIdx.x / blocks) * (256 / k.cvb);
+    p.run = first + threadIdx.x / k.cvb;
+    p.base = min(first, k.runs - 1) * k.run;
     // the last vector ends with the last channel: where V does not divide the channels it works out some of its neighbour's once more, to the same
     // values, and no access has to ask how many channels are left (fewer than V of them: V = 1)
     p.c = min(v * V, k.a.cols - V); p.ok = v < k.cv;
     return p;
 }
 
+// The rows that a block's threads work on, of one tensor, through a buffer descriptor: a row is a 32-bit offset (one addition from row to row), rows behind
+// the tensor read as zeros, and an offset of NOWHERE reads zeros and stores nothing, which serves in place of branches.  Host code sees to it that a
+// block's rows span less than 2^31 bytes.
+constexpr unsigned NOWHERE = 0xf0000000u;
+template <class T, int V> struct Span {
+    __amdgpu_buffer_rsrc_t rs; unsigned ld;                      // bytes from row to row
+    __device__ __forceinline__ Span(const void* p, int64_t stride, int base, int rows, int cols) : ld((unsigned)stride * (unsigned)sizeof(T)) {
+        const int64_t bytes = ((int64_t)(rows - base - 1) * stride + cols) * (int64_t)sizeof(T);
+        rs = __builtin_amdgcn_make_buffer_rsrc((void*)((const T*)p + (int64_t)base * stride), 0, (int)min(bytes, (int64_t)0x7fffffff), 0x00020000);
+    }
+    __device__ __forceinline__ void store(unsigned at, const float (&f)[V]) const {
+        Pack<T, V> q;
+#pragma unroll
+        for (int i = 0; i < V; ++i) q.v[i] = (T)f[i];
+        if constexpr (V * sizeof(T) == 16) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, q), rs, at, 0, 0);
+        else if constexpr (V * sizeof(T) == 8) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, q), rs, at, 0, 0);
+        else if constexpr (V * sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, q), rs, at, 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, q), rs, at, 0, 0);
+    }
+};
 // V elements as they came: 16-bit ones two to a register
 template <class T, int V> struct Raw {
     static constexpr int N = (V * (int)sizeof(T) + 3) / 4;
     unsigned w[N];
-    __device__ __forceinline__ void load(const T* p) {
-        if constexpr (V * sizeof(T) % 4 != 0) w[0] = __builtin_bit_cast(unsigned short, *p);
-        else {
-            struct __attribute__((packed, aligned(sizeof(T)))) W { unsigned v[N]; };
-            const W q = *(const W*)p;
-#pragma unroll
-            for (int i = 0; i < N; ++i) w[i] = q.v[i];
-        }
+    __device__ __forceinline__ void load(const Span<T, V>& s, unsigned at) {
+        if constexpr (N == 4) { const u32x4 q = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(s.rs, at, 0, 0)); w[0] = q[0]; w[1] = q[1]; w[2] = q[2]; w[3] = q[3]; }
+        else if constexpr (N == 2) { const u32x2 q = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(s.rs, at, 0, 0)); w[0] = q[0]; w[1] = q[1]; }
+        else if constexpr (sizeof(T) == 4) w[0] = __builtin_amdgcn_raw_buffer_load_b32(s.rs, at, 0, 0);
+        else w[0] = __builtin_amdgcn_raw_buffer_load_b16(s.rs, at, 0, 0);
     }
     __device__ __forceinline__ void get(float (&f)[V]) const {
 #pragma unroll
@@ -75,7 +99,7 @@ template <class T, int V> struct Raw {
         }
     }
 };
-template <class T, int K, int V> __global__ __launch_bounds__(256) void conv1d_fwd_kernel(const ConvArgs k) {
+template <class T, int K, int V, bool SILU> __global__ __launch_bounds__(256) void conv1d_fwd_kernel(const ConvArgs k) {
     const vc_conv1d_args& a = k.a;
     const Place p = place(k, V);
     if (!p.ok) return;
@@ -92,14 +116,14 @@ template <class T, int K, int V> __global__ __launch_bounds__(256) void conv1d_f
         return;
     }
     const Filter<T, K, V> w(a, p.c);
-    int r = p.run * FWD_RUN;
-    const int r1 = min(r + FWD_RUN, k.m.rows);
-    const T* x = (const T*)a.x + p.c;
-    T* y = (T*)a.y + p.c;
+    int r = p.run * k.run;
+    const int r1 = min(r + k.run, k.m.rows);
+    const Span<T, V> X(a.x, a.x_ld, p.base, k.m.rows, a.cols), Y(a.y, a.y_ld, p.base, k.m.rows, a.cols);
+    const unsigned ch = p.c * (unsigned)sizeof(T);
     for (int s = seq_of(k.m, r); r < r1; ++s) {
         if (s >= k.m.n_seqs) {                                   // rows behind the last utterance
-            float f[V] = {};
-            if (a.zero_tail) for (; r < r1; ++r) store_vec<T, V>(y + (int64_t)r * a.y_ld, f);
+            const float f[V] = {};
+            if (a.zero_tail) for (; r < r1; ++r) Y.store((r - p.base) * Y.ld + ch, f);
             return;
         }
         const int b = seq_begin(k.m, s), hi = min(seq_end(k.m, s, b), r1);
@@ -107,47 +131,40 @@ template <class T, int K, int V> __global__ __launch_bounds__(256) void conv1d_f
         float win[K][V];
 #pragma unroll
         for (int i = 0; i < K - 1; ++i) frame<T, V>(a, s, b, r - b - (K - 1) + i, p.c, win[i]);
-        auto step = [&](const float (&f)[V]) {
-            float o[V];
+        unsigned from = (r - p.base) * X.ld + ch, to = (r - p.base) * Y.ld + ch;
+        // AHEAD rows are worked on while the next are on their way; what rows past the end give is dropped
+        Raw<T, V> next[AHEAD];
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                win[K - 1][e] = f[e];
-                float q = w.b[e];
+        for (int i = 0; i < AHEAD; ++i) next[i].load(X, from + i * X.ld);
+        for (; r < hi; r += AHEAD) {
+            Raw<T, V> now[AHEAD];
+            from += AHEAD * X.ld;
 #pragma unroll
-                for (int i = 0; i < K; ++i) q = fmaf(w.w[i][e], win[i][e], q);
-                o[e] = a.silu ? q * sigmoid_acc(q) : q;
+            for (int i = 0; i < AHEAD; ++i) { now[i] = next[i]; next[i].load(X, r + AHEAD < hi ? from + i * X.ld : NOWHERE); }
 #pragma unroll
-                for (int i = 0; i < K - 1; ++i) win[i][e] = win[i + 1][e];
+            for (int i = 0; i < AHEAD; ++i) {
+                now[i].get(win[K - 1]);
+                float o[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    float q = w.b[e];
+#pragma unroll
+                    for (int j = 0; j < K; ++j) q = fmaf(w.w[j][e], win[j][e], q);
+                    o[e] = SILU ? q * sigmoid_acc(q) : q;
+#pragma unroll
+                    for (int j = 0; j < K - 1; ++j) win[j][e] = win[j + 1][e];
+                }
+                Y.store(r + i < hi ? to + i * Y.ld : NOWHERE, o);
             }
-            store_vec<T, V>(y + (int64_t)r * a.y_ld, o);
-            ++r;
-        };
-        // FWD_AHEAD rows are worked on while the next are on their way; rows past the end read the last one and are not used
-        Raw<T, V> next[FWD_AHEAD];
-        auto fetch = [&](int at) {
-#pragma unroll
-            for (int i = 0; i < FWD_AHEAD; ++i) next[i].load(x + (int64_t)min(at + i, hi - 1) * a.x_ld);
-        };
-        fetch(r);
-        while (r < hi) {
-            Raw<T, V> now[FWD_AHEAD];
-#pragma unroll
-            for (int i = 0; i < FWD_AHEAD; ++i) now[i] = next[i];
-            if (r + FWD_AHEAD < hi) fetch(r + FWD_AHEAD);
-#pragma unroll
-            for (int i = 0; i < FWD_AHEAD; ++i) {
-                if (r >= hi) break;
-                float f[V];
-                now[i].get(f);
-                step(f);
-            }
+            to += AHEAD * Y.ld;
         }
+        r = hi;
     }
 }
 
 // g of one frame, from the K frames it looks at
-template <int K, int V> __device__ __forceinline__ void pre_gradient(const float (&win)[K][V], const float (&w)[K][V], const float (&b)[V], bool silu, float (&g)[V]) {
-    if (!silu) return;
+template <bool SILU, int K, int V> __device__ __forceinline__ void pre_gradient(const float (&win)[K][V], const float (&w)[K][V], const float (&b)[V], float (&g)[V]) {
+    if constexpr (!SILU) return;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         float q = b[e];
@@ -160,21 +177,23 @@ template <int K, int V> __device__ __forceinline__ void pre_gradient(const float
 // A run's dx needs the K - 1 frames' g behind it as well: they are worked out again there.  dx of a frame gathers in a register ring while the
 // frames that look at it go by.
 // Four channels a thread: eight would fill the registers (filter, window, ring and its share of dw are K vectors each) and leave too few waves to wait with.
-template <class T, int K, int V> __global__ __launch_bounds__(256) void conv1d_bwd_kernel(const ConvArgs k) {
+template <class T, int K, int V, bool SILU> __global__ __launch_bounds__(256) void conv1d_bwd_kernel(const ConvArgs k) {
     __shared__ float red[256 * V];
     const vc_conv1d_args& a = k.a;
     const Place p = place(k, V);
     float dw[K][V] = {}, db[V] = {};
     if (p.ok && p.run < k.runs) {
         const Filter<T, K, V> w(a, p.c);
-        int r = p.run * BWD_RUN;
-        const int r1 = min(r + BWD_RUN, k.m.rows);
-        const T *x = (const T*)a.x + p.c, *dy = (const T*)a.dy + p.c;
-        T* dx = a.dx ? (T*)a.dx + p.c : nullptr;
+        int r = p.run * k.run;
+        const int r1 = min(r + k.run, k.m.rows);
+        const bool want_dx = a.dx != nullptr;
+        const Span<T, V> X(a.x, a.x_ld, p.base, k.m.rows, a.cols), DY(a.dy, a.dy_ld, p.base, k.m.rows, a.cols),
+            DX(want_dx ? a.dx : a.dy, want_dx ? a.dx_ld : a.dy_ld, p.base, k.m.rows, a.cols);
+        const unsigned ch = p.c * (unsigned)sizeof(T);
         for (int s = seq_of(k.m, r); r < r1; ++s) {
             if (s >= k.m.n_seqs) {
-                float f[V] = {};
-                if (a.zero_tail && dx) for (; r < r1; ++r) store_vec<T, V>(dx + (int64_t)r * a.dx_ld, f);
+                const float f[V] = {};
+                if (a.zero_tail && want_dx) for (; r < r1; ++r) DX.store((r - p.base) * DX.ld + ch, f);
                 break;
             }
             const int b = seq_begin(k.m, s), end = seq_end(k.m, s, b), lo = r, hi = min(end, r1);
@@ -182,66 +201,56 @@ template <class T, int K, int V> __global__ __launch_bounds__(256) void conv1d_b
             float win[K][V], ring[K][V] = {};                    // ring[i]: dx of frame r - (K-1) + i so far
 #pragma unroll
             for (int i = 0; i < K - 1; ++i) frame<T, V>(a, s, b, lo - b - (K - 1) + i, p.c, win[i]);
-            auto emit = [&](int at, const float (&d)[V]) {       // row `at` has all but its share of the final state's gradient
-                if (!dx || at < lo || at >= hi) return;
-                float o[V] = {};
-                if (a.dfinal && at >= end - (K - 1))
-                    load_vec<T, V>((const T*)a.dfinal + ((int64_t)s * (K - 1) + at - (end - (K - 1))) * a.cols + p.c, o);
-#pragma unroll
-                for (int e = 0; e < V; ++e) o[e] += d[e];
-                store_vec<T, V>(dx + (int64_t)at * a.dx_ld, o);
-            };
-            auto step = [&](const float (&f)[V], float (&g)[V]) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) win[K - 1][e] = f[e];
-                pre_gradient<K, V>(win, w.w, w.b, a.silu, g);
-                if (r < hi) {
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        db[e] += g[e];
-#pragma unroll
-                        for (int i = 0; i < K; ++i) dw[i][e] = fmaf(g[e], win[i][e], dw[i][e]);
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-#pragma unroll
-                    for (int i = 0; i < K; ++i) ring[i][e] = fmaf(w.w[i][e], g[e], ring[i][e]);
-                emit(r - (K - 1), ring[0]);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-#pragma unroll
-                    for (int i = 0; i < K - 1; ++i) { win[i][e] = win[i + 1][e]; ring[i][e] = ring[i + 1][e]; }
-                    ring[K - 1][e] = 0.f;
-                }
-                ++r;
-            };
-            const int stop = min(end, hi + (dx ? K - 1 : 0));
-            // BWD_AHEAD rows are worked on while the next are on their way; rows past the end read the last one and are not used
-            Raw<T, V> xn[BWD_AHEAD], gn[BWD_AHEAD];
+            // K - 1 rows more than the run's: their g where the utterance has them, zeros behind its end.  AHEAD rows are worked on while the next are
+            // on their way
+            const int stop = want_dx ? hi + K - 1 : hi;
+            unsigned xo = (r - p.base) * X.ld + ch, go = (r - p.base) * DY.ld + ch, to = (r - (K - 1) - p.base) * DX.ld + ch;
+            Raw<T, V> xn[AHEAD], gn[AHEAD];
             auto fetch = [&](int at) {
 #pragma unroll
-                for (int i = 0; i < BWD_AHEAD; ++i) {
-                    const int64_t row = min(at + i, stop - 1);
-                    xn[i].load(x + row * a.x_ld); gn[i].load(dy + row * a.dy_ld);
+                for (int i = 0; i < AHEAD; ++i) {
+                    const bool in = at + i < min(end, stop);
+                    xn[i].load(X, in ? xo + i * X.ld : NOWHERE); gn[i].load(DY, in ? go + i * DY.ld : NOWHERE);
                 }
+                xo += AHEAD * X.ld; go += AHEAD * DY.ld;
             };
             fetch(r);
-            while (r < stop) {
-                Raw<T, V> xc[BWD_AHEAD], gc[BWD_AHEAD];
+            for (; r < stop; r += AHEAD) {
+                Raw<T, V> xc[AHEAD], gc[AHEAD];
 #pragma unroll
-                for (int i = 0; i < BWD_AHEAD; ++i) { xc[i] = xn[i]; gc[i] = gn[i]; }
-                if (r + BWD_AHEAD < stop) fetch(r + BWD_AHEAD);
+                for (int i = 0; i < AHEAD; ++i) { xc[i] = xn[i]; gc[i] = gn[i]; }
+                fetch(r + AHEAD);
 #pragma unroll
-                for (int i = 0; i < BWD_AHEAD; ++i) {
-                    if (r >= stop) break;
-                    float f[V], g[V];
-                    xc[i].get(f); gc[i].get(g);
-                    step(f, g);
+                for (int i = 0; i < AHEAD; ++i) {
+                    float g[V];
+                    xc[i].get(win[K - 1]); gc[i].get(g);
+                    pre_gradient<SILU, K, V>(win, w.w, w.b, g);
+                    const bool mine = r + i < hi;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const float gm = mine ? g[e] : 0.f;
+                        db[e] += gm;
+#pragma unroll
+                        for (int j = 0; j < K; ++j) {
+                            dw[j][e] = fmaf(gm, win[j][e], dw[j][e]);
+                            ring[j][e] = j == K - 1 ? w.w[j][e] * g[e] : fmaf(w.w[j][e], g[e], ring[j][e]);
+                        }
+                    }
+                    const int at = r + i - (K - 1);              // has all its shares now, but that of the final state's gradient
+                    if (a.dfinal && at >= lo && at < hi && at >= end - (K - 1)) {
+                        float o[V];
+                        load_vec<T, V>((const T*)a.dfinal + ((int64_t)s * (K - 1) + at - (end - (K - 1))) * a.cols + p.c, o);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) ring[0][e] += o[e];
+                    }
+                    DX.store(want_dx && at >= lo && at < hi ? to + i * DX.ld : NOWHERE, ring[0]);
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+#pragma unroll
+                        for (int j = 0; j < K - 1; ++j) { win[j][e] = win[j + 1][e]; ring[j][e] = ring[j + 1][e]; }
                 }
+                to += AHEAD * DX.ld;
             }
-#pragma unroll
-            for (int i = 0; i < K - 1; ++i) emit(stop - (K - 1) + i, ring[i]);      // the utterance's last frames, nothing behind them
             r = hi;
         }
     } else if (p.ok && a.dinitial && p.run - k.runs < k.m.n_seqs) {
@@ -257,7 +266,7 @@ template <class T, int K, int V> __global__ __launch_bounds__(256) void conv1d_b
             float g[V] = {};
             frame<T, V>(a, s, b, t, p.c, win[K - 1]);
             load_vec<T, V>((const T*)a.dy + (int64_t)(b + t) * a.dy_ld + p.c, g);
-            pre_gradient<K, V>(win, w.w, w.b, a.silu, g);
+            pre_gradient<SILU, K, V>(win, w.w, w.b, g);
 #pragma unroll
             for (int i = 0; i < K - 1; ++i)                      // frame t's tap j looks at frame t - (K-1) + j = i - (K-1)
                 if (i - t >= 0)
@@ -343,22 +352,38 @@ static int check_conv1d(const char* who, const vc_conv1d_args* a, int v, int mos
     k->part = nullptr;
     return 0;
 }
+static void set_runs(ConvArgs& k, int longest, int shortest) {
+    for (k.run = longest; k.run > shortest && (int64_t)k.m.rows * k.cv < (int64_t)k.run * 64 * RUN_WAVES;) k.run /= 2;
+    k.runs = (k.m.rows + k.run - 1) / k.run;
+}
 static int conv_grid(const char* who, const ConvArgs& k, bool seqs, unsigned* grid) {
     const int per = 256 / k.cvb;
     const int64_t g = (int64_t)((k.cv + k.cvb - 1) / k.cvb) * (((int64_t)k.runs + (seqs ? k.m.n_seqs : 0) + per - 1) / per);
     VC_ARG(g < (1LL << 31), "%s: too many rows and channels for one launch", who);
+    // the rows of a block, with the frames that its runs look at ahead and behind, by 32-bit offsets
+    const int64_t span = std::min((int64_t)per * k.run, (int64_t)k.m.rows) + 16;
+    for (int64_t ld : {k.a.x_ld, k.a.y ? k.a.y_ld : 0, k.a.dy ? k.a.dy_ld : 0, k.a.dx ? k.a.dx_ld : 0})
+        VC_ARG(ld >= 0 && (span * ld + k.a.cols) * seq_esize(k.a.type) < (1LL << 31), "%s: a row stride of %lld elements is out of range", who, (long long)ld);
     *grid = (unsigned)g;
     return 0;
 }
 template <class T, int K> static int fwd_k(const ConvArgs& k, unsigned grid, hipStream_t s) {
-    if (k.v == 1) hipLaunchKernelGGL((conv1d_fwd_kernel<T, K, 1>), dim3(grid), dim3(256), 0, s, k);
-    else hipLaunchKernelGGL((conv1d_fwd_kernel<T, K, 16 / (int)sizeof(T)>), dim3(grid), dim3(256), 0, s, k);
+    constexpr int V = 16 / (int)sizeof(T);
+    if (k.v == 1) {
+        if (k.a.silu) hipLaunchKernelGGL((conv1d_fwd_kernel<T, K, 1, true>), dim3(grid), dim3(256), 0, s, k);
+        else hipLaunchKernelGGL((conv1d_fwd_kernel<T, K, 1, false>), dim3(grid), dim3(256), 0, s, k);
+    } else if (k.a.silu) hipLaunchKernelGGL((conv1d_fwd_kernel<T, K, V, true>), dim3(grid), dim3(256), 0, s, k);
+    else hipLaunchKernelGGL((conv1d_fwd_kernel<T, K, V, false>), dim3(grid), dim3(256), 0, s, k);
     VC_HIP(hipGetLastError());
     return 0;
 }
 template <class T, int K> static int bwd_k(const ConvArgs& k, unsigned grid, hipStream_t s) {
-    if (k.v == 1) hipLaunchKernelGGL((conv1d_bwd_kernel<T, K, 1>), dim3(grid), dim3(256), 0, s, k);
-    else hipLaunchKernelGGL((conv1d_bwd_kernel<T, K, BWD_V>), dim3(grid), dim3(256), 0, s, k);
+    constexpr int V = BWD_V;
+    if (k.v == 1) {
+        if (k.a.silu) hipLaunchKernelGGL((conv1d_bwd_kernel<T, K, 1, true>), dim3(grid), dim3(256), 0, s, k);
+        else hipLaunchKernelGGL((conv1d_bwd_kernel<T, K, 1, false>), dim3(grid), dim3(256), 0, s, k);
+    } else if (k.a.silu) hipLaunchKernelGGL((conv1d_bwd_kernel<T, K, V, true>), dim3(grid), dim3(256), 0, s, k);
+    else hipLaunchKernelGGL((conv1d_bwd_kernel<T, K, V, false>), dim3(grid), dim3(256), 0, s, k);
     VC_HIP(hipGetLastError());
     return 0;
 }
@@ -378,7 +403,7 @@ extern "C" int vc_causal_conv1d_fwd(const vc_conv1d_args* a, void* stream) {
     VC_ARG(a->w && (a->rows == 0 || (a->x && a->y)), "vc_causal_conv1d_fwd: null pointer");
     VC_ARG(!a->final_state || a->final_state != a->initial, "vc_causal_conv1d_fwd: final_state may not be initial");
     if (a->rows == 0 && !a->final_state) return 0;
-    k.runs = (k.m.rows + FWD_RUN - 1) / FWD_RUN;
+    set_runs(k, FWD_RUN, FWD_SHORT);
     unsigned grid; VC_CHECK(conv_grid("vc_causal_conv1d_fwd", k, a->final_state != nullptr, &grid));
     return SEQ_TYPES(a->type, conv1d_fwd, k, grid, (hipStream_t)stream);
 }
@@ -386,13 +411,13 @@ extern "C" int vc_causal_conv1d_fwd(const vc_conv1d_args* a, void* stream) {
 static int conv_parts(const ConvArgs& k) { const int per = 256 / k.cvb; return (k.runs + per - 1) / per; }
 extern "C" int64_t vc_causal_conv1d_bwd_work(const vc_conv1d_args* a) {
     ConvArgs k; if (check_conv1d("vc_causal_conv1d_bwd_work", a, BWD_V, BWD_WIDE, &k)) return VC_E_ARG;
-    k.runs = (k.m.rows + BWD_RUN - 1) / BWD_RUN;
+    set_runs(k, BWD_RUN, BWD_SHORT);
     return (int64_t)conv_parts(k) * (a->taps + 1) * a->cols;
 }
 extern "C" int vc_causal_conv1d_bwd(const vc_conv1d_args* a, void* stream) {
     ConvArgs k; VC_CHECK(check_conv1d("vc_causal_conv1d_bwd", a, BWD_V, BWD_WIDE, &k));
     VC_ARG(a->w && (a->rows == 0 || (a->x && a->dy)), "vc_causal_conv1d_bwd: null pointer");
-    k.runs = (k.m.rows + BWD_RUN - 1) / BWD_RUN;
+    set_runs(k, BWD_RUN, BWD_SHORT);
     const bool params = a->dw || a->dbias;
     const int64_t need = (int64_t)conv_parts(k) * (a->taps + 1) * a->cols;
     if (params && need && (!a->work || a->work_floats < need)) { vc_set_error("vc_causal_conv1d_bwd: work is too small (%lld floats needed)", (long long)need); return VC_E_NOMEM; }
