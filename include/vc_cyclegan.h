@@ -256,7 +256,8 @@ int vc_rms_norm_bwd(const void* dy, int64_t dy_ld, const void* dsum, int64_t dsu
  *   p[t][c] = bias[c] + sum_k w[k][c] x[t - (taps-1) + k][c];   y = p * sigmoid(p) (silu != 0) or p
  * w [taps][cols], 2 <= taps <= 8; bias may be NULL.  Frames before an utterance come from initial [n_seqs][taps-1][cols] (type; oldest first;
  * NULL: zeros).  final [n_seqs][taps-1][cols] (may be NULL) receives the last taps-1 frames, what the next call of a stream takes as initial;
- * final may not be initial. */
+ * final may not be initial.  Row strides: up to 2^15 elements, 2^20 from 256 channels on (a block's rows
+ * lie within 2^31 bytes). */
 typedef struct {
     const void* x; const float* w; const float* bias; const void* initial; const int32_t* offsets;
     void* y; void* final_state;

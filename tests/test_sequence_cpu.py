@@ -220,3 +220,21 @@ def test_python_refuses_cpu_tensors(L):
         S.selective_scan(x, x, torch.zeros(8, 4), x[..., :4], x[..., :4])
     with pytest.raises(ValueError, match='no CPU path'):
         S.selective_scan_step(x[0], x[0], torch.zeros(8, 4), x[0, :, :4], x[0, :, :4], torch.zeros(3, 8, 4))
+
+
+def test_conv_refuses_strides_beyond_a_block(L):
+    """a block of the convolution reaches its rows with 32-bit offsets, so a stride of 2^30 elements is refused, and a negative one"""
+    f, b = L.lib.vc_causal_conv1d_fwd, L.lib.vc_causal_conv1d_bwd
+    big = 1 << 30
+    for bad in (dict(x_ld=big), dict(y_ld=big), dict(x_ld=-8), dict(y_ld=-8)):
+        assert f(C.byref(_conv(L, **bad)), NULL_STREAM) == -1, bad
+        assert b'row stride' in L.lib.vc_last_error()
+    full = dict(dy=4096, dx=4096, dx_ld=8, dy_ld=8)
+    for bad in (dict(x_ld=big), dict(dy_ld=big), dict(dx_ld=big), dict(dx_ld=-8)):
+        assert b(C.byref(_conv(L, **{**full, **bad})), NULL_STREAM) == -1, bad
+        assert b'row stride' in L.lib.vc_last_error()
+
+
+def test_binding_is_built_from_these_sources(L):
+    from voice_converter_cyclegan_amd import sequence as S
+    assert S._seq.build_id == L._bmod.binding_id()

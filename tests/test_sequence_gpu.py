@@ -708,3 +708,107 @@ def test_rows_behind_the_last_utterance_are_left_without_zero_tail(S):
     ca = _lib.Conv1dArgs(x=v['x'].data_ptr(), w=w.data_ptr(), offsets=off.data_ptr(), y=y.data_ptr(), x_ld=24, y_ld=24, rows=40, cols=24, taps=4, n_seqs=2, type=0, silu=1)
     _lib.check(_lib.lib.vc_causal_conv1d_fwd(C.byref(ca), torch.cuda.current_stream().cuda_stream))
     assert (y[31:] == 7).all() and (y[:31] != 7).all()
+
+
+# ------------------------------------------------------------------------------------------------------- autograd's corners
+
+def _three(S):
+    """each operator on leaves of its own: (output, leaves)"""
+    x, gamma, res = rnd(1, 12, 16).requires_grad_(True), (1 + rnd(2, 16, scale=0.1)).requires_grad_(True), rnd(3, 12, 16).requires_grad_(True)
+    yield S.rms_norm(x, gamma, res)[0], [x, gamma, res]
+    x, w = rnd(4, 3, 4, 16).requires_grad_(True), rnd(5, 4, 16).requires_grad_(True)
+    yield S.causal_conv1d(x, w), [x, w]
+    v = {k: t.detach().clone().requires_grad_(True) for k, t in scan_inputs(12, 16, 4, 1, F32, 1).items()}
+    yield (S.selective_scan(v['x'][None], v['dt'][None], v['A'], v['B'][None], v['C'][None], D=v['D'], z=v['z'][None], dt_bias=v['dt_bias']),
+           [v[k] for k in ('x', 'dt', 'A', 'B', 'C', 'D', 'z', 'dt_bias')])
+
+
+def test_gradients_kept_accumulated_and_not_differentiated_twice(S):
+    for y, leaves in _three(S):
+        dy = rnd(9, *y.shape)
+        first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+        again = torch.autograd.grad(y, leaves, dy, create_graph=True)
+        for a, b in zip(first, again):
+            assert torch.equal(a, b.detach())
+        with pytest.raises(RuntimeError, match='differentiated twice'):
+            torch.autograd.grad(again[0].sum(), leaves, retain_graph=True)
+        del again
+        y.backward(dy, retain_graph=True)
+        y.backward(dy)
+        for t, a in zip(leaves, first):
+            assert torch.equal(t.grad, a + a)
+        with pytest.raises(RuntimeError):
+            y.backward(dy)                                        # what was saved is gone
+
+
+def test_changing_an_input_in_place_is_noticed(S):
+    for y, leaves in _three(S):
+        with torch.no_grad():
+            leaves[1].mul_(2.0)
+        with pytest.raises(RuntimeError, match='inplace'):
+            y.backward(rnd(9, *y.shape))
+
+
+def test_moving_a_state_on_is_noticed(S):
+    state, w = rnd(1, 2, 3, 16), rnd(2, 4, 16)
+    t = rnd(3, 2, 3, 16).requires_grad_(True)
+    held = (t * state).sum()                                      # keeps the state for its gradient
+    S.causal_conv1d_step(rnd(4, 2, 16), state, w)
+    with pytest.raises(RuntimeError, match='inplace'):
+        held.backward()
+    v, pool = scan_inputs(2, 16, 4, 1, F32, 1), rnd(5, 2, 16, 4)
+    t = rnd(6, 2, 16, 4).requires_grad_(True)
+    held = (t * pool).sum()
+    S.selective_scan_step(v['x'], v['dt'], v['A'], v['B'], v['C'], pool)
+    with pytest.raises(RuntimeError, match='inplace'):
+        held.backward()
+
+
+def test_nothing_is_held_once_the_outputs_are_gone(S):
+    import gc
+
+    def use(backward):
+        for y, leaves in _three(S):
+            if backward:
+                y.backward(rnd(9, *y.shape))
+    use(True)
+    for backward in (False, True):
+        gc.collect(); torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        for _ in range(3):
+            use(backward)
+        gc.collect()
+        assert torch.cuda.memory_allocated() == before
+
+
+def test_what_memory_alone_does_not_tell_is_refused(S):
+    gamma = torch.ones(8, device=DEV)
+    negated = torch.view_as_complex(rnd(1, 6, 8, 2)).conj().imag
+    assert negated.is_neg()
+    with pytest.raises(ValueError, match='negated'):
+        S.rms_norm(negated, gamma)
+    assert torch.equal(S.rms_norm(negated.resolve_neg(), gamma), S.rms_norm(negated.clone(), gamma))
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level():
+        dual = fw.make_dual(rnd(2, 6, 8), rnd(3, 6, 8))
+        with pytest.raises(NotImplementedError, match='forward mode'):
+            S.rms_norm(dual, gamma)
+    with pytest.raises(ValueError):
+        S.rms_norm(torch.ones((), device=DEV), gamma)
+    x = rnd(4, 6, 8).requires_grad_(True)                         # a lazily negated gradient
+    y = S.rms_norm(x, gamma)
+    a, = torch.autograd.grad(y, x, negated, retain_graph=True)
+    b, = torch.autograd.grad(y, x, negated.resolve_neg())
+    assert torch.equal(a, b)
+
+
+def test_rows_far_apart(S):
+    """a few channels of very wide rows: copied where the kernel's 32-bit offsets would not reach"""
+    wide = rnd(1, 9, (1 << 17) + 8)
+    x, w, off = wide[:, 3:7], rnd(2, 4, 4), offsets_of([5, 4])
+    assert torch.equal(S.causal_conv1d(x, w, seq_offsets=off), S.causal_conv1d(x.contiguous(), w, seq_offsets=off))
+    leaf = wide.clone().requires_grad_(True)
+    g, = torch.autograd.grad(S.causal_conv1d(leaf[:, 3:7], w, seq_offsets=off), leaf, x)
+    leaf2 = x.contiguous().requires_grad_(True)
+    g2, = torch.autograd.grad(S.causal_conv1d(leaf2, w, seq_offsets=off), leaf2, x.contiguous())
+    assert torch.equal(g[:, 3:7], g2)

@@ -6,7 +6,6 @@
 // Host code only; no kernel and no HIP call is made here but through that library.
 #include <torch/csrc/utils/pybind.h>
 #include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
@@ -70,13 +69,26 @@ int type_code(const Tensor& t) {
         default: return -1;
     }
 }
+// what its memory alone does not tell: a lazily negated view, a tangent (these operators have reverse gradients only), another layout
+void ordinary(const Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(t.layout() == at::kStrided && !t.is_neg(), name, " must be a dense tensor that is not negated lazily (resolve_neg() makes one)");
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name, " has a tangent: forward mode differentiation is not offered");
+}
+int narrow(int64_t n, const char* name) {
+    TORCH_CHECK_VALUE(n >= 0 && n < (int64_t{1} << 31), n, " ", name, " are too many");
+    return (int)n;
+}
 void activation(const Tensor& t, const char* name) {
     TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a tensor on a GPU (there is no CPU path)");
     TORCH_CHECK_VALUE(type_code(t) >= 0, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+    TORCH_CHECK_VALUE(t.dim() >= 1, name, " must be [..., channels]");
+    ordinary(t, name);
+    narrow(t.size(-1), "channels");
 }
 void like(const Tensor& t, const Tensor& ref, const char* name, at::IntArrayRef shape, at::ScalarType dtype) {
     TORCH_CHECK_VALUE(t.scalar_type() == dtype && t.device() == ref.device(), name, " must be a ", dtype, " tensor on ", ref.device());
     TORCH_CHECK_VALUE(t.sizes() == shape, name, " must have shape ", shape, ", got ", t.sizes());
+    ordinary(t, name);
 }
 void like(const OptTensor& t, const Tensor& ref, const char* name, at::IntArrayRef shape, at::ScalarType dtype) {
     if (t) like(*t, ref, name, shape, dtype);
@@ -107,7 +119,12 @@ struct Rows {
     }
     explicit Rows(const OptTensor& from) { if (from) *this = Rows(*from); }
     void* p() const { return ptr(t); }
+    Rows&& within(int64_t most) && { if (ld > most && !t.is_contiguous()) { t = t.contiguous(); ld = t.size(-1); } return std::move(*this); }
 };
+// Widest row strides that are taken in place: below what the kernels' 32-bit offsets reach (a block of the convolution has up to 8192 rows, and up to 256
+// rows where they are of 256 channels or more); rows that lie further apart are copied
+int64_t conv_ld(const Tensor& x) { return x.size(-1) < 256 ? 1 << 15 : 1 << 20; }
+constexpr int64_t SCAN_LD = 1 << 24;
 // B or C of a scan: [..., states] or [..., groups, states] beside x [..., channels]
 struct Grouped {
     Tensor t; int64_t ld = 0; int groups = 1;
@@ -117,21 +134,34 @@ struct Grouped {
         const bool one = from.dim() == x.dim();
         TORCH_CHECK_VALUE((one || from.dim() == x.dim() + 1) && from.size(-1) == states && from.sizes().slice(0, x.dim() - 1) == lead && (one || from.size(-2) > 0),
                           name, " must be ", lead, " + [groups, ", states, "] or + [", states, "], got ", from.sizes());
+        ordinary(from, name);
+        TORCH_CHECK_VALUE(one || from.size(-2) <= x.size(-1), name, " has more groups than there are channels");
         groups = one ? 1 : (int)from.size(-2);
         const int64_t w = groups * states;
         if (from.is_contiguous()) { t = from; ld = w; return; }
         t = from.reshape({-1, groups, states});
         if ((states > 1 && t.stride(2) != 1) || (groups > 1 && t.stride(1) != states)) t = t.contiguous();
         ld = t.size(0) > 1 ? t.stride(0) : w;
+        if (ld > SCAN_LD && !t.is_contiguous()) { t = t.contiguous(); ld = w; }
     }
 };
 
-// what a backward pass returns where a graph of it is being built: it cannot be differentiated again
-variable_list once(variable_list out, const char* what) {
+// Where a graph of a backward pass is being built, its results hang on a node that leads to all that they depend on and refuses to be run: whichever way
+// a second differentiation comes, it meets an error and no missing gradient.
+struct Twice : public Node {
+    std::string what;
+    std::string name() const override { return "CannotBeDifferentiatedTwice"; }
+    variable_list apply(variable_list&&) override { throw std::runtime_error(what + " cannot be differentiated twice"); }
+};
+variable_list once(variable_list out, const Node& backward, const variable_list& grads, const char* what) {
     if (!at::GradMode::is_enabled()) return out;
-    auto fn = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " cannot be differentiated twice", (int64_t)out.size());
-    for (auto& o : out) if (o.defined()) o = o.detach().set_requires_grad(true);
-    return (*fn)(std::move(out));
+    auto n = std::shared_ptr<Twice>(new Twice(), torch::autograd::deleteNode);
+    n->what = what;
+    auto edges = backward.next_edges();
+    for (const auto& g : grads) if (g.defined() && g.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(g));
+    n->set_next_edges(std::move(edges));
+    for (auto& o : out) if (o.defined()) { o = o.detach(); torch::autograd::set_history(o, n); }
+    return out;
 }
 template <class N, class... Ts> std::shared_ptr<N> node_for(const Ts&... inputs) {
     auto n = std::shared_ptr<N>(new N(), torch::autograd::deleteNode);
@@ -161,9 +191,9 @@ struct NormBackward : public Node {
             if (need_r && !one) dres = fresh(t.sizes(), t);
             if (need_g) dg = rows ? fresh(g.sizes(), g) : at::zeros(g.sizes(), g.options());
             if (rows) {
-                const Rows tr(t), dy(grads[0].defined() ? grads[0] : at::zeros(t.sizes(), t.options().dtype(x_type)));
+                const Rows tr(t), dy(grads[0].defined() ? grads[0].resolve_neg() : at::zeros(t.sizes(), t.options().dtype(x_type)));
                 Rows ds;
-                if (residual && grads.size() > 1 && grads[1].defined()) ds = Rows(grads[1]);
+                if (residual && grads.size() > 1 && grads[1].defined()) ds = Rows(grads[1].resolve_neg());
                 const Tensor gc = g.contiguous();
                 Tensor work;
                 const int64_t n = need_g ? L.rms_norm_bwd_work(rows, (int)cols) : 0;
@@ -174,7 +204,7 @@ struct NormBackward : public Node {
             if (need_r && one) dres = dx;
             if (!need_x) dx = Tensor();
         }
-        return once({dx, dg, dres}, "rms_norm");
+        return once({dx, dg, dres}, *this, grads, "rms_norm");
     }
 };
 void norm_inputs(const Tensor& x, const Tensor& gamma, const OptTensor& residual, double eps) {
@@ -240,14 +270,18 @@ Utterances utterances(const Tensor& x, const OptTensor& offsets) {
     if (!offsets) {
         TORCH_CHECK_VALUE(x.dim() == 3, "x must be [batch, frames, channels], or [rows, channels] with seq_offsets; got ", x.sizes());
         TORCH_CHECK_VALUE(x.size(0) > 0, "x holds no utterance");
+        narrow(x.size(0), "utterances");
         return {x.size(0), x.size(0) * x.size(1)};
     }
     TORCH_CHECK_VALUE(x.dim() == 2, "with seq_offsets x must be [rows, channels], got ", x.sizes());
     TORCH_CHECK_VALUE(offsets->scalar_type() == at::kInt && offsets->device() == x.device() && offsets->dim() == 1 && offsets->numel() >= 2,
                       "seq_offsets must be an int32 tensor [utterances + 1] on ", x.device());
+    ordinary(*offsets, "seq_offsets");
+    narrow(offsets->numel() - 1, "utterances");
     return {offsets->numel() - 1, x.size(0)};
 }
 void check_slots(const OptTensor& slots, int64_t rows, int64_t pool, const Tensor& ref) {
+    narrow(rows, "streams"); narrow(pool, "states");
     if (slots) like(*slots, ref, "slots", {rows}, at::kInt);
     else TORCH_CHECK_VALUE(rows <= pool, rows, " frames without slots, and a state of ", pool);
 }
@@ -265,7 +299,7 @@ struct ConvPlan { int64_t n, rows; bool silu; };
 struct ConvCall {
     vc_conv1d_args a{}; Rows x; Tensor w, bias, initial, offsets;
     ConvCall(const Tensor& x_, const Tensor& w_, const OptTensor& bias_, const OptTensor& initial_, const OptTensor& offsets_, const ConvPlan& p)
-        : x(x_), w(w_.contiguous()), bias(plain(bias_)), initial(plain(initial_)), offsets(plain(offsets_)) {
+        : x(Rows(x_).within(conv_ld(x_))), w(w_.contiguous()), bias(plain(bias_)), initial(plain(initial_)), offsets(plain(offsets_)) {
         a.x = x.p(); a.x_ld = x.ld; a.w = (const float*)ptr(w); a.bias = (const float*)ptr(bias); a.initial = ptr(initial); a.offsets = (const int32_t*)ptr(offsets);
         a.rows = p.rows; a.cols = (int)x_.size(-1); a.taps = (int)w.size(0); a.n_seqs = (int)p.n; a.type = type_code(x_); a.silu = p.silu; a.zero_tail = 1;
     }
@@ -286,8 +320,8 @@ struct ConvBackward : public Node {
             at::NoGradGuard ng;
             const c10::DeviceGuard guard(xv.device());
             ConvCall k(xv, wv, optional(bv), optional(iv), optional(ov), plan);
-            const Rows dy(grads[0].defined() ? grads[0] : at::zeros(xv.sizes(), xv.options()));
-            const Tensor df = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : Tensor();
+            const Rows dy = Rows(grads[0].defined() ? grads[0].resolve_neg() : at::zeros(xv.sizes(), xv.options())).within(conv_ld(xv));
+            const Tensor df = grads.size() > 1 && grads[1].defined() ? grads[1].resolve_neg().contiguous() : Tensor();
             if (task_should_compute_output(0)) dx = fresh(xv.sizes(), xv);
             if (task_should_compute_output(1)) dw = fresh(wv.sizes(), wv);
             if (bv.defined() && task_should_compute_output(2)) db = fresh(bv.sizes(), bv);
@@ -300,7 +334,7 @@ struct ConvBackward : public Node {
             k.a.work = (float*)ptr(work);
             check(L.causal_conv1d_bwd(&k.a, stream->of(xv.device())), "vc_causal_conv1d_bwd");
         }
-        return once({dx, dw, db, di}, "causal_conv1d");
+        return once({dx, dw, db, di}, *this, grads, "causal_conv1d");
     }
 };
 py::object causal_conv1d(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& initial, const OptTensor& offsets, bool silu, bool want_final) {
@@ -367,7 +401,7 @@ struct ScanCall {
     vc_scan_args a{}; Rows x, dt, z; Grouped B, C; Tensor A, D, dt_bias, initial, offsets;
     ScanCall(const Tensor& x_, const Tensor& dt_, const Tensor& A_, const Tensor& B_, const Tensor& C_, const OptTensor& D_, const OptTensor& z_, const OptTensor& bias_,
              const OptTensor& initial_, const OptTensor& offsets_, const ScanPlan& p)
-        : x(x_), dt(dt_), z(z_), B(B_, x_, A_.size(1), "B"), C(C_, x_, A_.size(1), "C"), A(A_.contiguous()), D(plain(D_)), dt_bias(plain(bias_)), initial(plain(initial_)),
+        : x(Rows(x_).within(SCAN_LD)), dt(Rows(dt_).within(SCAN_LD)), z(Rows(z_).within(SCAN_LD)), B(B_, x_, A_.size(1), "B"), C(C_, x_, A_.size(1), "C"), A(A_.contiguous()), D(plain(D_)), dt_bias(plain(bias_)), initial(plain(initial_)),
           offsets(plain(offsets_)) {
         same_groups(B, C, x_);
         a.x = x.p(); a.dt = dt.p(); a.z = z.p(); a.B = ptr(B.t); a.C = ptr(C.t); a.A = (const float*)ptr(A); a.D = (const float*)ptr(D); a.dt_bias = (const float*)ptr(dt_bias);
@@ -393,8 +427,8 @@ struct ScanBackward : public Node {
             at::NoGradGuard ng;
             const c10::DeviceGuard guard(xv.device());
             ScanCall k(xv, tv, Av, Bv, Cv, optional(Dv), optional(zv), optional(bv), optional(iv), optional(ov), plan);
-            const Rows dy(grads[0].defined() ? grads[0] : at::zeros(xv.sizes(), xv.options()));
-            const Tensor df = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : Tensor();
+            const Rows dy = Rows(grads[0].defined() ? grads[0].resolve_neg() : at::zeros(xv.sizes(), xv.options())).within(SCAN_LD);
+            const Tensor df = grads.size() > 1 && grads[1].defined() ? grads[1].resolve_neg().contiguous() : Tensor();
             dx = fresh(xv.sizes(), xv); ddt = fresh(tv.sizes(), xv); dB = fresh(Bv.sizes(), xv); dC = fresh(Cv.sizes(), xv); dA = fresh(Av.sizes(), Av);
             if (zv.defined()) dz = fresh(zv.sizes(), xv);
             if (Dv.defined()) dD = fresh(Dv.sizes(), Av);
@@ -412,7 +446,7 @@ struct ScanBackward : public Node {
         }
         variable_list out{dx, ddt, dA, dB, dC, dD, dz, db, di};
         for (size_t i = 0; i < out.size(); ++i) if (!task_should_compute_output(i)) out[i] = Tensor();
-        return once(std::move(out), "selective_scan");
+        return once(std::move(out), *this, grads, "selective_scan");
     }
 };
 py::object selective_scan(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const OptTensor& D, const OptTensor& z, const OptTensor& dt_bias,
