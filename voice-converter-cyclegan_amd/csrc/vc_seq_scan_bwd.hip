@@ -318,6 +318,7 @@ template <class T> __global__ __launch_bounds__(256) void scan_finish_kernel(con
         dst += g * a.states + n;
         if (r >= tail) { if (a.zero_tail) *dst = (T)0.f; return; }
         float s = 0.f;
+#pragma unroll 8
         for (int b = 0; b < k.nblk; ++b) s += k.part[((int64_t)(g * k.nblk + b) * k.m.rows + r) * (2 * np) + m];
         *dst = (T)s;
         return;
