@@ -812,3 +812,73 @@ def test_rows_far_apart(S):
     leaf2 = x.contiguous().requires_grad_(True)
     g2, = torch.autograd.grad(S.causal_conv1d(leaf2, w, seq_offsets=off), leaf2, x.contiguous())
     assert torch.equal(g[:, 3:7], g2)
+
+
+# --------------------------------------------------------------------------------------------------- more than 2^31 elements
+
+def big(rows, cols, seed, **kw):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return torch.empty(rows, cols, device=DEV, dtype=BF16).normal_(generator=g, **kw)
+
+
+def test_rows_beyond_32_bit_offsets(S):
+    """2^21 + 70 rows of 1040 channels are more than 2^31 elements and 2^32 bytes: the last rows against the definition.  bf16, bounds as everywhere here."""
+    rows, cols, tail = (1 << 21) + 70, 1040, 70
+    lengths = [64] * (rows // 64 - 1) + [64 + rows % 64]
+    off = offsets_of(lengths)
+    x, dy = big(rows, cols, 1), big(rows, cols, 2)
+    last = slice(rows - tail, rows)                               # the last utterance
+    assert lengths[-1] == tail
+    gamma = 1 + rnd(3, cols, scale=0.1)
+    x.requires_grad_(True)
+    y = S.rms_norm(x, gamma)
+    dx, = torch.autograd.grad(y, x, dy)
+    ref, dt, _ = O.rms_norm(x.detach()[last], gamma, 1e-6, dy[last])
+    _, dt_m, _ = O.rms_norm(x.detach()[last], gamma, 1e-6, dy[last], absolute=True)
+    close(y[last], ref, ref.abs(), 37, 'norm')
+    close(dx[last], dt, dt_m, 111, 'norm dx')
+    del y, dx
+    w, b = rnd(4, 4, cols, scale=0.5), rnd(5, cols, scale=0.1)
+    y = S.causal_conv1d(x, w, b, seq_offsets=off)
+    dx, = torch.autograd.grad(y, x, dy)
+    r = O.conv1d(x.detach()[last].cpu(), w, b, None, [tail], True, dy[last].cpu())
+    m = O.conv1d(x.detach()[last].cpu(), w, b, None, [tail], True, dy[last].cpu(), absolute=True)
+    close(y[last], r['y'], m['p'], 24, 'conv')
+    close(dx[last], r['dx'], m['dx'], 24, 'conv dx')
+    del y, dx
+    v = scan_inputs(tail, cols, 4, 1, BF16, 1)
+    dt = big(rows, cols, 6).clamp_(-0.1, 0.5)
+    B, Cm = (big(rows, 4, s) for s in (7, 8))
+    leaves = [t.requires_grad_(True) for t in (x, dt, B, Cm)]
+    y = S.selective_scan(x, dt, v['A'], B, Cm, D=v['D'], dt_bias=v['dt_bias'], seq_offsets=off, max_len=70)
+    got = torch.autograd.grad(y, leaves, dy)
+    cut = dict(x=x.detach()[last], dt=dt.detach()[last], A=v['A'], B=B.detach()[last].view(tail, 1, 4), C=Cm.detach()[last].view(tail, 1, 4), D=v['D'], z=None,
+               dt_bias=v['dt_bias'], initial=None, lengths=[tail], dy=dy[last])
+    r, m = O.scan(**cut), O.scan(**cut, absolute=True)
+    held = lasts(r, v['A'], tail)
+    close(y[last], r['y'], m['y'], 3 * held + 44, 'scan')
+    for name, g in zip(('x', 'dt', 'B', 'C'), got):
+        close(g[last].reshape(r['d' + name].shape), r['d' + name], m['d' + name], 6 * held + tail + cols + 64, 'scan d' + name)
+
+
+def test_slots_beyond_32_bit_offsets(S):
+    """the last entry of a pool of more than 2^31 numbers moves on as the first one does"""
+    n, cols, states = (1 << 17) + 5, 1024, 17
+    pool = torch.zeros(n, cols, states, device=DEV)
+    v = scan_inputs(1, cols, states, 1, BF16, 1)
+    pool[0] = pool[n - 1] = v['initial'][0]
+    assert pool.numel() > 1 << 31
+    two = {k: v[k].repeat(2, *[1] * (v[k].dim() - 1)) for k in ('x', 'dt', 'z', 'B', 'C')}
+    y = S.selective_scan_step(two['x'], two['dt'], v['A'], two['B'], two['C'], pool, D=v['D'], z=two['z'], dt_bias=v['dt_bias'],
+                              slots=torch.tensor([0, n - 1], dtype=torch.int32, device=DEV))
+    assert torch.equal(y[0], y[1]) and torch.equal(pool[0], pool[n - 1]) and not torch.equal(pool[0], v['initial'][0])
+    assert (pool[1] == 0).all() and (pool[n - 2] == 0).all()
+    del pool
+    n, cols = (1 << 19) + 9, 1366
+    state = torch.zeros(n, 3, cols, device=DEV, dtype=BF16)
+    state[0] = state[n - 1] = rnd(1, 3, cols, dtype=BF16)
+    assert state.numel() > 1 << 31
+    x = rnd(2, 1, cols, dtype=BF16).repeat(2, 1)
+    y = S.causal_conv1d_step(x, state, rnd(3, 4, cols), slots=torch.tensor([n - 1, 0], dtype=torch.int32, device=DEV))
+    assert torch.equal(y[0], y[1]) and torch.equal(state[0], state[n - 1]) and torch.equal(state[0, 2], x[0])
+    assert (state[1] == 0).all() and (state[n - 2] == 0).all()

@@ -342,7 +342,7 @@ static int check_conv1d(const char* who, const vc_conv1d_args* a, int v, int mos
     VC_ARG(a, "%s: null pointer", who);
     VC_ARG(seq_type_ok(a->type), "%s: type must be VC_F32, VC_BF16 or VC_F16", who);
     VC_ARG(a->taps >= 2 && a->taps <= 8, "%s: 2 to 8 taps, got %d", who, a->taps);
-    VC_ARG(a->rows >= 0 && a->rows < (1LL << 31) - (1 << 16) && a->cols > 0 && a->n_seqs > 0, "%s: bad sizes (rows %lld, cols %d, n_seqs %d)", who, (long long)a->rows, a->cols, a->n_seqs);
+    VC_ARG(a->rows >= 0 && a->rows + (int64_t)std::max(a->n_seqs, 0) < (1LL << 31) - (1 << 16) && a->cols > 0 && a->n_seqs > 0, "%s: bad sizes (rows %lld, cols %d, n_seqs %d)", who, (long long)a->rows, a->cols, a->n_seqs);
     VC_ARG(a->offsets || a->rows % a->n_seqs == 0, "%s: without offsets the rows divide into n_seqs equal utterances", who);
     k->a = *a;
     k->m = SeqMap{a->offsets, (int)a->rows, a->n_seqs, (int)(a->rows / a->n_seqs)};

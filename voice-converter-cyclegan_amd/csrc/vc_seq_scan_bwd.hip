@@ -308,19 +308,20 @@ template <class T> __global__ __launch_bounds__(256) void scan_finish_kernel(con
     __shared__ float red[4][64];
     const vc_scan_args& a = k.a;
     if ((int)blockIdx.x < bc) {
-        const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-        const int w = 2 * np * a.groups, tail = seq_tail(k.m);
-        if (i >= (int64_t)k.m.rows * w) return;
-        const int64_t r = i / w;
-        const int e = (int)(i - r * w), g = e / (2 * np), m = e % (2 * np), n = m % np;
-        if (n >= a.states) return;
-        T* dst = m < np ? (T*)a.dB + r * a.db_ld : (T*)a.dC + r * a.dc_ld;
-        dst += g * a.states + n;
-        if (r >= tail) { if (a.zero_tail) *dst = (T)0.f; return; }
-        float s = 0.f;
+        const int64_t w = (int64_t)2 * np * a.groups;
+        const int tail = seq_tail(k.m);
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)k.m.rows * w; i += (int64_t)bc * 256) {
+            const int64_t r = i / w;
+            const int e = (int)(i - r * w), g = e / (2 * np), m = e % (2 * np), n = m % np;
+            if (n >= a.states) continue;
+            T* dst = m < np ? (T*)a.dB + r * a.db_ld : (T*)a.dC + r * a.dc_ld;
+            dst += g * a.states + n;
+            if (r >= tail) { if (a.zero_tail) *dst = (T)0.f; continue; }
+            float s = 0.f;
 #pragma unroll 8
-        for (int b = 0; b < k.nblk; ++b) s += k.part[((int64_t)(g * k.nblk + b) * k.m.rows + r) * (2 * np) + m];
-        *dst = (T)s;
+            for (int b = 0; b < k.nblk; ++b) s += k.part[((int64_t)(g * k.nblk + b) * k.m.rows + r) * (2 * np) + m];
+            *dst = (T)s;
+        }
         return;
     }
     // dapart [items][cols * states], chpart [items][2 * cols]
@@ -367,10 +368,10 @@ extern "C" int64_t vc_selective_scan_bwd_work(const vc_scan_args* a) {
 }
 template <class T, int L, int NS> static int scan_bwd_l(const ScanK& k, hipStream_t s) {
     const int64_t blocks = (int64_t)k.a.groups * k.nblk * (k.items + (k.a.zero_tail && k.m.off ? 1 : 0));
-    const int64_t bc = ((int64_t)k.m.rows * 2 * L * NS * k.a.groups + 255) / 256;
+    const int64_t bc = std::min<int64_t>(((int64_t)k.m.rows * 2 * L * NS * k.a.groups + 255) / 256, 1 << 22);
     const int per = EDGE_WAVES * 64 / L, nblk1 = (k.cg + per - 1) / per;
     const int64_t eb = (int64_t)k.a.groups * nblk1 * k.items;
-    VC_ARG(blocks < (1LL << 31) && bc < (1LL << 31) && eb < (1LL << 31), "vc_selective_scan_bwd: too many utterances and channels for one launch");
+    VC_ARG(blocks < (1LL << 31) && eb < (1LL << 31), "vc_selective_scan_bwd: too many utterances and channels for one launch");
     if (k.chunk) {
         hipLaunchKernelGGL((scan_bwd_edge_kernel<T, L, NS>), dim3((unsigned)eb), dim3(64 * EDGE_WAVES), 0, s, k, nblk1);
         VC_CHECK(scan_carry(k, false, s));
