@@ -37,10 +37,10 @@ template <class T, int K, int V> struct Filter {
     }
 };
 // A block's threads: cvb vectors of channels (a power of two) next to each other, 256 / cvb runs of rows
-// Longest and shortest run of rows, and the waves below which a run is halved.  Long runs repeat fewer frames ahead of them (the gradient: and behind
+// Longest and shortest run of rows, and the waves below which a run is halved (a quarter of them once it has four rows).  Long runs repeat fewer frames ahead of them (the gradient: and behind
 // them, with their sigmoids), short ones leave enough threads.  Gradient of 8192 x 2048 bf16, 4 taps, with its forward pass: 45.7 us by runs of 32, 51.7
-// by 16, 55.8 by 64; of 1024 x 512: 16 by 8, 18.6 by 16, 23.7 by 32.  Forward alone, 9001 x 1000 fp32: 17.2 by 8, 17.7 by 4 and by 16.
-constexpr int FWD_RUN = 8, FWD_SHORT = 4, BWD_RUN = 32, BWD_SHORT = 8, RUN_WAVES = 1024;
+// by 16, 55.8 by 64; of 1024 x 512: 14.4 by 4, 15.1 by 2, 15.6 by 8, 23.7 by 32; of 92 x 37 in 60 utterances: 24 by 2, 39 by 8.  Forward alone, 9001 x 1000 fp32: 17.2 by 8, 17.7 by 4 and by 16.
+constexpr int FWD_RUN = 8, BWD_RUN = 32, SHORT_RUN = 2, RUN_WAVES = 1024;
 // Rows worked on while as many are on their way: with two in the forward pass 18.0 us in place of 17.2, in the gradient 48.9 in place of 45.7.
 constexpr int AHEAD = 4;
 constexpr int BWD_V = 4;                                         // channels of a thread of the gradient
@@ -352,8 +352,8 @@ static int check_conv1d(const char* who, const vc_conv1d_args* a, int v, int mos
     k->part = nullptr;
     return 0;
 }
-static void set_runs(ConvArgs& k, int longest, int shortest) {
-    for (k.run = longest; k.run > shortest && (int64_t)k.m.rows * k.cv < (int64_t)k.run * 64 * RUN_WAVES;) k.run /= 2;
+static void set_runs(ConvArgs& k, int longest) {
+    for (k.run = longest; k.run > SHORT_RUN && (int64_t)k.m.rows * k.cv < (int64_t)k.run * 64 * (k.run > 4 ? RUN_WAVES : RUN_WAVES / 4);) k.run /= 2;
     k.runs = (k.m.rows + k.run - 1) / k.run;
 }
 static int conv_grid(const char* who, const ConvArgs& k, bool seqs, unsigned* grid) {
@@ -403,7 +403,7 @@ extern "C" int vc_causal_conv1d_fwd(const vc_conv1d_args* a, void* stream) {
     VC_ARG(a->w && (a->rows == 0 || (a->x && a->y)), "vc_causal_conv1d_fwd: null pointer");
     VC_ARG(!a->final_state || a->final_state != a->initial, "vc_causal_conv1d_fwd: final_state may not be initial");
     if (a->rows == 0 && !a->final_state) return 0;
-    set_runs(k, FWD_RUN, FWD_SHORT);
+    set_runs(k, FWD_RUN);
     unsigned grid; VC_CHECK(conv_grid("vc_causal_conv1d_fwd", k, a->final_state != nullptr, &grid));
     return SEQ_TYPES(a->type, conv1d_fwd, k, grid, (hipStream_t)stream);
 }
@@ -411,13 +411,13 @@ extern "C" int vc_causal_conv1d_fwd(const vc_conv1d_args* a, void* stream) {
 static int conv_parts(const ConvArgs& k) { const int per = 256 / k.cvb; return (k.runs + per - 1) / per; }
 extern "C" int64_t vc_causal_conv1d_bwd_work(const vc_conv1d_args* a) {
     ConvArgs k; if (check_conv1d("vc_causal_conv1d_bwd_work", a, BWD_V, BWD_WIDE, &k)) return VC_E_ARG;
-    set_runs(k, BWD_RUN, BWD_SHORT);
+    set_runs(k, BWD_RUN);
     return (int64_t)conv_parts(k) * (a->taps + 1) * a->cols;
 }
 extern "C" int vc_causal_conv1d_bwd(const vc_conv1d_args* a, void* stream) {
     ConvArgs k; VC_CHECK(check_conv1d("vc_causal_conv1d_bwd", a, BWD_V, BWD_WIDE, &k));
     VC_ARG(a->w && (a->rows == 0 || (a->x && a->dy)), "vc_causal_conv1d_bwd: null pointer");
-    set_runs(k, BWD_RUN, BWD_SHORT);
+    set_runs(k, BWD_RUN);
     const bool params = a->dw || a->dbias;
     const int64_t need = (int64_t)conv_parts(k) * (a->taps + 1) * a->cols;
     if (params && need && (!a->work || a->work_floats < need)) { vc_set_error("vc_causal_conv1d_bwd: work is too small (%lld floats needed)", (long long)need); return VC_E_NOMEM; }

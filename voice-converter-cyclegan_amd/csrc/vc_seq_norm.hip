@@ -394,7 +394,7 @@ int seq_sum_parts(const float* part, int parts, int64_t n, float* dst0, int64_t 
 // Rows of 2048 bf16 with 8-bit output (8832 of them): 58 us by a wave with four vectors a thread, whose registers leave four waves a SIMD, 53 by 128
 // threads, 45 by 256; rows of 1024: 32 us by a wave, 40 by 128 or 256 threads.
 #define NORM_LAYOUT(nv, F) \
-    ((nv) <= 64 ? F(64, 1) : (nv) <= 128 ? F(64, 2) : (nv) <= 256 ? F(256, 1) : (nv) <= 512 ? F(256, 2) : (nv) <= 1024 ? F(256, 4) : F(1024, 2))
+    ((nv) <= 64 ? F(64, 1) : (nv) <= 128 ? F(64, 2) : (nv) <= 256 ? F(256, 1) : (nv) <= 512 ? F(256, 2) : (nv) <= 1024 ? F(512, 2) : F(1024, 2))
 static int norm_tpr(int64_t nv) { return nv <= 128 ? 64 : nv <= 1024 ? 256 : 1024; }
 constexpr int64_t NORM_MOST = 2048;                              // vectors of the longest row that registers hold
 static int64_t norm_vectors(int cols, int type) { const int v = 16 / seq_esize(type); return (cols + v - 1) / v; }
@@ -425,13 +425,16 @@ static int norm_bwd_blocks(int64_t rows, int cols, int type) {
     const int64_t rpb = nv <= 128 ? 4 : 1, most = norm_tpr(nv) == 1024 ? 256 : 1024;
     return (int)std::min<int64_t>((rows + rpb - 1) / rpb, most);
 }
+template <class T, class S, int TPR, int ITEMS> static void launch_bwd(const NormRowArgs& a, int blocks, hipStream_t s) {
+    hipLaunchKernelGGL((rms_bwd_kernel<T, S, TPR, ITEMS>), dim3(blocks), dim3(TPR == 64 ? 256 : TPR), 0, s, a);
+}
 template <class T, class S> static int norm_bwd_t(const NormRowArgs& a, int type, float* dgamma, hipStream_t s) {
     const int64_t nv = norm_vectors(a.cols, type);
     const int blocks = norm_bwd_blocks(a.rows, a.cols, type);
     if (nv > NORM_MOST) hipLaunchKernelGGL((rms_bwd_long_kernel<T, S>), dim3(blocks), dim3(1024), 0, s, a);
     else {
-#define F(TPR, ITEMS) hipLaunchKernelGGL((rms_bwd_kernel<T, S, TPR, ITEMS>), dim3(blocks), dim3(TPR == 64 ? 256 : TPR), 0, s, a)
-        if (nv <= 64) F(64, 1); else if (nv <= 128) F(64, 2); else if (nv <= 256) F(256, 1); else if (nv <= 512) F(256, 2); else if (nv <= 1024) F(256, 4); else F(1024, 2);
+#define F(TPR, ITEMS) launch_bwd<T, S, TPR, ITEMS>(a, blocks, s)
+        NORM_LAYOUT(nv, F);
 #undef F
     }
     VC_HIP(hipGetLastError());

@@ -18,7 +18,7 @@ constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f, 
 
 struct ScanK {
     vc_scan_args a; SeqMap m;
-    int cg, nblk;                  // channels of a group; blocks that cover them
+    int cg, nblk, waves;           // channels of a group; blocks that cover them, and the waves of each
     int slots;                     // slots in all
     // How the time axis is shared out: items are whole utterances (chunk = 0), or runs of `chunk` slots whatever utterances these belong to.
     // In the second form a first pass works out what each run does to a state that enters it, h -> exp(A sum_delta) h + edge, and the main pass begins

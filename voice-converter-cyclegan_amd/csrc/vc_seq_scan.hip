@@ -10,7 +10,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_ed
     __shared__ float lds[FWD_WAVES][TILE * NP];
     const vc_scan_args& a = k.a;
     const int nblk = a.groups * k.nblk, item = blockIdx.x / nblk, blk = blockIdx.x - item * nblk;
-    const Lane<L, NS> w(k, FWD_WAVES, blk);
+    const Lane<L, NS> w(k, k.waves, blk);
     const int c = w.c, j = w.j, n0 = w.n0, nn = w.nn;
     const Rows<T, L> X(a.x, a.x_ld, a.cols, c, j), DT(a.dt, a.dt_ld, a.cols, c, j);
     const States<T, NP> B(a.B, a.b_ld, w.g, a.states, w.lane);
@@ -66,34 +66,62 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_ed
     if (blk == 0 && threadIdx.x == 0) k.cut[item] = cut;
 }
 
-// Second pass of a split axis: from what every run hands on to what enters it, run by run for one state a thread.  Reads ahead: the chain is one
-// multiply-add a run.
-__global__ __launch_bounds__(64) void scan_carry_kernel(const ScanK k, bool forward) {
-    constexpr int AHEAD = 16;
+// Second pass of a split axis: from what every run hands on to what enters it, for 16 states a block.  64 threads share a state's runs: each goes through
+// its own as if nothing entered them, what they do together -- h -> exp2(p) h + e, or e behind a cut -- is combined over the threads before, and each
+// goes through its own once more from there.
+constexpr int CARRY_W = 16, CARRY_SEGS = 64;
+__global__ __launch_bounds__(CARRY_W * CARRY_SEGS) void scan_carry_kernel(const ScanK k, bool forward) {
+    constexpr int KEEP = 8;
+    __shared__ float ps[CARRY_SEGS][CARRY_W], es[CARRY_SEGS][CARRY_W];
+    __shared__ int cs[CARRY_SEGS][CARRY_W];
     const vc_scan_args& a = k.a;
-    const int64_t n = (int64_t)a.cols * a.states, i = (int64_t)blockIdx.x * 64 + threadIdx.x;
-    if (i >= n) return;
-    const int c = (int)(i / a.states);
+    const int x = threadIdx.x % CARRY_W, seg = threadIdx.x / CARRY_W;
+    const int64_t n = (int64_t)a.cols * a.states, at = (int64_t)blockIdx.x * CARRY_W + x, i = min(at, n - 1);      // past the last state: the last one again, not stored
+    const int c = (int)(i / a.states), each = (k.items + CARRY_SEGS - 1) / CARRY_SEGS, first = min(seg * each, k.items), last = min(first + each, k.items);
     const float A2 = a.A[i] * LOG2E;
-    float h = 0.f;
-    for (int r0 = 0; r0 < k.items; r0 += AHEAD) {
-        float e[AHEAD], sd[AHEAD]; int cut[AHEAD];
+    float e[KEEP], p[KEEP]; int cut[KEEP];
+    auto fetch = [&](int r0) {
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int at = min(r0 + u, k.items - 1), r = forward ? at : k.items - 1 - at;
-            e[u] = k.edge[r * n + i]; sd[u] = k.sum_delta[(int64_t)r * a.cols + c]; cut[u] = k.cut[r];
+        for (int u = 0; u < KEEP; ++u) {
+            const int q = min(r0 + u, k.items - 1), r = forward ? q : k.items - 1 - q;
+            e[u] = k.edge[r * n + i]; p[u] = A2 * k.sum_delta[(int64_t)r * a.cols + c]; cut[u] = k.cut[r];
         }
+    };
+    float h = 0.f, sum = 0.f; int any = 0;
+    for (int r0 = first; r0 < last; r0 += KEEP) {
+        fetch(r0);
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            if (r0 + u >= k.items) break;
-            k.edge[(forward ? r0 + u : k.items - 1 - r0 - u) * n + i] = h;
-            h = carried(A2 * sd[u], h, e[u], cut[u]);
+        for (int u = 0; u < KEEP; ++u) {
+            if (r0 + u >= last) break;
+            h = carried(p[u], h, e[u], cut[u]); sum += p[u]; any |= cut[u];
+        }
+    }
+    ps[seg][x] = sum; es[seg][x] = h; cs[seg][x] = any;
+    __syncthreads();
+    for (int d = 1; d < CARRY_SEGS; d *= 2) {
+        const int b = max(seg - d, 0);
+        const float pb = ps[b][x], eb = es[b][x]; const int cb = cs[b][x];
+        __syncthreads();
+        if (seg >= d) {
+            h = carried(sum, eb, h, any); sum += pb; any |= cb;
+            ps[seg][x] = sum; es[seg][x] = h; cs[seg][x] = any;
+        }
+        __syncthreads();
+    }
+    h = seg ? es[seg - 1][x] : 0.f;
+    for (int r0 = first; r0 < last; r0 += KEEP) {
+        if (last - first > KEEP) fetch(r0);
+#pragma unroll
+        for (int u = 0; u < KEEP; ++u) {
+            if (r0 + u >= last) break;
+            if (at < n) k.edge[(forward ? r0 + u : k.items - 1 - r0 - u) * n + i] = h;
+            h = carried(p[u], h, e[u], cut[u]);
         }
     }
 }
 int scan_carry(const ScanK& k, bool forward, hipStream_t s) {
     if (k.items <= CARRY_ITEMS) return 0;
-    hipLaunchKernelGGL(scan_carry_kernel, dim3((unsigned)(((int64_t)k.a.cols * k.a.states + 63) / 64)), dim3(64), 0, s, k, forward);
+    hipLaunchKernelGGL(scan_carry_kernel, dim3((unsigned)(((int64_t)k.a.cols * k.a.states + CARRY_W - 1) / CARRY_W)), dim3(CARRY_W * CARRY_SEGS), 0, s, k, forward);
     VC_HIP(hipGetLastError());
     return 0;
 }
@@ -108,13 +136,13 @@ template <int NS> struct RowPair {                                // B and C of 
     }
 };
 
-// One block walks the slots of one item for FWD_WAVES * 64 / L channels.  The next tile's rows are on their way while a tile is worked on.
+// One block walks the slots of one item for its waves * 64 / L channels.  The next tile's rows are on their way while a tile is worked on.
 template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_fwd_kernel(const ScanK k) {
     constexpr int NP = L * NS, NB = TILE / L;
     __shared__ float lds[FWD_WAVES][2][TILE * NP];
     const vc_scan_args& a = k.a;
     const int nblk = a.groups * k.nblk, item = blockIdx.x / nblk, blk = blockIdx.x - item * nblk;
-    const Lane<L, NS> w(k, FWD_WAVES, blk);
+    const Lane<L, NS> w(k, k.waves, blk);
     const int c = w.c, j = w.j, n0 = w.n0, nn = w.nn;
     const Rows<T, L> Y(a.y, a.y_ld, a.cols, c, j, w.ok);
     if (item == k.items) {                                       // rows behind the last utterance
@@ -252,11 +280,11 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_st
     }
 }
 
-// Whole utterances where these fill the card side by side (WALK_WAVES: two waves a SIMD), else runs of slots: as many as make run_waves waves, though
-// of no fewer than sqrt(slots / 32) slots, for a wave goes through all runs before its own.  Runs cost their first pass on top, 0.7 of the main pass.
+// Whole utterances where these fill the card side by side (WALK_WAVES: two waves a SIMD), else runs of slots: as many as make run_waves waves.  Runs
+// cost their first pass on top, 0.7 of the main pass, and more than CARRY_ITEMS of them the pass between.
 // Measured, bf16, 16 states: 1 x 8192 frames x 1024 channels 2880 us as one walk, 162 / 112 / 103 / 103 us in runs for 1024 / 2048 / 4096 / 8192 waves;
 // 1 x 128 x 1024 20 us walked, 10 in runs; 64 x 128 x 1024 (4096 waves side by side) 54 us walked, 94 in runs; 16 x 512 x 1024 (1024) 92 and 103, its
-// training step 380 and 332.
+// training step 380 and 332.  Few channels, training: 1 x 16384 x 64 82 us in runs of a slot, 99 in runs of six; 1 x 1152 x 33 36 and 54 (of two).
 constexpr int64_t WALK_WAVES = 2048, FWD_RUN_WAVES = 4096;
 int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_waves, ScanK* k) {
     VC_ARG(a, "%s: null pointer", who);
@@ -278,9 +306,10 @@ int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_wa
     k->m = SeqMap{a->offsets, (int)a->rows, a->n_seqs, (int)(a->rows / a->n_seqs)};
     k->cg = a->cols / a->groups;
     k->slots = (int)(a->rows / TILE) + a->n_seqs;
-    const int per = waves * 64 / scan_lanes(a->states);          // channels of a block
-    k->nblk = (k->cg + per - 1) / per;
-    const int64_t row_waves = (int64_t)a->groups * ((k->cg + 64 / scan_lanes(a->states) - 1) / (64 / scan_lanes(a->states)));      // waves that a frame's channels fill
+    const int cw = 64 / scan_lanes(a->states), need = (k->cg + cw - 1) / cw;     // channels of a wave; waves that a group's channels fill
+    k->nblk = (need + waves - 1) / waves;
+    k->waves = (need + k->nblk - 1) / k->nblk;                   // no wave without a channel, but for the last block's
+    const int64_t row_waves = (int64_t)a->groups * need;         // waves that a frame's channels fill
     const int64_t longest = !a->offsets ? k->m.len : a->max_len > 0 ? a->max_len : a->rows;
     // utterances that run side by side for as long as the longest lasts
     const int64_t side = longest > 0 ? std::max<int64_t>(1, a->rows / longest) : a->n_seqs;
@@ -288,7 +317,7 @@ int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_wa
     const int64_t want = std::max<int64_t>(1, run_waves / row_waves);
     // ... and runs where utterances are many and short: their first pass then has little to do, and the sums over items stay few
     if ((side * row_waves < WALK_WAVES && longest > 4 * TILE) || a->n_seqs > 4 * want) {
-        k->chunk = (int)std::max<int64_t>((int64_t)ceil(sqrt(k->slots / 32.0)), (k->slots + want - 1) / want);
+        k->chunk = (int)((k->slots + want - 1) / want);
         k->items = (k->slots + k->chunk - 1) / k->chunk;
         if (k->items == 1) { k->items = a->n_seqs; k->chunk = 0; }
     }
@@ -313,10 +342,10 @@ template <class T, int L, int NS> static int scan_fwd_l(const ScanK& k, hipStrea
     const int64_t per = (int64_t)k.a.groups * k.nblk, blocks = per * (k.items + (k.a.zero_tail && k.m.off ? 1 : 0));
     VC_ARG(blocks < (1LL << 31), "vc_selective_scan_fwd: too many utterances and channels for one launch");
     if (k.chunk) {
-        hipLaunchKernelGGL((scan_edge_kernel<T, L, NS>), dim3((unsigned)(per * k.items)), dim3(64 * FWD_WAVES), 0, s, k);
+        hipLaunchKernelGGL((scan_edge_kernel<T, L, NS>), dim3((unsigned)(per * k.items)), dim3(64 * k.waves), 0, s, k);
         VC_CHECK(scan_carry(k, true, s));
     }
-    hipLaunchKernelGGL((scan_fwd_kernel<T, L, NS>), dim3((unsigned)blocks), dim3(64 * FWD_WAVES), 0, s, k);
+    hipLaunchKernelGGL((scan_fwd_kernel<T, L, NS>), dim3((unsigned)blocks), dim3(64 * k.waves), 0, s, k);
     VC_HIP(hipGetLastError());
     return 0;
 }

@@ -62,14 +62,12 @@ template <int L, int NS> __device__ __forceinline__ int item_at(int it, int j) {
 }
 
 // First pass of a split axis: what each run hands on to the one before it.  Only rows up to the end of the run's first utterance matter.
-constexpr int EDGE_WAVES = 4;
-template <class T, int L, int NS> __global__ __launch_bounds__(64 * EDGE_WAVES) void scan_bwd_edge_kernel(const ScanK k, int nblk1) {
+template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES) void scan_bwd_edge_kernel(const ScanK k) {
     constexpr int NP = L * NS, NB = TILE / L;
-    __shared__ float lds[EDGE_WAVES][TILE * NP];
+    __shared__ float lds[BWD_WAVES][TILE * NP];
     const vc_scan_args& a = k.a;
-    const int nblk = a.groups * nblk1, item = blockIdx.x / nblk, blk = blockIdx.x - item * nblk;
-    ScanK kk = k; kk.nblk = nblk1;
-    const Lane<L, NS> w(kk, EDGE_WAVES, blk);
+    const int nblk = a.groups * k.nblk, item = blockIdx.x / nblk, blk = blockIdx.x - item * nblk;
+    const Lane<L, NS> w(k, k.waves, blk);
     const int c = w.c, j = w.j, n0 = w.n0, nn = w.nn;
     const bool has_z = a.z != nullptr;
     const Rows<T, L> DT(a.dt, a.dt_ld, a.cols, c, j), DY(a.dy, a.dy_ld, a.cols, c, j), Z(has_z ? a.z : a.dy, has_z ? a.z_ld : a.dy_ld, a.cols, c, j);
@@ -133,13 +131,15 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * EDGE_WAVES) 
 
 // Rows whose decays are worked out a second time on the way back: 4 NS registers for 4 NS exponentials of a tile, without which some would spill
 template <class T> constexpr int AGAIN = sizeof(T) == 4 ? 6 : 4;
-template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES, L == 16 && NS == 4 ? 1 : 2) void scan_bwd_kernel(const ScanK k) {
+// FULL: BWD_WAVES a block, known to the compiler (8192 x 1024, 16 states: 204 us with the forward pass in place of 208); fewer where a group's channels need no more
+template <class T, int L, int NS, bool FULL> __global__ __launch_bounds__(64 * BWD_WAVES, L == 16 && NS == 4 ? 1 : 2) void scan_bwd_kernel(const ScanK k) {
     constexpr int NP = L * NS, NB = TILE / L, WV = BWD_WAVES, R = RED<L, NS>;
     __shared__ float lds[WV][2][TILE * NP];
     __shared__ float red[2][WV][TILE * R];                       // two of them: one barrier a tile
     const vc_scan_args& a = k.a;
     const int nblk = a.groups * k.nblk, item = blockIdx.x / nblk, blk = blockIdx.x - item * nblk;
-    const Lane<L, NS> w(k, WV, blk);
+    const int waves = FULL ? WV : k.waves;
+    const Lane<L, NS> w(k, waves, blk);
     const int c = w.c, j = w.j, n0 = w.n0, nn = w.nn;
     const bool has_z = a.z != nullptr;
     const Rows<T, L> DX(a.dx, a.dx_ld, a.cols, c, j, w.ok), DDT(a.ddt, a.ddt_ld, a.cols, c, j, w.ok), DZ(a.dz, a.dz_ld, a.cols, c, j, w.ok);
@@ -162,6 +162,8 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES, L
     if (k.chunk) cur.find(q1 - 1); else cur.load(item);
     if (k.chunk && cur.base + cur.tiles > q1) carry_in<NS, false>(k, item, c, n0, nn, w.full, A2, dhc);
     float dDacc = 0.f, dbacc = 0.f;
+    // waves that this block has not got add nothing (there before the first sums are taken: a barrier lies between)
+    for (int o = waves * TILE * R + threadIdx.x; o < WV * TILE * R; o += 64 * waves) red[0][0][o] = red[1][0][o] = 0.f;
     float *Bs = lds[w.wave][0], *Cs = lds[w.wave][1];
     int turn = 0;
     for (int q = q1 - 1; q >= q0;) {                             // the utterances of the item, the last one first
@@ -274,7 +276,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES, L
             DDT.store(tt, b, dv);
         });
         __syncthreads();
-        for (int o = threadIdx.x; o < nr * 2 * NP; o += 64 * WV) {
+        for (int o = threadIdx.x; o < nr * 2 * NP; o += 64 * waves) {
             const int t = o / (2 * NP), e = o % (2 * NP), n = e % NP, it = (e / NP) * NS + n % NS;
             const float* at = red[turn][0] + t * R + item_at<L, NS>(it, n / NS);
             float f[WV * SPLIT<L, NS>];
@@ -303,9 +305,9 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES, L
 }
 
 // What the main pass left in parts: dB and dC are summed over the blocks of a group and rounded once (blocks [0, bc)), dA, dD and ddt_bias over the items
-// (one column of sums for 64 lanes and 4 waves).
+// (16 columns of sums a block, 16 threads a column).
 template <class T> __global__ __launch_bounds__(256) void scan_finish_kernel(const ScanK k, int np, int bc) {
-    __shared__ float red[4][64];
+    __shared__ float red[16][17];
     const vc_scan_args& a = k.a;
     if ((int)blockIdx.x < bc) {
         const int64_t w = (int64_t)2 * np * a.groups;
@@ -325,27 +327,30 @@ template <class T> __global__ __launch_bounds__(256) void scan_finish_kernel(con
         return;
     }
     // dapart [items][cols * states], chpart [items][2 * cols]
-    const int64_t na = (int64_t)a.cols * a.states, i = (int64_t)(blockIdx.x - bc) * 64 + (threadIdx.x & 63);
+    const int64_t na = (int64_t)a.cols * a.states, i = (int64_t)(blockIdx.x - bc) * 16 + (threadIdx.x & 15);
     const bool second = i >= na;
     const int64_t e = second ? i - na : i, width = second ? 2 * (int64_t)a.cols : na;
     const float* src = second ? k.chpart : k.dapart;
-    const int w = threadIdx.x >> 6;
+    const int w = threadIdx.x >> 4;
     float s = 0.f;
     if (e < width) {
         int q = w;
-        for (; q + 28 < k.items; q += 32) {
+        for (; q + 112 < k.items; q += 128) {
             float v[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = src[(q + 4 * u) * width + e];
+            for (int u = 0; u < 8; ++u) v[u] = src[(q + 16 * u) * width + e];
 #pragma unroll
             for (int u = 0; u < 8; ++u) s += v[u];
         }
-        for (; q < k.items; q += 4) s += src[q * width + e];
+#pragma unroll 4
+        for (; q < k.items; q += 16) s += src[q * width + e];
     }
-    red[w][threadIdx.x & 63] = s;
+    red[w][threadIdx.x & 15] = s;
     __syncthreads();
     if (w || e >= width) return;
-    s = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+    s = 0.f;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) s += red[u][threadIdx.x];
     if (!second) a.dA[e] = s;
     else if (e < a.cols) { if (a.dD) a.dD[e] = s; }
     else if (a.ddt_bias) a.ddt_bias[e - a.cols] = s;
@@ -369,15 +374,15 @@ extern "C" int64_t vc_selective_scan_bwd_work(const vc_scan_args* a) {
 template <class T, int L, int NS> static int scan_bwd_l(const ScanK& k, hipStream_t s) {
     const int64_t blocks = (int64_t)k.a.groups * k.nblk * (k.items + (k.a.zero_tail && k.m.off ? 1 : 0));
     const int64_t bc = std::min<int64_t>(((int64_t)k.m.rows * 2 * L * NS * k.a.groups + 255) / 256, 1 << 22);
-    const int per = EDGE_WAVES * 64 / L, nblk1 = (k.cg + per - 1) / per;
-    const int64_t eb = (int64_t)k.a.groups * nblk1 * k.items;
+    const int64_t eb = (int64_t)k.a.groups * k.nblk * k.items;
     VC_ARG(blocks < (1LL << 31) && eb < (1LL << 31), "vc_selective_scan_bwd: too many utterances and channels for one launch");
     if (k.chunk) {
-        hipLaunchKernelGGL((scan_bwd_edge_kernel<T, L, NS>), dim3((unsigned)eb), dim3(64 * EDGE_WAVES), 0, s, k, nblk1);
+        hipLaunchKernelGGL((scan_bwd_edge_kernel<T, L, NS>), dim3((unsigned)eb), dim3(64 * k.waves), 0, s, k);
         VC_CHECK(scan_carry(k, false, s));
     }
-    hipLaunchKernelGGL((scan_bwd_kernel<T, L, NS>), dim3((unsigned)blocks), dim3(64 * BWD_WAVES), 0, s, k);
-    const int64_t pc = ((int64_t)k.a.cols * (k.a.states + 2) + 63) / 64;
+    if (k.waves == BWD_WAVES) hipLaunchKernelGGL((scan_bwd_kernel<T, L, NS, true>), dim3((unsigned)blocks), dim3(64 * BWD_WAVES), 0, s, k);
+    else hipLaunchKernelGGL((scan_bwd_kernel<T, L, NS, false>), dim3((unsigned)blocks), dim3(64 * k.waves), 0, s, k);
+    const int64_t pc = ((int64_t)k.a.cols * (k.a.states + 2) + 15) / 16;
     VC_ARG(bc + pc < (1LL << 31), "vc_selective_scan_bwd: too many rows and channels for one launch");
     hipLaunchKernelGGL((scan_finish_kernel<T>), dim3((unsigned)(bc + pc)), dim3(256), 0, s, k, L * NS, (int)bc);
     VC_HIP(hipGetLastError());
