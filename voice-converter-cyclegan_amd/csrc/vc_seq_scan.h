@@ -23,7 +23,7 @@ struct ScanK {
     // How the time axis is shared out: items are whole utterances (chunk = 0), or runs of `chunk` slots whatever utterances these belong to.
     // In the second form a first pass works out what each run does to a state that enters it, h -> exp(A sum_delta) h + edge, and the main pass begins
     // with the sum of what the runs before it hand on.  `cut` marks the runs that hand on nothing of what enters (an utterance begins or ends there).
-    int items, chunk;
+    int items, chunk; bool once;   // once: what enters the runs is worked out by a pass of its own
     float *edge, *sum_delta; int* cut;             // [items][cols][states], [items][cols], [items]
     float *part, *dapart, *chpart; // backward: partial sums of dB / dC, dA, and of dD and ddt_bias
 };
@@ -209,7 +209,9 @@ int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_wa
 int64_t scan_edge_floats(const ScanK& k);                        // of edge, sum_delta and cut
 void scan_edge_place(ScanK* k, float* work);
 // What enters run `item` from the runs before it (behind it where !FORWARD).  Up to CARRY_ITEMS runs every wave goes through them itself, which saves a
-// launch; more are gone through once for all by scan_carry, which puts what enters a run in the place of what it hands on.
+// launch (half as many where lanes lack states and load them one by one); more are gone through once for all by scan_carry, which puts what enters a run in
+// the place of what it hands on.  1 x 8192 x 1024 (64 runs) 102 us by the waves, 106 by scan_carry, 512 rows (33) 17 and 23; 617 x 277 with 21 states (53
+// runs) 26 and 23.
 constexpr int CARRY_ITEMS = 64;
 // exp2(p) h + e, or e where nothing is handed on.  In two halves: the factor of a whole run may leave the range of fp32 where its product with h does not
 // (frame by frame it would not either), and a state of zero stays one under any factor.
@@ -221,7 +223,7 @@ int scan_carry(const ScanK& k, bool forward, hipStream_t s);
 template <int NS, bool FORWARD> __device__ __forceinline__ void carry_in(const ScanK& k, int item, int c, int n0, int nn, bool full, const float (&A2)[NS], float (&h)[NS]) {
     constexpr int AT_ONCE = 8;                                   // runs whose loads are on their way together: the chain itself is one multiply-add a run
     const vc_scan_args& a = k.a;
-    if (k.items > CARRY_ITEMS) {
+    if (k.once) {
         load_state<NS>(k.edge + ((int64_t)item * a.cols + c) * a.states + n0, h, nn, full);
         return;
     }

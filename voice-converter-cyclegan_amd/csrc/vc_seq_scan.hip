@@ -120,7 +120,7 @@ __global__ __launch_bounds__(CARRY_W * CARRY_SEGS) void scan_carry_kernel(const 
     }
 }
 int scan_carry(const ScanK& k, bool forward, hipStream_t s) {
-    if (k.items <= CARRY_ITEMS) return 0;
+    if (!k.once) return 0;
     hipLaunchKernelGGL(scan_carry_kernel, dim3((unsigned)(((int64_t)k.a.cols * k.a.states + CARRY_W - 1) / CARRY_W)), dim3(CARRY_W * CARRY_SEGS), 0, s, k, forward);
     VC_HIP(hipGetLastError());
     return 0;
@@ -320,6 +320,7 @@ int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_wa
         k->chunk = (int)((k->slots + want - 1) / want);
         k->items = (k->slots + k->chunk - 1) / k->chunk;
         if (k->items == 1) { k->items = a->n_seqs; k->chunk = 0; }
+        k->once = k->items > (a->states == scan_padded(a->states) ? CARRY_ITEMS : CARRY_ITEMS / 2);
     }
     return 0;
 }
