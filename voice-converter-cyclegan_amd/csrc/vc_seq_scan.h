@@ -63,7 +63,11 @@ template <int CTRL> __device__ __forceinline__ float dpp_all(float x) {
 // lane i's value of the L lanes that share a channel
 template <int L, int I> __device__ __forceinline__ float from_lane(float v) {
     if constexpr (L == 4) return dpp_all<I * 0x55>(v);          // quad_perm [i,i,i,i]
-    else return dpp_all<0x150 + I>(v);                          // row_newbcast:i
+    else if constexpr (L == 16) return dpp_all<0x150 + I>(v);   // row_newbcast:i
+    else {                                                      // row_newbcast:i, and :8 + i for the upper eight lanes of a row
+        const int x = __builtin_bit_cast(int, v);
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_amdgcn_mov_dpp(x, 0x150 + I, 0xf, 0xf, true), x, 0x158 + I, 0xf, 0xc, false));
+    }
 }
 // one step of sums_by_row: rows kept by one bit of the lane, the others handed to the lane that keeps them
 template <int CTRL, int N> __device__ __forceinline__ void halve(float (&v)[N], bool up) {
@@ -75,31 +79,30 @@ template <int CTRL, int N> __device__ __forceinline__ void halve(float (&v)[N], 
 }
 // v[i] = this lane's share of row i; lane j gets the sum of row j over the L lanes (L - 1 additions in place of L log2 L)
 template <int L> __device__ __forceinline__ float sums_by_row(float (&v)[L], int j) {
-    if constexpr (L == 16) {
-        halve<0x128, 16>(v, j & 8);                              // row_ror:8
-        float w[8], q[4], p[2];
+    if constexpr (L == 16) halve<0x128, 16>(v, j & 8);           // row_ror:8
+    if constexpr (L >= 8) {
+        float w[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = v[i];
         halve<0x141, 8>(w, j & 4);                               // row_half_mirror
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = w[i];
-        halve<0x4E, 4>(q, j & 2);
-        p[0] = q[0]; p[1] = q[1];
-        halve<0xB1, 2>(p, j & 1);
-        return p[0];
-    } else {
-        float p[2];
-        halve<0x4E, 4>(v, j & 2);                                // quad_perm [2,3,0,1]
-        p[0] = v[0]; p[1] = v[1];
-        halve<0xB1, 2>(p, j & 1);                                // quad_perm [1,0,3,2]
-        return p[0];
+        for (int i = 0; i < 4; ++i) v[i] = w[i];
     }
+    float q[4], p[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = v[i];
+    halve<0x4E, 4>(q, j & 2);                                    // quad_perm [2,3,0,1]
+    p[0] = q[0]; p[1] = q[1];
+    halve<0xB1, 2>(p, j & 1);                                    // quad_perm [1,0,3,2]
+    return p[0];
 }
 // sum over the L lanes of a channel, in all of them
 template <int L> __device__ __forceinline__ float channel_sum(float v) {
     if constexpr (L == 16) return row16_sum(v);
     v += dpp_all<0xB1>(v);
-    return v + dpp_all<0x4E>(v);
+    v += dpp_all<0x4E>(v);
+    if constexpr (L == 8) v += dpp_all<0x141>(v);
+    return v;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -200,10 +203,11 @@ template <int NS> __device__ __forceinline__ void store_state(float* p, const fl
     if (full) store_vec<float, NS>(p, h); else store_some<float, NS>(p, h, nn);
 }
 
-// which register layout serves a number of states, and how many channels a block of `waves` waves covers
+// Which register layout serves a number of states.  Four states a lane carry a row's fixed costs better than two: 64 x 128 x 1024 bf16, 32 states 94 us by
+// 8 lanes of four, 140 by 16 of two (training 398 and 556).
 #define SCAN_LAYOUT(T, states, F, ...) \
-    ((states) <= 8 ? F<T, 4, 2>(__VA_ARGS__) : (states) <= 16 ? F<T, 4, 4>(__VA_ARGS__) : (states) <= 32 ? F<T, 16, 2>(__VA_ARGS__) : F<T, 16, 4>(__VA_ARGS__))
-static inline int scan_lanes(int states) { return states <= 16 ? 4 : 16; }
+    ((states) <= 8 ? F<T, 4, 2>(__VA_ARGS__) : (states) <= 16 ? F<T, 4, 4>(__VA_ARGS__) : (states) <= 32 ? F<T, 8, 4>(__VA_ARGS__) : F<T, 16, 4>(__VA_ARGS__))
+static inline int scan_lanes(int states) { return states <= 16 ? 4 : states <= 32 ? 8 : 16; }
 static inline int scan_padded(int states) { return states <= 8 ? 8 : states <= 16 ? 16 : states <= 32 ? 32 : 64; }
 int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_waves, ScanK* k);
 int64_t scan_edge_floats(const ScanK& k);                        // of edge, sum_delta and cut

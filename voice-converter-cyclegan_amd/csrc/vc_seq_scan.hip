@@ -1,10 +1,10 @@
 // vc_seq_scan.hip -- selective state space scan: prompts and single frames (vc_seq_scan.h says how the work is laid out).
 #include "vc_seq_scan.h"
-#include <cmath>
 
 constexpr int FWD_WAVES = 4;
 
-// First pass of a split axis: what each run hands on.  Only rows from the last utterance's beginning on matter.
+// First pass of a split axis: what each run hands on.  Only rows from the last utterance's beginning on matter.  Bound by vector issue: a product, an
+// exponential and two multiply-adds a state; 1 x 8192 x 1024 bf16, 16 states: 39 us, the main pass 63.
 template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_edge_kernel(const ScanK k) {
     constexpr int NP = L * NS, NB = TILE / L;
     __shared__ float lds[FWD_WAVES][TILE * NP];
@@ -68,7 +68,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_ed
 
 // Second pass of a split axis: from what every run hands on to what enters it, for 16 states a block.  64 threads share a state's runs: each goes through
 // its own as if nothing entered them, what they do together -- h -> exp2(p) h + e, or e behind a cut -- is combined over the threads before, and each
-// goes through its own once more from there.
+// goes through its own once more from there.  A launch and a few trips to memory: 5 to 8 us, where one thread a state took 15 for 109 runs.
 constexpr int CARRY_W = 16, CARRY_SEGS = 64;
 __global__ __launch_bounds__(CARRY_W * CARRY_SEGS) void scan_carry_kernel(const ScanK k, bool forward) {
     constexpr int KEEP = 8;
@@ -137,6 +137,8 @@ template <int NS> struct RowPair {                                // B and C of 
 };
 
 // One block walks the slots of one item for its waves * 64 / L channels.  The next tile's rows are on their way while a tile is worked on.
+// Bound by vector issue: a row and channel costs a lane a product, an exponential (two slots) and three multiply-adds for each of its states, and its share
+// of softplus, gate and sums.  64 x 128 x 1024 bf16, 16 states: 52 us with the vector units busy 85 % of the time (the bytes alone would take 14).
 template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_fwd_kernel(const ScanK k) {
     constexpr int NP = L * NS, NB = TILE / L;
     __shared__ float lds[FWD_WAVES][2][TILE * NP];
@@ -236,7 +238,7 @@ struct ScanStepArgs {
     int64_t x_ld, dt_ld, z_ld, b_ld, c_ld, y_ld; int rows, n_slots, cols, states, groups, softplus;
 };
 // Bound by the state's traffic: L lanes a channel as in the scan, STEP_U channels a lane group.  Everything is asked for before the earlier rows' slots are
-// looked through; a slot outside the pool reads entry 0 and drops it.
+// looked through; a slot outside the pool reads entry 0 and drops it.  256 streams x 2048 bf16, 16 states: 16.7 us, 4.3 TB/s; one of 1024: 3.8 us.
 constexpr int STEP_U = 2;
 template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_step_kernel(const ScanStepArgs a) {
     constexpr int G = 256 / L;                                   // lane groups of a block

@@ -2,6 +2,8 @@
 //   dh_t = C_t dp_t + a_{t+1} dh_{t+1} (dp = dy * gate, a = exp(delta A));  with q_t = dh_t a_t h_{t-1}:
 //   dA = sum_t q delta;  ddelta = sum_n q A + x sum_n dh B;  dx = D dp + delta sum_n dh B;  dB = sum_c dh delta x;  dC = sum_c dp h
 // A tile's states are worked out again from the one the forward kept in front of it: a and h of its 16 rows stay in registers for the way back.
+// Bound by vector issue: six slots a state on the way there, eight and five for the sums over channels on the way back, two waves a SIMD (the registers).
+// 64 x 128 x 1024 bf16, 16 states: 134 us, the vector units busy 76 % of the time.
 #include "vc_seq_scan.h"
 
 constexpr int BWD_WAVES = 4;                                     // of a block.  8 leave half as many partial sums of dB and dC and cost 2 %: more waves stand at a barrier together
@@ -28,7 +30,7 @@ template <int N> __device__ __forceinline__ void across_16(float (&v)[N]) {
         v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     }
 }
-// dst[i][64]: 2 NS = 8 values and L = 4: one a lane, item = bit3 + 2 bit4 + 4 bit5; 4 values: one a lane (the last channel steps not taken for L = 4),
+// dst[i][64]: 2 NS = 8 values and L = 4 or 8: one a lane, item = bit3 + 2 bit4 + 4 bit5; 4 values: one a lane (the last channel steps not taken for L = 4),
 // item = bit4 + 2 bit5; 8 values and L = 16: two a lane, item = i + 2 bit4 + 4 bit5
 template <int L, int NS> __device__ __forceinline__ void reduce_to_lds(float (&v)[2 * NS], float* dst, int lane) {
     if constexpr (NS == 4) {
@@ -38,7 +40,7 @@ template <int L, int NS> __device__ __forceinline__ void reduce_to_lds(float (&v
         for (int i = 0; i < 4; ++i) w[i] = v[i];
         across_16<4>(w);
         u[0] = w[0]; u[1] = w[1];
-        if constexpr (L == 4) {
+        if constexpr (L <= 8) {
             halve<0x128, 2>(u, lane & 8);                        // row_ror:8
             dst[lane] = u[0];
         } else {
@@ -54,14 +56,15 @@ template <int L, int NS> __device__ __forceinline__ void reduce_to_lds(float (&v
 }
 template <int L, int NS> constexpr int RED = (L == 16 && NS == 4) ? 128 : 64;      // floats a wave leaves for one row
 // what one wave left of item `it` (0..NS-1 dB, NS.. dC) of lane j of the channels: SPLIT numbers to be added
-template <int L, int NS> constexpr int SPLIT = L == 16 ? 1 : NS == 4 ? 2 : 4;
+template <int L, int NS> constexpr int SPLIT = L >= 8 ? 1 : NS == 4 ? 2 : 4;
 template <int L, int NS> __device__ __forceinline__ int item_at(int it, int j) {
-    if constexpr (L == 4 && NS == 4) return ((it & 1) << 3) + ((it & 2) << 3) + ((it & 4) << 3) + j;
+    if constexpr (L <= 8 && NS == 4) return ((it & 1) << 3) + ((it & 2) << 3) + ((it & 4) << 3) + j;
     else if constexpr (NS == 4) return (it & 1) * 64 + ((it & 2) << 3) + ((it & 4) << 3) + j;
     else return ((it & 1) << 4) + ((it & 2) << 4) + j;
 }
 
-// First pass of a split axis: what each run hands on to the one before it.  Only rows up to the end of the run's first utterance matter.
+// First pass of a split axis: what each run hands on to the one before it.  Only rows up to the end of the run's first utterance matter.  Bound by vector
+// issue, like the forward's; 2208 x 1002 fp32, 12 states: 16 us.
 template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES) void scan_bwd_edge_kernel(const ScanK k) {
     constexpr int NP = L * NS, NB = TILE / L;
     __shared__ float lds[BWD_WAVES][TILE * NP];
@@ -305,7 +308,7 @@ template <class T, int L, int NS, bool FULL> __global__ __launch_bounds__(64 * B
 }
 
 // What the main pass left in parts: dB and dC are summed over the blocks of a group and rounded once (blocks [0, bc)), dA, dD and ddt_bias over the items
-// (16 columns of sums a block, 16 threads a column).
+// (16 columns of sums a block, 16 threads a column).  64 x 128 x 1024: 6 us.
 template <class T> __global__ __launch_bounds__(256) void scan_finish_kernel(const ScanK k, int np, int bc) {
     __shared__ float red[16][17];
     const vc_scan_args& a = k.a;
