@@ -882,3 +882,42 @@ def test_slots_beyond_32_bit_offsets(S):
     y = S.causal_conv1d_step(x, state, rnd(3, 4, cols), slots=torch.tensor([n - 1, 0], dtype=torch.int32, device=DEV))
     assert torch.equal(y[0], y[1]) and torch.equal(state[0], state[n - 1]) and torch.equal(state[0, 2], x[0])
     assert (state[1] == 0).all() and (state[n - 2] == 0).all()
+
+
+@pytest.mark.parametrize('cols,states,kind', [(16, 4, F32), (20, 16, BF16), (6, 21, F32)])
+def test_scan_of_very_many_runs(S, cols, states, kind):
+    """few channels and thousands of frames: hundreds of runs of a tile, what enters them worked out by a pass of its own, several runs a thread"""
+    lengths = [7000, 0, 1500, 33, 700]
+    n, rows = len(lengths), sum(lengths)
+    v = scan_inputs(rows, cols, states, 1, kind, n)
+    dy, df = rnd(20, rows, cols, dtype=kind), rnd(21, n, cols, states)
+    leaves = [t.requires_grad_(True) for t in v.values()]
+    y, final = S.selective_scan(v['x'], v['dt'], v['A'], v['B'], v['C'], D=v['D'], z=v['z'], dt_bias=v['dt_bias'], initial_state=v['initial'],
+                                seq_offsets=offsets_of(lengths), return_final_state=True)
+    r = O.scan(**v, lengths=lengths, dy=dy, dfinal=df)
+    m = O.scan(**v, lengths=lengths, dy=dy, dfinal=df, absolute=True)
+    last = lasts(r, v['A'], max(lengths))
+    close(y, r['y'], m['y'], 3 * last + states + 40, 'y')
+    close(final, r['final'], m['final'], 3 * last + states + 40, 'final')
+    for (name, _), got in zip(v.items(), torch.autograd.grad((y, final), leaves, (dy, df))):
+        close(got, r['d' + name], m['d' + name], 6 * last + rows + cols + states + 60, 'd' + name)
+
+
+def test_a_state_that_grows_through_very_many_runs(S):
+    """A > 0 over 640 runs: the factor of many runs together leaves the range of fp32, a state of zero stays one, and one that starts late stays finite"""
+    rows, cols, n = 10240, 16, 4
+    x = torch.zeros(1, rows, cols, device=DEV)
+    x[0, rows - 300] = 1.0                                        # nothing before it
+    dt = torch.full((1, rows, cols), 0.2, device=DEV)
+    A = torch.full((cols, n), 0.5, device=DEV)
+    one = torch.ones(1, rows, n, device=DEV)
+    with torch.no_grad():
+        y, final = S.selective_scan(x, dt, A, one, one, softplus=False, return_final_state=True)
+    assert (y[0, :rows - 300] == 0).all() and torch.isfinite(y).all()
+    steps = torch.arange(300, dtype=torch.float64)
+    want = n * 0.2 * torch.exp(0.1 * steps)                       # e^30 at the end
+    got = y[0, rows - 300:, 0].cpu().double()
+    # a frame: two units for the exponential, one for the product, 0.3 for the exponent; over all: 0.2 and log2(e) as fp32 have them, and the exponents of
+    # the runs' sums, which end at 43
+    assert ((got - want).abs() <= want * U * (4 * 300 + 200)).all()
+    assert torch.allclose(final, y[0, -1, 0] / n, rtol=1e-6)

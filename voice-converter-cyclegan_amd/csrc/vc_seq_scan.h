@@ -209,7 +209,7 @@ template <int NS> __device__ __forceinline__ void store_state(float* p, const fl
     ((states) <= 8 ? F<T, 4, 2>(__VA_ARGS__) : (states) <= 16 ? F<T, 4, 4>(__VA_ARGS__) : (states) <= 32 ? F<T, 8, 4>(__VA_ARGS__) : F<T, 16, 4>(__VA_ARGS__))
 static inline int scan_lanes(int states) { return states <= 16 ? 4 : states <= 32 ? 8 : 16; }
 static inline int scan_padded(int states) { return states <= 8 ? 8 : states <= 16 ? 16 : states <= 32 ? 32 : 64; }
-int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_waves, ScanK* k);
+int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_waves, double margin, ScanK* k);
 int64_t scan_edge_floats(const ScanK& k);                        // of edge, sum_delta and cut
 void scan_edge_place(ScanK* k, float* work);
 // What enters run `item` from the runs before it (behind it where !FORWARD).  Up to CARRY_ITEMS runs every wave goes through them itself, which saves a

@@ -282,13 +282,16 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_st
     }
 }
 
-// Whole utterances where these fill the card side by side (WALK_WAVES: two waves a SIMD), else runs of slots: as many as make run_waves waves.  Runs
-// cost their first pass on top, 0.7 of the main pass, and more than CARRY_ITEMS of them the pass between.
-// Measured, bf16, 16 states: 1 x 8192 frames x 1024 channels 2880 us as one walk, 162 / 112 / 103 / 103 us in runs for 1024 / 2048 / 4096 / 8192 waves;
-// 1 x 128 x 1024 20 us walked, 10 in runs; 64 x 128 x 1024 (4096 waves side by side) 54 us walked, 94 in runs; 16 x 512 x 1024 (1024) 92 and 103, its
-// training step 380 and 332.  Few channels, training: 1 x 16384 x 64 82 us in runs of a slot, 99 in runs of six; 1 x 1152 x 33 36 and 54 (of two).
-constexpr int64_t WALK_WAVES = 2048, FWD_RUN_WAVES = 4096;
-int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_waves, ScanK* k) {
+// Whole utterances, each walked by its own waves, or runs of slots, as many as make run_waves waves.  With w waves a SIMD side by side a row of the longest
+// utterance takes about max(0.18, 0.1 w) us walked; in runs all rows are shared out, at 0.16 us a row for w = 1, since the first pass costs 0.7 of the main
+// one, and the passes before the main one cost a few us more, the more waves the more (`margin`).  So walk where longest * (0.18 - 0.16 w) < 6 + margin w.
+// Measured, bf16, 16 states, 1024 channels, forward (walked and in runs): 1 x 8192 frames 2880 and 103, 1 x 128 20 and 10, 1 x 32 6.9 and 9.1, 8 x 128 21
+// and 27, 8 x 256 47 and 38, 16 x 512 91 and 102, 16 x 1024 194 and 185, 16 x 2048 400 and 338, 24 x 100 27 and 47, 64 x 128 54 and 94; the gradient 8 x 128 55 and 46, 16 x 512
+// 214 and 210, 24 x 100 66 and 78, 1 x 32 the same.  1 x 8192 in runs for 1024 / 2048 / 4096 / 8192 waves: 162 / 112 / 103 / 103.  Few channels, training:
+// 1 x 16384 x 64 82 in runs of a slot, 99 in runs of six.
+constexpr int64_t FWD_RUN_WAVES = 4096;
+constexpr double FWD_MARGIN = 14;
+int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_waves, double margin, ScanK* k) {
     VC_ARG(a, "%s: null pointer", who);
     VC_ARG(seq_type_ok(a->type), "%s: type must be VC_F32, VC_BF16 or VC_F16", who);
     VC_ARG(a->states >= 1 && a->states <= 64, "%s: 1 to 64 states, got %d", who, a->states);
@@ -318,7 +321,9 @@ int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_wa
     k->items = a->n_seqs; k->chunk = 0;
     const int64_t want = std::max<int64_t>(1, run_waves / row_waves);
     // ... and runs where utterances are many and short: their first pass then has little to do, and the sums over items stay few
-    if ((side * row_waves < WALK_WAVES && longest > 4 * TILE) || a->n_seqs > 4 * want) {
+    const double w = side * row_waves / 1024.0;                  // waves a SIMD, walked
+    const bool walk = longest * (0.18 - 0.16 * w) < 6 + margin * w;
+    if (!walk || a->n_seqs > 4 * want) {
         k->chunk = (int)((k->slots + want - 1) / want);
         k->items = (k->slots + k->chunk - 1) / k->chunk;
         if (k->items == 1) { k->items = a->n_seqs; k->chunk = 0; }
@@ -333,11 +338,11 @@ void scan_edge_place(ScanK* k, float* work) {
     k->cut = (int*)(k->sum_delta + (int64_t)k->items * k->a.cols);
 }
 extern "C" int64_t vc_selective_scan_saved(const vc_scan_args* a) {
-    ScanK k; if (scan_setup("vc_selective_scan_saved", a, FWD_WAVES, FWD_RUN_WAVES, &k)) return VC_E_ARG;
+    ScanK k; if (scan_setup("vc_selective_scan_saved", a, FWD_WAVES, FWD_RUN_WAVES, FWD_MARGIN, &k)) return VC_E_ARG;
     return (int64_t)k.slots * a->cols * a->states;
 }
 extern "C" int64_t vc_selective_scan_fwd_work(const vc_scan_args* a) {
-    ScanK k; if (scan_setup("vc_selective_scan_fwd_work", a, FWD_WAVES, FWD_RUN_WAVES, &k)) return VC_E_ARG;
+    ScanK k; if (scan_setup("vc_selective_scan_fwd_work", a, FWD_WAVES, FWD_RUN_WAVES, FWD_MARGIN, &k)) return VC_E_ARG;
     return scan_edge_floats(k);
 }
 
@@ -354,7 +359,7 @@ template <class T, int L, int NS> static int scan_fwd_l(const ScanK& k, hipStrea
 }
 template <class T> static int scan_fwd_t(const ScanK& k, hipStream_t s) { return SCAN_LAYOUT(T, k.a.states, scan_fwd_l, k, s); }
 extern "C" int vc_selective_scan_fwd(const vc_scan_args* a, void* stream) {
-    ScanK k; VC_CHECK(scan_setup("vc_selective_scan_fwd", a, FWD_WAVES, FWD_RUN_WAVES, &k));
+    ScanK k; VC_CHECK(scan_setup("vc_selective_scan_fwd", a, FWD_WAVES, FWD_RUN_WAVES, FWD_MARGIN, &k));
     VC_ARG(a->A && (a->rows == 0 || (a->x && a->dt && a->B && a->C && a->y)), "vc_selective_scan_fwd: null pointer");
     VC_ARG(!a->final_state || a->final_state != a->initial, "vc_selective_scan_fwd: final_state may not be initial");
     if (a->saved && a->saved_floats < (int64_t)k.slots * a->cols * a->states) { vc_set_error("vc_selective_scan_fwd: saved is too small"); return VC_E_NOMEM; }

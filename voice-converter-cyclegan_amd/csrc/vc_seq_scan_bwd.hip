@@ -359,10 +359,11 @@ template <class T> __global__ __launch_bounds__(256) void scan_finish_kernel(con
     else if (a.ddt_bias) a.ddt_bias[e - a.cols] = s;
 }
 
+constexpr double BWD_MARGIN = 4;
 constexpr int64_t BWD_RUN_WAVES = 2048;                          // two waves a SIMD is what its registers allow
 static int bwd_setup(const char* who, const vc_scan_args* a, ScanK* k, int64_t* floats) {
     VC_ARG(a, "%s: null pointer", who);
-    VC_CHECK(scan_setup(who, a, BWD_WAVES, BWD_RUN_WAVES, k));
+    VC_CHECK(scan_setup(who, a, BWD_WAVES, BWD_RUN_WAVES, BWD_MARGIN, k));
     const int64_t part = (int64_t)a->groups * k->nblk * a->rows * 2 * scan_padded(a->states);
     const int64_t da = (int64_t)k->items * a->cols * a->states, ch = (int64_t)k->items * 2 * a->cols;
     *floats = part + da + ch + scan_edge_floats(*k);
