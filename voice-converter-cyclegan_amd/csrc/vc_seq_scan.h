@@ -213,10 +213,9 @@ int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_wa
 int64_t scan_edge_floats(const ScanK& k);                        // of edge, sum_delta and cut
 void scan_edge_place(ScanK* k, float* work);
 // What enters run `item` from the runs before it (behind it where !FORWARD).  Up to CARRY_ITEMS runs every wave goes through them itself, which saves a
-// launch (half as many where lanes lack states and load them one by one); more are gone through once for all by scan_carry, which puts what enters a run in
-// the place of what it hands on.  1 x 8192 x 1024 (64 runs) 102 us by the waves, 106 by scan_carry, 512 rows (33) 17 and 23; 617 x 277 with 21 states (53
-// runs) 26 and 23.
-constexpr int CARRY_ITEMS = 64;
+// launch; more are gone through once for all by scan_carry, which puts what enters a run in the place of what it hands on.  1 x 8192 x 1024 (64 runs)
+// 102 us by the waves, 100 by scan_carry; 1 x 512 x 1024 (33) 17 and 18; 8 x 128 x 1024 training (up to 32) 70 and 74.
+constexpr int CARRY_ITEMS = 32;
 // exp2(p) h + e, or e where nothing is handed on.  In two halves: the factor of a whole run may leave the range of fp32 where its product with h does not
 // (frame by frame it would not either), and a state of zero stays one under any factor.
 __device__ __forceinline__ float carried(float p, float h, float e, int cut) {

@@ -66,18 +66,19 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_ed
     if (blk == 0 && threadIdx.x == 0) k.cut[item] = cut;
 }
 
-// Second pass of a split axis: from what every run hands on to what enters it, for 16 states a block.  64 threads share a state's runs: each goes through
+// Second pass of a split axis: from what every run hands on to what enters it, for 16 states a block.  SEGS threads share a state's runs: each goes through
 // its own as if nothing entered them, what they do together -- h -> exp2(p) h + e, or e behind a cut -- is combined over the threads before, and each
-// goes through its own once more from there.  A launch and a few trips to memory: 5 to 8 us, where one thread a state took 15 for 109 runs.
-constexpr int CARRY_W = 16, CARRY_SEGS = 64;
-__global__ __launch_bounds__(CARRY_W * CARRY_SEGS) void scan_carry_kernel(const ScanK k, bool forward) {
+// goes through its own once more from there.  A launch and a few trips to memory: 4 to 8 us, where one thread a state took 15 for 109 runs.  Up to 128 runs
+// 16 threads are enough (2208 x 1002 x 12: 4 us less than by 64), for 425 runs they cost 8 us more.
+constexpr int CARRY_W = 16;
+template <int SEGS> __global__ __launch_bounds__(CARRY_W * SEGS) void scan_carry_kernel(const ScanK k, bool forward) {
     constexpr int KEEP = 8;
-    __shared__ float ps[CARRY_SEGS][CARRY_W], es[CARRY_SEGS][CARRY_W];
-    __shared__ int cs[CARRY_SEGS][CARRY_W];
+    __shared__ float ps[SEGS][CARRY_W], es[SEGS][CARRY_W];
+    __shared__ int cs[SEGS][CARRY_W];
     const vc_scan_args& a = k.a;
     const int x = threadIdx.x % CARRY_W, seg = threadIdx.x / CARRY_W;
     const int64_t n = (int64_t)a.cols * a.states, at = (int64_t)blockIdx.x * CARRY_W + x, i = min(at, n - 1);      // past the last state: the last one again, not stored
-    const int c = (int)(i / a.states), each = (k.items + CARRY_SEGS - 1) / CARRY_SEGS, first = min(seg * each, k.items), last = min(first + each, k.items);
+    const int c = (int)(i / a.states), each = (k.items + SEGS - 1) / SEGS, first = min(seg * each, k.items), last = min(first + each, k.items);
     const float A2 = a.A[i] * LOG2E;
     float e[KEEP], p[KEEP]; int cut[KEEP];
     auto fetch = [&](int r0) {
@@ -98,7 +99,7 @@ __global__ __launch_bounds__(CARRY_W * CARRY_SEGS) void scan_carry_kernel(const 
     }
     ps[seg][x] = sum; es[seg][x] = h; cs[seg][x] = any;
     __syncthreads();
-    for (int d = 1; d < CARRY_SEGS; d *= 2) {
+    for (int d = 1; d < SEGS; d *= 2) {
         const int b = max(seg - d, 0);
         const float pb = ps[b][x], eb = es[b][x]; const int cb = cs[b][x];
         __syncthreads();
@@ -121,7 +122,9 @@ __global__ __launch_bounds__(CARRY_W * CARRY_SEGS) void scan_carry_kernel(const 
 }
 int scan_carry(const ScanK& k, bool forward, hipStream_t s) {
     if (!k.once) return 0;
-    hipLaunchKernelGGL(scan_carry_kernel, dim3((unsigned)(((int64_t)k.a.cols * k.a.states + CARRY_W - 1) / CARRY_W)), dim3(CARRY_W * CARRY_SEGS), 0, s, k, forward);
+    const dim3 grid((unsigned)(((int64_t)k.a.cols * k.a.states + CARRY_W - 1) / CARRY_W));
+    if (k.items <= 128) hipLaunchKernelGGL(scan_carry_kernel<16>, grid, dim3(CARRY_W * 16), 0, s, k, forward);
+    else hipLaunchKernelGGL(scan_carry_kernel<64>, grid, dim3(CARRY_W * 64), 0, s, k, forward);
     VC_HIP(hipGetLastError());
     return 0;
 }
@@ -327,7 +330,7 @@ int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_wa
         k->chunk = (int)((k->slots + want - 1) / want);
         k->items = (k->slots + k->chunk - 1) / k->chunk;
         if (k->items == 1) { k->items = a->n_seqs; k->chunk = 0; }
-        k->once = k->items > (a->states == scan_padded(a->states) ? CARRY_ITEMS : CARRY_ITEMS / 2);
+        k->once = k->items > CARRY_ITEMS;
     }
     return 0;
 }
