@@ -219,9 +219,9 @@ int vc_adam_tf_update(float* p, float* m, float* v, const float* g, int64_t n,
  * Types (`type`, the activations of one call): VC_F32, VC_BF16, VC_F16.  Parameters, recurrent states, statistics, and parameter gradients
  * are fp32.  All sums are taken in fp32, in a fixed order: there are no atomics and two runs on the same inputs are bitwise equal.
  * Utterances: `offsets` (device, int32, n_seqs + 1 entries, rising) packs n_seqs utterances of any length, zero included, one behind the
- * other: utterance s is rows [offsets[s], offsets[s+1]).  NULL: n_seqs utterances of rows / n_seqs frames each.  Offsets are clamped into
+ * other: utterance s is rows [offsets[s], offsets[s+1]); the first may begin behind row 0.  NULL: n_seqs utterances of rows / n_seqs frames each.  Offsets are clamped into
  * [0, rows] on the device (they are not read back), so wrong ones give wrong numbers and no access outside the tensors.
- * Rows behind the last utterance are left as they were in every output, or cleared where `zero_tail` is set.
+ * Rows behind the last utterance and ahead of the first are left as they were in every output, or cleared where `zero_tail` is set.
  * Slots (`slots`, device, int32, one per row of a single-frame call): which entry of the state pool a row belongs to; NULL: row r has entry r.
  * A row whose slot lies outside [0, n_slots), or that an earlier row of the call has already named, is padding: y gets zeros, no state moves.  At most
  * 4096 rows a call with slots, 65535 without. */

@@ -921,3 +921,48 @@ def test_a_state_that_grows_through_very_many_runs(S):
     # the runs' sums, which end at 43
     assert ((got - want).abs() <= want * U * (4 * 300 + 200)).all()
     assert torch.allclose(final, y[0, -1, 0] / n, rtol=1e-6)
+
+
+@pytest.mark.parametrize('head', [5, 16, 100, 801])
+@pytest.mark.parametrize('lengths', [[40, 3], [0, 700, 20], [0, 0, 9], [400]])
+def test_utterances_that_begin_behind_row_zero(S, head, lengths):
+    """offsets cut out of a longer list: rows ahead of the first utterance belong to none, are not read, and give zeros"""
+    n, live, cols, taps = len(lengths), sum(lengths), 24, 4
+    rows = head + live + 4
+    v = scan_inputs(rows, cols, 16, 1, F32, n)
+    dy, df = rnd(20, rows, cols), rnd(21, n, cols, 16)
+    for t in [v[k] for k in ('x', 'dt', 'z', 'B', 'C')] + [dy]:
+        t[:head] = float('nan')
+        t[head + live:] = float('nan')
+    off = offsets_of(lengths) + head
+    w, init, dcf = rnd(2, taps, cols, scale=0.5), rnd(3, n, taps - 1, cols), rnd(4, n, taps - 1, cols)
+    mid = slice(head, head + live)
+    leaves = [v['x'].requires_grad_(True), w.requires_grad_(True), init.requires_grad_(True)]
+    y, final = S.causal_conv1d(*leaves[:2], initial_state=init, seq_offsets=off, return_final_state=True)
+    dx, dw, di = torch.autograd.grad((y, final), leaves, (dy, dcf))
+    r = O.conv1d(v['x'][mid].detach(), w, None, init, lengths, True, dy[mid], dcf)
+    m = O.conv1d(v['x'][mid].detach(), w, None, init, lengths, True, dy[mid], dcf, absolute=True)
+    close(y[mid], r['y'], m['p'], taps + 20, 'conv')
+    assert torch.equal(final.detach().double().cpu(), r['final'])
+    close(dx[mid], r['dx'], m['dx'], taps + 20, 'conv dx')
+    close(dw, r['dw'], m['dw'], taps + 20 + live, 'conv dw')
+    close(di, r['dinitial'], m['dinitial'], taps + 20, 'conv dinitial')
+    for t in (y, dx):
+        assert (t[:head] == 0).all() and (t[head + live:] == 0).all()
+    for hint in (None, max(lengths)):
+        leaves = [t.detach().requires_grad_(True) for t in v.values()]
+        u = dict(zip(v, leaves))
+        y, final = S.selective_scan(u['x'], u['dt'], u['A'], u['B'], u['C'], D=u['D'], z=u['z'], dt_bias=u['dt_bias'], initial_state=u['initial'], seq_offsets=off,
+                                    max_len=hint, return_final_state=True)
+        grads = dict(zip(v, torch.autograd.grad((y, final), leaves, (dy, df))))
+        cut = {k: t.detach()[mid] if k in ('x', 'dt', 'z', 'B', 'C') else t.detach() for k, t in v.items()}
+        r, m = O.scan(**cut, lengths=lengths, dy=dy[mid], dfinal=df), O.scan(**cut, lengths=lengths, dy=dy[mid], dfinal=df, absolute=True)
+        last = lasts(r, v['A'], max(lengths))
+        close(y[mid], r['y'], m['y'], 3 * last + 56, 'y')
+        close(final, r['final'], m['final'], 3 * last + 56, 'final')
+        for k, got in grads.items():
+            rowwise = k in ('x', 'dt', 'z', 'B', 'C')
+            close(got[mid] if rowwise else got, r['d' + k], m['d' + k], 6 * last + rows + cols + 76, 'd' + k)
+            if rowwise:
+                assert (got[:head] == 0).all() and (got[head + live:] == 0).all(), k
+        assert (y[:head] == 0).all() and (y[head + live:] == 0).all()

@@ -41,7 +41,8 @@ template <class T, int V> __device__ __forceinline__ void store_some(T* p, const
 struct SeqMap { const int* off; int rows, n_seqs, len; };
 __device__ __forceinline__ int seq_begin(const SeqMap& m, int s) { return m.off ? min(max(m.off[s], 0), m.rows) : s * m.len; }
 __device__ __forceinline__ int seq_end(const SeqMap& m, int s, int begin) { return m.off ? max(seq_begin(m, s + 1), begin) : begin + m.len; }
-// rows behind the last utterance start here
+// the utterances begin here (rows ahead of it belong to none), and rows behind the last one here
+__device__ __forceinline__ int seq_head(const SeqMap& m) { return m.off ? seq_begin(m, 0) : 0; }
 __device__ __forceinline__ int seq_tail(const SeqMap& m) { return m.off ? seq_begin(m, m.n_seqs) : m.rows; }
 
 // 1 / (1 + e^-x) through the reciprocal instruction (one unit in the last place; e^-x overflows to infinity, whose reciprocal is 0)

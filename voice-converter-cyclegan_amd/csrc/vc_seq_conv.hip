@@ -7,7 +7,7 @@
 
 struct ConvArgs { vc_conv1d_args a; SeqMap m; int v, cv, cvb, run, runs; float* part; };   // v channels a thread, cv such vectors, cvb of them next to each other; runs of `run` rows
 
-// the utterance row r lies in: the last s with begin(s) <= r; n_seqs where r lies behind the last utterance
+// the utterance row r >= seq_head lies in: the last s with begin(s) <= r; n_seqs where r lies behind the last utterance
 __device__ __forceinline__ int seq_of(const SeqMap& m, int r) {
     if (!m.off) return r / m.len;
     if (r >= seq_tail(m)) return m.n_seqs;
@@ -120,6 +120,10 @@ template <class T, int K, int V, bool SILU> __global__ __launch_bounds__(256) vo
     const int r1 = min(r + k.run, k.m.rows);
     const Span<T, V> X(a.x, a.x_ld, p.base, k.m.rows, a.cols), Y(a.y, a.y_ld, p.base, k.m.rows, a.cols);
     const unsigned ch = p.c * (unsigned)sizeof(T);
+    for (const int head = min(seq_head(k.m), r1); r < head; ++r) {           // rows ahead of the first utterance
+        const float f[V] = {};
+        if (a.zero_tail) Y.store((r - p.base) * Y.ld + ch, f);
+    }
     for (int s = seq_of(k.m, r); r < r1; ++s) {
         if (s >= k.m.n_seqs) {                                   // rows behind the last utterance
             const float f[V] = {};
@@ -191,6 +195,10 @@ template <class T, int K, int V, bool SILU> __global__ __launch_bounds__(256) vo
         const Span<T, V> X(a.x, a.x_ld, p.base, k.m.rows, a.cols), DY(a.dy, a.dy_ld, p.base, k.m.rows, a.cols),
             DX(want_dx ? a.dx : a.dy, want_dx ? a.dx_ld : a.dy_ld, p.base, k.m.rows, a.cols);
         const unsigned ch = p.c * (unsigned)sizeof(T);
+        for (const int head = min(seq_head(k.m), r1); r < head; ++r) {
+            const float f[V] = {};
+            if (a.zero_tail && want_dx) DX.store((r - p.base) * DX.ld + ch, f);
+        }
         for (int s = seq_of(k.m, r); r < r1; ++s) {
             if (s >= k.m.n_seqs) {
                 const float f[V] = {};

@@ -150,7 +150,8 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_fw
     const Lane<L, NS> w(k, k.waves, blk);
     const int c = w.c, j = w.j, n0 = w.n0, nn = w.nn;
     const Rows<T, L> Y(a.y, a.y_ld, a.cols, c, j, w.ok);
-    if (item == k.items) {                                       // rows behind the last utterance
+    if (item == k.items) {                                       // rows ahead of the first utterance and behind the last one
+        Y.clear(0, seq_head(k.m), c, j);
         Y.clear(seq_tail(k.m), k.m.rows, c, j);
         return;
     }
@@ -171,7 +172,8 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_fw
     for (int q = q0; q < q1;) {                                  // the utterances of the item
         const int64_t hs = ((int64_t)cur.s * a.cols + c) * a.states + n0;
         const int k0 = max(q - cur.base, 0), k1 = min(cur.tiles, q1 - cur.base);
-        if (q == cur.base) {
+        const bool begins = q <= cur.base && cur.base < q1;      // (ahead of the first utterance lie slots of none)
+        if (begins) {
 #pragma unroll
             for (int i = 0; i < NS; ++i) h[i] = 0.f;
             if (a.initial) load_state<NS>(a.initial + hs, h, nn, w.full);
@@ -229,7 +231,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_fw
             });
             wave_lds_fence();
         }
-        if (a.final_state && w.ok && (cur.tiles ? k0 < cur.tiles && k1 == cur.tiles : q == cur.base)) store_state<NS>(a.final_state + hs, h, nn, w.full);
+        if (a.final_state && w.ok && (cur.tiles ? k0 < cur.tiles && k1 == cur.tiles : begins)) store_state<NS>(a.final_state + hs, h, nn, w.full);
         if (cur.next >= q1) break;
         q = max(cur.next, q + 1);
         cur.load(cur.s + 1);

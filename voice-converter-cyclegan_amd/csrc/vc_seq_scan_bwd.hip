@@ -146,10 +146,11 @@ template <class T, int L, int NS, bool FULL> __global__ __launch_bounds__(64 * B
     const int c = w.c, j = w.j, n0 = w.n0, nn = w.nn;
     const bool has_z = a.z != nullptr;
     const Rows<T, L> DX(a.dx, a.dx_ld, a.cols, c, j, w.ok), DDT(a.ddt, a.ddt_ld, a.cols, c, j, w.ok), DZ(a.dz, a.dz_ld, a.cols, c, j, w.ok);
-    if (item == k.items) {                                       // rows behind the last utterance
-        const int tail = seq_tail(k.m);
+    if (item == k.items) {                                       // rows ahead of the first utterance and behind the last one
+        const int head = seq_head(k.m), tail = seq_tail(k.m);
+        DX.clear(0, head, c, j); DDT.clear(0, head, c, j);
         DX.clear(tail, k.m.rows, c, j); DDT.clear(tail, k.m.rows, c, j);
-        if (has_z) DZ.clear(tail, k.m.rows, c, j);
+        if (has_z) { DZ.clear(0, head, c, j); DZ.clear(tail, k.m.rows, c, j); }
         return;
     }
     const Rows<T, L> X(a.x, a.x_ld, a.cols, c, j), DT(a.dt, a.dt_ld, a.cols, c, j), DY(a.dy, a.dy_ld, a.cols, c, j), Z(has_z ? a.z : a.dy, has_z ? a.z_ld : a.dy_ld, a.cols, c, j);
@@ -294,7 +295,7 @@ template <class T, int L, int NS, bool FULL> __global__ __launch_bounds__(64 * B
         }
         turn ^= 1;
       }
-      if (cur.base >= q0 && a.dinitial && w.ok) store_state<NS>(a.dinitial + hs, dhc, nn, w.full);       // its beginning lies in this item
+      if (cur.base >= q0 && cur.base < q1 && a.dinitial && w.ok) store_state<NS>(a.dinitial + hs, dhc, nn, w.full);       // its beginning lies in this item
       if (cur.base <= q0 || cur.s == 0) break;
       q = min(cur.base, q) - 1;
       cur.load(cur.s - 1);
@@ -314,14 +315,14 @@ template <class T> __global__ __launch_bounds__(256) void scan_finish_kernel(con
     const vc_scan_args& a = k.a;
     if ((int)blockIdx.x < bc) {
         const int64_t w = (int64_t)2 * np * a.groups;
-        const int tail = seq_tail(k.m);
+        const int head = seq_head(k.m), tail = seq_tail(k.m);
         for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)k.m.rows * w; i += (int64_t)bc * 256) {
             const int64_t r = i / w;
             const int e = (int)(i - r * w), g = e / (2 * np), m = e % (2 * np), n = m % np;
             if (n >= a.states) continue;
             T* dst = m < np ? (T*)a.dB + r * a.db_ld : (T*)a.dC + r * a.dc_ld;
             dst += g * a.states + n;
-            if (r >= tail) { if (a.zero_tail) *dst = (T)0.f; continue; }
+            if (r < head || r >= tail) { if (a.zero_tail) *dst = (T)0.f; continue; }
             float s = 0.f;
 #pragma unroll 8
             for (int b = 0; b < k.nblk; ++b) s += k.part[((int64_t)(g * k.nblk + b) * k.m.rows + r) * (2 * np) + m];

@@ -8,7 +8,8 @@ operators look back only: a model of them trains on packed utterances and conver
     v = selective_scan(u, dt, A, B, C, D=D, z=z)      # all earlier frames, through a state of `states` numbers a channel
 
 Frames are rows: tensors are [batch, frames, channels], or [rows, channels] with `seq_offsets` (int32, [n + 1], rising, on the same device) where
-utterances of different lengths lie one behind the other; lengths of zero are fine, and rows behind the last utterance give zeros.  Any row
+utterances of different lengths lie one behind the other; lengths of zero are fine, and rows ahead of the first
+utterance or behind the last give zeros.  Any row
 stride is taken in place (column slices of a product, for one).  Activations are fp32, bf16 or fp16 (one type in a call); parameters, recurrent
 states and parameter gradients are fp32, and every sum is.  The kernels are those of include/vc_cyclegan.h; gradients are deterministic.
 
