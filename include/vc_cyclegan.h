@@ -216,6 +216,7 @@ int vc_adam_tf_update(float* p, float* m, float* v, const float* g, int64_t n,
  *
  * Layout: frame-major.  A tensor is rows x channels, channel stride 1, `*_ld` elements from row to row (a column slice of a wider product is
  * passed in place; 0 repeats one row).  Row strides, pointers and channel counts need no alignment beyond the element's own.
+ * Channels: up to 2^24 (the norm: 2^28).
  * Types (`type`, the activations of one call): VC_F32, VC_BF16, VC_F16.  Parameters, recurrent states, statistics, and parameter gradients
  * are fp32.  All sums are taken in fp32, in a fixed order: there are no atomics and two runs on the same inputs are bitwise equal.
  * Utterances: `offsets` (device, int32, n_seqs + 1 entries, rising) packs n_seqs utterances of any length, zero included, one behind the

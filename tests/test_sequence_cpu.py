@@ -238,3 +238,16 @@ def test_conv_refuses_strides_beyond_a_block(L):
 def test_binding_is_built_from_these_sources(L):
     from voice_converter_cyclegan_amd import sequence as S
     assert S._seq.build_id == L._bmod.binding_id()
+
+
+def test_more_channels_than_an_index_holds_are_refused(L):
+    """column indexes are 31 bits with room for what a thread steps over"""
+    for cols in ((1 << 28) + 1, (1 << 31) - 1):
+        assert L.lib.vc_rms_norm_fwd(ONE, cols, None, 0, ONE, ONE, cols, None, 0, None, 1e-6, 1, cols, 0, 0, NULL_STREAM) == -1
+        assert L.lib.vc_rms_norm_bwd_work(1, cols) == -1
+    for cols in ((1 << 24) + 1, (1 << 31) - 1):
+        assert L.lib.vc_causal_conv1d_fwd(C.byref(_conv(L, cols=cols)), NULL_STREAM) == -1
+        assert L.lib.vc_causal_conv1d_bwd_work(C.byref(_conv(L, cols=cols))) == -1
+        assert L.lib.vc_causal_conv1d_step(ONE, cols, ONE, None, ONE, None, ONE, cols, 1, 1, cols, 4, 0, 1, NULL_STREAM) == -1
+        assert L.lib.vc_selective_scan_fwd(C.byref(_scan(L, cols=cols)), NULL_STREAM) == -1
+        assert L.lib.vc_selective_scan_step(ONE, cols, ONE, cols, None, 0, ONE, 16, ONE, 16, ONE, None, None, ONE, None, ONE, cols, 1, 1, cols, 16, 1, 0, 1, NULL_STREAM) == -1

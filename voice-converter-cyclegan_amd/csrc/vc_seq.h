@@ -9,6 +9,8 @@
 // VC_ARG inside a function that returns the status itself
 #define SEQ_TYPES(type, F, ...) ((type) == VC_F32 ? F<float>(__VA_ARGS__) : (type) == VC_BF16 ? F<__bf16>(__VA_ARGS__) : F<_Float16>(__VA_ARGS__))
 static inline int seq_esize(int type) { return type == VC_F32 ? 4 : 2; }
+// Channels of a call: column indexes of the norm and of the convolution, and what they step over, then stay within 31 bits
+constexpr int64_t NORM_COLS = 1 << 28, SEQ_COLS = 1 << 24;
 static inline bool seq_type_ok(int type) { return type == VC_F32 || type == VC_BF16 || type == VC_F16; }
 
 // V elements in one access at any address the element type itself allows: gfx950 takes 16-byte global accesses at any alignment, so odd

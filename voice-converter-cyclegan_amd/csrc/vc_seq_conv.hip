@@ -352,7 +352,7 @@ static int check_conv1d(const char* who, const vc_conv1d_args* a, int v, int mos
     VC_ARG(a, "%s: null pointer", who);
     VC_ARG(seq_type_ok(a->type), "%s: type must be VC_F32, VC_BF16 or VC_F16", who);
     VC_ARG(a->taps >= 2 && a->taps <= 8, "%s: 2 to 8 taps, got %d", who, a->taps);
-    VC_ARG(a->rows >= 0 && a->rows + (int64_t)std::max(a->n_seqs, 0) < (1LL << 31) - (1 << 16) && a->cols > 0 && a->n_seqs > 0, "%s: bad sizes (rows %lld, cols %d, n_seqs %d)", who, (long long)a->rows, a->cols, a->n_seqs);
+    VC_ARG(a->rows >= 0 && a->rows + (int64_t)std::max(a->n_seqs, 0) < (1LL << 31) - (1 << 16) && a->cols > 0 && a->cols <= SEQ_COLS && a->n_seqs > 0, "%s: bad sizes (rows %lld, cols %d, n_seqs %d)", who, (long long)a->rows, a->cols, a->n_seqs);
     VC_ARG(a->offsets || a->rows % a->n_seqs == 0, "%s: without offsets the rows divide into n_seqs equal utterances", who);
     k->a = *a;
     k->m = SeqMap{a->offsets, (int)a->rows, a->n_seqs, (int)(a->rows / a->n_seqs)};
@@ -441,7 +441,7 @@ extern "C" int vc_causal_conv1d_step(const void* x, int64_t x_ld, void* state, c
                                      void* y, int64_t y_ld, int rows, int n_slots, int cols, int taps, int type, int silu, void* stream) {
     VC_ARG(seq_type_ok(type), "vc_causal_conv1d_step: type must be VC_F32, VC_BF16 or VC_F16");
     VC_ARG(taps >= 2 && taps <= 8, "vc_causal_conv1d_step: 2 to 8 taps, got %d", taps);
-    VC_ARG(rows >= 0 && rows <= 65535 && n_slots > 0 && cols > 0, "vc_causal_conv1d_step: bad sizes (rows %d, n_slots %d, cols %d)", rows, n_slots, cols);
+    VC_ARG(rows >= 0 && rows <= 65535 && n_slots > 0 && cols > 0 && cols <= SEQ_COLS, "vc_causal_conv1d_step: bad sizes (rows %d, n_slots %d, cols %d)", rows, n_slots, cols);
     VC_ARG(slots || rows <= n_slots, "vc_causal_conv1d_step: %d rows without slots, and %d slots", rows, n_slots);
     VC_ARG(!slots || rows <= MAX_SLOT_ROWS, "vc_causal_conv1d_step: at most %d rows with slots, got %d", MAX_SLOT_ROWS, rows);
     if (rows == 0) return 0;

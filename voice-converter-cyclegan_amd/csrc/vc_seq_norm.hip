@@ -446,7 +446,7 @@ template <class T> static int norm_bwd(const NormRowArgs& a, bool wide, int type
 }
 
 static int check_norm(const char* who, int64_t rows, int cols, int type, int sum_type) {
-    VC_ARG(rows >= 0 && rows < (1LL << 31) && cols > 0, "%s: bad sizes (rows %lld, cols %d)", who, (long long)rows, cols);
+    VC_ARG(rows >= 0 && rows < (1LL << 31) && cols > 0 && cols <= NORM_COLS, "%s: bad sizes (rows %lld, cols %d)", who, (long long)rows, cols);
     VC_ARG(seq_type_ok(type), "%s: type must be VC_F32, VC_BF16 or VC_F16", who);
     VC_ARG(sum_type == type || sum_type == VC_F32, "%s: the residual stream has the activations' type or fp32", who);
     return 0;

@@ -304,7 +304,7 @@ int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_wa
     VC_ARG(a->rows >= 0 && a->n_seqs > 0 && a->rows + (int64_t)TILE * a->n_seqs < (1LL << 31), "%s: bad sizes (rows %lld, n_seqs %d)", who, (long long)a->rows, a->n_seqs);
     VC_ARG(a->offsets || a->rows % a->n_seqs == 0, "%s: without offsets the rows divide into n_seqs equal utterances", who);
     for (int64_t ld : {a->x_ld, a->dt_ld, a->z ? a->z_ld : 0, a->b_ld, a->c_ld, a->y ? a->y_ld : 0, a->dy ? a->dy_ld : 0})
-        VC_ARG(ld >= 0 && ld <= MAX_LD && a->cols <= MAX_LD, "%s: row strides lie between 0 and 2^24 elements", who);
+        VC_ARG(ld >= 0 && ld <= MAX_LD && a->cols <= SEQ_COLS, "%s: row strides lie between 0 and 2^24 elements", who);
     if (a->rows > 1) {
         VC_ARG(!a->y || a->y_ld >= a->cols, "%s: rows of y overlap", who);
         VC_ARG(!a->dx || (a->dx_ld >= a->cols && a->dx_ld <= MAX_LD && a->ddt_ld >= a->cols && a->ddt_ld <= MAX_LD), "%s: row strides of dx and ddt lie between cols and 2^24", who);
@@ -389,7 +389,7 @@ extern "C" int vc_selective_scan_step(const void* x, int64_t x_ld, const void* d
                                       int rows, int n_slots, int cols, int states, int groups, int type, int softplus, void* stream) {
     VC_ARG(seq_type_ok(type), "vc_selective_scan_step: type must be VC_F32, VC_BF16 or VC_F16");
     VC_ARG(states >= 1 && states <= 64, "vc_selective_scan_step: 1 to 64 states, got %d", states);
-    VC_ARG(rows >= 0 && rows <= 65535 && n_slots > 0 && cols > 0 && groups > 0 && cols % groups == 0,
+    VC_ARG(rows >= 0 && rows <= 65535 && n_slots > 0 && cols > 0 && cols <= SEQ_COLS && groups > 0 && cols % groups == 0,
            "vc_selective_scan_step: bad sizes (rows %d, n_slots %d, cols %d, groups %d)", rows, n_slots, cols, groups);
     VC_ARG(slots || rows <= n_slots, "vc_selective_scan_step: %d rows without slots, and %d slots", rows, n_slots);
     VC_ARG(!slots || rows <= MAX_SLOT_ROWS, "vc_selective_scan_step: at most %d rows with slots, got %d", MAX_SLOT_ROWS, rows);

@@ -8,10 +8,10 @@ operators look back only: a model of them trains on packed utterances and conver
     v = selective_scan(u, dt, A, B, C, D=D, z=z)      # all earlier frames, through a state of `states` numbers a channel
 
 Frames are rows: tensors are [batch, frames, channels], or [rows, channels] with `seq_offsets` (int32, [n + 1], rising, on the same device) where
-utterances of different lengths lie one behind the other; lengths of zero are fine, and rows ahead of the first
-utterance or behind the last give zeros.  Any row
-stride is taken in place (column slices of a product, for one).  Activations are fp32, bf16 or fp16 (one type in a call); parameters, recurrent
-states and parameter gradients are fp32, and every sum is.  The kernels are those of include/vc_cyclegan.h; gradients are deterministic.
+utterances of different lengths lie one behind the other; lengths of zero are fine, and rows ahead of the first utterance
+or behind the last give zeros.  Any row stride is taken in place (column slices of a product, for one).  Activations are fp32, bf16 or fp16 (one type in
+a call); parameters, recurrent states and parameter gradients are fp32, and every sum is.  The kernels are those of include/vc_cyclegan.h; gradients are
+deterministic.
 
 A backward pass that is captured into a graph must not meet an eager autograd graph of the same leaves that is still alive: torch's gradient
 accumulators belong to the stream they were made on.  Drop the eager outputs first."""
@@ -66,7 +66,7 @@ def causal_conv1d_step(x, state, w, bias=None, slots=None, silu=True):
     """One frame of each of x's [streams, channels]: y, and `state` [pool, taps - 1, channels] moved on by a frame in place.
 
     slots (int32 [streams]): the stream's entry in the pool; without them stream i has entry i.  A stream whose slot lies outside the pool, or is
-    named by an earlier stream of the call, is padding: its y is zero and no state moves.  At most 4096 streams a call with slots."""
+    named by an earlier stream of the call, is padding: its y is zero and no state moves.  At most 4096 streams a call with slots, 65535 without."""
     return _seq.causal_conv1d_step(x, state, w, bias, slots, bool(silu))
 
 
