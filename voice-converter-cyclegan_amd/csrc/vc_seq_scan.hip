@@ -4,7 +4,7 @@
 constexpr int FWD_WAVES = 4;
 
 // First pass of a split axis: what each run hands on.  Only rows from the last utterance's beginning on matter.  Bound by vector issue: a product, an
-// exponential and two multiply-adds a state; 1 x 8192 x 1024 bf16, 16 states: 39 us, the main pass 63.
+// exponential and two multiply-adds a state; 1 x 8192 x 1024 bf16, 16 states: 39 us, the main pass 54.
 template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_edge_kernel(const ScanK k) {
     constexpr int NP = L * NS, NB = TILE / L;
     __shared__ float lds[FWD_WAVES][TILE * NP];
