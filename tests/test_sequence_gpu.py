@@ -966,3 +966,38 @@ def test_utterances_that_begin_behind_row_zero(S, head, lengths):
             if rowwise:
                 assert (got[:head] == 0).all() and (got[head + live:] == 0).all(), k
         assert (y[:head] == 0).all() and (y[head + live:] == 0).all()
+
+
+@pytest.mark.parametrize('kind,stream', [(BF16, F32), (F32, F32), (F16, F16)])
+def test_large_calls_equal_their_parts(S, kind, stream):
+    """outputs of more than 8 MiB are stored past the L2s: the same bits as in parts that are not, odd channel counts and tails included"""
+    rows, cols = 4300, 1001
+    x, res, gamma = rnd(1, rows, cols, dtype=kind), rnd(2, rows, cols, dtype=stream), 1 + rnd(3, cols, scale=0.1)
+    dy, ds = rnd(4, rows, cols, dtype=kind), rnd(5, rows, cols, dtype=stream)
+    parts = [slice(0, 1000), slice(1000, 2000), slice(2000, 3000), slice(3000, rows)]
+    assert rows * cols * x.element_size() >= 8 << 20 > 1300 * cols * x.element_size()
+
+    def norm(p):
+        a, b = x[p].detach().requires_grad_(True), res[p].detach().requires_grad_(True)
+        y, s = S.rms_norm(a, gamma, b)
+        return [y, s] + list(torch.autograd.grad((y, s), (a, b), (dy[p], ds[p]))) + list(S.rms_norm_e4m3(x[p], gamma, res[p]))
+    for i, (a, *b) in enumerate(zip(norm(slice(0, rows)), *[norm(p) for p in parts])):
+        assert torch.equal(a.float(), torch.cat(b).float()), i
+    w, lengths = rnd(6, 4, cols, scale=0.5), [1000, 1000, 1000, 1300]
+
+    def conv(p, lens):
+        a = x[p].detach().requires_grad_(True)
+        y = S.causal_conv1d(a, w, seq_offsets=offsets_of(lens))
+        return [y] + list(torch.autograd.grad(y, a, dy[p]))
+    for i, (a, *b) in enumerate(zip(conv(slice(0, rows), lengths), *[conv(p, [n]) for p, n in zip(parts, lengths)])):
+        assert torch.equal(a, torch.cat(b)), i
+    for states in (16, 13):
+        v = scan_inputs(900, 200, states, 1, kind, 1)
+        pool = rnd(7, 900, 200, states)
+        halves = pool.clone()
+        assert pool.numel() * 4 >= 8 << 20 > pool.numel() * 2
+
+        def step(p, state):
+            return S.selective_scan_step(v['x'][p], v['dt'][p], v['A'], v['B'][p], v['C'][p], state, D=v['D'], z=v['z'][p], dt_bias=v['dt_bias'])
+        y = step(slice(0, 900), pool)
+        assert torch.equal(y, torch.cat([step(slice(0, 450), halves[:450]), step(slice(450, 900), halves[450:])])) and torch.equal(pool, halves)

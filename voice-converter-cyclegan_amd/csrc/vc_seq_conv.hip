@@ -5,7 +5,7 @@
 // apart from the K - 1 frames ahead of a run.  Measured: 9001 x 1000 fp32 forward 16.3 us (4.4 TB/s of a copy's 5.0), 8192 x 2048 bf16 16 us.
 #include "vc_seq.h"
 
-struct ConvArgs { vc_conv1d_args a; SeqMap m; int v, cv, cvb, run, runs; float* part; };   // v channels a thread, cv such vectors, cvb of them next to each other; runs of `run` rows
+struct ConvArgs { vc_conv1d_args a; SeqMap m; int v, cv, cvb, run, runs; bool past; float* part; };   // v channels a thread, cv such vectors, cvb of them next to each other; runs of `run` rows
 
 // the utterance row r >= seq_head lies in: the last s with begin(s) <= r; n_seqs where r lies behind the last utterance
 __device__ __forceinline__ int seq_of(const SeqMap& m, int r) {
@@ -71,14 +71,16 @@ template <class T, int V> struct Span {
         const int64_t bytes = ((int64_t)(rows - base - 1) * stride + cols) * (int64_t)sizeof(T);
         rs = __builtin_amdgcn_make_buffer_rsrc((void*)((const T*)p + (int64_t)base * stride), 0, (int)min(bytes, (int64_t)0x7fffffff), 0x00020000);
     }
-    __device__ __forceinline__ void store(unsigned at, const float (&f)[V]) const {
+    // PAST: the L2s are not to keep it
+    template <bool PAST> __device__ __forceinline__ void store(unsigned at, const float (&f)[V]) const {
+        constexpr int POLICY = PAST ? 2 : 0;                     // non-temporal or not
         Pack<T, V> q;
 #pragma unroll
         for (int i = 0; i < V; ++i) q.v[i] = (T)f[i];
-        if constexpr (V * sizeof(T) == 16) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, q), rs, at, 0, 0);
-        else if constexpr (V * sizeof(T) == 8) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, q), rs, at, 0, 0);
-        else if constexpr (V * sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, q), rs, at, 0, 0);
-        else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, q), rs, at, 0, 0);
+        if constexpr (V * sizeof(T) == 16) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, q), rs, at, 0, POLICY);
+        else if constexpr (V * sizeof(T) == 8) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, q), rs, at, 0, POLICY);
+        else if constexpr (V * sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, q), rs, at, 0, POLICY);
+        else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, q), rs, at, 0, POLICY);
     }
 };
 // V elements as they came: 16-bit ones two to a register
@@ -99,7 +101,7 @@ template <class T, int V> struct Raw {
         }
     }
 };
-template <class T, int K, int V, bool SILU> __global__ __launch_bounds__(256) void conv1d_fwd_kernel(const ConvArgs k) {
+template <class T, int K, int V, bool SILU, bool PAST> __global__ __launch_bounds__(256) void conv1d_fwd_kernel(const ConvArgs k) {
     const vc_conv1d_args& a = k.a;
     const Place p = place(k, V);
     if (!p.ok) return;
@@ -122,12 +124,12 @@ template <class T, int K, int V, bool SILU> __global__ __launch_bounds__(256) vo
     const unsigned ch = p.c * (unsigned)sizeof(T);
     for (const int head = min(seq_head(k.m), r1); r < head; ++r) {           // rows ahead of the first utterance
         const float f[V] = {};
-        if (a.zero_tail) Y.store((r - p.base) * Y.ld + ch, f);
+        if (a.zero_tail) Y.template store<PAST>((r - p.base) * Y.ld + ch, f);
     }
     for (int s = seq_of(k.m, r); r < r1; ++s) {
         if (s >= k.m.n_seqs) {                                   // rows behind the last utterance
             const float f[V] = {};
-            if (a.zero_tail) for (; r < r1; ++r) Y.store((r - p.base) * Y.ld + ch, f);
+            if (a.zero_tail) for (; r < r1; ++r) Y.template store<PAST>((r - p.base) * Y.ld + ch, f);
             return;
         }
         const int b = seq_begin(k.m, s), hi = min(seq_end(k.m, s, b), r1);
@@ -158,7 +160,7 @@ template <class T, int K, int V, bool SILU> __global__ __launch_bounds__(256) vo
 #pragma unroll
                     for (int j = 0; j < K - 1; ++j) win[j][e] = win[j + 1][e];
                 }
-                Y.store(r + i < hi ? to + i * Y.ld : NOWHERE, o);
+                Y.template store<PAST>(r + i < hi ? to + i * Y.ld : NOWHERE, o);
             }
             to += AHEAD * Y.ld;
         }
@@ -182,7 +184,7 @@ template <bool SILU, int K, int V> __device__ __forceinline__ void pre_gradient(
 // frames that look at it go by.
 // 8192 x 2048 bf16: 26 us, 3.9 TB/s, the vector units busy 82 % of the time with the pre-activation and its sigmoid once more.
 // Four channels a thread: eight would fill the registers (filter, window, ring and its share of dw are K vectors each) and leave too few waves to wait with.
-template <class T, int K, int V, bool SILU> __global__ __launch_bounds__(256) void conv1d_bwd_kernel(const ConvArgs k) {
+template <class T, int K, int V, bool SILU, bool PAST> __global__ __launch_bounds__(256) void conv1d_bwd_kernel(const ConvArgs k) {
     __shared__ float red[256 * V];
     const vc_conv1d_args& a = k.a;
     const Place p = place(k, V);
@@ -197,12 +199,12 @@ template <class T, int K, int V, bool SILU> __global__ __launch_bounds__(256) vo
         const unsigned ch = p.c * (unsigned)sizeof(T);
         for (const int head = min(seq_head(k.m), r1); r < head; ++r) {
             const float f[V] = {};
-            if (a.zero_tail && want_dx) DX.store((r - p.base) * DX.ld + ch, f);
+            if (a.zero_tail && want_dx) DX.template store<PAST>((r - p.base) * DX.ld + ch, f);
         }
         for (int s = seq_of(k.m, r); r < r1; ++s) {
             if (s >= k.m.n_seqs) {
                 const float f[V] = {};
-                if (a.zero_tail && want_dx) for (; r < r1; ++r) DX.store((r - p.base) * DX.ld + ch, f);
+                if (a.zero_tail && want_dx) for (; r < r1; ++r) DX.template store<PAST>((r - p.base) * DX.ld + ch, f);
                 break;
             }
             const int b = seq_begin(k.m, s), end = seq_end(k.m, s, b), lo = r, hi = min(end, r1);
@@ -252,7 +254,7 @@ template <class T, int K, int V, bool SILU> __global__ __launch_bounds__(256) vo
 #pragma unroll
                         for (int e = 0; e < V; ++e) ring[0][e] += o[e];
                     }
-                    DX.store(want_dx && at >= lo && at < hi ? to + i * DX.ld : NOWHERE, ring[0]);
+                    DX.template store<PAST>(want_dx && at >= lo && at < hi ? to + i * DX.ld : NOWHERE, ring[0]);
 #pragma unroll
                     for (int e = 0; e < V; ++e)
 #pragma unroll
@@ -360,6 +362,7 @@ static int check_conv1d(const char* who, const vc_conv1d_args* a, int v, int mos
     k->cv = (a->cols + k->v - 1) / k->v;
     for (k->cvb = 1; k->cvb < k->cv && k->cvb < most;) k->cvb *= 2;
     k->part = nullptr;
+    k->past = a->rows * a->cols * seq_esize(a->type) >= STREAM_BYTES;
     return 0;
 }
 static void set_runs(ConvArgs& k, int longest) {
@@ -379,21 +382,23 @@ static int conv_grid(const char* who, const ConvArgs& k, bool seqs, unsigned* gr
 }
 template <class T, int K> static int fwd_k(const ConvArgs& k, unsigned grid, hipStream_t s) {
     constexpr int V = 16 / (int)sizeof(T);
-    if (k.v == 1) {
-        if (k.a.silu) hipLaunchKernelGGL((conv1d_fwd_kernel<T, K, 1, true>), dim3(grid), dim3(256), 0, s, k);
-        else hipLaunchKernelGGL((conv1d_fwd_kernel<T, K, 1, false>), dim3(grid), dim3(256), 0, s, k);
-    } else if (k.a.silu) hipLaunchKernelGGL((conv1d_fwd_kernel<T, K, V, true>), dim3(grid), dim3(256), 0, s, k);
-    else hipLaunchKernelGGL((conv1d_fwd_kernel<T, K, V, false>), dim3(grid), dim3(256), 0, s, k);
+#define F(V, SILU, PAST) hipLaunchKernelGGL((conv1d_fwd_kernel<T, K, V, SILU, PAST>), dim3(grid), dim3(256), 0, s, k)
+    if (k.v == 1) { if (k.a.silu) F(1, true, false); else F(1, false, false); }       // fewer channels than a vector
+    else if (k.past) { if (k.a.silu) F(V, true, true); else F(V, false, true); }
+    else if (k.a.silu) F(V, true, false);
+    else F(V, false, false);
+#undef F
     VC_HIP(hipGetLastError());
     return 0;
 }
 template <class T, int K> static int bwd_k(const ConvArgs& k, unsigned grid, hipStream_t s) {
     constexpr int V = BWD_V;
-    if (k.v == 1) {
-        if (k.a.silu) hipLaunchKernelGGL((conv1d_bwd_kernel<T, K, 1, true>), dim3(grid), dim3(256), 0, s, k);
-        else hipLaunchKernelGGL((conv1d_bwd_kernel<T, K, 1, false>), dim3(grid), dim3(256), 0, s, k);
-    } else if (k.a.silu) hipLaunchKernelGGL((conv1d_bwd_kernel<T, K, V, true>), dim3(grid), dim3(256), 0, s, k);
-    else hipLaunchKernelGGL((conv1d_bwd_kernel<T, K, V, false>), dim3(grid), dim3(256), 0, s, k);
+#define F(V, SILU, PAST) hipLaunchKernelGGL((conv1d_bwd_kernel<T, K, V, SILU, PAST>), dim3(grid), dim3(256), 0, s, k)
+    if (k.v == 1) { if (k.a.silu) F(1, true, false); else F(1, false, false); }       // fewer channels than a vector
+    else if (k.past) { if (k.a.silu) F(V, true, true); else F(V, false, true); }
+    else if (k.a.silu) F(V, true, false);
+    else F(V, false, false);
+#undef F
     VC_HIP(hipGetLastError());
     return 0;
 }

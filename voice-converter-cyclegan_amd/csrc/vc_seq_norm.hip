@@ -8,7 +8,7 @@ struct NormRowArgs {
     const void* x; const void* res; const float* gamma; void* y; void* sum; float* rstd; float* scale;
     const void* dy; const void* dsum; void* dx; void* dres; float* part;
     int64_t x_ld, res_ld, y_ld, sum_ld, dy_ld, dsum_ld, dx_ld, dres_ld;
-    float eps; int64_t rows; int cols, group;
+    float eps; int64_t rows; int cols, group; bool past;         // past: stores that go past the L2s
 };
 
 // sum / largest over the TPR threads of a row; every one gets it.  TPR = 64: a wave, no barrier; else the block
@@ -142,7 +142,7 @@ template <class T, class S, bool E4M3, int TPR, int ITEMS> __global__ __launch_b
                 const int c = (i * TPR + t) * V;
 #pragma unroll
                 for (int e = 0; e < V; ++e) f[i][e] = (float)(S)(f[i][e] + g[i][e]);
-                if (left[i] > 0) store_some<S, V>((S*)a.sum + r * a.sum_ld + c, f[i], left[i]);
+                if (left[i] > 0) store_out<S, V>((S*)a.sum + r * a.sum_ld + c, f[i], left[i], a.past);
             }
         }
         float ss = 0.f;
@@ -163,7 +163,7 @@ template <class T, class S, bool E4M3, int TPR, int ITEMS> __global__ __launch_b
         if constexpr (!E4M3) {
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i)
-                if (left[i] > 0) store_some<T, V>((T*)a.y + r * a.y_ld + (i * TPR + t) * V, f[i], left[i]);
+                if (left[i] > 0) store_out<T, V>((T*)a.y + r * a.y_ld + (i * TPR + t) * V, f[i], left[i], a.past);
         } else {
             Quant k[ITEMS];
             if (a.group == 0) {
@@ -308,8 +308,8 @@ template <class T, class S, int TPR, int ITEMS> __global__ __launch_bounds__(TPR
 #pragma unroll
             for (int e = 0; e < V; ++e) g[i][e] = fmaf(rstd, fmaf(-th[i][e], m, g[i][e]), ds[i][e]);
             if (left[i] <= 0) continue;
-            if (a.dx) store_some<T, V>((T*)a.dx + r * a.dx_ld + c, g[i], left[i]);
-            if (a.dres) store_some<S, V>((S*)a.dres + r * a.dres_ld + c, g[i], left[i]);
+            if (a.dx) store_out<T, V>((T*)a.dx + r * a.dx_ld + c, g[i], left[i], a.past);
+            if (a.dres) store_out<S, V>((S*)a.dres + r * a.dres_ld + c, g[i], left[i], a.past);
         }
     }
     if (!a.part) return;
@@ -458,6 +458,7 @@ static int norm_entry(const char* who, NormRowArgs& a, int type, int sum_type, b
     VC_ARG(a.eps > 0.f, "%s: eps must be positive", who);
     if (!a.res) sum_type = type;
     const bool wide = sum_type == VC_F32 && type != VC_F32;
+    a.past = a.rows * a.cols * seq_esize(type) >= STREAM_BYTES;
     return SEQ_TYPES(type, norm_fwd, a, wide, e4m3, (hipStream_t)stream);
 }
 extern "C" int vc_rms_norm_fwd(const void* x, int64_t x_ld, const void* residual, int64_t res_ld, const float* gamma,
@@ -495,6 +496,7 @@ extern "C" int vc_rms_norm_bwd(const void* dy, int64_t dy_ld, const void* dsum, 
     NormRowArgs a{};
     a.dy = dy; a.dy_ld = dy_ld; a.dsum = dsum; a.dsum_ld = dsum_ld; a.sum = (void*)sum; a.sum_ld = sum_ld; a.rstd = (float*)rstd; a.gamma = gamma;
     a.dx = dx; a.dx_ld = dx_ld; a.dres = dres; a.dres_ld = dres_ld; a.rows = rows; a.cols = cols; a.part = dgamma ? work : nullptr;
+    a.past = rows * cols * seq_esize(type) >= STREAM_BYTES;
     return SEQ_TYPES(type, norm_bwd, a, sum_type == VC_F32 && type != VC_F32, type, dgamma, (hipStream_t)stream);
 }
 

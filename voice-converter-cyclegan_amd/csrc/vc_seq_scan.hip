@@ -240,7 +240,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_fw
 
 struct ScanStepArgs {
     const void *x, *dt, *z, *B, *C; const float *A, *D, *dt_bias; float* state; const int* slots; void* y;
-    int64_t x_ld, dt_ld, z_ld, b_ld, c_ld, y_ld; int rows, n_slots, cols, states, groups, softplus;
+    int64_t x_ld, dt_ld, z_ld, b_ld, c_ld, y_ld; int rows, n_slots, cols, states, groups, softplus; bool past;
 };
 // Bound by the state's traffic: L lanes a channel as in the scan, STEP_U channels a lane group.  Everything is asked for before the earlier rows' slots are
 // looked through; a slot outside the pool reads entry 0 and drops it.  256 streams x 2048 bf16, 16 states: 16.7 us, 4.3 TB/s; one of 1024: 3.8 us.
@@ -281,7 +281,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_st
             sum = fmaf(C[u][e], h[u][e], sum);
         }
         float* hp = a.state + ((int64_t)mine * a.cols + c) * a.states + n0;
-        store_state<NS>(hp, h[u], nn, full);
+        store_out<float, NS>(hp, h[u], nn, a.past);
         sum = channel_sum<L>(sum) + D[u] * x[u];
         if (j == 0) *y = (T)(a.z ? sum * (z[u] * sigmoid_acc(z[u])) : sum);
     }
@@ -395,6 +395,6 @@ extern "C" int vc_selective_scan_step(const void* x, int64_t x_ld, const void* d
     VC_ARG(!slots || rows <= MAX_SLOT_ROWS, "vc_selective_scan_step: at most %d rows with slots, got %d", MAX_SLOT_ROWS, rows);
     if (rows == 0) return 0;
     VC_ARG(x && dt && B && C && A && state && y, "vc_selective_scan_step: null pointer");
-    const ScanStepArgs a{x, dt, z, B, C, A, D, dt_bias, state, slots, y, x_ld, dt_ld, z_ld, b_ld, c_ld, y_ld, rows, n_slots, cols, states, groups, softplus};
+    const ScanStepArgs a{x, dt, z, B, C, A, D, dt_bias, state, slots, y, x_ld, dt_ld, z_ld, b_ld, c_ld, y_ld, rows, n_slots, cols, states, groups, softplus, (int64_t)rows * cols * states * 4 >= STREAM_BYTES};
     return SEQ_TYPES(type, scan_step_t, a, (hipStream_t)stream);
 }
