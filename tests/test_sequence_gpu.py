@@ -968,6 +968,22 @@ def test_utterances_that_begin_behind_row_zero(S, head, lengths):
         assert (y[:head] == 0).all() and (y[head + live:] == 0).all()
 
 
+@pytest.mark.parametrize('kind,stream', [(BF16, BF16), (BF16, F32), (F32, F32)])
+def test_large_norms_equal_their_parts(S, kind, stream):
+    """inputs of more than 32 MiB are loaded past the L2s as well"""
+    rows, cols = 17000, 1024
+    x, res, gamma = rnd(1, rows, cols, dtype=kind), rnd(2, rows, cols, dtype=stream), 1 + rnd(3, cols, scale=0.1)
+    dy, ds = rnd(4, rows, cols, dtype=kind), rnd(5, rows, cols, dtype=stream)
+    parts = [slice(i, min(i + 2000, rows)) for i in range(0, rows, 2000)]
+
+    def norm(p):
+        a, b = x[p].detach().requires_grad_(True), res[p].detach().requires_grad_(True)
+        y, s = S.rms_norm(a, gamma, b)
+        return [y, s] + list(torch.autograd.grad((y, s), (a, b), (dy[p], ds[p]))) + list(S.rms_norm_e4m3(x[p], gamma, res[p], group=128))
+    for i, (a, *b) in enumerate(zip(norm(slice(0, rows)), *[norm(p) for p in parts])):
+        assert torch.equal(a.float(), torch.cat(b).float()), i
+
+
 @pytest.mark.parametrize('kind,stream', [(BF16, F32), (F32, F32), (F16, F16)])
 def test_large_calls_equal_their_parts(S, kind, stream):
     """outputs of more than 8 MiB are stored past the L2s: the same bits as in parts that are not, odd channel counts and tails included"""

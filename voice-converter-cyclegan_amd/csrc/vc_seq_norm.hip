@@ -8,7 +8,7 @@ struct NormRowArgs {
     const void* x; const void* res; const float* gamma; void* y; void* sum; float* rstd; float* scale;
     const void* dy; const void* dsum; void* dx; void* dres; float* part;
     int64_t x_ld, res_ld, y_ld, sum_ld, dy_ld, dsum_ld, dx_ld, dres_ld;
-    float eps; int64_t rows; int cols, group; bool past;         // past: stores that go past the L2s
+    float eps; int64_t rows; int cols, group; bool past, past_in;     // stores, loads that go past the L2s
 };
 
 // sum / largest over the TPR threads of a row; every one gets it.  TPR = 64: a wave, no barrier; else the block
@@ -126,7 +126,7 @@ template <class T, class S, bool E4M3, int TPR, int ITEMS> __global__ __launch_b
             const int c = (i * TPR + t) * V;
 #pragma unroll
             for (int e = 0; e < V; ++e) f[i][e] = 0.f;
-            if (left[i] > 0) load_some<T, V>((const T*)a.x + r * a.x_ld + c, f[i], left[i]);
+            if (left[i] > 0) load_in<T, V>((const T*)a.x + r * a.x_ld + c, f[i], left[i], a.past_in);
         }
         if (a.res) {
             float g[ITEMS][V];
@@ -135,7 +135,7 @@ template <class T, class S, bool E4M3, int TPR, int ITEMS> __global__ __launch_b
                 const int c = (i * TPR + t) * V;
 #pragma unroll
                 for (int e = 0; e < V; ++e) g[i][e] = 0.f;
-                if (left[i] > 0) load_some<S, V>((const S*)a.res + r * a.res_ld + c, g[i], left[i]);
+                if (left[i] > 0) load_in<S, V>((const S*)a.res + r * a.res_ld + c, g[i], left[i], a.past_in);
             }
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
@@ -284,9 +284,9 @@ template <class T, class S, int TPR, int ITEMS> __global__ __launch_bounds__(TPR
 #pragma unroll
             for (int e = 0; e < V; ++e) { th[i][e] = 0.f; g[i][e] = 0.f; ds[i][e] = 0.f; }
             if (left[i] > 0) {
-                load_some<S, V>((const S*)a.sum + r * a.sum_ld + c, th[i], left[i]);
-                load_some<T, V>((const T*)a.dy + r * a.dy_ld + c, g[i], left[i]);
-                if (a.dsum) load_some<S, V>((const S*)a.dsum + r * a.dsum_ld + c, ds[i], left[i]);
+                load_in<S, V>((const S*)a.sum + r * a.sum_ld + c, th[i], left[i], a.past_in);
+                load_in<T, V>((const T*)a.dy + r * a.dy_ld + c, g[i], left[i], a.past_in);
+                if (a.dsum) load_in<S, V>((const S*)a.dsum + r * a.dsum_ld + c, ds[i], left[i], a.past_in);
             }
         }
         const float rstd = a.rstd[r];
@@ -451,6 +451,12 @@ static int check_norm(const char* who, int64_t rows, int cols, int type, int sum
     VC_ARG(sum_type == type || sum_type == VC_F32, "%s: the residual stream has the activations' type or fp32", who);
     return 0;
 }
+static void set_past(NormRowArgs& a, int type) {
+    const int64_t e = seq_esize(type), bytes = a.rows * a.cols * e;
+    a.past = bytes >= STREAM_BYTES;
+    a.past_in = bytes >= LOAD_BYTES;
+    for (int64_t n : {(int64_t)a.cols, a.x_ld, a.res_ld, a.sum_ld, a.dy_ld, a.dsum_ld}) a.past_in = a.past_in && n * e % 128 == 0;     // no line shared by rows
+}
 static int norm_entry(const char* who, NormRowArgs& a, int type, int sum_type, bool e4m3, void* stream) {
     VC_CHECK(check_norm(who, a.rows, a.cols, type, sum_type));
     if (a.rows == 0) return 0;
@@ -458,7 +464,7 @@ static int norm_entry(const char* who, NormRowArgs& a, int type, int sum_type, b
     VC_ARG(a.eps > 0.f, "%s: eps must be positive", who);
     if (!a.res) sum_type = type;
     const bool wide = sum_type == VC_F32 && type != VC_F32;
-    a.past = a.rows * a.cols * seq_esize(type) >= STREAM_BYTES;
+    set_past(a, type);
     return SEQ_TYPES(type, norm_fwd, a, wide, e4m3, (hipStream_t)stream);
 }
 extern "C" int vc_rms_norm_fwd(const void* x, int64_t x_ld, const void* residual, int64_t res_ld, const float* gamma,
@@ -496,7 +502,7 @@ extern "C" int vc_rms_norm_bwd(const void* dy, int64_t dy_ld, const void* dsum, 
     NormRowArgs a{};
     a.dy = dy; a.dy_ld = dy_ld; a.dsum = dsum; a.dsum_ld = dsum_ld; a.sum = (void*)sum; a.sum_ld = sum_ld; a.rstd = (float*)rstd; a.gamma = gamma;
     a.dx = dx; a.dx_ld = dx_ld; a.dres = dres; a.dres_ld = dres_ld; a.rows = rows; a.cols = cols; a.part = dgamma ? work : nullptr;
-    a.past = rows * cols * seq_esize(type) >= STREAM_BYTES;
+    set_past(a, type);
     return SEQ_TYPES(type, norm_bwd, a, sum_type == VC_F32 && type != VC_F32, type, dgamma, (hipStream_t)stream);
 }
 
