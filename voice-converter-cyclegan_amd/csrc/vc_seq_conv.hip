@@ -2,7 +2,7 @@
 //   p[t] = bias + sum_k w[k] x[t - (K-1) + k];  y = p sigmoid(p) or p
 //   g = dy * (p sigmoid(p))';  dx[u] = sum_k w[k] g[u + (K-1) - k];  dw[k] = sum_t g[t] x[t - (K-1) + k];  dbias = sum_t g[t]
 // Bound by HBM.  A thread walks a run of rows for one 16-byte vector of channels with the last K frames in registers, so a row is fetched once,
-// apart from the K - 1 frames ahead of a run.  Measured: 9001 x 1000 fp32 forward 16.3 us (4.4 TB/s of a copy's 5.0), 8192 x 2048 bf16 16 us.
+// apart from the K - 1 frames ahead of a run.  Measured: 9001 x 1000 fp32 forward 17 us (4.3 TB/s of a copy's 5.0), 8192 x 2048 bf16 15.4 us, 4.4 TB/s.
 #include "vc_seq.h"
 
 struct ConvArgs { vc_conv1d_args a; SeqMap m; int v, cv, cvb, run, runs; bool past; float* part; };   // v channels a thread, cv such vectors, cvb of them next to each other; runs of `run` rows
@@ -38,7 +38,7 @@ template <class T, int K, int V> struct Filter {
 };
 // A block's threads: cvb vectors of channels (a power of two) next to each other, 256 / cvb runs of rows
 // Longest and shortest run of rows, and the waves below which a run is halved (a quarter of them once it has four rows).  Long runs repeat fewer frames ahead of them (the gradient: and behind
-// them, with their sigmoids), short ones leave enough threads.  Gradient of 8192 x 2048 bf16, 4 taps, with its forward pass: 45.7 us by runs of 32, 51.7
+// them, with their sigmoids), short ones leave enough threads.  (Before stores went past the L2s.)  Gradient of 8192 x 2048 bf16, 4 taps, with its forward pass: 45.7 us by runs of 32, 51.7
 // by 16, 55.8 by 64; of 1024 x 512: 14.4 by 4, 15.1 by 2, 15.6 by 8, 23.7 by 32; of 92 x 37 in 60 utterances: 24 by 2, 39 by 8.  Forward alone, 9001 x 1000 fp32: 17.2 by 8, 17.7 by 4 and by 16.
 constexpr int FWD_RUN = 8, BWD_RUN = 32, SHORT_RUN = 2, RUN_WAVES = 1024;
 // Rows worked on while as many are on their way: with two in the forward pass 18.0 us in place of 17.2, in the gradient 48.9 in place of 45.7.
@@ -182,7 +182,7 @@ template <bool SILU, int K, int V> __device__ __forceinline__ void pre_gradient(
 }
 // A run's dx needs the K - 1 frames' g behind it as well: they are worked out again there.  dx of a frame gathers in a register ring while the
 // frames that look at it go by.
-// 8192 x 2048 bf16: 26 us, 3.9 TB/s, the vector units busy 82 % of the time with the pre-activation and its sigmoid once more.
+// 8192 x 2048 bf16: 23 to 25 us, 4.2 TB/s, the vector units busy 82 % of the time with the pre-activation and its sigmoid once more.
 // Four channels a thread: eight would fill the registers (filter, window, ring and its share of dw are K vectors each) and leave too few waves to wait with.
 template <class T, int K, int V, bool SILU, bool PAST> __global__ __launch_bounds__(256) void conv1d_bwd_kernel(const ConvArgs k) {
     __shared__ float red[256 * V];

@@ -103,7 +103,7 @@ template <int V> __device__ __forceinline__ float rest_of(const float (&p)[V], c
 constexpr float NO_REST = -3.0e38f;
 
 // A row of up to TPR * ITEMS vectors in registers.  Threads walk the rows with a stride of the grid, so gamma is read once for all of them.
-// 16384 x 1024 bf16 with a residual: 32 us, 4.2 TB/s (a copy 5.0); 8832 x 2048 bf16 on an fp32 stream to 8 bits: 45 us, 4.4 TB/s; 1 x 512: 2.8 us.
+// 16384 x 1024 bf16 with a residual: 28 us, 4.8 TB/s (a copy 5.0); 8832 x 2048 bf16 on an fp32 stream to 8 bits: 38 us, 5.2 TB/s; 1 x 512: 2.9 us.
 template <class T, class S, bool E4M3, int TPR, int ITEMS> __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_fwd_kernel(const NormRowArgs a) {
     constexpr int V = 16 / (int)sizeof(T), RPB = TPR == 64 ? 4 : 1;
     __shared__ float red[TPR / 64 > 0 ? TPR / 64 : 1];
@@ -260,7 +260,7 @@ template <class T, class S, bool E4M3> __global__ __launch_bounds__(1024) void r
     }
 }
 
-// Gradient.  Every thread keeps its columns' share of dgamma over all rows it walks; a block leaves one row of `part`.  16384 x 1024 bf16: 31 us, 4.3 TB/s.
+// Gradient.  Every thread keeps its columns' share of dgamma over all rows it walks; a block leaves one row of `part`.  16384 x 1024 bf16: 30 us, 4.4 TB/s.
 template <class T, class S, int TPR, int ITEMS> __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_bwd_kernel(const NormRowArgs a) {
     constexpr int V = 16 / (int)sizeof(T), RPB = TPR == 64 ? 4 : 1;
     __shared__ float red[TPR / 64 > 0 ? TPR / 64 : 1];
@@ -392,7 +392,7 @@ int seq_sum_parts(const float* part, int parts, int64_t n, float* dst0, int64_t 
 }
 
 // How a row of nv vectors is held: by a wave with up to two vectors a thread, which needs no barrier; longer ones by a block of 256, then of 1024.
-// Rows of 2048 bf16 with 8-bit output (8832 of them): 58 us by a wave with four vectors a thread, whose registers leave four waves a SIMD, 53 by 128
+// (Before loads and stores went past the L2s.)  Rows of 2048 bf16 with 8-bit output (8832 of them): 58 us by a wave with four vectors a thread, whose registers leave four waves a SIMD, 53 by 128
 // threads, 45 by 256; rows of 1024: 32 us by a wave, 40 by 128 or 256 threads; 2535 rows of 4352 to 8 bits: 40 us by 256 threads, 36 by 512, 38 by 1024.
 #define NORM_LAYOUT(nv, F) \
     ((nv) <= 64 ? F(64, 1) : (nv) <= 128 ? F(64, 2) : (nv) <= 256 ? F(256, 1) : (nv) <= 512 ? F(256, 2) : (nv) <= 1024 ? F(512, 2) : F(1024, 2))

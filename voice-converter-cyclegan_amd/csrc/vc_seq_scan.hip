@@ -243,7 +243,7 @@ struct ScanStepArgs {
     int64_t x_ld, dt_ld, z_ld, b_ld, c_ld, y_ld; int rows, n_slots, cols, states, groups, softplus; bool past;
 };
 // Bound by the state's traffic: L lanes a channel as in the scan, STEP_U channels a lane group.  Everything is asked for before the earlier rows' slots are
-// looked through; a slot outside the pool reads entry 0 and drops it.  256 streams x 2048 bf16, 16 states: 16.7 us, 4.3 TB/s; one of 1024: 3.8 us.
+// looked through; a slot outside the pool reads entry 0 and drops it.  256 streams x 2048 bf16, 16 states: 16.3 us, 4.4 TB/s; one of 1024: 3.8 us.
 constexpr int STEP_U = 2;
 template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_step_kernel(const ScanStepArgs a) {
     constexpr int G = 256 / L;                                   // lane groups of a block
