@@ -1017,3 +1017,53 @@ def test_large_calls_equal_their_parts(S, kind, stream):
             return S.selective_scan_step(v['x'][p], v['dt'][p], v['A'], v['B'][p], v['C'][p], state, D=v['D'], z=v['z'][p], dt_bias=v['dt_bias'])
         y = step(slice(0, 900), pool)
         assert torch.equal(y, torch.cat([step(slice(0, 450), halves[:450]), step(slice(450, 900), halves[450:])])) and torch.equal(pool, halves)
+
+
+# ------------------------------------------------------------------------------------------- 8 bits: which side of a border
+
+def e4m3_of(v):
+    """64-bit v to the nearest e4m3 value, ties to even, as the numbers they stand for; and how far v lies from the next border, relative to v"""
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp_min(2.0 ** -6))) - 3)
+    n = v / step
+    return (torch.round(n) * step).clamp(-448, 448), ((n.abs() - torch.floor(n.abs()) - 0.5).abs() / n.abs().clamp_min(2.0 ** -60))
+
+
+@pytest.mark.parametrize('kind', [F32, BF16, F16])
+@pytest.mark.parametrize('cols,group', [(1024, 0), (1024, 32), (1024, 128), (2048, 64), (8192, 0), (33280, 0), (33280, 128)])
+def test_norm_e4m3_beside_a_border(S, kind, cols, group):
+    """Quotients 448 t gamma / max|t gamma| that lie within 2^-24 of a border between two e4m3 values, in registers and in long rows: every one has to go to
+    the side of it that the quotient in 64 bits lies on.  The kernel holds the quotient as a sum of two fp32 numbers: what it leaves out are products of two
+    rounding errors, at most 8 of 2^-48 = 2^-45 of the value, so only what lies within 2^-40 of its border (64-bit arithmetic rounds too, by 2^-52) may differ."""
+    g = torch.Generator().manual_seed(cols + group)
+    wide = group or cols
+    x = (1 + torch.rand(1, cols, generator=g)).to(kind)
+    x64 = x.double()[0]
+    top = x64.view(-1, wide)[:, :1].repeat_interleave(wide, 1).view(-1)                      # max|t gamma| of a group: its first column's, where gamma is 1
+    e, m = torch.randint(-8, 6, (cols,), generator=g).double(), torch.randint(0, 8, (cols,), generator=g).double()
+    border = torch.where(e == -8, (m + 0.5) * 2.0 ** -9, (8.5 + m) * torch.exp2(e) / 2)      # from half the least value to 248
+    gamma = (border / 448 * top / x64).float()
+    gamma.view(-1, wide)[:, 0] = 1.0
+    sign = torch.where(torch.rand(cols, generator=g) < 0.5, -1.0, 1.0)
+    q, scale = S.rms_norm_e4m3(x.to(DEV), (gamma * sign).to(DEV), group=group)
+    p = x64 * (gamma * sign).double()
+    v = p * 448 / p.view(-1, wide).abs().amax(-1, keepdim=True).repeat_interleave(wide, 1).view(-1)
+    want, far = e4m3_of(v)
+    assert (far < 2.0 ** -23).sum() > 0.9 * cols * (wide - 1) / wide
+    clear = far > 2.0 ** -40
+    assert clear.sum() > 0.9 * cols
+    wrong = (q[0].float().cpu().double() != want) & clear
+    assert not wrong.any(), '%d of %d on the wrong side' % (int(wrong.sum()), cols)
+
+
+@pytest.mark.parametrize('kind,stream,group', [(BF16, F32, 128), (F32, F32, 0), (F16, F16, 32)])
+def test_norm_e4m3_of_many_rows_is_the_nearest_value(S, kind, stream, group):
+    """17 million ordinary values: nearest in 64 bits, apart from those within 2^-40 of a border; a quotient in fp32 gets several wrong"""
+    rows, cols = 16384, 1024
+    x, res, gamma = rnd(1, rows, cols, dtype=kind), rnd(2, rows, cols, dtype=stream, scale=3.0), 1 + rnd(3, cols, scale=0.1)
+    q, scale, total = S.rms_norm_e4m3(x, gamma, res, group=group)
+    p = total.double() * gamma.double()
+    v = (p.view(rows, -1, group or cols) * 448 / p.view(rows, -1, group or cols).abs().amax(-1, keepdim=True)).view(rows, cols)
+    want, far = e4m3_of(v)
+    clear = far > 2.0 ** -40
+    assert clear.float().mean() > 0.999
+    assert int(((q.float().double() != want) & clear).sum()) == 0
