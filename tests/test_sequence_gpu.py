@@ -1067,3 +1067,22 @@ def test_norm_e4m3_of_many_rows_is_the_nearest_value(S, kind, stream, group):
     clear = far > 2.0 ** -40
     assert clear.float().mean() > 0.999
     assert int(((q.float().double() != want) & clear).sum()) == 0
+
+
+@pytest.mark.parametrize('cols', [256, 33280])
+def test_norm_e4m3_of_tiny_rows(S, cols):
+    """Groups under the least scale (max|y| below 2^-100) that are not zero, and products t gamma so small that 448 over the largest leaves fp32 while the norm
+    itself is above the least scale (a tiny eps): the values and scales of the definition.  rstd is off by cols / 64 + 8 roundings (a sum of squares of a
+    thread's columns, steps across lanes and waves, a root and a quotient), and two products follow."""
+    u = rnd(1, 2, cols)
+    k = cols / 64 + 12
+    for size, eps in ((1e-30, 1e-6), (3e-34, 1e-6), (3e-37, 1e-14), (1e-39, 1e-18)):
+        x, gamma = u * size, torch.ones(cols, device=DEV)
+        q, scale = S.rms_norm_e4m3(x, gamma, eps=eps, group=128)
+        y = O.rms_norm(x, gamma, eps).view(2, -1, 128)
+        want = y.abs().amax(-1).clamp_min(2.0 ** -100) / 448
+        close(scale, want, want, k, 'scale %g %g' % (size, eps))
+        v = q.float().double().cpu().view(2, -1, 128)
+        assert torch.isfinite(v).all(), (size, eps)
+        ideal = y / want[..., None]
+        assert ((v - ideal).abs() <= ideal.abs() * (2.0 ** -4 + k * U) + 2.0 ** -10 + k * U).all(), (size, eps, float((v - ideal).abs().max()))

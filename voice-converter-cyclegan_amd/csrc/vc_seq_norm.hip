@@ -86,9 +86,11 @@ struct Quant { float first, factor, correction, scale; };
 __device__ __forceinline__ Quant quant_of(unsigned bits, float rest, float rstd) {
     const float top = __uint_as_float(bits), y = top * rstd;
     Quant q;
-    if (y >= LEAST_TOP) {
-        q.first = 1.f; q.factor = E4M3_TOP / top; q.scale = y / E4M3_TOP;
-        q.correction = (fmaf(-q.factor, top, E4M3_TOP) - q.factor * rest) / E4M3_TOP;
+    if (y >= LEAST_TOP) {                                        // (448 / top would leave fp32 below 2^-119: products that small take 2^100 first)
+        q.first = top < 0x1p-100f ? 0x1p100f : 1.f;
+        const float t = top * q.first;
+        q.factor = E4M3_TOP / t; q.scale = y / E4M3_TOP;
+        q.correction = (fmaf(-q.factor, t, E4M3_TOP) - q.factor * (rest * q.first)) / E4M3_TOP;
     } else { q.first = rstd; q.factor = E4M3_TOP / LEAST_TOP; q.correction = 0.f; q.scale = y != y ? y : LEAST_TOP / E4M3_TOP; }
     return q;
 }
