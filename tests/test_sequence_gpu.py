@@ -1086,3 +1086,26 @@ def test_norm_e4m3_of_tiny_rows(S, cols):
         assert torch.isfinite(v).all(), (size, eps)
         ideal = y / want[..., None]
         assert ((v - ideal).abs() <= ideal.abs() * (2.0 ** -4 + k * U) + 2.0 ** -10 + k * U).all(), (size, eps, float((v - ideal).abs().max()))
+
+
+@pytest.mark.parametrize('kind', [F32, BF16, F16])
+@pytest.mark.parametrize('rows', [20, 1500])
+def test_scan_from_an_infinite_state(S, kind, rows):
+    """an infinite state wears off by no factor above zero: infinite with its sign to the end, frame by frame and over runs whose whole factor leaves fp32; the
+    gradient that an infinite one of the final state leaves behind is infinite back to the first frame"""
+    cols, states = 12, 8
+    v = scan_inputs(rows, cols, states, 1, kind, 1)
+    v['C'], v['z'] = v['C'].abs() + 0.5, v['z'].abs() + 0.5
+    sign = torch.tensor([1.0, -1.0, 1.0], device=DEV).repeat(4)
+    sick = torch.tensor([True, True, False], device=DEV).repeat(4)
+    v['initial'][:, sick] = float('inf') * sign[sick, None]
+    call = lambda u: S.selective_scan(u['x'], u['dt'], u['A'], u['B'], u['C'], D=u['D'], z=u['z'], dt_bias=u['dt_bias'], initial_state=u['initial'],  # noqa: E731
+                                      seq_offsets=offsets_of([rows]), return_final_state=True)
+    y, final = call(v)
+    assert (y[:, sick] == float('inf') * sign[sick]).all() and (final[:, sick] == float('inf') * sign[sick, None]).all()
+    assert torch.isfinite(y[:, ~sick]).all() and torch.isfinite(final[:, ~sick]).all()
+    v['initial'] = torch.zeros_like(v['initial']).requires_grad_(True)
+    df = torch.zeros(1, cols, states, device=DEV)
+    df[:, sick] = float('inf') * sign[sick, None]
+    d, = torch.autograd.grad(call(v)[1], v['initial'], df)
+    assert torch.equal(d, df)

@@ -217,9 +217,10 @@ void scan_edge_place(ScanK* k, float* work);
 // 102 us by the waves, 100 by scan_carry; 1 x 512 x 1024 (33) 17 and 18; 8 x 128 x 1024 training (up to 32) 70 and 74.
 constexpr int CARRY_ITEMS = 32;
 // exp2(p) h + e, or e where nothing is handed on.  In two halves: the factor of a whole run may leave the range of fp32 where its product with h does not
-// (frame by frame it would not either), and a state of zero stays one under any factor.
+// (frame by frame it would not either), and a state of zero stays one under any factor.  A factor that is only too small for fp32 is 2^-252 in place of 0, which
+// leaves nothing of a finite state and an infinite one as it is (0 would make it no number).
 __device__ __forceinline__ float carried(float p, float h, float e, int cut) {
-    const float f = exp2_fast(0.5f * p);
+    const float f = fmaxf(exp2_fast(0.5f * p), p >= -3.4e38f ? 0x1p-126f : 0.f);             // (where p is no number, e is none)
     return cut || h == 0.f ? e : fmaf(f * h, f, e);
 }
 int scan_carry(const ScanK& k, bool forward, hipStream_t s);
