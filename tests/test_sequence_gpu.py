@@ -1109,3 +1109,125 @@ def test_scan_from_an_infinite_state(S, kind, rows):
     df[:, sick] = float('inf') * sign[sick, None]
     d, = torch.autograd.grad(call(v)[1], v['initial'], df)
     assert torch.equal(d, df)
+
+
+# ------------------------------------------------------------------------------------------------- steps of zero and beyond
+
+def masked_scan(kind, lengths, cols, states, fill, seed=1):
+    """scan_inputs with frames whose dt is `fill`: the first two of every utterance, a stretch in it, the last one, and all of the second utterance"""
+    rows = sum(lengths)
+    v = scan_inputs(rows, cols, states, 1, kind, len(lengths), seed)
+    mask = torch.zeros(rows, dtype=torch.bool)
+    at = 0
+    for i, m in enumerate(lengths):
+        mask[at:at + 2] = True
+        mask[at + m // 3:at + m // 2] = True
+        mask[at + m - 1:at + m] = True
+        if i == 1:
+            mask[at:at + m] = True
+        at += m
+    v['dt'][mask.to(DEV)] = fill
+    return v, mask
+
+
+def least_of(kind):
+    return [float('-inf'), torch.finfo(kind).min]
+
+
+@pytest.mark.parametrize('kind', [F32, BF16, F16])
+@pytest.mark.parametrize('which', [0, 1])
+@pytest.mark.parametrize('lengths,hint', [([23, 18, 40], 40), ([700, 20, 900], None), ([2000], None)])
+def test_scan_of_masked_frames(S, kind, which, lengths, hint):
+    """dt = -inf or the type's lowest value is a step of zero (softplus is 0 in 64 bits, and in fp32): the state stays as it is, y = C h + D x, dt has no
+    gradient there, and nothing else of the utterance notices; walked and in runs"""
+    cols, states = 24, 16
+    v, mask = masked_scan(kind, lengths, cols, states, least_of(kind)[which])
+    rows = sum(lengths)
+    dy, df = rnd(20, rows, cols, dtype=kind), rnd(21, len(lengths), cols, states)
+    leaves = [t.requires_grad_(True) for t in v.values()]
+    y, final = S.selective_scan(v['x'], v['dt'], v['A'], v['B'], v['C'], D=v['D'], z=v['z'], dt_bias=v['dt_bias'], initial_state=v['initial'],
+                                seq_offsets=offsets_of(lengths), max_len=hint, return_final_state=True)
+    r = O.scan(**v, lengths=lengths, dy=dy, dfinal=df)
+    m = O.scan(**v, lengths=lengths, dy=dy, dfinal=df, absolute=True)
+    assert all(torch.isfinite(t).all() for t in r.values())
+    steps = r['delta'][~mask]                                     # masked frames carry a term by a factor of exactly 1: they do not wear it
+    last = min(max(lengths), 17 / float(steps.min() * v['A'].detach().abs().min()))
+    close(y, r['y'], m['y'], 3 * last + states + 40, 'y')
+    close(final, r['final'], m['final'], 3 * last + states + 40, 'final')
+    if len(lengths) > 1:
+        assert torch.equal(final[1], v['initial'][1])
+    grads = dict(zip(v, torch.autograd.grad((y, final), leaves, (dy, df))))
+    assert (grads['dt'][mask.to(DEV)] == 0).all()
+    for name, got in grads.items():
+        over = rows if name in ('A', 'D', 'dt_bias') else cols if name in ('B', 'C') else 0
+        close(got, r['d' + name], m['d' + name], 6 * last + over + states + 60, 'd' + name)
+
+
+@pytest.mark.parametrize('kind', [F32, BF16, F16])
+@pytest.mark.parametrize('which', [0, 1])
+def test_single_frames_of_masked_streams(S, kind, which):
+    """a masked frame of a live stream leaves its state as it is"""
+    v = scan_inputs(6, 40, 16, 1, kind, 6)
+    v['dt'][1::2] = least_of(kind)[which]
+    pool = v['initial'].clone()
+    y = S.selective_scan_step(v['x'], v['dt'], v['A'], v['B'][:, 0], v['C'][:, 0], pool, D=v['D'], z=v['z'], dt_bias=v['dt_bias'])
+    r, m = O.scan(**v, lengths=[1] * 6), O.scan(**v, lengths=[1] * 6, absolute=True)
+    close(y, r['y'], m['y'], 59, 'y')
+    close(pool, r['final'], m['final'], 59, 'state')
+    assert torch.equal(pool[1::2], v['initial'][1::2])
+
+
+@pytest.mark.parametrize('kind', [F32, BF16, F16])
+@pytest.mark.parametrize('rows', [40, 1500])
+def test_scan_of_the_largest_steps(S, kind, rows):
+    """dt = the type's largest value: softplus is dt itself, the state forgets everything and takes delta x B.  x is small there (2^-30, in fp16 2^-8) and dy
+    (2^-20), so that neither h nor a gradient leaves its type; what is 1e29 large wears off over the frames behind, and so do the bounds"""
+    cols, states, big = 24, 4, torch.finfo(kind).max
+    v = scan_inputs(rows, cols, states, 1, kind, 1)
+    at = [5, rows // 2]
+    v['dt'][at] = big
+    v['x'][at] *= 2.0 ** (-8 if kind == F16 else -30)
+    v['C'] *= 2.0 ** -8                                           # y within fp16
+    v['z'] = v['z'].clamp(-2, 2)
+    dy = (rnd(20, rows, cols) * 2.0 ** -20).to(kind) if kind != F16 else rnd(20, rows, cols, dtype=kind) * 2.0 ** -10
+    leaves = [t.requires_grad_(True) for t in v.values()]
+    y, final = S.selective_scan(v['x'], v['dt'], v['A'], v['B'], v['C'], D=v['D'], z=v['z'], dt_bias=v['dt_bias'], initial_state=v['initial'],
+                                seq_offsets=offsets_of([rows]), return_final_state=True)
+    r, m = O.scan(**v, lengths=[rows], dy=dy), O.scan(**v, lengths=[rows], dy=dy, absolute=True)
+    assert all(torch.isfinite(t.to(kind)).all() for k, t in r.items() if k in ('y', 'dx', 'ddt', 'dz', 'dB', 'dC')), 'inputs out of range'
+    last = lasts(r, v['A'], rows)
+    close(y, r['y'], m['y'], 3 * last + states + 40, 'y')
+    close(final, r['final'], m['final'], 3 * last + states + 40, 'final')
+    for name, got in zip(v, torch.autograd.grad(y, leaves, dy)):
+        over = rows if name in ('A', 'D', 'dt_bias') else cols if name in ('B', 'C') else 0
+        close(got, r['d' + name], m['d' + name], 6 * last + over + states + 60, 'd' + name)
+    pool = v['initial'].detach().repeat(2, 1, 1)
+    w = {k: t.detach()[at] if k in ('x', 'dt', 'z', 'B', 'C') else t.detach() for k, t in v.items()}
+    y = S.selective_scan_step(w['x'], w['dt'], w['A'], w['B'][:, 0], w['C'][:, 0], pool, D=w['D'], z=w['z'], dt_bias=w['dt_bias'])
+    w['initial'] = v['initial'].detach().repeat(2, 1, 1)
+    r, m = O.scan(**w, lengths=[1, 1]), O.scan(**w, lengths=[1, 1], absolute=True)
+    close(y, r['y'], m['y'], 59, 'step')
+    close(pool, r['final'], m['final'], 59, 'state')
+
+
+@pytest.mark.parametrize('kind', [F32, BF16, F16])
+@pytest.mark.parametrize('rows', [9, 1500])
+def test_scan_of_infinite_and_undefined_steps(S, kind, rows):
+    """dt = inf: softplus is infinite, and so are a channel's states from there on, with the sign of x B; dt = NaN is NaN from there on.  One sign a channel"""
+    cols, states = 12, 8
+    v = scan_inputs(rows, cols, states, 1, kind, 1)
+    v['x'] = (v['x'].abs() + 0.5) * torch.tensor([1.0, -1.0, -1.0], device=DEV, dtype=kind).repeat(4)
+    v['B'], v['C'], v['z'] = v['B'].abs() + 0.5, v['C'].abs() + 0.5, v['z'].abs() + 0.5
+    v['dt'][4, 1::2] = float('inf')
+    v['dt'][4, 2::4] = float('nan')
+    r = O.scan(**v, lengths=[rows])
+    assert torch.isinf(r['y'][4:, 1::2]).all() and torch.isnan(r['y'][4:, 2::4]).all() and torch.isfinite(r['y'][:, ::4]).all()
+    y, final = S.selective_scan(v['x'], v['dt'], v['A'], v['B'], v['C'], D=v['D'], z=v['z'], dt_bias=v['dt_bias'], initial_state=v['initial'],
+                                seq_offsets=offsets_of([rows]), return_final_state=True)
+    pool = v['initial'].clone()
+    one = torch.stack([S.selective_scan_step(v['x'][i:i + 1], v['dt'][i:i + 1], v['A'], v['B'][i:i + 1, 0], v['C'][i:i + 1, 0], pool, D=v['D'], z=v['z'][i:i + 1],
+                                             dt_bias=v['dt_bias'])[0] for i in range(rows)])
+    for got, ref in ((y, r['y']), (one, r['y']), (final, r['final']), (pool, r['final'])):
+        got = got.cpu().double()
+        assert torch.equal(torch.isnan(got), torch.isnan(ref))
+        assert torch.equal(torch.where(torch.isinf(got), got.sign(), torch.zeros_like(got)), torch.where(torch.isinf(ref), ref.sign(), torch.zeros_like(ref)))

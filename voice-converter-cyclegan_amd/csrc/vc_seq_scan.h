@@ -106,19 +106,22 @@ template <int L> __device__ __forceinline__ float channel_sum(float v) {
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-// softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|) in (0, 1], and its slope.  log(1 + e) = 2 atanh(e / (2 + e)) by its series: the argument is at
-// most 1/3, seven terms leave 1.4e-8, and a small e keeps all its bits (a logarithm of the rounded 1 + e would lose them: steps of 0.001 are ordinary here)
+// softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|) in [0, 1], and its slope.  log(1 + e) = 2 atanh(e / (2 + e)) by its series: the argument is at
+// most 1/3, seven terms leave 1.4e-8, and a small e keeps all its bits (a logarithm of the rounded 1 + e would lose them: steps of 0.001 are ordinary here).
+// dt masked by -inf or its type's lowest value is a step of exactly 0 with a slope of 0, the largest value or inf is a step of itself, a NaN stays one.
 __device__ __forceinline__ float softplus(float v, float& slope) {
-    // e^-|v| with what the product with log2 e rounds off put back: the exponential alone would be off by |v| 2^-24 of itself
-    const float av = fabsf(v), t = -av * LOG2E, lo = fmaf(-av, LOG2E, -t) - av * LOG2E_REST;
+    // e^-|v| with what the product with log2 e rounds off put back: the exponential alone would be off by |v| 2^-24 of itself.  |v| counts up to 128, where
+    // e is 0 in fp32: beyond 2^127 the product would leave fp32 and what it rounds off be no number
+    const float av = fminf(fabsf(v), 128.f), t = -av * LOG2E, lo = fmaf(-av, LOG2E, -t) - av * LOG2E_REST;
     float e = exp2_fast(t);
     e = fmaf(e, lo * LN2, e);
     const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
     float p = 1.f / 13.f;
     p = fmaf(p, q, 1.f / 11.f); p = fmaf(p, q, 1.f / 9.f); p = fmaf(p, q, 1.f / 7.f); p = fmaf(p, q, 1.f / 5.f); p = fmaf(p, q, 1.f / 3.f); p = fmaf(p, q, 1.f);
     const float r = __builtin_amdgcn_rcpf(1.f + e);
-    slope = v >= 0.f ? r : e * r;
-    return fmaxf(v, 0.f) + 2.f * s * p + (v - v);                // v - v: a NaN stays one (fmaxf drops it)
+    const bool below = v < 0.f;                                  // (of a NaN not: it goes on into the sum)
+    slope = below ? e * r : r;
+    return fmaf(2.f * s, p, below ? 0.f : v);
 }
 
 // A tensor of rows as a lane uses it: through a buffer descriptor of the tile's rows, whose bounds check gives zeros for the rows that a short tile
