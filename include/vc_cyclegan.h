@@ -215,7 +215,8 @@ int vc_adam_tf_update(float* p, float* m, float* v, const float* g, int64_t n,
  * recordings.  These operators look back only, so a model built of them trains on packed utterances and runs on a live stream frame by frame.
  *
  * Layout: frame-major.  A tensor is rows x channels, channel stride 1, `*_ld` elements from row to row (a column slice of a wider product is
- * passed in place; 0 repeats one row).  Row strides, pointers and channel counts need no alignment beyond the element's own.
+ * passed in place; 0 repeats one row).  Row strides, pointers and channel counts need no alignment beyond the element's own.  Rows of an output may not
+ * overlap: its stride is at least its width (any value where there is one row).
  * Channels: up to 2^24 (the norm: 2^28).
  * Types (`type`, the activations of one call): VC_F32, VC_BF16, VC_F16.  Parameters, recurrent states, statistics, and parameter gradients
  * are fp32.  All sums are taken in fp32, in a fixed order: there are no atomics and two runs on the same inputs are bitwise equal.
@@ -235,7 +236,7 @@ int vc_seq_version(void);              /* revision of this section: 1 */
  *   t = x + residual, rounded to sum_type and stored in `sum`;   rstd = 1 / sqrt(mean(t^2) + eps);   y = t * rstd * gamma
  * The norm reads t as it is stored, so the backward pass needs `sum` and rstd alone.  residual NULL: t = x (sum is not written and may be
  * NULL, sum_type == type).  rstd [rows] may be NULL.  eps > 0: a row of zeros gives zeros.  sum_type: type or VC_F32.
- * x, y, residual, sum: y may be x, sum may be residual. */
+ * x, y, residual, sum: y may be x, sum may be residual, with the same row stride. */
 int vc_rms_norm_fwd(const void* x, int64_t x_ld, const void* residual, int64_t res_ld, const float* gamma,
                     void* y, int64_t y_ld, void* sum, int64_t sum_ld, float* rstd, float eps,
                     int64_t rows, int cols, int type, int sum_type, void* stream);
@@ -257,7 +258,7 @@ int vc_rms_norm_bwd(const void* dy, int64_t dy_ld, const void* dsum, int64_t dsu
  *   p[t][c] = bias[c] + sum_k w[k][c] x[t - (taps-1) + k][c];   y = p * sigmoid(p) (silu != 0) or p
  * w [taps][cols], 2 <= taps <= 8; bias may be NULL.  Frames before an utterance come from initial [n_seqs][taps-1][cols] (type; oldest first;
  * NULL: zeros).  final [n_seqs][taps-1][cols] (may be NULL) receives the last taps-1 frames, what the next call of a stream takes as initial;
- * final may not be initial.  Row strides: up to 2^15 elements, 2^20 from 256 channels on (a block's rows
+ * final may not be initial, nor y be x, dx be x or dy, dinitial be initial or dfinal.  Row strides: up to 2^15 elements, 2^20 from 256 channels on (a block's rows
  * lie within 2^31 bytes). */
 typedef struct {
     const void* x; const float* w; const float* bias; const void* initial; const int32_t* offsets;
@@ -282,7 +283,7 @@ int vc_causal_conv1d_step(const void* x, int64_t x_ld, void* state, const int32_
  *   y[t][c] = (sum_n C[t][g][n] h[t][c][n] + D[c] x[t][c]) * z[t][c] sigmoid(z[t][c])
  * with g = c / (cols / groups): the channels of a group share B and C.  A [cols][states] fp32, finite, 1 <= states <= 64.  D, z, dt_bias may be NULL
  * (no skip, no gate, no bias).  B, C: row stride b_ld / c_ld, group g at + g * states.  initial [n_seqs][cols][states] fp32 (NULL: zeros);
- * final_state likewise (NULL: not wanted); final_state may not be initial.  Row strides: at most 2^24 elements, those of outputs at least their row. */
+ * final_state likewise (NULL: not wanted); final_state may not be initial, nor dinitial be dfinal.  Row strides: at most 2^24 elements, those of outputs at least their row. */
 typedef struct {
     const void *x, *dt, *z, *B, *C; const float *A, *D, *dt_bias; const float* initial; const int32_t* offsets;
     void* y; float* final_state;

@@ -251,3 +251,46 @@ def test_more_channels_than_an_index_holds_are_refused(L):
         assert L.lib.vc_causal_conv1d_step(ONE, cols, ONE, None, ONE, None, ONE, cols, 1, 1, cols, 4, 0, 1, NULL_STREAM) == -1
         assert L.lib.vc_selective_scan_fwd(C.byref(_scan(L, cols=cols)), NULL_STREAM) == -1
         assert L.lib.vc_selective_scan_step(ONE, cols, ONE, cols, None, 0, ONE, 16, ONE, 16, ONE, None, None, ONE, None, ONE, cols, 1, 1, cols, 16, 1, 0, 1, NULL_STREAM) == -1
+
+
+def test_output_rows_that_overlap_are_refused(L):
+    """rows of an output closer than their width would be written by several threads in no order; one row has no stride"""
+    f, q, b = L.lib.vc_rms_norm_fwd, L.lib.vc_rms_norm_e4m3, L.lib.vc_rms_norm_bwd
+
+    def fwd(x_ld=8, res_ld=8, y_ld=8, sum_ld=8, y=ONE, rows=4):
+        return f(C.c_void_p(1 << 20), x_ld, C.c_void_p(1 << 21), res_ld, ONE, y, y_ld, C.c_void_p(1 << 22), sum_ld, None, 1e-6, rows, 8, 0, 0, NULL_STREAM)
+    for bad in (dict(x_ld=-8), dict(res_ld=-1), dict(y_ld=7), dict(y_ld=0), dict(y_ld=-8), dict(sum_ld=7), dict(y=C.c_void_p(1 << 20), x_ld=9)):
+        assert fwd(**bad) == -1 and b'row stride' in L.lib.vc_last_error(), bad
+    assert q(ONE, 96, None, 0, ONE, ONE, 95, ONE, None, 0, 1e-6, 4, 96, 32, 0, 0, NULL_STREAM) == -1 and b'row stride' in L.lib.vc_last_error()
+    args = [ONE, 8, ONE, 8, ONE, 8, ONE, ONE, ONE, 8, ONE, 8, None, None, 0, 4, 8, 0, 0, NULL_STREAM]
+    for i, v in ((1, -8), (3, -8), (5, -8), (9, 7), (9, -8), (11, 7), (11, 0)):
+        bad = list(args)
+        bad[i] = v
+        assert b(*bad) == -1 and b'row stride' in L.lib.vc_last_error(), (i, v)
+    f, b = L.lib.vc_causal_conv1d_fwd, L.lib.vc_causal_conv1d_bwd
+    for v in (0, 7):
+        assert f(C.byref(_conv(L, y_ld=v)), NULL_STREAM) == -1 and b'row stride' in L.lib.vc_last_error()
+        assert b(C.byref(_conv(L, dy=8192, dx=16384, dx_ld=v, dy_ld=8)), NULL_STREAM) == -1 and b'row stride' in L.lib.vc_last_error()
+    s = L.lib.vc_causal_conv1d_step
+    args = [ONE, 8, ONE, None, ONE, None, ONE, 8, 2, 4, 8, 4, 0, 1, NULL_STREAM]
+    for i, v in ((1, -8), (7, 7), (7, 0), (7, -8)):
+        bad = list(args)
+        bad[i] = v
+        assert s(*bad) == -1 and b'row stride' in L.lib.vc_last_error(), (i, v)
+    s = L.lib.vc_selective_scan_step
+    args = [ONE, 8, ONE, 8, ONE, 8, ONE, 16, ONE, 16, ONE, None, None, ONE, None, ONE, 8, 2, 4, 8, 16, 1, 0, 1, NULL_STREAM]
+    for i, v in ((1, -8), (3, -8), (5, -8), (7, -1), (9, -1), (16, 7), (16, 0)):
+        bad = list(args)
+        bad[i] = v
+        assert s(*bad) == -1 and b'row stride' in L.lib.vc_last_error(), (i, v)
+
+
+def test_convolution_in_place_is_refused(L):
+    """a run of rows looks at frames that another one writes to: its output may not be its input, nor a gradient what it is taken from"""
+    f, b = L.lib.vc_causal_conv1d_fwd, L.lib.vc_causal_conv1d_bwd
+    assert f(C.byref(_conv(L, y=4096)), NULL_STREAM) == -1 and b'in place' in L.lib.vc_last_error()
+    full = dict(dy=8192, dx=16384, dx_ld=8, dy_ld=8, initial=1 << 20, dfinal=1 << 21, dinitial=1 << 22)
+    for bad in (dict(dx=4096), dict(dx=8192), dict(dinitial=1 << 20), dict(dinitial=1 << 21)):
+        assert b(C.byref(_conv(L, **{**full, **bad})), NULL_STREAM) == -1 and b'in place' in L.lib.vc_last_error(), bad
+    a = dict(dy=4096, dx=4096, ddt=4096, dB=4096, dC=4096, dA=4096, saved=4096, saved_floats=1 << 20, work=4096, work_floats=1 << 20, dy_ld=8, dx_ld=8, ddt_ld=8, db_ld=16, dc_ld=16)
+    assert L.lib.vc_selective_scan_bwd(C.byref(_scan(L, dinitial=1 << 20, dfinal=1 << 20, **a)), NULL_STREAM) == -1 and b'in place' in L.lib.vc_last_error()

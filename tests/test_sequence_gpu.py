@@ -1231,3 +1231,32 @@ def test_scan_of_infinite_and_undefined_steps(S, kind, rows):
         got = got.cpu().double()
         assert torch.equal(torch.isnan(got), torch.isnan(ref))
         assert torch.equal(torch.where(torch.isinf(got), got.sign(), torch.zeros_like(got)), torch.where(torch.isinf(ref), ref.sign(), torch.zeros_like(ref)))
+
+
+def test_one_row_of_any_stride(S):
+    """a call of a single row takes no stride from its arguments: 0 (or any other) means the same as its width, in outputs too"""
+    from voice_converter_cyclegan_amd import _lib
+    import ctypes as C
+    cols, states = 24, 16
+    v = scan_inputs(1, cols, states, 1, F32, 1)
+    dy = rnd(20, 1, cols)
+    leaves = [v[k].requires_grad_(True) for k in ('x', 'dt', 'A', 'B', 'C', 'z')]
+    y0 = S.selective_scan(v['x'][None], v['dt'][None], v['A'], v['B'][None], v['C'][None], z=v['z'][None])
+    want = torch.autograd.grad(y0, leaves, dy[None])
+    for ld in (0, 5, cols, 1 << 28):
+        out = {k: torch.full((cols, states) if k == 'dA' else (1, states) if k in ('dB', 'dC') else (1, cols), 7.0, device=DEV) for k in ('y', 'dx', 'ddt', 'dz', 'dA', 'dB', 'dC')}
+        a = _lib.ScanArgs(x=v['x'].data_ptr(), dt=v['dt'].data_ptr(), z=v['z'].data_ptr(), B=v['B'].data_ptr(), C=v['C'].data_ptr(), A=v['A'].data_ptr(), dy=dy.data_ptr(),
+                          x_ld=cols, dt_ld=cols, z_ld=cols, b_ld=states, c_ld=states, dy_ld=cols, y_ld=ld, dx_ld=ld, ddt_ld=ld, dz_ld=ld, db_ld=ld, dc_ld=ld,
+                          rows=1, cols=cols, states=states, groups=1, n_seqs=1, type=0, softplus=1, **{k: t.data_ptr() for k, t in out.items()})
+        a.saved_floats = _lib.lib.vc_selective_scan_saved(C.byref(a))
+        assert a.saved_floats > 0, _lib.lib.vc_last_error()
+        a.work_floats = max(_lib.lib.vc_selective_scan_fwd_work(C.byref(a)), _lib.lib.vc_selective_scan_bwd_work(C.byref(a)))
+        saved, work = torch.empty(a.saved_floats, device=DEV), torch.empty(a.work_floats, device=DEV)
+        a.saved, a.work = saved.data_ptr(), work.data_ptr()
+        stream = torch.cuda.current_stream().cuda_stream
+        _lib.check(_lib.lib.vc_selective_scan_fwd(C.byref(a), stream))
+        _lib.check(_lib.lib.vc_selective_scan_bwd(C.byref(a), stream))
+        torch.cuda.synchronize()
+        assert torch.equal(out['y'], y0[0].detach()), ld
+        for k, w in zip(('dx', 'ddt', 'dA', 'dB', 'dC', 'dz'), want):
+            assert torch.equal(out[k].view(w.shape), w), (k, ld)

@@ -369,7 +369,7 @@ static void set_runs(ConvArgs& k, int longest) {
     for (k.run = longest; k.run > SHORT_RUN && (int64_t)k.m.rows * k.cv < (int64_t)k.run * 64 * (k.run > 4 ? RUN_WAVES : RUN_WAVES / 4);) k.run /= 2;
     k.runs = (k.m.rows + k.run - 1) / k.run;
 }
-static int conv_grid(const char* who, const ConvArgs& k, bool seqs, unsigned* grid) {
+static int conv_grid(const char* who, const ConvArgs& k, bool seqs, int64_t out_ld, unsigned* grid) {
     const int per = 256 / k.cvb;
     const int64_t g = (int64_t)((k.cv + k.cvb - 1) / k.cvb) * (((int64_t)k.runs + (seqs ? k.m.n_seqs : 0) + per - 1) / per);
     VC_ARG(g < (1LL << 31), "%s: too many rows and channels for one launch", who);
@@ -377,6 +377,7 @@ static int conv_grid(const char* who, const ConvArgs& k, bool seqs, unsigned* gr
     const int64_t span = std::min((int64_t)per * k.run, (int64_t)k.m.rows) + 16;
     for (int64_t ld : {k.a.x_ld, k.a.y ? k.a.y_ld : 0, k.a.dy ? k.a.dy_ld : 0, k.a.dx ? k.a.dx_ld : 0})
         VC_ARG(ld >= 0 && (span * ld + k.a.cols) * seq_esize(k.a.type) < (1LL << 31), "%s: a row stride of %lld elements is out of range", who, (long long)ld);
+    VC_ARG(k.m.rows <= 1 || out_ld >= k.a.cols, "%s: a row stride of %lld elements: rows of an output of %d channels overlap", who, (long long)out_ld, k.a.cols);
     *grid = (unsigned)g;
     return 0;
 }
@@ -419,7 +420,8 @@ extern "C" int vc_causal_conv1d_fwd(const vc_conv1d_args* a, void* stream) {
     VC_ARG(!a->final_state || a->final_state != a->initial, "vc_causal_conv1d_fwd: final_state may not be initial");
     if (a->rows == 0 && !a->final_state) return 0;
     set_runs(k, FWD_RUN);
-    unsigned grid; VC_CHECK(conv_grid("vc_causal_conv1d_fwd", k, a->final_state != nullptr, &grid));
+    unsigned grid; VC_CHECK(conv_grid("vc_causal_conv1d_fwd", k, a->final_state != nullptr, a->y_ld, &grid));
+    VC_ARG(a->rows == 0 || a->y != a->x, "vc_causal_conv1d_fwd: not in place: a run of rows looks at frames that another one writes");
     return SEQ_TYPES(a->type, conv1d_fwd, k, grid, (hipStream_t)stream);
 }
 // rows of `part`: one for each block's runs
@@ -437,7 +439,9 @@ extern "C" int vc_causal_conv1d_bwd(const vc_conv1d_args* a, void* stream) {
     const int64_t need = (int64_t)conv_parts(k) * (a->taps + 1) * a->cols;
     if (params && need && (!a->work || a->work_floats < need)) { vc_set_error("vc_causal_conv1d_bwd: work is too small (%lld floats needed)", (long long)need); return VC_E_NOMEM; }
     if (params) k.part = a->work;
-    unsigned grid; VC_CHECK(conv_grid("vc_causal_conv1d_bwd", k, a->dinitial != nullptr, &grid));
+    unsigned grid; VC_CHECK(conv_grid("vc_causal_conv1d_bwd", k, a->dinitial != nullptr, a->dx ? a->dx_ld : a->cols, &grid));
+    VC_ARG((!a->dx || a->rows == 0 || (a->dx != a->x && a->dx != a->dy)) && (!a->dinitial || (a->dinitial != a->initial && a->dinitial != a->dfinal)),
+           "vc_causal_conv1d_bwd: not in place: a run of rows looks at frames that another one writes");
     if (grid) VC_CHECK(SEQ_TYPES(a->type, conv1d_bwd, k, grid, (hipStream_t)stream));
     // no rows: no parts, and the sums are zeros
     return params ? seq_sum_parts(k.part, conv_parts(k), (int64_t)(a->taps + 1) * a->cols, a->dw, (int64_t)a->taps * a->cols, a->dbias, (hipStream_t)stream) : 0;
@@ -451,6 +455,7 @@ extern "C" int vc_causal_conv1d_step(const void* x, int64_t x_ld, void* state, c
     VC_ARG(!slots || rows <= MAX_SLOT_ROWS, "vc_causal_conv1d_step: at most %d rows with slots, got %d", MAX_SLOT_ROWS, rows);
     if (rows == 0) return 0;
     VC_ARG(x && state && w && y, "vc_causal_conv1d_step: null pointer");
+    VC_ARG(rows == 1 || (x_ld >= 0 && y_ld >= cols), "vc_causal_conv1d_step: a row stride is out of range, or rows of y overlap");
     const ConvStepArgs a{x, state, slots, w, bias, y, x_ld, y_ld, rows, n_slots, cols, taps, silu};
     return SEQ_TYPES(type, conv1d_step, a, (hipStream_t)stream);
 }

@@ -457,6 +457,13 @@ static int check_norm(const char* who, int64_t rows, int cols, int type, int sum
     VC_ARG(sum_type == type || sum_type == VC_F32, "%s: the residual stream has the activations' type or fp32", who);
     return 0;
 }
+// rows of an output closer than their width would be written by several threads in no order; a single row has no stride
+static int check_ld(const char* who, const NormRowArgs& a, std::initializer_list<int64_t> in, std::initializer_list<int64_t> out) {
+    if (a.rows <= 1) return 0;
+    for (int64_t ld : in) VC_ARG(ld >= 0, "%s: a row stride of %lld elements is out of range", who, (long long)ld);
+    for (int64_t ld : out) VC_ARG(ld >= a.cols, "%s: a row stride of %lld elements: rows of an output of %d columns overlap", who, (long long)ld, a.cols);
+    return 0;
+}
 static void set_past(NormRowArgs& a, int type) {
     const int64_t e = seq_esize(type), bytes = a.rows * a.cols * e;
     a.past = bytes >= STREAM_BYTES;
@@ -468,6 +475,9 @@ static int norm_entry(const char* who, NormRowArgs& a, int type, int sum_type, b
     if (a.rows == 0) return 0;
     VC_ARG(a.x && a.gamma && a.y && (!a.res || a.sum), "%s: null pointer", who);
     VC_ARG(a.eps > 0.f, "%s: eps must be positive", who);
+    VC_CHECK(check_ld(who, a, {a.x_ld, a.res ? a.res_ld : 0}, {a.y_ld, a.res ? a.sum_ld : a.cols}));
+    VC_ARG(a.rows <= 1 || ((a.y != a.x || a.y_ld == a.x_ld) && (!a.res || a.sum != a.res || a.sum_ld == a.res_ld)), "%s: in place, but with another row stride", who);
+    VC_ARG(!e4m3 || a.y != a.x, "%s: q may not be x", who);
     if (!a.res) sum_type = type;
     const bool wide = sum_type == VC_F32 && type != VC_F32;
     set_past(a, type);
@@ -508,6 +518,7 @@ extern "C" int vc_rms_norm_bwd(const void* dy, int64_t dy_ld, const void* dsum, 
     NormRowArgs a{};
     a.dy = dy; a.dy_ld = dy_ld; a.dsum = dsum; a.dsum_ld = dsum_ld; a.sum = (void*)sum; a.sum_ld = sum_ld; a.rstd = (float*)rstd; a.gamma = gamma;
     a.dx = dx; a.dx_ld = dx_ld; a.dres = dres; a.dres_ld = dres_ld; a.rows = rows; a.cols = cols; a.part = dgamma ? work : nullptr;
+    VC_CHECK(check_ld("vc_rms_norm_bwd", a, {dy_ld, dsum ? dsum_ld : 0, sum_ld}, {dx ? dx_ld : cols, dres ? dres_ld : cols}));
     set_past(a, type);
     return SEQ_TYPES(type, norm_bwd, a, sum_type == VC_F32 && type != VC_F32, type, dgamma, (hipStream_t)stream);
 }

@@ -303,7 +303,7 @@ int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_wa
     VC_ARG(a->cols > 0 && a->groups > 0 && a->cols % a->groups == 0, "%s: groups (%d) must divide cols (%d)", who, a->groups, a->cols);
     VC_ARG(a->rows >= 0 && a->n_seqs > 0 && a->rows + (int64_t)TILE * a->n_seqs < (1LL << 31), "%s: bad sizes (rows %lld, n_seqs %d)", who, (long long)a->rows, a->n_seqs);
     VC_ARG(a->offsets || a->rows % a->n_seqs == 0, "%s: without offsets the rows divide into n_seqs equal utterances", who);
-    for (int64_t ld : {a->x_ld, a->dt_ld, a->z ? a->z_ld : 0, a->b_ld, a->c_ld, a->y ? a->y_ld : 0, a->dy ? a->dy_ld : 0})
+    for (int64_t ld : {a->x_ld, a->dt_ld, a->z ? a->z_ld : 0, a->b_ld, a->c_ld, a->y && a->rows > 1 ? a->y_ld : 0, a->dy ? a->dy_ld : 0})
         VC_ARG(ld >= 0 && ld <= MAX_LD && a->cols <= SEQ_COLS, "%s: row strides lie between 0 and 2^24 elements", who);
     if (a->rows > 1) {
         VC_ARG(!a->y || a->y_ld >= a->cols, "%s: rows of y overlap", who);
@@ -313,6 +313,8 @@ int scan_setup(const char* who, const vc_scan_args* a, int waves, int64_t run_wa
     }
     *k = ScanK{};
     k->a = *a;
+    // one row has no stride: the rows that its tile lacks are to lie behind it all the same, so that what is stored to them is dropped
+    if (a->rows == 1) k->a.y_ld = k->a.dx_ld = k->a.ddt_ld = k->a.dz_ld = a->cols;
     k->m = SeqMap{a->offsets, (int)a->rows, a->n_seqs, (int)(a->rows / a->n_seqs)};
     k->cg = a->cols / a->groups;
     k->slots = (int)(a->rows / TILE) + a->n_seqs;
@@ -395,6 +397,7 @@ extern "C" int vc_selective_scan_step(const void* x, int64_t x_ld, const void* d
     VC_ARG(!slots || rows <= MAX_SLOT_ROWS, "vc_selective_scan_step: at most %d rows with slots, got %d", MAX_SLOT_ROWS, rows);
     if (rows == 0) return 0;
     VC_ARG(x && dt && B && C && A && state && y, "vc_selective_scan_step: null pointer");
+    VC_ARG(rows == 1 || (x_ld >= 0 && dt_ld >= 0 && (!z || z_ld >= 0) && b_ld >= 0 && c_ld >= 0 && y_ld >= cols), "vc_selective_scan_step: a row stride is out of range, or rows of y overlap");
     const ScanStepArgs a{x, dt, z, B, C, A, D, dt_bias, state, slots, y, x_ld, dt_ld, z_ld, b_ld, c_ld, y_ld, rows, n_slots, cols, states, groups, softplus, (int64_t)rows * cols * states * 4 >= STREAM_BYTES};
     return SEQ_TYPES(type, scan_step_t, a, (hipStream_t)stream);
 }

@@ -399,6 +399,7 @@ extern "C" int vc_selective_scan_bwd(const vc_scan_args* a, void* stream) {
     VC_CHECK(bwd_setup("vc_selective_scan_bwd", a, &k, &need));
     VC_ARG(a->A && a->dA && (a->rows == 0 || (a->x && a->dt && a->B && a->C && a->dy && a->dx && a->ddt && a->dB && a->dC && a->saved)), "vc_selective_scan_bwd: null pointer");
     VC_ARG(!a->z || a->dz || a->rows == 0, "vc_selective_scan_bwd: z has a gradient, dz is null");
+    VC_ARG(!a->dinitial || a->dinitial != a->dfinal, "vc_selective_scan_bwd: dinitial may not be dfinal: not in place, an utterance's beginning and end may lie in two runs");
     if (!a->z) k.a.dz = nullptr;
     if (a->saved_floats < vc_selective_scan_saved(a) && a->rows) { vc_set_error("vc_selective_scan_bwd: saved is too small"); return VC_E_NOMEM; }
     if (a->work_floats < need || !a->work) { vc_set_error("vc_selective_scan_bwd: work is too small (%lld floats needed)", (long long)need); return VC_E_NOMEM; }
