@@ -1260,3 +1260,51 @@ def test_one_row_of_any_stride(S):
         assert torch.equal(out['y'], y0[0].detach()), ld
         for k, w in zip(('dx', 'ddt', 'dA', 'dB', 'dC', 'dz'), want):
             assert torch.equal(out[k].view(w.shape), w), (k, ld)
+
+
+# -------------------------------------------------------------------------------------------------- far out on the sigmoid
+
+def test_gates_and_activations_of_large_magnitude(S):
+    """p sigmoid(p) and its slope relative to themselves, in fp32 and far to both sides (rounding the exponential's argument alone would cost |p| 2^-24).
+    Roundings of 2^-24: the exponential 2 (one unit in the last place) and its correction 1, 1 + e 1, the reciprocal 2, e times it 1, p times it 1 = 8; slope
+    s (1 + p (1 - s)), relative to s (1 + |p|): s 7, 1 - s 2, the multiply-add and the product 1 each = 11; the scan multiplies once more."""
+    n = 512
+    p = torch.cat([-torch.linspace(2.0, 80.0, n), torch.linspace(2.0, 80.0, n)]) + 0.3 * torch.rand(2 * n, generator=torch.Generator().manual_seed(1))
+    p = p.to(DEV)
+    s64 = 1 / (1 + torch.exp(-p.cpu().double()))
+    y64, d64 = O.silu(p.cpu().double()), O.dsilu(p.cpu().double())
+    dmag = s64 * (1 + p.cpu().double().abs())
+    w = torch.tensor([0.0, 1.0], device=DEV)[:, None].repeat(1, 2 * n)
+    x = p[None, None].clone().requires_grad_(True)
+    y = S.causal_conv1d(x, w)
+    close(y[0, 0], y64, y64.abs(), 8, 'convolution')
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    close(dx[0, 0], d64, dmag, 11, 'convolution, slope')
+    close(S.causal_conv1d_step(p[None], torch.zeros(1, 1, 2 * n, device=DEV), w)[0], y64, y64.abs(), 8, 'convolution, single frame')
+    one, bc = torch.ones(1, 1, 2 * n, device=DEV), torch.zeros(1, 1, 4, device=DEV)
+    A, D = -torch.ones(2 * n, 4, device=DEV), torch.ones(2 * n, device=DEV)
+    z = p[None, None].clone().requires_grad_(True)
+    y = S.selective_scan(one, one, A, bc, bc, D=D, z=z)
+    close(y[0, 0], y64, y64.abs(), 9, 'gate')
+    dz, = torch.autograd.grad(y, z, torch.ones_like(y))
+    close(dz[0, 0], d64, dmag, 13, 'gate, slope')
+    pool = torch.zeros(1, 2 * n, 4, device=DEV)
+    close(S.selective_scan_step(one[0], one[0], A, bc[0], bc[0], pool, D=D, z=p[None])[0], y64, y64.abs(), 9, 'gate, single frame')
+
+
+@pytest.mark.parametrize('kind', [F32, BF16, F16])
+def test_gates_and_activations_at_the_ends_of_a_type(S, kind):
+    """the lowest value gates to zero with a slope of zero, the largest to itself with a slope of one"""
+    ends = torch.tensor([torch.finfo(kind).min, torch.finfo(kind).max, -200.0, 200.0], device=DEV, dtype=kind)
+    y0, d0 = ends.clamp_min(0), torch.tensor([0.0, 1.0, 0.0, 1.0], device=DEV, dtype=kind)
+    w = torch.tensor([0.0, 1.0], device=DEV)[:, None].repeat(1, 4)
+    x = ends[None, None].clone().requires_grad_(True)
+    y = S.causal_conv1d(x, w)
+    assert torch.equal(y[0, 0], y0) and torch.equal(torch.autograd.grad(y, x, torch.ones_like(y))[0][0, 0], d0)
+    assert torch.equal(S.causal_conv1d_step(ends[None], torch.zeros(1, 1, 4, device=DEV, dtype=kind), w)[0], y0)
+    one, bc = torch.ones(1, 1, 4, device=DEV, dtype=kind), torch.zeros(1, 1, 4, device=DEV, dtype=kind)
+    A, D = -torch.ones(4, 4, device=DEV), torch.ones(4, device=DEV)
+    z = ends[None, None].clone().requires_grad_(True)
+    y = S.selective_scan(one, one, A, bc, bc, D=D, z=z)
+    assert torch.equal(y[0, 0], y0) and torch.equal(torch.autograd.grad(y, z, torch.ones_like(y))[0][0, 0], d0)
+    assert torch.equal(S.selective_scan_step(one[0], one[0], A, bc[0], bc[0], torch.zeros(1, 4, 4, device=DEV), D=D, z=ends[None])[0], y0)

@@ -84,8 +84,22 @@ __device__ __forceinline__ int seq_end(const SeqMap& m, int s, int begin) { retu
 __device__ __forceinline__ int seq_head(const SeqMap& m) { return m.off ? seq_begin(m, 0) : 0; }
 __device__ __forceinline__ int seq_tail(const SeqMap& m) { return m.off ? seq_begin(m, m.n_seqs) : m.rows; }
 
-// 1 / (1 + e^-x) through the reciprocal instruction (one unit in the last place; e^-x overflows to infinity, whose reciprocal is 0)
-__device__ __forceinline__ float sigmoid_acc(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f, LN2_REST = -1.90465429995776804525e-9f;       // log 2 = LN2 + LN2_REST
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// e^v for -128 <= v <= 88.72 (0 where it leaves fp32 downwards): 2^t of t = v log2 e as it is rounded, and what that leaves out put back, e^c = 1 + c with
+// c = v - t log 2: the exponential alone would be off by |v| 2^-24 of itself
+__device__ __forceinline__ float exp_acc(float v) {
+    const float t = v * LOG2E, c = fmaf(t, -LN2_REST, fmaf(t, -LN2, v)), e = exp2_fast(t);
+    return fmaf(e, c, e);
+}
+// 1 / (1 + e^-x) for activations of type T.  fp32: 6 roundings of 2^-24 relative to itself, the exponential 2 and its correction, 1 + e, the reciprocal 2.
+// Beyond the bounds it is 0 (the reciprocal of 2^127.99 is flushed) and 1; of a NaN a number, but everything here multiplies it by x.
+// 16-bit activations: without the correction, off by |x| 2^-24 of itself for negative x; what it goes into is rounded by 2^-9 or 2^-12 (and parameter
+// gradients add it to terms that are not that small).  8192 x 2048 bf16 convolution and gradient 41 us so, 46 with it; 9001 x 1000 fp32 17.6 without, 18.1 with.
+template <class T> __device__ __forceinline__ float sigmoid(float x) {
+    if constexpr (sizeof(T) == 4) return __builtin_amdgcn_rcpf(1.f + exp_acc(-__builtin_amdgcn_fmed3f(x, -88.72f, 128.f)));
+    else return __builtin_amdgcn_rcpf(1.f + __expf(-x));
+}
 // Single-frame calls.  The slot row r names; whether it is padding: a slot outside the pool, or one that an earlier row of the call names.  A wave looks
 // through the earlier rows itself (no barrier); MAX_SLOT_ROWS bounds how many there are.
 constexpr int MAX_SLOT_ROWS = 4096;

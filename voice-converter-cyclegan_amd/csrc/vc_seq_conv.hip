@@ -156,7 +156,7 @@ template <class T, int K, int V, bool SILU, bool PAST> __global__ __launch_bound
                     float q = w.b[e];
 #pragma unroll
                     for (int j = 0; j < K; ++j) q = fmaf(w.w[j][e], win[j][e], q);
-                    o[e] = SILU ? q * sigmoid_acc(q) : q;
+                    o[e] = SILU ? q * sigmoid<T>(q) : q;
 #pragma unroll
                     for (int j = 0; j < K - 1; ++j) win[j][e] = win[j + 1][e];
                 }
@@ -169,14 +169,14 @@ template <class T, int K, int V, bool SILU, bool PAST> __global__ __launch_bound
 }
 
 // g of one frame, from the K frames it looks at
-template <bool SILU, int K, int V> __device__ __forceinline__ void pre_gradient(const float (&win)[K][V], const float (&w)[K][V], const float (&b)[V], float (&g)[V]) {
+template <class T, bool SILU, int K, int V> __device__ __forceinline__ void pre_gradient(const float (&win)[K][V], const float (&w)[K][V], const float (&b)[V], float (&g)[V]) {
     if constexpr (!SILU) return;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         float q = b[e];
 #pragma unroll
         for (int i = 0; i < K; ++i) q = fmaf(w[i][e], win[i][e], q);
-        const float sg = sigmoid_acc(q);
+        const float sg = sigmoid<T>(q);
         g[e] *= sg * fmaf(q, 1.f - sg, 1.f);
     }
 }
@@ -235,7 +235,7 @@ template <class T, int K, int V, bool SILU, bool PAST> __global__ __launch_bound
                 for (int i = 0; i < AHEAD; ++i) {
                     float g[V];
                     xc[i].get(win[K - 1]); gc[i].get(g);
-                    pre_gradient<SILU, K, V>(win, w.w, w.b, g);
+                    pre_gradient<T, SILU, K, V>(win, w.w, w.b, g);
                     const bool mine = r + i < hi;
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
@@ -277,7 +277,7 @@ template <class T, int K, int V, bool SILU, bool PAST> __global__ __launch_bound
             float g[V] = {};
             frame<T, V>(a, s, b, t, p.c, win[K - 1]);
             load_vec<T, V>((const T*)a.dy + (int64_t)(b + t) * a.dy_ld + p.c, g);
-            pre_gradient<SILU, K, V>(win, w.w, w.b, g);
+            pre_gradient<T, SILU, K, V>(win, w.w, w.b, g);
 #pragma unroll
             for (int i = 0; i < K - 1; ++i)                      // frame t's tap j looks at frame t - (K-1) + j = i - (K-1)
                 if (i - t >= 0)
@@ -341,7 +341,7 @@ template <class T> __global__ __launch_bounds__(256) void conv1d_step_kernel(con
     if (c >= a.cols) return;
     T* y = (T*)a.y + (int64_t)r * a.y_ld + c;
     if (padding) { *y = (T)0.f; return; }
-    *y = (T)(a.silu ? p * sigmoid_acc(p) : p);
+    *y = (T)(a.silu ? p * sigmoid<T>(p) : p);
     T* to = (T*)a.state + (int64_t)mine * (a.taps - 1) * a.cols + c;
 #pragma unroll
     for (int k = 0; k < 7; ++k) {

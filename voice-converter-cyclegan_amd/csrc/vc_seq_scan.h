@@ -14,7 +14,6 @@
 #include "vc_seq.h"
 
 constexpr int TILE = 16;
-constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f, LOG2E_REST = 1.92596299112661746887e-8f;     // log2 e = LOG2E + LOG2E_REST
 
 struct ScanK {
     vc_scan_args a; SeqMap m;
@@ -105,16 +104,11 @@ template <int L> __device__ __forceinline__ float channel_sum(float v) {
     return v;
 }
 
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|) in [0, 1], and its slope.  log(1 + e) = 2 atanh(e / (2 + e)) by its series: the argument is at
 // most 1/3, seven terms leave 1.4e-8, and a small e keeps all its bits (a logarithm of the rounded 1 + e would lose them: steps of 0.001 are ordinary here).
 // dt masked by -inf or its type's lowest value is a step of exactly 0 with a slope of 0, the largest value or inf is a step of itself, a NaN stays one.
 __device__ __forceinline__ float softplus(float v, float& slope) {
-    // e^-|v| with what the product with log2 e rounds off put back: the exponential alone would be off by |v| 2^-24 of itself.  |v| counts up to 128, where
-    // e is 0 in fp32: beyond 2^127 the product would leave fp32 and what it rounds off be no number
-    const float av = fminf(fabsf(v), 128.f), t = -av * LOG2E, lo = fmaf(-av, LOG2E, -t) - av * LOG2E_REST;
-    float e = exp2_fast(t);
-    e = fmaf(e, lo * LN2, e);
+    const float e = exp_acc(-fminf(fabsf(v), 128.f));            // (beyond 128 it is 0 in fp32; beyond 2^127 what its argument rounds off would be no number)
     const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
     float p = 1.f / 13.f;
     p = fmaf(p, q, 1.f / 11.f); p = fmaf(p, q, 1.f / 9.f); p = fmaf(p, q, 1.f / 7.f); p = fmaf(p, q, 1.f / 5.f); p = fmaf(p, q, 1.f / 3.f); p = fmaf(p, q, 1.f);

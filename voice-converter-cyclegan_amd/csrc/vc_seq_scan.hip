@@ -197,7 +197,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_fw
                 const float v = (float)tr[b] + bias, d = a.softplus ? softplus(v, slope) : v, xv = (float)xr[b];
                 delta[b] = b * L + j < nr ? d : 0.f;
                 dtx[b] = b * L + j < nr ? d * xv : 0.f;
-                gate[b] = has_z ? (float)zr[b] * sigmoid_acc((float)zr[b]) : 1.f;
+                gate[b] = has_z ? (float)zr[b] * sigmoid<T>((float)zr[b]) : 1.f;
                 skip[b] = Dc * xv;
             }
             if (kt + 1 < k1) fetch(kt + 1);
@@ -283,7 +283,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(256) void scan_st
         float* hp = a.state + ((int64_t)mine * a.cols + c) * a.states + n0;
         store_out<float, NS>(hp, h[u], nn, a.past);
         sum = channel_sum<L>(sum) + D[u] * x[u];
-        if (j == 0) *y = (T)(a.z ? sum * (z[u] * sigmoid_acc(z[u])) : sum);
+        if (j == 0) *y = (T)(a.z ? sum * (z[u] * sigmoid<T>(z[u])) : sum);
     }
 }
 

@@ -108,7 +108,7 @@ template <class T, int L, int NS> __global__ __launch_bounds__(64 * BWD_WAVES) v
             const float v = (float)tr[b] + bias, d = a.softplus ? softplus(v, slope) : v;
             delta[b] = ok ? d : 0.f;
             sd += delta[b];
-            dp[b] = ok ? has_z ? (float)gr[b] * ((float)zr[b] * sigmoid_acc((float)zr[b])) : (float)gr[b] : 0.f;
+            dp[b] = ok ? has_z ? (float)gr[b] * ((float)zr[b] * sigmoid<T>((float)zr[b])) : (float)gr[b] : 0.f;
         }
         if (kt > k0) fetch(kt - 1);
         wave_lds_fence();
@@ -207,7 +207,7 @@ template <class T, int L, int NS, bool FULL> __global__ __launch_bounds__(64 * B
             dtx[b] = delta[b] * xv[b];
             dp[b] = g; dzf[b] = 0.f;
             if (has_z) {
-                const float zv = ok ? (float)zr[b] : 0.f, sg = sigmoid_acc(zv);
+                const float zv = ok ? (float)zr[b] : 0.f, sg = sigmoid<T>(zv);
                 dp[b] = g * (zv * sg);
                 dzf[b] = g * (sg * (1.f + zv * (1.f - sg)));
             }
