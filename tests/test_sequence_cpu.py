@@ -294,3 +294,26 @@ def test_convolution_in_place_is_refused(L):
         assert b(C.byref(_conv(L, **{**full, **bad})), NULL_STREAM) == -1 and b'in place' in L.lib.vc_last_error(), bad
     a = dict(dy=4096, dx=4096, ddt=4096, dB=4096, dC=4096, dA=4096, saved=4096, saved_floats=1 << 20, work=4096, work_floats=1 << 20, dy_ld=8, dx_ld=8, ddt_ld=8, db_ld=16, dc_ld=16)
     assert L.lib.vc_selective_scan_bwd(C.byref(_scan(L, dinitial=1 << 20, dfinal=1 << 20, **a)), NULL_STREAM) == -1 and b'in place' in L.lib.vc_last_error()
+
+
+@pytest.mark.parametrize('lacks', ['nothing', 'torch', 'a compiler', 'headers'])
+def test_the_library_is_built_first_and_without_torch(L, monkeypatch, capsys, lacks):
+    """the binding comes behind the C-ABI library, and what only the binding needs does not stop the library"""
+    import importlib.util
+    import sys
+    spec = importlib.util.spec_from_file_location('_vcb', L._bmod.__file__)
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    done = []
+    monkeypatch.setattr(b, 'build_library', lambda force, verbose: done.append('library') or b.LIB)
+    monkeypatch.setattr(b, 'build_binding', lambda force, verbose: done.append('binding'))
+    if lacks == 'torch':
+        monkeypatch.setitem(sys.modules, 'torch', None)
+    elif lacks == 'a compiler':
+        monkeypatch.setenv('CXX', 'no-such-compiler')
+    elif lacks == 'headers':
+        import sysconfig
+        monkeypatch.setattr(sysconfig, 'get_paths', lambda: {'include': '/nonexistent'})
+    assert b.build() == b.LIB
+    assert done == (['library', 'binding'] if lacks == 'nothing' else ['library'])
+    assert ('not built' in capsys.readouterr().out) == (lacks != 'nothing')

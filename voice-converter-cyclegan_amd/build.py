@@ -91,6 +91,23 @@ def binding_id():
     return h.hexdigest()[:16]
 
 
+def binding_lacks():
+    """What the binding cannot be built without and this machine has not got (None: nothing).  The C-ABI library needs none of it."""
+    import shutil
+    import sysconfig
+    try:
+        import torch
+    except ImportError as e:
+        return 'torch cannot be imported (%s)' % e
+    cxx = os.environ.get('CXX', 'g++')
+    if not shutil.which(cxx):
+        return 'there is no host compiler %s' % cxx
+    for header in (os.path.join(os.path.dirname(torch.__file__), 'include', 'torch', 'csrc', 'utils', 'pybind.h'), os.path.join(sysconfig.get_paths()['include'], 'Python.h')):
+        if not os.path.exists(header):
+            return 'there is no %s' % header
+    return None
+
+
 def build_binding(force=False, verbose=True):
     import sysconfig
     import torch
@@ -110,7 +127,17 @@ def build_binding(force=False, verbose=True):
 
 
 def build(force=False, verbose=True):
-    build_binding(force, verbose)
+    """The library, then the binding where it can be built; without it sequence.py says so at import, and everything else works."""
+    lib = build_library(force, verbose)
+    lacks = binding_lacks()
+    if lacks is None:
+        build_binding(force, verbose)
+    else:
+        print('[vcgan] the torch binding of the sequence operators is not built: ' + lacks, flush=True)
+    return lib
+
+
+def build_library(force=False, verbose=True):
     if not force and not needs_build():
         return LIB
     hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
