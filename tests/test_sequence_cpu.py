@@ -317,3 +317,11 @@ def test_the_library_is_built_first_and_without_torch(L, monkeypatch, capsys, la
     assert b.build() == b.LIB
     assert done == (['library', 'binding'] if lacks == 'nothing' else ['library'])
     assert ('not built' in capsys.readouterr().out) == (lacks != 'nothing')
+
+
+def test_norm_gradient_workspace_goes_by_the_layout(L):
+    """a row of dgamma's sums for each block: four rows a block up to 128 vectors, at most 1024 blocks, 256 where a block has 1024 threads (from 1025 vectors of
+    16 bytes on; the larger of what fp32 and 16-bit rows take)"""
+    for cols, few, many in ((512, 25, 1024), (1024, 100, 1024), (4096, 100, 1024), (8192, 100, 1024), (8200, 100, 256), (16384, 100, 256), (40000, 100, 256)):
+        assert L.lib.vc_rms_norm_bwd_work(100, cols) == few * cols, cols
+        assert L.lib.vc_rms_norm_bwd_work(1 << 20, cols) == many * cols, cols

@@ -397,12 +397,16 @@ int seq_sum_parts(const float* part, int parts, int64_t n, float* dst0, int64_t 
     return 0;
 }
 
-// How a row of nv vectors is held: by a wave with up to two vectors a thread, which needs no barrier; longer ones by a block of 256, then of 1024.
+// How a row of nv vectors is held: by a wave with up to two vectors a thread, which needs no barrier; longer ones by a block of 256, 512, then of 1024.
 // (Before loads and stores went past the L2s.)  Rows of 2048 bf16 with 8-bit output (8832 of them): 58 us by a wave with four vectors a thread, whose registers leave four waves a SIMD, 53 by 128
 // threads, 45 by 256; rows of 1024: 32 us by a wave, 40 by 128 or 256 threads; 2535 rows of 4352 to 8 bits: 40 us by 256 threads, 36 by 512, 38 by 1024.
 #define NORM_LAYOUT(nv, F) \
     ((nv) <= 64 ? F(64, 1) : (nv) <= 128 ? F(64, 2) : (nv) <= 256 ? F(256, 1) : (nv) <= 512 ? F(256, 2) : (nv) <= 1024 ? F(512, 2) : F(1024, 2))
-static int norm_tpr(int64_t nv) { return nv <= 128 ? 64 : nv <= 1024 ? 256 : 1024; }
+static int norm_tpr(int64_t nv) {                                // threads of a row: 64 (four rows a block), or a block
+#define F(TPR, ITEMS) TPR
+    return NORM_LAYOUT(nv, F);
+#undef F
+}
 constexpr int64_t NORM_MOST = 2048;                              // vectors of the longest row that registers hold
 static int64_t norm_vectors(int cols, int type) { const int v = 16 / seq_esize(type); return (cols + v - 1) / v; }
 
@@ -428,8 +432,8 @@ template <class T> static int norm_fwd(const NormRowArgs& a, bool wide, bool e4m
 }
 // Blocks of the gradient: enough to fill the card, few enough that their rows of `part` cost little beside the activations
 static int norm_bwd_blocks(int64_t rows, int cols, int type) {
-    const int64_t nv = norm_vectors(cols, type);
-    const int64_t rpb = nv <= 128 ? 4 : 1, most = norm_tpr(nv) == 1024 ? 256 : 1024;
+    const int tpr = norm_tpr(norm_vectors(cols, type));
+    const int64_t rpb = tpr == 64 ? 4 : 1, most = tpr == 1024 ? 256 : 1024;
     return (int)std::min<int64_t>((rows + rpb - 1) / rpb, most);
 }
 template <class T, class S, int TPR, int ITEMS> static void launch_bwd(const NormRowArgs& a, int blocks, hipStream_t s) {
