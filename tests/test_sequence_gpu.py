@@ -1308,3 +1308,25 @@ def test_gates_and_activations_at_the_ends_of_a_type(S, kind):
     y = S.selective_scan(one, one, A, bc, bc, D=D, z=z)
     assert torch.equal(y[0, 0], y0) and torch.equal(torch.autograd.grad(y, z, torch.ones_like(y))[0][0, 0], d0)
     assert torch.equal(S.selective_scan_step(one[0], one[0], A, bc[0], bc[0], torch.zeros(1, 4, 4, device=DEV), D=D, z=ends[None])[0], y0)
+
+
+@pytest.mark.parametrize('kind,stream,rows,cols', [(BF16, BF16, 24000, 1024), (F16, F16, 6000, 4096), (F32, F32, 12000, 1024), (BF16, None, 50000, 1024), (F32, None, 24000, 1024)])
+def test_norms_that_read_past_the_l2s_equal_their_parts(S, kind, stream, rows, cols):
+    """from 88 MiB of inputs on every pass loads past the L2s: the same bits as in parts that do not; with and without a residual, and a gradient of the sum"""
+    x, gamma, dy = rnd(1, rows, cols, dtype=kind), 1 + rnd(3, cols, scale=0.1), rnd(4, rows, cols, dtype=kind)
+    res, ds = (None, None) if stream is None else (rnd(2, rows, cols, dtype=stream), rnd(5, rows, cols, dtype=stream))
+    assert x.numel() * x.element_size() * (1 if res is None else 2) >= 88 << 20
+    step = rows // 8
+
+    def norm(p):
+        a = x[p].detach().requires_grad_(True)
+        if res is None:
+            y = S.rms_norm(a, gamma)
+            return [y] + list(torch.autograd.grad(y, a, dy[p])) + list(S.rms_norm_e4m3(x[p], gamma, group=64))
+        b = res[p].detach().requires_grad_(True)
+        y, s = S.rms_norm(a, gamma, b)
+        return [y, s] + list(torch.autograd.grad((y, s), (a, b), (dy[p], ds[p]), retain_graph=True)) + list(torch.autograd.grad(y, a, dy[p])) \
+            + list(S.rms_norm_e4m3(x[p], gamma, res[p], group=64))
+    whole, parts = norm(slice(0, rows)), [norm(slice(i, min(i + step, rows))) for i in range(0, rows, step)]
+    for i, (a, *b) in enumerate(zip(whole, *parts)):
+        assert torch.equal(a.float(), torch.cat(b).float()), i

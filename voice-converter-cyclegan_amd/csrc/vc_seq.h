@@ -60,10 +60,14 @@ template <class T, int V> __device__ __forceinline__ void store_out(T* p, const 
     store_some<T, V>(p, f, n);
 }
 
-// ... and such loads, where a thread takes a vector in one access (two would fetch their line twice) and rows share no line.  Only from LOAD_BYTES on: of
-// smaller inputs the last level of cache may still hold much.  Norm of 16384 x 1024 bf16 and its gradient 73 us without, 62 with; to 8 bits 8832 x 2048
-// 43 and 38, 2048 x 8192 35 and 38; norm of 16384 x 2048 and the product behind it 86 and 78, of 8192 x 2048 51 and 53, of 8192 x 1024 (not chosen) 32 and 35.
-constexpr int64_t LOAD_BYTES = 32 << 20;                         // of one tensor
+// ... and such loads, where a thread takes a vector in one access (two would fetch their line twice) and rows share no line.  Only where a pass reads
+// LOAD_BYTES or more in all: of fewer the last level of cache may still hold much.  Norm kernels of 1024 or 2048 columns on three sets of tensors in turn, us
+// without and with, by what a pass reads: forward of bf16 rows 64 MiB 24.3 and 24.9, 80 MiB 29.4 and 30.0, 88 MiB 39.8 and 32.5, 128 MiB 54.8 and 46.1; of fp32
+// rows 64 MiB 21.3 and 24.2, 80 MiB 26.0 and 29.6, 88 MiB 33.1 and 32.3, 128 MiB 48.7 and 45.3; to 8 bits 64 MiB 32.2 and 32.5 (2048 x 8192: 38.1 and 41.2), 80 MiB
+// 41.4 and 38.1, 96 MiB 48.9 and 45.1; gradient 60 MiB 26.1 and 25.5, 84 MiB 37.4 and 33.3, 96 MiB 40.8 and 34.0, fp32 33.6 and 34.7 (1024 columns 33.3 and 29.9),
+// 192 MiB 75.7 and 61.0, fp32 56.3 and 56.1.  Between a kernel that has just written the input and one that reads the result such loads win at all sizes
+// (16-bit rows up to 10 %, fp32 1 %); below the border they are left out for the calls that find their inputs in the cache.
+constexpr int64_t LOAD_BYTES = 88 << 20;                         // of all tensors that a pass reads
 template <class T, int V> __device__ __forceinline__ void load_in(const T* p, float (&f)[V], int n, bool past) {
     if constexpr (V * sizeof(T) == 16) {
         if (past && n >= V) {

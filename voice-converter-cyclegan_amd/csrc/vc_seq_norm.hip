@@ -468,11 +468,12 @@ static int check_ld(const char* who, const NormRowArgs& a, std::initializer_list
     for (int64_t ld : out) VC_ARG(ld >= a.cols, "%s: a row stride of %lld elements: rows of an output of %d columns overlap", who, (long long)ld, a.cols);
     return 0;
 }
-static void set_past(NormRowArgs& a, int type) {
-    const int64_t e = seq_esize(type), bytes = a.rows * a.cols * e;
-    a.past = bytes >= STREAM_BYTES;
-    a.past_in = bytes >= LOAD_BYTES;
-    for (int64_t n : {(int64_t)a.cols, a.x_ld, a.res_ld, a.sum_ld, a.dy_ld, a.dsum_ld}) a.past_in = a.past_in && n * e % 128 == 0;     // no line shared by rows
+static void set_past(NormRowArgs& a, int type, bool wide) {
+    const int64_t e = seq_esize(type), es = wide ? 4 : e, n = a.rows * a.cols;
+    a.past = n * e >= STREAM_BYTES;
+    const int64_t read = a.dy ? n * (e + (a.dsum ? 2 : 1) * es) : n * (e + (a.res ? es : 0));
+    a.past_in = read >= LOAD_BYTES;
+    for (int64_t w : {(int64_t)a.cols, a.x_ld, a.res_ld, a.sum_ld, a.dy_ld, a.dsum_ld}) a.past_in = a.past_in && w * e % 128 == 0;     // no line shared by rows
 }
 static int norm_entry(const char* who, NormRowArgs& a, int type, int sum_type, bool e4m3, void* stream) {
     VC_CHECK(check_norm(who, a.rows, a.cols, type, sum_type));
@@ -484,7 +485,7 @@ static int norm_entry(const char* who, NormRowArgs& a, int type, int sum_type, b
     VC_ARG(!e4m3 || a.y != a.x, "%s: q may not be x", who);
     if (!a.res) sum_type = type;
     const bool wide = sum_type == VC_F32 && type != VC_F32;
-    set_past(a, type);
+    set_past(a, type, wide);
     return SEQ_TYPES(type, norm_fwd, a, wide, e4m3, (hipStream_t)stream);
 }
 extern "C" int vc_rms_norm_fwd(const void* x, int64_t x_ld, const void* residual, int64_t res_ld, const float* gamma,
@@ -523,8 +524,9 @@ extern "C" int vc_rms_norm_bwd(const void* dy, int64_t dy_ld, const void* dsum, 
     a.dy = dy; a.dy_ld = dy_ld; a.dsum = dsum; a.dsum_ld = dsum_ld; a.sum = (void*)sum; a.sum_ld = sum_ld; a.rstd = (float*)rstd; a.gamma = gamma;
     a.dx = dx; a.dx_ld = dx_ld; a.dres = dres; a.dres_ld = dres_ld; a.rows = rows; a.cols = cols; a.part = dgamma ? work : nullptr;
     VC_CHECK(check_ld("vc_rms_norm_bwd", a, {dy_ld, dsum ? dsum_ld : 0, sum_ld}, {dx ? dx_ld : cols, dres ? dres_ld : cols}));
-    set_past(a, type);
-    return SEQ_TYPES(type, norm_bwd, a, sum_type == VC_F32 && type != VC_F32, type, dgamma, (hipStream_t)stream);
+    const bool wide = sum_type == VC_F32 && type != VC_F32;
+    set_past(a, type, wide);
+    return SEQ_TYPES(type, norm_bwd, a, wide, type, dgamma, (hipStream_t)stream);
 }
 
 extern "C" int vc_seq_version(void) { return 1; }
