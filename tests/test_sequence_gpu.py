@@ -1330,3 +1330,28 @@ def test_norms_that_read_past_the_l2s_equal_their_parts(S, kind, stream, rows, c
     whole, parts = norm(slice(0, rows)), [norm(slice(i, min(i + step, rows))) for i in range(0, rows, step)]
     for i, (a, *b) in enumerate(zip(whole, *parts)):
         assert torch.equal(a.float(), torch.cat(b).float()), i
+
+
+# ------------------------------------------------------------------------------------------ gradients by what they add over
+
+@pytest.mark.parametrize('lengths,hint', [([4000], None), ([900, 7, 0, 1500], None), ([70] * 40, 70)])
+@pytest.mark.parametrize('cols,states,groups,kind', [(48, 16, 1, F32), (26, 12, 2, F32), (40, 16, 1, BF16)])
+def test_scan_gradients_add_over_what_their_bounds_count(S, lengths, hint, cols, states, groups, kind):
+    """dx, ddt, dz and dinitial add over states only, dB and dC over a group's channels as well, dA, dD and ddt_bias over the rows: bounds that count no more.
+    States forget fast here (delta |A| >= 0.5: 2^-24 is left after 34 frames), so the recurrence's own share is small."""
+    rows, n = sum(lengths), len(lengths)
+    v = scan_inputs(rows, cols, states, groups, kind, n)
+    v['A'] = v['A'] - 10.0
+    dy, df = rnd(20, rows, cols, dtype=kind), rnd(21, n, cols, states)
+    leaves = [t.requires_grad_(True) for t in v.values()]
+    y, final = S.selective_scan(v['x'], v['dt'], v['A'], v['B'], v['C'], D=v['D'], z=v['z'], dt_bias=v['dt_bias'], initial_state=v['initial'],
+                                seq_offsets=offsets_of(lengths), max_len=hint, return_final_state=True)
+    r = O.scan(**v, lengths=lengths, dy=dy, dfinal=df)
+    m = O.scan(**v, lengths=lengths, dy=dy, dfinal=df, absolute=True)
+    last = lasts(r, v['A'], max(lengths))
+    assert last < 50
+    close(y, r['y'], m['y'], 3 * last + states + 40, 'y')
+    close(final, r['final'], m['final'], 3 * last + states + 40, 'final')
+    for (name, _), got in zip(v.items(), torch.autograd.grad((y, final), leaves, (dy, df))):
+        over = rows if name in ('A', 'D', 'dt_bias') else cols // groups if name in ('B', 'C') else 0
+        close(got, r['d' + name], m['d' + name], 6 * last + over + states + 60, 'd' + name)
