@@ -242,7 +242,8 @@ int vc_rms_norm_fwd(const void* x, int64_t x_ld, const void* residual, int64_t r
                     int64_t rows, int cols, int type, int sum_type, void* stream);
 /* The same with y in 8 bits: q [rows][cols] OCP e4m3 (one byte each), y ~= q * scale.  group: columns that share a scale: 32, 64 or 128
  * (dividing cols), or 0 for the whole row; scale [rows][cols/group or 1], contiguous.  scale = max|y| / 448 of the fp32 y (not below 2^-100 / 448),
- * q = y / scale rounded to nearest even.  A group that holds a NaN or an infinity gets a NaN or infinite scale: it stands for no numbers. */
+ * q = y / scale rounded to nearest even.  A group that holds a NaN or an infinity gets a NaN or infinite scale: it stands for no numbers
+ * (|t gamma| beyond fp32 counts as infinite). */
 int vc_rms_norm_e4m3(const void* x, int64_t x_ld, const void* residual, int64_t res_ld, const float* gamma,
                      void* q, int64_t q_ld, float* scale, void* sum, int64_t sum_ld, float eps,
                      int64_t rows, int cols, int group, int type, int sum_type, void* stream);
@@ -278,7 +279,8 @@ int vc_causal_conv1d_step(const void* x, int64_t x_ld, void* state, const int32_
                           void* y, int64_t y_ld, int rows, int n_slots, int cols, int taps, int type, int silu, void* stream);
 
 /* Selective state space scan along the rows:
- *   delta = softplus(dt + dt_bias) (softplus != 0) or dt + dt_bias
+ *   delta = softplus(dt + dt_bias) (softplus != 0) or dt + dt_bias.  softplus of -inf or of the type's lowest value is 0 (the frame leaves the state as it
+ *   is, and dt has no gradient); a delta of +inf, or delta x beyond fp32, leaves infinities or NaN in its channel from there on
  *   h[t][c][n] = exp(delta[t][c] A[c][n]) h[t-1][c][n] + delta[t][c] x[t][c] B[t][g][n]
  *   y[t][c] = (sum_n C[t][g][n] h[t][c][n] + D[c] x[t][c]) * z[t][c] sigmoid(z[t][c])
  * with g = c / (cols / groups): the channels of a group share B and C.  A [cols][states] fp32, finite, 1 <= states <= 64.  D, z, dt_bias may be NULL

@@ -6,7 +6,7 @@
 #include <algorithm>
 #include <type_traits>
 
-// VC_ARG inside a function that returns the status itself
+// F<T>(arguments) for the element type that `type` names
 #define SEQ_TYPES(type, F, ...) ((type) == VC_F32 ? F<float>(__VA_ARGS__) : (type) == VC_BF16 ? F<__bf16>(__VA_ARGS__) : F<_Float16>(__VA_ARGS__))
 static inline int seq_esize(int type) { return type == VC_F32 ? 4 : 2; }
 // Channels of a call: column indexes of the norm and of the convolution, and what they step over, then stay within 31 bits

@@ -109,7 +109,7 @@ template <int V> __device__ __forceinline__ float rest_of(const float (&p)[V], c
 constexpr float NO_REST = -3.0e38f;
 
 // A row of up to TPR * ITEMS vectors in registers.  Threads walk the rows with a stride of the grid, so gamma is read once for all of them.
-// 16384 x 1024 bf16 with a residual: 28 us, 4.8 TB/s (a copy 5.0); 8832 x 2048 bf16 on an fp32 stream to 8 bits: 38 us, 5.2 TB/s; 1 x 512: 2.9 us.
+// 16384 x 1024 bf16 with a residual: 28 us, 4.8 TB/s (a copy 5.0); 8832 x 2048 bf16 on an fp32 stream to 8 bits: 39 us, 5.1 TB/s; 1 x 512: 2.9 us.
 template <class T, class S, bool E4M3, int TPR, int ITEMS> __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_fwd_kernel(const NormRowArgs a) {
     constexpr int V = 16 / (int)sizeof(T), RPB = TPR == 64 ? 4 : 1;
     __shared__ float red[TPR / 64 > 0 ? TPR / 64 : 1];

@@ -3,7 +3,7 @@
 //   dA = sum_t q delta;  ddelta = sum_n q A + x sum_n dh B;  dx = D dp + delta sum_n dh B;  dB = sum_c dh delta x;  dC = sum_c dp h
 // A tile's states are worked out again from the one the forward kept in front of it: a and h of its 16 rows stay in registers for the way back.
 // Bound by vector issue: six slots a state on the way there, eight and five for the sums over channels on the way back, two waves a SIMD (the registers).
-// 64 x 128 x 1024 bf16, 16 states: 134 us, the vector units busy 84 % of the time.
+// 64 x 128 x 1024 bf16, 16 states: 136 us, the vector units busy 83 % of the time.
 #include "vc_seq_scan.h"
 
 constexpr int BWD_WAVES = 4;                                     // of a block.  8 leave half as many partial sums of dB and dC and cost 2 %: more waves stand at a barrier together

@@ -8,10 +8,10 @@ operators look back only: a model of them trains on packed utterances and conver
     v = selective_scan(u, dt, A, B, C, D=D, z=z)      # all earlier frames, through a state of `states` numbers a channel
 
 Frames are rows: tensors are [batch, frames, channels], or [rows, channels] with `seq_offsets` (int32, [n + 1], rising, on the same device) where
-utterances of different lengths lie one behind the other; lengths of zero are fine, and rows ahead of the first utterance
-or behind the last give zeros.  Any row stride is taken in place (column slices of a product, for one).  Activations are fp32, bf16 or fp16 (one type in
-a call); parameters, recurrent states and parameter gradients are fp32, and every sum is.  The kernels are those of include/vc_cyclegan.h; gradients are
-deterministic.
+utterances of different lengths lie one behind the other; lengths of zero are fine, and rows ahead of the first utterance or behind the last give
+zeros.  Rows are taken in place (column slices of a product, for one) unless they lie very far apart, more than 2^15 elements for the convolution (2^20 from
+256 channels on) and 2^24 for the scan: those are copied.  Activations are fp32, bf16 or fp16 (one type in a call); parameters, recurrent states and
+parameter gradients are fp32, and every sum is.  The kernels are those of include/vc_cyclegan.h; gradients are deterministic.
 
 A backward pass that is captured into a graph must not meet an eager autograd graph of the same leaves that is still alive: torch's gradient
 accumulators belong to the stream they were made on.  Drop the eager outputs first."""
@@ -77,6 +77,7 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, initial_state=N
 
     x, dt, z: [batch, frames, channels] or packed [rows, channels]; A [channels, states] (finite, 1 to 64 states); B, C: [..., states] shared by all
     channels, or [..., groups, states], the channels of a group next to each other; D, dt_bias [channels].  softplus=False: delta = dt + dt_bias.
+    A frame masked by dt = -inf or its type's lowest value leaves the state as it is.
     initial_state [utterances, channels, states] (float32; zeros otherwise); return_final_state: (y, the state behind each utterance's last frame).
     max_len: the longest utterance where the program knows it: how a packed call is split, never what it gives."""
     return _seq.selective_scan(x, dt, A, B, C, D, z, dt_bias, initial_state, seq_offsets, max_len or 0, bool(softplus), bool(return_final_state))
